@@ -124,7 +124,9 @@ typedef enum {
 } tq_status;
 
 typedef enum { TQ_DTYPE_F32 = 0, TQ_DTYPE_F16 = 1, TQ_DTYPE_BF16 = 2 } tq_dtype;
-typedef enum { TQ_TYPE_TQ2_0 = 2, TQ_TYPE_TQ3_0 = 3, TQ_TYPE_TQ4_0 = 4 } tq_type;
+typedef enum { TQ_TYPE_TQ2_0 = 2, TQ_TYPE_TQ3_0 = 3, TQ_TYPE_TQ4_0 = 4,
+               TQ_TYPE_Q8 = 8   /* paged caches only: int8 codes, one scale per 16 tokens and head (below) */
+} tq_type;
 
 const char *tq_status_string(tq_status s);
 /* message of the last failure on the calling thread ("" if none) */
@@ -355,6 +357,83 @@ tq_status tq_kv_append_paged_cuda(tq_type type, const void *src, tq_dtype src_dt
                                   int n_kv_heads, int head_dim, const tq_kv_pages *pages, int64_t n_new,
                                   const int32_t *pos, int rotate, int opt_passes, int32_t *overflow,
                                   void *stream);
+
+/* ── rotation by position, and the paged append with it on the way ────────────
+ *
+ * Rotary positions with one or several axes (no counterpart in the reference C; the rotation that its
+ * prototype's tests combine with the Hadamard rotation, prototype/tests/test_rope_invariance.py:69-135).
+ * Pair i of a head row, elements (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved, turns by the
+ * angle p * inv_freq[i], p the token's position on axis axis[i]:
+ *   (a, b) -> (a cos - b sin, b cos + a sin),   cos and sin times scale;
+ * elements from rotary_dim on stay as they are.  inverse turns back, which is also the rotation's gradient
+ * (scale included).  Angles are exact for every int32 position: the cosines and sines are those of 64-bit
+ * arithmetic rounded to float32.  inv_freq is float64 device memory: any frequencies (a base, a scaling
+ * rule, one set per axis) come as values.  |inv_freq| must be below 2^31.  axis entries outside
+ * [0, n_axes) read the nearest axis.
+ */
+typedef struct {
+    const double *inv_freq;     /* device [rotary_dim / 2] */
+    const int32_t *axis;        /* device [rotary_dim / 2], or NULL: every pair on axis 0 */
+    const int32_t *positions;   /* device [n_axes][batch][n_new] */
+    int n_axes;
+    int rotary_dim;             /* a multiple of 16, at most head_dim */
+    int interleaved;
+    int inverse;
+    double scale;               /* 1, or a factor on the rotated part (0 = 1) */
+} tq_rope;
+/* rows [batch][heads][n_new][head_dim] of src and dst at strides in elements (batch, head, token); the
+ * last dimension is contiguous and every row starts on a 16-byte boundary */
+typedef struct {
+    const void *src;   void *dst;
+    int heads;
+    int64_t src_stride[3], dst_stride[3];
+} tq_head_rows;
+
+/* Rotates x (and x2, optional: e.g. queries and keys) in one launch; dst may be src (with its strides).
+ * head_dim: a multiple of 8, at most 512. */
+tq_status tq_rotary_cuda(const tq_rope *rope, tq_dtype dtype, int batch, int64_t n_new, int head_dim,
+                         const tq_head_rows *x, const tq_head_rows *x2, void *stream);
+
+/*
+ * A step's rows into a paged cache in one launch: keys are rotated by position (rope.inv_freq not NULL),
+ * Hadamard-rotated (rotate != 0) and quantized into the K pool, values are Hadamard-rotated and quantized
+ * into the V pool, queries (q.heads > 0) are rotated by position into q.dst.  k and v: src only, n_kv_heads
+ * heads each.  Row t of sequence b goes to token slot pos[b] + t (pos NULL: slot t) as in
+ * tq_kv_append_paged_cuda; rope.positions NULL takes the slot as the position.  Rows t >= new_len[b] (a
+ * padded batch; new_len NULL: none) are neither stored nor counted; their queries are rotated all the same.
+ * Rows without a place are counted in *overflow, one per key and one per value row.  The TQ blocks equal
+ * rotation in float32 followed by tq_kv_append_paged_cuda bit for bit (no optimal rounding).
+ *
+ * Pools: TQ2_0 / TQ3_0 / TQ4_0 keys with TQ4_0 values (tq_kv_pages above), or TQ_TYPE_Q8 for both:
+ *   codes  int8  [num_pages][n_kv_heads][page_size][head_dim]
+ *   scale  float [num_pages][n_kv_heads][page_size / TQ_Q8_BLOCK]
+ * A value is code * scale, |code| <= 127, one scale for the head rows of TQ_Q8_BLOCK consecutive slots:
+ * max |x| / 127 over the rows stored in the block.  It starts anew when slot 0 of the block is written and
+ * grows when a later row needs it; then the block's earlier codes are rounded to the new scale.  Slots
+ * behind the last row keep their codes.  Scales below 2^-100 are stored as 0.  Inputs must be finite.
+ * head_dim 128 or 256.  Two sequences of a call must not share a page that they write.
+ */
+#define TQ_Q8_BLOCK 16
+typedef struct {
+    int batch, n_kv_heads, head_dim;
+    int64_t n_new;
+    tq_dtype dtype;             /* of k, v, q and the rotated queries */
+    tq_head_rows k, v, q;
+    tq_rope rope;               /* inverse must be 0 */
+    void *k_pool;               tq_type k_type;
+    float *k_scale;             /* TQ_TYPE_Q8 only */
+    void *v_pool;               tq_type v_type;
+    float *v_scale;
+    const int32_t *pos;         /* device [batch] */
+    const int32_t *new_len;     /* device [batch] */
+    int rotate;
+    int32_t *overflow;          /* device, optional */
+} tq_rotary_append_args;
+tq_status tq_kv_append_rotary_paged_cuda(const tq_rotary_append_args *a, const tq_kv_pages *pages, void *stream);
+/* values of n_blocks 16-token blocks of 8-bit pages: y[i] = codes[i] * scale[i / (16 head_dim)], rounded to
+ * y_dtype; head_dim 128 or 256 */
+tq_status tq_dequantize_q8_cuda(const int8_t *codes, const float *scale, void *y, tq_dtype y_dtype,
+                                int64_t n_blocks, int head_dim, void *stream);
 
 /* log-sum-exp merge of n_parts partial results o[n_parts][n_rows][head_dim] with
  * natural-log lse[n_parts][n_rows] into out[n_rows][head_dim] (+ lse_out, optional):

@@ -18,7 +18,7 @@ def load_library():
 
 def __getattr__(name):
     # torch-backed submodules load on first use so the C-ABI layer imports without torch
-    if name in ("ops", "attention", "distributed", "turboquant"):
+    if name in ("ops", "attention", "distributed", "paged", "turboquant"):
         import importlib
         return importlib.import_module(f"{__name__}.{name}")
     raise AttributeError(name)

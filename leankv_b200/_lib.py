@@ -21,6 +21,8 @@ STATUS_NAMES = {0: "TQ_SUCCESS", 1: "TQ_ERROR_INVALID_VALUE", 2: "TQ_ERROR_UNSUP
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 TQ_PEER_HANDLE_BYTES = 64   # bytes of a tq_peer_exchange_create handle
 TYPE_TQ2_0, TYPE_TQ3_0, TYPE_TQ4_0 = 2, 3, 4
+TYPE_Q8 = 8                 # int8 codes of 8-bit pages
+Q8_BLOCK = 16               # token slots that share a scale there
 BLOCK_BYTES = {TYPE_TQ2_0: 10, TYPE_TQ3_0: 14, TYPE_TQ4_0: 18}
 QK = 32
 
@@ -102,6 +104,10 @@ SIGNATURES = {
     # KV-cache append
     "tq_kv_append_cuda": (_i32, [_i32, _v, _i32, _v, _i32, _i32, _i32, _i64, _i64, _v, _i32, _i32, _v, _v]),
     "tq_kv_append_paged_cuda": (_i32, [_i32, _v, _i32, _v, _i32, _i32, _i32, _v, _i64, _v, _i32, _i32, _v, _v]),
+    # rotary positions, paged append with the rotation on the way, 8-bit pages (argument blocks: leankv_b200.ops)
+    "tq_rotary_cuda": (_i32, [_v, _i32, _i32, _i64, _i32, _v, _v, _v]),
+    "tq_kv_append_rotary_paged_cuda": (_i32, [_v, _v, _v]),
+    "tq_dequantize_q8_cuda": (_i32, [_v, _v, _v, _i32, _i64, _i32, _v]),
     # split-sequence merge over peer memory (exchange handles are opaque pointers)
     "tq_peer_exchange_create": (_i32, [_i32, _i32, _i64, _i32, C.c_uint32, _v, _v]),
     "tq_peer_exchange_connect": (_i32, [_v, _v]),

@@ -1,0 +1,154 @@
+// tq_capi_q8.cu — extern "C" entry points of the rotary operators and the 8-bit paged cache.
+#include <cmath>
+
+#include "leankv_tq.h"
+#include "tq_capi_internal.h"
+#include "tq_common.cuh"
+#include "tq_rope.h"
+
+using namespace tq;
+
+// rows of 8 elements at a time: base and strides on 16-byte boundaries
+static tq_status rows_check(const tq_head_rows* x, bool has_dst, size_t eb, const char* name) {
+    if (x->heads <= 0) return set_error(TQ_ERROR_INVALID_VALUE, "%s: bad head count", name);
+    if (!x->src || (has_dst && !x->dst)) return set_error(TQ_ERROR_INVALID_VALUE, "%s: null pointer", name);
+    uintptr_t m = (uintptr_t)x->src | (has_dst ? (uintptr_t)x->dst : 0);
+    for (int i = 0; i < 3; ++i)
+        m |= (uintptr_t)(x->src_stride[i] * (int64_t)eb) | (has_dst ? (uintptr_t)(x->dst_stride[i] * (int64_t)eb) : 0);
+    if (m & 15) return set_error(TQ_ERROR_MISALIGNED, "%s: rows must start on 16-byte boundaries", name);
+    if (has_dst && x->src == x->dst)
+        for (int i = 0; i < 3; ++i)
+            if (x->src_stride[i] != x->dst_stride[i])
+                return set_error(TQ_ERROR_INVALID_VALUE, "%s: in place needs equal strides", name);
+    return TQ_SUCCESS;
+}
+
+static HeadRows rows_of(const tq_head_rows* x) {
+    HeadRows r;
+    r.src = x->src;
+    r.dst = x->dst;
+    r.heads = x->heads;
+    for (int i = 0; i < 3; ++i) {
+        r.ss[i] = x->src_stride[i];
+        r.ds[i] = x->dst_stride[i];
+    }
+    return r;
+}
+
+static tq_status rope_check(const tq_rope* p, int head_dim, bool need_positions, Rope* r) {
+    if (p->rotary_dim <= 0 || p->rotary_dim > head_dim || p->rotary_dim % 16)
+        return set_error(TQ_ERROR_INVALID_VALUE, "rotary_dim=%d (a multiple of 16, at most head_dim)", p->rotary_dim);
+    if (!p->inv_freq || (need_positions && !p->positions)) return set_error(TQ_ERROR_INVALID_VALUE, "null frequencies or positions");
+    if (p->n_axes <= 0 || p->n_axes > 16) return set_error(TQ_ERROR_INVALID_VALUE, "n_axes=%d (1 .. 16)", p->n_axes);
+    if (!std::isfinite(p->scale)) return set_error(TQ_ERROR_INVALID_VALUE, "scale is not finite");
+    if (((uintptr_t)p->inv_freq & 7) || (((uintptr_t)p->axis | (uintptr_t)p->positions) & 3))
+        return set_error(TQ_ERROR_MISALIGNED, "frequencies, axes or positions not aligned to their element size");
+    r->inv_freq = p->inv_freq;
+    r->axis = p->axis;
+    r->positions = p->positions;
+    r->n_axes = p->n_axes;
+    r->rotary_dim = p->rotary_dim;
+    r->interleaved = p->interleaved != 0;
+    r->inverse = p->inverse != 0;
+    r->scale = p->scale != 0.0 ? p->scale : 1.0;
+    return TQ_SUCCESS;
+}
+
+extern "C" tq_status tq_rotary_cuda(const tq_rope* rope, tq_dtype dtype, int batch, int64_t n_new, int head_dim,
+                                    const tq_head_rows* x, const tq_head_rows* x2, void* stream) {
+    clear_error();
+    if (!rope || !x) return set_error(TQ_ERROR_INVALID_VALUE, "null argument");
+    if (!dtype_ok(dtype)) return set_error(TQ_ERROR_INVALID_VALUE, "unknown dtype %d", (int)dtype);
+    if (batch < 0 || n_new < 0 || n_new > INT32_MAX) return set_error(TQ_ERROR_INVALID_VALUE, "bad batch or token count");
+    if (head_dim <= 0 || head_dim % 8 || head_dim > 512)
+        return set_error(TQ_ERROR_UNSUPPORTED, "head_dim=%d (a multiple of 8, at most 512)", head_dim);
+    RotaryRun r;
+    tq_status s = rope_check(rope, head_dim, batch > 0 && n_new > 0, &r.rope);
+    if (s) return s;
+    if (batch == 0 || n_new == 0) return TQ_SUCCESS;
+    if ((s = rows_check(x, true, dtype_bytes(dtype), "x"))) return s;
+    if (x2 && (s = rows_check(x2, true, dtype_bytes(dtype), "x2"))) return s;
+    r.batch = batch;
+    r.head_dim = head_dim;
+    r.dtype = (int)dtype;
+    r.n_new = n_new;
+    r.x[0] = rows_of(x);
+    if (x2) r.x[1] = rows_of(x2);
+    return cuda_status(launch_rotary(r, (cudaStream_t)stream), "rotary kernel launch");
+}
+
+extern "C" tq_status tq_kv_append_rotary_paged_cuda(const tq_rotary_append_args* a, const tq_kv_pages* pg, void* stream) {
+    clear_error();
+    if (!a) return set_error(TQ_ERROR_INVALID_VALUE, "null argument block");
+    if (!dtype_ok(a->dtype)) return set_error(TQ_ERROR_INVALID_VALUE, "unknown dtype %d", (int)a->dtype);
+    if (a->batch < 0 || a->n_kv_heads <= 0 || a->n_new < 0 || a->n_new > INT32_MAX)
+        return set_error(TQ_ERROR_INVALID_VALUE, "bad batch / head / row counts");
+    if (a->head_dim != 128 && a->head_dim != 256)
+        return set_error(TQ_ERROR_UNSUPPORTED, "head_dim %d (supported: 128, 256)", a->head_dim);
+    const bool q8 = a->k_type == TQ_TYPE_Q8;
+    if (q8 ? a->v_type != TQ_TYPE_Q8
+           : (a->v_type != TQ_TYPE_TQ4_0 || (a->k_type != TQ_TYPE_TQ4_0 && a->k_type != TQ_TYPE_TQ3_0 && a->k_type != TQ_TYPE_TQ2_0)))
+        return set_error(TQ_ERROR_UNSUPPORTED, "block types K=%d V=%d (supported: K TQ4_0, TQ3_0 or TQ2_0 with V TQ4_0, or Q8 for both)",
+                         (int)a->k_type, (int)a->v_type);
+    int shift = 0;
+    tq_status s = pages_check(pg, a->batch, &shift);
+    if (s) return s;
+    RotaryAppendRun r;
+    if (a->rope.inv_freq) {
+        if ((s = rope_check(&a->rope, a->head_dim, false, &r.rope))) return s;
+        if (a->rope.inverse) return set_error(TQ_ERROR_INVALID_VALUE, "the append rotates forward only");
+        if (!a->rope.positions && a->rope.n_axes != 1)
+            return set_error(TQ_ERROR_INVALID_VALUE, "several axes need positions");
+    } else if (a->q.heads > 0) {
+        return set_error(TQ_ERROR_INVALID_VALUE, "queries without a rotation");
+    }
+    if (a->batch == 0 || a->n_new == 0) return TQ_SUCCESS;
+    const size_t eb = dtype_bytes(a->dtype);
+    if (a->k.heads != a->n_kv_heads || a->v.heads != a->n_kv_heads)
+        return set_error(TQ_ERROR_INVALID_VALUE, "k and v must have n_kv_heads heads");
+    if (a->q.heads < 0) return set_error(TQ_ERROR_INVALID_VALUE, "bad query head count");
+    if ((s = rows_check(&a->k, false, eb, "k")) || (s = rows_check(&a->v, false, eb, "v"))) return s;
+    if (a->q.heads > 0 && (s = rows_check(&a->q, true, eb, "q"))) return s;
+    if (!a->k_pool || !a->v_pool || (q8 && (!a->k_scale || !a->v_scale))) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
+    if (((uintptr_t)a->k_pool | (uintptr_t)a->v_pool) & 15) return set_error(TQ_ERROR_MISALIGNED, "pools must be 16-byte aligned");
+    if (((uintptr_t)a->k_scale | (uintptr_t)a->v_scale | (uintptr_t)a->pos | (uintptr_t)a->new_len | (uintptr_t)a->overflow) & 3)
+        return set_error(TQ_ERROR_MISALIGNED, "scales, lengths or overflow not 4-byte aligned");
+    r.batch = a->batch;
+    r.head_dim = a->head_dim;
+    r.n_kv_heads = a->n_kv_heads;
+    r.dtype = (int)a->dtype;
+    r.n_new = a->n_new;
+    r.k = rows_of(&a->k);
+    r.v = rows_of(&a->v);
+    if (a->q.heads > 0) r.q = rows_of(&a->q);
+    r.kd.pool = static_cast<uint8_t*>(a->k_pool);
+    r.kd.scale = a->k_scale;
+    r.kd.type = (int)a->k_type;
+    r.vd.pool = static_cast<uint8_t*>(a->v_pool);
+    r.vd.scale = a->v_scale;
+    r.vd.type = (int)a->v_type;
+    r.pages = pg->page_table;
+    r.max_pages = pg->max_pages_per_seq;
+    r.num_pages = pg->num_pages;
+    r.page_shift = shift;
+    r.pos = a->pos;
+    r.new_len = a->new_len;
+    r.rotate = a->rotate != 0;
+    r.norm = fwht_norm(a->head_dim);
+    r.overflow = a->overflow;
+    return cuda_status(launch_rotary_append(r, (cudaStream_t)stream), "rotary append kernel launch");
+}
+
+extern "C" tq_status tq_dequantize_q8_cuda(const int8_t* codes, const float* scale, void* y, tq_dtype y_dtype,
+                                           int64_t n_blocks, int head_dim, void* stream) {
+    clear_error();
+    if (!dtype_ok(y_dtype)) return set_error(TQ_ERROR_INVALID_VALUE, "unknown output dtype %d", (int)y_dtype);
+    if (head_dim != 128 && head_dim != 256) return set_error(TQ_ERROR_UNSUPPORTED, "head_dim %d (supported: 128, 256)", head_dim);
+    if (n_blocks < 0) return set_error(TQ_ERROR_INVALID_VALUE, "n_blocks=%lld", (long long)n_blocks);
+    if (n_blocks == 0) return TQ_SUCCESS;
+    if (!codes || !scale || !y) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
+    if ((((uintptr_t)codes | (uintptr_t)y) & 15) || ((uintptr_t)scale & 3))
+        return set_error(TQ_ERROR_MISALIGNED, "codes and y must be 16-byte aligned, scales 4-byte aligned");
+    return cuda_status(launch_dequantize_q8(codes, scale, y, (int)y_dtype, n_blocks, head_dim, (cudaStream_t)stream),
+                       "dequantize kernel launch");
+}

@@ -6,7 +6,9 @@ TQ4_0 or (n_blocks, 14) for TQ3_0 — the byte layout of src/ggml-tq.h:131-141.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
@@ -14,6 +16,7 @@ from . import _lib as L
 
 QK = L.QK
 TQ2_0, TQ3_0, TQ4_0 = L.TYPE_TQ2_0, L.TYPE_TQ3_0, L.TYPE_TQ4_0
+Q8, Q8_BLOCK = L.TYPE_Q8, L.Q8_BLOCK
 BLOCK_BYTES = L.BLOCK_BYTES
 _DTYPES = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16}
 
@@ -183,6 +186,264 @@ def kv_append_paged(src: torch.Tensor, pool: torch.Tensor, page_table: torch.Ten
                                              int(rotate), int(opt_passes),
                                              overflow.data_ptr() if overflow is not None else None, _stream(src)))
     return pool
+
+
+# ── rotation by position ─────────────────────────────────────────────────────
+
+class Rotary(NamedTuple):
+    """How head rows turn with their positions (tq_rope in include/leankv_tq.h).
+
+    inv_freq: float64 CUDA tensor [rotary_dim / 2], the angle of each pair per position step
+    (rotary_frequencies() gives the usual ones; scaling rules come as values).  axis: int32 CUDA tensor
+    [rotary_dim / 2], the position axis of each pair (rotary_axes()), None for one axis.  Pairs are the
+    elements (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; scale multiplies the turned part.
+    """
+    inv_freq: torch.Tensor
+    axis: torch.Tensor | None = None
+    interleaved: bool = False
+    scale: float = 1.0
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
+    """theta^(-2 i / rotary_dim), i = 0 .. rotary_dim / 2 - 1, as float64."""
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    return (float(theta) ** (-2.0 * i / rotary_dim)).to(device)
+
+
+def rotary_axes(sections, device="cuda", interleaved: bool = False) -> torch.Tensor:
+    """Position axis of each pair, int32: sections[a] pairs turn with axis a, in consecutive runs, or, when
+    interleaved, dealt out in turn (pair 0 to axis 0, pair 1 to axis 1, ...) until an axis has its share."""
+    left = [int(n) for n in sections]
+    if not left or min(left) < 0:
+        raise ValueError("sections must be counts of pairs, one per axis")
+    if not interleaved:
+        return torch.tensor([a for a, n in enumerate(left) for _ in range(n)], dtype=torch.int32, device=device)
+    order = []
+    while any(left):
+        for a, n in enumerate(left):
+            if n:
+                order.append(a)
+                left[a] -= 1
+    return torch.tensor(order, dtype=torch.int32, device=device)
+
+
+class _Rope(C.Structure):
+    """Mirror of tq_rope (include/leankv_tq.h)."""
+    _fields_ = [("inv_freq", C.c_void_p), ("axis", C.c_void_p), ("positions", C.c_void_p), ("n_axes", C.c_int),
+                ("rotary_dim", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int), ("scale", C.c_double)]
+
+
+class _HeadRows(C.Structure):
+    """Mirror of tq_head_rows (include/leankv_tq.h)."""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("heads", C.c_int), ("src_stride", C.c_int64 * 3),
+                ("dst_stride", C.c_int64 * 3)]
+
+
+class _RotaryAppendArgs(C.Structure):
+    """Mirror of tq_rotary_append_args (include/leankv_tq.h)."""
+    _fields_ = [("batch", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("n_new", C.c_int64),
+                ("dtype", C.c_int), ("k", _HeadRows), ("v", _HeadRows), ("q", _HeadRows), ("rope", _Rope),
+                ("k_pool", C.c_void_p), ("k_type", C.c_int), ("k_scale", C.c_void_p), ("v_pool", C.c_void_p),
+                ("v_type", C.c_int), ("v_scale", C.c_void_p), ("pos", C.c_void_p), ("new_len", C.c_void_p),
+                ("rotate", C.c_int), ("overflow", C.c_void_p)]
+
+
+def _on_device(t: torch.Tensor):
+    """Launches go to the current device: make it the tensor's."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _same_device(t: torch.Tensor, *others) -> None:
+    for o in others:
+        if o is not None and o.device != t.device:
+            raise ValueError(f"tensors on {t.device} and {o.device}")
+
+
+def _check_rows(t: torch.Tensor, name: str) -> None:
+    if t.dim() != 4 or t.dtype not in _DTYPES or (t.shape[3] > 1 and t.stride(3) != 1):
+        raise ValueError(f"{name} must be a f32/f16/bf16 [batch, heads, tokens, head_dim] tensor, head_dim contiguous")
+
+
+def _rows(src: torch.Tensor, dst: torch.Tensor | None = None) -> _HeadRows:
+    s = src.stride()
+    if dst is None:
+        return _HeadRows(src.data_ptr(), None, src.shape[1], (s[0], s[1], s[2]))
+    d = dst.stride()
+    return _HeadRows(src.data_ptr(), dst.data_ptr(), src.shape[1], (s[0], s[1], s[2]), (d[0], d[1], d[2]))
+
+
+def _rope(rope: Rotary, like: torch.Tensor, positions: torch.Tensor | None, inverse: bool) -> _Rope:
+    f, ax = rope.inv_freq, rope.axis
+    _need_cuda(f)
+    if f.dtype != torch.float64 or f.dim() != 1 or not f.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float64 [rotary_dim / 2] tensor")
+    if ax is not None:
+        _need_cuda(ax)
+        if ax.dtype != torch.int32 or ax.shape != f.shape or not ax.is_contiguous():
+            raise ValueError("axis must be a contiguous int32 tensor of inv_freq's shape")
+    axes = 1
+    if positions is not None:
+        _need_cuda(positions)
+        if positions.dtype != torch.int32 or not positions.is_contiguous() or positions.dim() not in (2, 3) \
+                or positions.shape[-2] != like.shape[0] or positions.shape[-1] != like.shape[2]:
+            raise ValueError("positions must be a contiguous int32 [batch, tokens] or [axes, batch, tokens] tensor")
+        axes = positions.shape[0] if positions.dim() == 3 else 1
+        if axes > 1 and ax is None:
+            raise ValueError("positions of several axes need the axis of each pair")
+    _same_device(like, f, ax, positions)
+    return _Rope(f.data_ptr(), None if ax is None else ax.data_ptr(), None if positions is None else positions.data_ptr(),
+                 axes, 2 * f.shape[0], int(rope.interleaved), int(inverse), float(rope.scale))
+
+
+def _rotary_out(t: torch.Tensor, out: torch.Tensor | None, name: str) -> torch.Tensor:
+    if out is None:
+        # token-major memory, as the projections on either side have it
+        return torch.empty((t.shape[0], t.shape[2], t.shape[1], t.shape[3]), dtype=t.dtype, device=t.device).transpose(1, 2)
+    _need_cuda(out)
+    if out.shape != t.shape or out.dtype != t.dtype or (out.shape[3] > 1 and out.stride(3) != 1):
+        raise ValueError(f"{name} must have the shape and type of its input, head_dim contiguous")
+    return out
+
+
+def rotary(q: torch.Tensor, positions: torch.Tensor, rope: Rotary, k: torch.Tensor | None = None,
+           inverse: bool = False, out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Rotates head rows by their positions (tq_rotary_cuda); q (and k, in the same launch) are
+    [batch, heads, tokens, head_dim] of any batch, head and token strides.
+
+    positions: int32 [batch, tokens], or [axes, batch, tokens] with rope.axis naming each pair's axis.
+    Computed in float32 with angles exact at every position, rounded once.  inverse turns back: the
+    gradient of the inputs from that of the outputs.  out / k_out: destinations (may be q / k themselves).
+    Returns the rotated q, or (q, k)."""
+    _need_cuda(q)
+    _check_rows(q, "q")
+    if k is not None:
+        _need_cuda(k)
+        _check_rows(k, "k")
+        if k.dtype != q.dtype or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]:
+            raise ValueError("k must have q's type, batch, tokens and head_dim")
+    if positions is None:
+        raise ValueError("positions are needed")
+    r = _rope(rope, q, positions, inverse)
+    out = _rotary_out(q, out, "out")
+    k_out = _rotary_out(k, k_out, "k_out") if k is not None else None
+    _same_device(q, k, out, k_out)
+    if q.shape[1] == 0 or (k is not None and k.shape[1] == 0):
+        raise ValueError("no heads")
+    with _on_device(q):
+        L.check(L.load().tq_rotary_cuda(C.byref(r), _DTYPES[q.dtype], q.shape[0], q.shape[2], q.shape[3],
+                                        C.byref(_rows(q, out)), C.byref(_rows(k, k_out)) if k is not None else None,
+                                        _stream(q)))
+    return out if k is None else (out, k_out)
+
+
+def kv_append_rotary_paged(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                           page_table: torch.Tensor, pos: torch.Tensor | None = None, rope: Rotary | None = None,
+                           positions: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                           q_out: torch.Tensor | None = None, new_len: torch.Tensor | None = None,
+                           k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                           rotate: bool = True, overflow: torch.Tensor | None = None) -> torch.Tensor | None:
+    """A step's rows into a paged cache in one launch (tq_kv_append_rotary_paged_cuda): keys are rotated by
+    position and quantized into k_pool, values quantized into v_pool, queries rotated.
+
+    k, v [batch, n_kv_heads, n_new, head_dim] and q [batch, n_q_heads, n_new, head_dim] may have any batch,
+    head and token strides (views of one projection's output).  Row t of sequence b goes to slot pos[b] + t
+    of its pages.  rope None stores the keys unturned; positions default to the slots.  Pools: uint8 TQ
+    blocks as in kv_append_paged (TQ2_0 / TQ3_0 / TQ4_0 keys, TQ4_0 values), or int8
+    [num_pages, n_kv_heads, page_size, head_dim] with float32 scales k_scale / v_scale
+    [num_pages, n_kv_heads, page_size / 16] (both pools).  new_len (int32 [batch]): rows t >= new_len[b] of
+    a padded batch are not stored.  rotate: the head_dim Hadamard rotation, as the attention expects.
+    Rows without a place are counted into overflow, keys and values each.  Returns the rotated q (in q_out
+    when given, which may be q), or None without q."""
+    _need_cuda(k, v, k_pool, v_pool, page_table)
+    _check_rows(k, "k")
+    _check_rows(v, "v")
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v must have the same shape and type")
+    B, H, n_new, D = k.shape
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B \
+            or not page_table.is_contiguous():
+        raise ValueError("page_table must be a contiguous int32 [batch, max_pages_per_seq] tensor")
+    if not k_pool.is_contiguous() or not v_pool.is_contiguous() or k_pool.shape[:3] != v_pool.shape[:3] \
+            or k_pool.dim() < 4 or k_pool.shape[1] != H:
+        raise ValueError("pools must be contiguous, with the same pages, n_kv_heads and page size")
+    pages, _, page_size = k_pool.shape[:3]
+    if k_pool.dtype == torch.int8:
+        kt = vt = Q8
+        if k_pool.shape != (pages, H, page_size, D) or v_pool.shape != k_pool.shape or v_pool.dtype != torch.int8:
+            raise ValueError("8-bit pools must be int8 [num_pages, n_kv_heads, page_size, head_dim], both")
+        for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if s is None:
+                raise ValueError(f"8-bit pools need {name}")
+            _need_cuda(s)
+            if s.dtype != torch.float32 or s.shape != (pages, H, page_size // Q8_BLOCK) or not s.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous float32 [num_pages, n_kv_heads, page_size / 16] tensor")
+    else:
+        kt = {n: t for t, n in BLOCK_BYTES.items()}.get(k_pool.shape[-1])
+        vt = TQ4_0
+        if k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 or kt is None \
+                or k_pool.shape != (pages, H, page_size, D // QK, BLOCK_BYTES[kt]) \
+                or v_pool.shape != (pages, H, page_size, D // QK, BLOCK_BYTES[TQ4_0]):
+            raise ValueError("pools must be uint8 [num_pages, n_kv_heads, page_size, head_dim/32, bytes] blocks, "
+                             "TQ4_0 for the values")
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("TQ pools have no scales")
+    for t, name in ((pos, "pos"), (new_len, "new_len")):
+        if t is not None:
+            _need_cuda(t)
+            if t.dtype != torch.int32 or t.numel() != B or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 [batch] tensor")
+    if overflow is not None:
+        _need_cuda(overflow)
+        if overflow.dtype != torch.int32:
+            raise ValueError("overflow must be an int32 tensor")
+    if positions is not None and rope is None:
+        raise ValueError("positions without a rotation")
+    if q is not None:
+        _need_cuda(q)
+        _check_rows(q, "q")
+        if q.dtype != k.dtype or q.shape[0] != B or q.shape[2] != n_new or q.shape[3] != D or q.shape[1] == 0:
+            raise ValueError("q must have k's type, batch, tokens and head_dim")
+        if rope is None:
+            raise ValueError("q without a rotation")
+        q_out = _rotary_out(q, q_out, "q_out")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _same_device(k, v, k_pool, v_pool, page_table, pos, new_len, k_scale, v_scale, q, q_out, overflow)
+    from .attention import make_pages
+    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+    a = _RotaryAppendArgs(B, H, D, n_new, _DTYPES[k.dtype], _rows(k), _rows(v),
+                          _HeadRows() if q is None else _rows(q, q_out),
+                          _Rope() if rope is None else _rope(rope, k, positions, False), ptr(k_pool), kt, ptr(k_scale),
+                          ptr(v_pool), vt, ptr(v_scale), ptr(pos), ptr(new_len), int(rotate), ptr(overflow))
+    with _on_device(k):
+        L.check(L.load().tq_kv_append_rotary_paged_cuda(C.byref(a), C.byref(make_pages(page_table, pages, page_size)),
+                                                        _stream(k)))
+    return q_out
+
+
+def dequantize_q8(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Values of 8-bit pages: int8 [..., tokens, head_dim] (tokens a multiple of 16, head_dim 128 or 256)
+    times float32 [..., tokens / 16], rounded to dtype."""
+    _need_cuda(codes, scale)
+    if codes.dtype != torch.int8 or not codes.is_contiguous() or codes.dim() < 2 or codes.shape[-2] % Q8_BLOCK:
+        raise ValueError("codes must be a contiguous int8 [..., tokens, head_dim] tensor, tokens a multiple of 16")
+    if scale.dtype != torch.float32 or not scale.is_contiguous() \
+            or scale.shape != (*codes.shape[:-2], codes.shape[-2] // Q8_BLOCK):
+        raise ValueError("scale must be a contiguous float32 [..., tokens / 16] tensor")
+    if out is None:
+        out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    else:
+        _need_cuda(out)
+        if out.shape != codes.shape or out.dtype not in _DTYPES or not out.is_contiguous():
+            raise ValueError("out must be a contiguous f32/f16/bf16 tensor of the codes' shape")
+    if out.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {out.dtype}")
+    _same_device(codes, scale, out)
+    with _on_device(codes):
+        L.check(L.load().tq_dequantize_q8_cuda(codes.data_ptr(), scale.data_ptr(), out.data_ptr(), _DTYPES[out.dtype],
+                                               scale.numel(), codes.shape[-1], _stream(codes)))
+    return out
 
 
 TQ2_1_BYTES = 44   # block_tq2_1: a TQ3_0 block and three TQ2_0 blocks per 128 elements
