@@ -435,6 +435,41 @@ tq_status tq_kv_append_rotary_paged_cuda(const tq_rotary_append_args *a, const t
 tq_status tq_dequantize_q8_cuda(const int8_t *codes, const float *scale, void *y, tq_dtype y_dtype,
                                 int64_t n_blocks, int head_dim, void *stream);
 
+/*
+ * Attention over 8-bit pages (TQ_TYPE_Q8 pools as tq_kv_append_rotary_paged_cuda writes them), for one query
+ * token per sequence, a few drafted tokens, or a prompt.  Query token i of sequence b's q_len[b] (NULL: n_new)
+ * is the cached token kv_len[b] - q_len[b] + i and, when causal, sees the tokens up to itself; else all
+ * kv_len[b] tokens (kv_len counts this step's rows, appended before).
+ *   q' = H q when rotate_q, s_j = sm_scale * q' . (code_j * scale), p = softmax(s),
+ *   out = sum_j p_j (code_j * scale), followed by H when v_rotated.
+ * Rows that see no token (empty sequences, tokens before the cache's first, rows i >= q_len[b]) give zeros and
+ * a log-sum-exp of -inf.  q and out: [batch][n_q_heads][n_new][head_dim] at element strides (batch, head,
+ * token), rows on 16-byte boundaries.  Products are f16 with fp32 sums: q' is scaled by its row's maximum and
+ * rounded to f16, codes are exact, weights are rounded to f16, statistics are fp32.  q must be finite.
+ * head_dim 128 or 256, any n_q_heads / n_kv_heads, page_size a power of two in 16 .. 65536.  A page id
+ * outside the pool that holds tokens a row would see is treated as holding none, and TQ_ERROR_INVALID_VALUE is
+ * stored in *status.  Work memory: tq_attention_q8_workspace_size() bytes, written before they are read; calls
+ * that can overlap need their own.
+ */
+typedef struct {
+    int batch, n_q_heads, n_kv_heads, head_dim;
+    int64_t n_new;              /* query tokens per sequence */
+    const void *q;              tq_dtype q_dtype;     int64_t q_stride[3];
+    void *out;                  tq_dtype out_dtype;   int64_t out_stride[3];
+    const int8_t *k_codes;      const float *k_scale;
+    const int8_t *v_codes;      const float *v_scale;
+    const int32_t *kv_len;      /* device [batch] */
+    const int32_t *q_len;       /* device [batch], or NULL */
+    int64_t max_kv_len;         /* about the largest kv_len: sizes the work split, not the result; 0 = capacity */
+    float sm_scale;             /* 0 = 1/sqrt(head_dim) */
+    int causal, rotate_q, v_rotated;
+    float *lse;                 /* optional [batch][n_q_heads][n_new], natural log */
+    int32_t *status;            /* optional device word, raised to TQ_ERROR_INVALID_VALUE by a bad page id */
+    void *workspace;            size_t workspace_bytes;
+} tq_attention_q8_args;
+size_t tq_attention_q8_workspace_size(const tq_attention_q8_args *a, const tq_kv_pages *pages);
+tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args *a, const tq_kv_pages *pages, void *stream);
+
 /* log-sum-exp merge of n_parts partial results o[n_parts][n_rows][head_dim] with
  * natural-log lse[n_parts][n_rows] into out[n_rows][head_dim] (+ lse_out, optional):
  * the split-by-sequence combine of the multi-GPU path (new) */

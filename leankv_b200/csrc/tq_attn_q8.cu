@@ -1,0 +1,619 @@
+// tq_attn_q8.cu — attention over 8-bit pages for few query rows: decode steps and drafted tokens.
+//
+// For query row i of a sequence (i of q_len tokens) and the KV head of its group:
+//   q' = H q (rotate_q),  s_j = sm_scale * sum_d q'_d c_jd * ks[j / 16],  p = softmax over the tokens it sees,
+//   o = sum_j p_j c'_jd * vs[j / 16],  out = H o (v_rotated).
+//
+// Work.  A unit is 16 or 32 query rows (tokens x heads of one group) of one (sequence, KV head); its tokens are
+// split over CTAs, and within a CTA over 8 warps that never wait for one another: a warp takes every 8th block
+// of 16 tokens (one scale block of K and V, 2 KB each at D = 128), which it copies into its own ring of
+// shared memory (cp.async, 16 bytes a lane).  Products are mma.sync m16n8k16 in f16 with fp32 accumulators:
+// with 1 to 40 rows per KV head the cache is read at memory speed, a tcgen05 tile (128 rows) would be mostly
+// empty, and its operands would have to go through shared memory once more after the conversion from 8 bits.
+//
+// Numbers.  A row of q' is scaled by its largest element and rounded to f16.  Codes are integers of 8 bits and
+// exact in f16.  K codes enter the product as subnormals (c + 128) 2^-24: one byte permute for two values;
+// 128 times the row's sum of q' is taken off in fp32.  V codes are made from 1024 + (c + 128) minus 1152
+// (the offset left in would cost up to 5 bits of the sum).  The V scale goes into the exponent:
+// p_j = 2^(s_j + log2 vs - m + 6), so that one multiply-add per score applies both scales and every product is
+// of f16 numbers near their row's largest, whatever the scales of other blocks; the sum of weights l takes
+// p_j / vs in fp32.  m is the largest s + log2 vs seen up to a slack of 8: rows are rescaled only when a score
+// exceeds m by more than that (p stays below 2^14, and is exact to f16's 11 bits down to 2^-20 of the largest).
+#include <type_traits>
+#include <utility>
+
+#include "tq_attn_q8.h"
+#include "tq_kernels.h"
+#include "tq_rope.h"
+#include "tq_rows.cuh"
+
+namespace tq {
+
+constexpr int Q8_WARPS = 8, Q8_THREADS = 32 * Q8_WARPS;
+constexpr float Q8_SHIFT = 6.0f, Q8_SLACK = 8.0f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ void load16(const void* p, int64_t at, float (&v)[16]) {
+    float a[8], b[8];
+    load8<T>(static_cast<const T*>(p) + at, a);
+    load8<T>(static_cast<const T*>(p) + at + 8, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { v[j] = a[j]; v[8 + j] = b[j]; }
+}
+__device__ __forceinline__ void load_row16(int dtype, const void* p, int64_t at, float (&v)[16]) {
+    if (dtype == DT_F32) load16<float>(p, at, v);
+    else if (dtype == DT_F16) load16<__half>(p, at, v);
+    else load16<__nv_bfloat16>(p, at, v);
+}
+template <typename T>
+__device__ __forceinline__ void put16(void* p, int64_t at, const float (&v)[16]) {
+    float a[8], b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { a[j] = v[j]; b[j] = v[8 + j]; }
+    store8<T>(static_cast<T*>(p) + at, a);
+    store8<T>(static_cast<T*>(p) + at + 8, b);
+}
+__device__ __forceinline__ void store_row16(int dtype, void* p, int64_t at, const float (&v)[16]) {
+    if (dtype == DT_F32) put16<float>(p, at, v);
+    else if (dtype == DT_F16) put16<__half>(p, at, v);
+    else put16<__nv_bfloat16>(p, at, v);
+}
+
+struct SeqLens {
+    int len, q_len;   // cached tokens (this step's included), query tokens
+};
+__device__ __forceinline__ SeqLens seq_lens(const Q8Run& r, int b) {
+    const int64_t cap = r.max_pages << r.page_shift;
+    int64_t len = r.kv_len[b], ql = r.q_len ? r.q_len[b] : r.n;
+    len = len < 0 ? 0 : (len > cap ? cap : len);
+    ql = ql < 0 ? 0 : (ql > r.n ? r.n : ql);
+    return {(int)len, (int)ql};
+}
+// last token that query token i sees (-1: none)
+__device__ __forceinline__ int last_seen(const Q8Run& r, const SeqLens& s, int i) {
+    if (i >= s.q_len) return -1;
+    const int lim = r.causal ? s.len - s.q_len + i : s.len - 1;
+    return lim < 0 ? -1 : lim;
+}
+
+// the 16-token block of a (sequence, KV head): its index in the pool (codes at 16 D times it, scale at it), or
+// -1 for a page outside the pool
+__device__ __forceinline__ int block_at(const Q8Run& r, int b, int h, int block) {
+    const int per = r.page_shift - 4;   // log2 blocks per page
+    const int32_t pg = r.pages[(int64_t)b * r.max_pages + (block >> per)];
+    if (pg < 0 || pg >= r.num_pages) return -1;
+    return (int)((((int64_t)pg * r.Hkv + h) << per) + (block & ((1 << per) - 1)));
+}
+
+template <int D, int MT> struct Q8Cfg {
+    static constexpr int ROWS = 16 * MT, NK = D / 16;
+    static constexpr int STAGES = D == 256 ? 3 : (MT == 1 ? 3 : 5);
+    static constexpr int BLOCK = 16 * D;                       // bytes of one tensor's block
+    static constexpr int RING = STAGES * 2 * BLOCK;            // per warp
+    static constexpr bool QREG = D == 128 && MT == 1;          // q' fragments stay in registers
+    static constexpr int QBYTES = MT * NK * 512;
+    static constexpr int MERGE = Q8_WARPS * ROWS * D * 4;      // the warps' sums, over the rings
+    static constexpr int RINGS = Q8_WARPS * RING > MERGE ? Q8_WARPS * RING : MERGE;
+    static constexpr int SMEM = RINGS + QBYTES + (2 * Q8_WARPS * ROWS + 4 * ROWS) * 4;
+    static constexpr int CTAS = QREG ? 2 : 1;
+};
+
+// Four 8-bit codes of a word, biased by 128, as f16 subnormals (c + 128) 2^-24: elements 0, 1 and 2, 3.
+__device__ __forceinline__ void bytes_sub(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    const uint32_t u = w ^ 0x80808080u;
+    lo = __byte_perm(u, 0u, 0x4140);
+    hi = __byte_perm(u, 0u, 0x4342);
+}
+
+// One unit's share of tokens.  Partial results go to part / part_lse (splits > 1), else to out / lse.
+template <int D, int MT>
+__global__ void __launch_bounds__(Q8_THREADS, Q8Cfg<D, MT>::CTAS)
+attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ part, float* __restrict__ part_lse) {
+    using C = Q8Cfg<D, MT>;
+    constexpr int ROWS = C::ROWS, NK = C::NK, HALVES = D / 128, LPR = D / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* s_q = smem + C::RINGS;
+    float* s_m = reinterpret_cast<float*>(s_q + C::QBYTES);   // [warp][row]
+    float* s_l = s_m + Q8_WARPS * ROWS;
+    float* s_f = s_l + Q8_WARPS * ROWS;                       // row's factor of the scores (log2 domain)
+    float* s_s = s_f + ROWS;                                  // 128 * sum of the row's f16 q'
+    int* s_lim = reinterpret_cast<int*>(s_s + ROWS);          // last token seen
+    float* s_lse = reinterpret_cast<float*>(s_lim + ROWS);
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int split = blockIdx.x % splits, rt = (blockIdx.x / splits) % row_tiles;
+    const int pair = blockIdx.x / splits / row_tiles, h = pair % r.Hkv, b = pair / r.Hkv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const SeqLens sl = seq_lens(r, b);
+    const int total_rows = (int)r.n * r.grp, row0 = rt * ROWS;
+
+    // rows row0 .. of the unit: row i * grp + head of group.  The tokens that any of them sees: [0, kv_end)
+    int last_i = (row0 + ROWS - 1) / r.grp;
+    if (last_i >= sl.q_len) last_i = sl.q_len - 1;
+    const int first_i = row0 / r.grp;
+    const int kv_end = last_i < first_i ? 0 : last_seen(r, sl, last_i) + 1;
+    const int per = ((kv_end + splits - 1) / splits + 127) & ~127;
+    const int64_t begin64 = (int64_t)split * per;
+    const int begin = begin64 < kv_end ? (int)begin64 : kv_end;
+    const int end = kv_end - begin < per ? kv_end : begin + per;
+    const int64_t unit = (int64_t)pair * row_tiles + rt;
+    if (begin >= end && splits > 1) {
+        if (threadIdx.x < ROWS) part_lse[(unit * splits + split) * ROWS + threadIdx.x] = -INFINITY;
+        return;
+    }
+
+    // ── this warp's blocks; the first copies go out before q' is prepared ──
+    const int nblk_all = (end - begin + 15) >> 4, blk0 = begin >> 4;
+    const int mine = nblk_all > warp ? (nblk_all - warp + Q8_WARPS - 1) / Q8_WARPS : 0;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * C::RING;
+    int nx_blk = -1, cu_blk = -1;                             // windows of 32 blocks, one per lane
+    float nx_ks = 0.0f, nx_vs = 0.0f, cu_ks = 0.0f, cu_vs = 0.0f;
+    auto window = [&](int i) {                                // blocks i .. i + 31 of this warp
+        nx_blk = -1;
+        nx_ks = nx_vs = 0.0f;
+        if (i + lane < mine) {
+            nx_blk = block_at(r, b, h, blk0 + warp + (i + lane) * Q8_WARPS);
+            if (nx_blk >= 0) {
+                nx_ks = r.ks[nx_blk];
+                nx_vs = r.vs[nx_blk];
+            } else if (r.status) {
+                atomicMax(r.status, 1);
+            }
+        }
+    };
+    auto issue = [&](int i) {
+        if (i < mine) {
+            if ((i & 31) == 0) window(i);
+            const int blk = __shfl_sync(0xffffffffu, nx_blk, i & 31);
+            if (blk >= 0) {
+                const uint32_t dst = ring + (i % C::STAGES) * (2 * C::BLOCK);
+                const int8_t* kp = r.k + (int64_t)blk * C::BLOCK;
+                const int8_t* vp = r.v + (int64_t)blk * C::BLOCK;
+                // 16-byte chunk c of row (token) x of a 128-byte half lies at chunk c ^ (x & 7)
+#pragma unroll
+                for (int e = 0; e < C::BLOCK / 512; ++e) {
+                    const int id = lane + 32 * e, half = id >> 7, x = (id >> 3) & 15, c = id & 7;
+                    const uint32_t at = half * 2048 + x * 128 + ((c ^ (x & 7)) << 4);
+                    const int64_t from = (int64_t)x * D + half * 128 + c * 16;
+                    cp16(dst + at, kp + from);
+                    cp16(dst + C::BLOCK + at, vp + from);
+                }
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
+
+    // ── q': Hadamard, row maximum, f16, in the order of the mma's A fragments ──
+    // k-step j = 8 half + jj of lane t covers elements 128 half + 32 t + 4 jj .. + 3 (so that a lane's K bytes
+    // are one run of 32), words a0, a2 = elements 0..1, 2..3 of row g; a1, a3 of row g + 8
+    for (int base = warp * (32 / LPR); base < ROWS; base += Q8_WARPS * (32 / LPR)) {
+        const int row = base + lane / LPR, e0 = (lane % LPR) * 16;
+        const int gr = row0 + row, i = gr / r.grp;
+        float v[16];
+        const bool live = gr < total_rows && i < sl.q_len;
+        if (live) {
+            load_row16(r.q_dtype, r.q, b * r.qs[0] + (h * r.grp + gr % r.grp) * r.qs[1] + (int64_t)i * r.qs[2] + e0, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+        }
+        if (r.rotate_q) fwht16<D>(v, r.norm);
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+        for (int o = 1; o < LPR; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
+        float sum = 0.0f;
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const __half2 p = __floats2half2_rn(v[2 * j] * inv, v[2 * j + 1] * inv);
+            sum += __low2float(p) + __high2float(p);
+            w[j] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+#pragma unroll
+        for (int o = 1; o < LPR; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int mt = row >> 4, rr = row & 15, half = e0 >> 7, tt = (e0 & 127) >> 5, jj0 = (e0 & 31) >> 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t* f = reinterpret_cast<uint32_t*>(s_q + ((mt * NK + half * 8 + jj0 + j) * 32 + (rr & 7) * 4 + tt) * 16);
+            f[rr >> 3] = w[2 * j];
+            f[2 + (rr >> 3)] = w[2 * j + 1];
+        }
+        if (lane % LPR == 0) {
+            s_f[row] = top * r.sm_scale * LOG2E;
+            s_s[row] = 128.0f * sum;
+            s_lim[row] = live ? last_seen(r, sl, i) : -1;
+        }
+    }
+    __syncthreads();
+
+    uint32_t qf[C::QREG ? NK : 1][4];
+    const uint32_t sq = (uint32_t)__cvta_generic_to_shared(s_q) + lane * 16;
+    if constexpr (C::QREG) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+            const uint4 w = lds128(sq + j * 512);
+            qf[j][0] = w.x; qf[j][1] = w.y; qf[j][2] = w.z; qf[j][3] = w.w;
+        }
+    }
+    float f[MT][2], fs[MT][2], m[MT][2], l[MT][2];
+    int lim[MT][2], lim_min = 0x7fffffff;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int row = mt * 16 + 8 * k + g;
+            f[mt][k] = s_f[row];
+            fs[mt][k] = s_f[row] * s_s[row];
+            lim[mt][k] = s_lim[row];
+            lim_min = lim[mt][k] < lim_min ? lim[mt][k] : lim_min;
+            m[mt][k] = -INFINITY;
+            l[mt][k] = 0.0f;
+        }
+    lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+    float o[MT][2 * NK][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 2 * NK; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
+
+    // ── blocks of 16 tokens ──
+    for (int i = 0; i < mine; ++i) {
+        cp_wait<C::STAGES - 2>();
+        __syncwarp();
+        if ((i & 31) == 0) { cu_blk = nx_blk; cu_ks = nx_ks; cu_vs = nx_vs; }
+        issue(i + C::STAGES - 1);   // into the stage that was read in the last turn
+        if (__shfl_sync(0xffffffffu, cu_blk, i & 31) < 0) continue;   // a page outside the pool holds nothing
+        const float ks = __shfl_sync(0xffffffffu, cu_ks, i & 31), vs = __shfl_sync(0xffffffffu, cu_vs, i & 31);
+        const uint32_t kt = ring + (i % C::STAGES) * (2 * C::BLOCK), vt = kt + C::BLOCK;
+
+        // scores: columns are tokens, n-tile 0 tokens 0..7, n-tile 1 tokens 8..15 (lane row g)
+        float s[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.0f;
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) {
+            uint32_t kw[2][8];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                const uint32_t row = kt + half * 2048 + (nt * 8 + g) * 128;
+                const uint4 x = lds128(row + (((2 * t) ^ g) << 4)), y = lds128(row + (((2 * t + 1) ^ g) << 4));
+                kw[nt][0] = x.x; kw[nt][1] = x.y; kw[nt][2] = x.z; kw[nt][3] = x.w;
+                kw[nt][4] = y.x; kw[nt][5] = y.y; kw[nt][6] = y.z; kw[nt][7] = y.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t b0[2], b1[2];
+                bytes_sub(kw[0][j], b0[0], b1[0]);
+                bytes_sub(kw[1][j], b0[1], b1[1]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    uint32_t a[4];
+                    if constexpr (C::QREG) {
+                        a[0] = qf[j][0]; a[1] = qf[j][1]; a[2] = qf[j][2]; a[3] = qf[j][3];
+                    } else {
+                        const uint4 w = lds128(sq + (mt * NK + half * 8 + j) * 512);
+                        a[0] = w.x; a[1] = w.y; a[2] = w.z; a[3] = w.w;
+                    }
+                    mma16816(s[mt][0], a, b0[0], b1[0]);
+                    mma16816(s[mt][1], a, b0[1], b1[1]);
+                }
+            }
+        }
+
+        // y = s * f ks + log2 vs (a block of zero values takes the smallest scale: its weights still count)
+        const float vse = vs > 0.0f ? vs : 0x1p-100f, lv = lg2(vse), iv = __frcp_rn(vse);
+        const int tok0 = (blk0 + warp + i * Q8_WARPS) << 4;
+        const bool edge = tok0 + 15 > lim_min;
+        bool over = false;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float a = f[mt][k] * ks * 0x1p24f, c = lv - fs[mt][k] * ks;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float y = fmaf(s[mt][nt][2 * k + e], a, c);
+                        if (edge && tok0 + nt * 8 + 2 * t + e > lim[mt][k]) y = -INFINITY;
+                        s[mt][nt][2 * k + e] = y;
+                        over |= y > m[mt][k] + Q8_SLACK;
+                    }
+            }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float top = fmaxf(fmaxf(s[mt][0][2 * k], s[mt][0][2 * k + 1]), fmaxf(s[mt][1][2 * k], s[mt][1][2 * k + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const float now = fmaxf(m[mt][k], top);
+                    const float w = now == -INFINITY ? 1.0f : ex2(m[mt][k] - now);
+                    m[mt][k] = now;
+                    l[mt][k] *= w;
+#pragma unroll
+                    for (int j = 0; j < 2 * NK; ++j) {
+                        o[mt][j][2 * k] *= w;
+                        o[mt][j][2 * k + 1] *= w;
+                    }
+                }
+        }
+        uint32_t pf[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float ref = m[mt][k] == -INFINITY ? 0.0f : m[mt][k] - Q8_SHIFT;
+                const float p0 = ex2(s[mt][0][2 * k] - ref), p1 = ex2(s[mt][0][2 * k + 1] - ref);
+                const float p2 = ex2(s[mt][1][2 * k] - ref), p3 = ex2(s[mt][1][2 * k + 1] - ref);
+                l[mt][k] = fmaf((p0 + p1) + (p2 + p3), iv, l[mt][k]);
+                pf[mt][k] = pack_h2(p0, p1);
+                pf[mt][2 + k] = pack_h2(p2, p3);
+            }
+
+        // out += P V: lane g's elements 16 g + j of each half (n-tile j), tokens 2t, 2t + 1, 2t + 8, 2t + 9
+        const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) {
+            uint32_t vw[4][4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int row = 2 * t + (x & 1) + 8 * (x >> 1);
+                const uint4 w = lds128(vt + half * 2048 + row * 128 + ((g ^ (row & 7)) << 4));
+                vw[x][0] = w.x ^ 0x80808080u; vw[x][1] = w.y ^ 0x80808080u;
+                vw[x][2] = w.z ^ 0x80808080u; vw[x][3] = w.w ^ 0x80808080u;
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t pr[4];   // byte pairs (token 2t, 2t + 1): elements 0, 1 | 2, 3; then tokens + 8
+                pr[0] = __byte_perm(vw[0][w], vw[1][w], 0x5140);
+                pr[1] = __byte_perm(vw[0][w], vw[1][w], 0x7362);
+                pr[2] = __byte_perm(vw[2][w], vw[3][w], 0x5140);
+                pr[3] = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t sel = (e & 1) ? 0x4342 : 0x4140;
+                    uint32_t b0 = __byte_perm(pr[e >> 1], 0x64646464u, sel), b1 = __byte_perm(pr[2 + (e >> 1)], 0x64646464u, sel);
+                    const __half2 h0 = __hsub2(*reinterpret_cast<__half2*>(&b0), off), h1 = __hsub2(*reinterpret_cast<__half2*>(&b1), off);
+                    b0 = *reinterpret_cast<const uint32_t*>(&h0);
+                    b1 = *reinterpret_cast<const uint32_t*>(&h1);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][half * 16 + 4 * w + e], pf[mt], b0, b1);
+                }
+            }
+        }
+    }
+    cp_wait<0>();
+
+    // ── the 8 warps' sums ──
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float x = l[mt][k];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            if (t == 0) {
+                s_m[warp * ROWS + mt * 16 + 8 * k + g] = m[mt][k];
+                s_l[warp * ROWS + mt * 16 + 8 * k + g] = x;
+            }
+        }
+    __syncthreads();   // every warp is done with its ring
+    // chunk c (4 floats) of a row at (c & ~7) | ((c ^ (4 row + (c >> 3))) & 7): no bank conflicts
+    float* sums = reinterpret_cast<float*>(smem);
+    auto cell = [&](int w, int row, int c) {
+        return sums + ((w * ROWS + row) * (D / 4) + ((c & ~7) | ((c ^ (4 * row + (c >> 3))) & 7))) * 4;
+    };
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int half = 0; half < HALVES; ++half)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)   // column 2t + e of n-tile j is element 16 (2t + e) + j
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int j = half * 16 + 4 * c;
+                        *reinterpret_cast<float4*>(cell(warp, mt * 16 + 8 * k + g, half * 32 + 8 * t + 4 * e + c)) =
+                            make_float4(o[mt][j][2 * k + e], o[mt][j + 1][2 * k + e], o[mt][j + 2][2 * k + e], o[mt][j + 3][2 * k + e]);
+                    }
+    __syncthreads();
+    for (int id = threadIdx.x; id < ROWS * (D / 4); id += Q8_THREADS) {
+        const int row = id / (D / 4), c = id % (D / 4);
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < Q8_WARPS; ++w) top = fmaxf(top, s_m[w * ROWS + row]);
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+        if (top != -INFINITY) {
+#pragma unroll
+            for (int w = 0; w < Q8_WARPS; ++w) {
+                const float e = ex2(s_m[w * ROWS + row] - top);
+                const float4 x = *reinterpret_cast<const float4*>(cell(w, row, c));
+                sum = fmaf(s_l[w * ROWS + row], e, sum);
+                a.x = fmaf(x.x, e, a.x); a.y = fmaf(x.y, e, a.y); a.z = fmaf(x.z, e, a.z); a.w = fmaf(x.w, e, a.w);
+            }
+            const float inv = __fdiv_rn(1.0f, sum);
+            a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
+        }
+        const float lse = top == -INFINITY ? -INFINITY : (top - Q8_SHIFT + lg2(sum)) * LN2;
+        if (splits > 1) {
+            const int64_t at = (unit * splits + split) * ROWS + row;
+            reinterpret_cast<float4*>(part + at * D)[c] = a;
+            if (c == 0) part_lse[at] = lse;
+        } else {
+            // back to shared memory, in place of warp 0's sums (this thread has read them all)
+            *reinterpret_cast<float4*>(cell(0, row, c)) = a;
+            if (c == 0) s_lse[row] = lse;
+        }
+    }
+    if (splits > 1) return;
+    __syncthreads();
+    for (int base = warp * (32 / LPR); base < ROWS; base += Q8_WARPS * (32 / LPR)) {
+        const int row = base + lane / LPR, e0 = (lane % LPR) * 16, gr = row0 + row, i = gr / r.grp;
+        float v[16];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float4 x = *reinterpret_cast<const float4*>(cell(0, row, e0 / 4 + c));
+            v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = x.z; v[4 * c + 3] = x.w;
+        }
+        if (r.v_rotated) fwht16<D>(v, r.norm);
+        if (gr < total_rows) {
+            const int hq = h * r.grp + gr % r.grp;
+            store_row16(r.out_dtype, r.out, b * r.os[0] + hq * r.os[1] + (int64_t)i * r.os[2] + e0, v);
+            if (r.lse && e0 == 0) r.lse[((int64_t)b * r.Hq + hq) * r.n + i] = s_lse[row];
+        }
+    }
+}
+
+// Merge of the splits' normalized partial rows by their log-sum-exp, in split order, then the Hadamard
+// transform and the output type.  D / 16 lanes take a row.
+template <int D>
+__global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int rows, int row_tiles, int splits,
+                                                            const float* __restrict__ part,
+                                                            const float* __restrict__ part_lse) {
+    constexpr int LPR = D / 16, RPC = 128 / LPR;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int total_rows = (int)r.n * r.grp;
+    const int64_t all = (int64_t)r.B * r.Hkv * total_rows;
+    const int64_t id = (int64_t)blockIdx.x * RPC + threadIdx.x / LPR;
+    const int e0 = (threadIdx.x % LPR) * 16;
+    const int64_t pair = id < all ? id / total_rows : 0;
+    const int gr = id < all ? (int)(id - pair * total_rows) : 0;
+    const int64_t unit = pair * row_tiles + gr / rows;
+    const float* pl = part_lse + unit * splits * rows + gr % rows;
+    float top = -INFINITY;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, pl[(int64_t)s * rows]);
+    float v[16], sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+    if (top != -INFINITY) {
+        for (int s = 0; s < splits; ++s) {
+            const float ls = pl[(int64_t)s * rows];
+            if (ls == -INFINITY) continue;
+            const float w = ex2((ls - top) * LOG2E);
+            sum += w;
+            const float4* x = reinterpret_cast<const float4*>(part + ((unit * splits + s) * rows + gr % rows) * D + e0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float4 y = x[c];
+                v[4 * c] = fmaf(w, y.x, v[4 * c]); v[4 * c + 1] = fmaf(w, y.y, v[4 * c + 1]);
+                v[4 * c + 2] = fmaf(w, y.z, v[4 * c + 2]); v[4 * c + 3] = fmaf(w, y.w, v[4 * c + 3]);
+            }
+        }
+        const float inv = __fdiv_rn(1.0f, sum);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] *= inv;
+    }
+    if (r.v_rotated) fwht16<D>(v, r.norm);
+    if (id >= all) return;
+    const int h = (int)(pair % r.Hkv), b = (int)(pair / r.Hkv), i = gr / r.grp, hq = h * r.grp + gr % r.grp;
+    store_row16(r.out_dtype, r.out, b * r.os[0] + hq * r.os[1] + (int64_t)i * r.os[2] + e0, v);
+    if (r.lse && e0 == 0) r.lse[((int64_t)b * r.Hq + hq) * r.n + i] = top == -INFINITY ? -INFINITY : top + lg2(sum) * LN2;
+}
+
+// ── plan and launch ────────────────────────────────────────────────────────
+
+Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
+    Q8Plan p;
+    const int64_t rows = n * grp;
+    p.rows = D == 128 && rows > 16 ? 32 : 16;
+    p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
+    const int64_t units = (int64_t)B * Hkv * p.row_tiles;
+    const int64_t slots = (int64_t)sm_count() * (D == 128 && p.rows == 16 ? 2 : 1);
+    // Splits: a CTA's time is its tokens plus a start and a merge worth about 384 tokens; the grid runs in
+    // waves of `slots` CTAs.  Take the number with the least waves * (tokens + 384).
+    const int64_t len = max_len > 0 ? max_len : 1;
+    int64_t best = INT64_MAX;
+    for (int s = 1; s <= 256; ++s) {
+        const int64_t per = ((len + s - 1) / s + 127) / 128 * 128;
+        if (s > 1 && (int64_t)(s - 1) * per >= len) continue;   // the last split would be empty
+        const int64_t waves = (units * s + slots - 1) / slots, cost = waves * (per + 384);
+        if (cost < best) { best = cost; p.splits = s; }
+    }
+    return p;
+}
+
+size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p) {
+    if (p.splits <= 1) return 0;
+    return (size_t)B * Hkv * p.row_tiles * p.splits * p.rows * (D + 1) * 4;
+}
+
+template <int D, int MT>
+static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
+    using C = Q8Cfg<D, MT>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t grid = (int64_t)r.B * r.Hkv * p.row_tiles * p.splits;
+    if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
+    attn_q8_kernel<D, MT><<<(unsigned)grid, Q8_THREADS, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st) {
+    float* part = static_cast<float*>(workspace);
+    float* part_lse = part + (size_t)r.B * r.Hkv * p.row_tiles * p.splits * p.rows * r.D;
+    cudaError_t e;
+    if (r.D == 256) e = launch_rows<256, 1>(r, p, part, part_lse, st);
+    else if (p.rows == 32) e = launch_rows<128, 2>(r, p, part, part_lse, st);
+    else e = launch_rows<128, 1>(r, p, part, part_lse, st);
+    if (e != cudaSuccess || p.splits <= 1) return e;
+    const int64_t rows = (int64_t)r.B * r.Hq * r.n, rpc = 128 / (r.D / 16);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((rows + rpc - 1) / rpc));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (r.D == 256) return cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<256>, r, p.rows, p.row_tiles, p.splits, (const float*)part, (const float*)part_lse);
+    return cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<128>, r, p.rows, p.row_tiles, p.splits, (const float*)part, (const float*)part_lse);
+}
+
+}  // namespace tq

@@ -1,0 +1,47 @@
+// tq_attn_q8.h — internal interface of the attention kernels over 8-bit pages.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace tq {
+
+struct Q8Run {
+    int B = 0, Hq = 0, Hkv = 0, grp = 1, D = 0;
+    int64_t n = 0;                 // query tokens of each sequence (padded)
+    const void* q = nullptr;
+    int q_dtype = 0;
+    int64_t qs[3] = {0, 0, 0};     // element strides: batch, head, token
+    void* out = nullptr;
+    int out_dtype = 0;
+    int64_t os[3] = {0, 0, 0};
+    const int8_t* k = nullptr;     // [num_pages][Hkv][page][D]
+    const int8_t* v = nullptr;
+    const float* ks = nullptr;     // [num_pages][Hkv][page / 16]
+    const float* vs = nullptr;
+    const int32_t* pages = nullptr;
+    int64_t max_pages = 0, num_pages = 0;
+    int page_shift = 4;
+    const int32_t* kv_len = nullptr;
+    const int32_t* q_len = nullptr;   // null: n
+    float sm_scale = 0.0f;
+    int causal = 1, rotate_q = 1, v_rotated = 1;
+    float norm = 1.0f;             // 1 / sqrt(D) of the Hadamard transform
+    float* lse = nullptr;          // [B][Hq][n]
+    int32_t* status = nullptr;
+};
+
+// Work split: a unit is one (sequence, KV head, tile of rows); `splits` CTAs share its tokens.
+struct Q8Plan {
+    int rows = 16;                 // query rows per unit
+    int row_tiles = 1;             // units per (sequence, KV head)
+    int splits = 1;
+    bool prompt = false;           // the tcgen05 kernel
+};
+
+Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len);
+size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p);
+cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st);
+
+}  // namespace tq

@@ -2,6 +2,7 @@
 #include <cmath>
 
 #include "leankv_tq.h"
+#include "tq_attn_q8.h"
 #include "tq_capi_internal.h"
 #include "tq_common.cuh"
 #include "tq_rope.h"
@@ -151,4 +152,70 @@ extern "C" tq_status tq_dequantize_q8_cuda(const int8_t* codes, const float* sca
         return set_error(TQ_ERROR_MISALIGNED, "codes and y must be 16-byte aligned, scales 4-byte aligned");
     return cuda_status(launch_dequantize_q8(codes, scale, y, (int)y_dtype, n_blocks, head_dim, (cudaStream_t)stream),
                        "dequantize kernel launch");
+}
+
+// ── attention ────────────────────────────────────────────────────────────────
+
+static tq_status q8_check(const tq_attention_q8_args* a, const tq_kv_pages* pg, Q8Run* r, Q8Plan* p) {
+    if (!a) return set_error(TQ_ERROR_INVALID_VALUE, "null argument block");
+    if (a->batch < 0 || a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->n_new < 0)
+        return set_error(TQ_ERROR_INVALID_VALUE, "bad batch / head / token counts");
+    if (a->n_q_heads % a->n_kv_heads) return set_error(TQ_ERROR_INVALID_VALUE, "n_q_heads %% n_kv_heads != 0");
+    if (a->head_dim != 128 && a->head_dim != 256)
+        return set_error(TQ_ERROR_UNSUPPORTED, "head_dim %d (supported: 128, 256)", a->head_dim);
+    if (!dtype_ok(a->q_dtype) || !dtype_ok(a->out_dtype)) return set_error(TQ_ERROR_INVALID_VALUE, "bad dtype");
+    int shift = 0;
+    tq_status s = pages_check(pg, a->batch, &shift);
+    if (s) return s;
+    const int64_t cap = pg->max_pages_per_seq << shift, grp = a->n_q_heads / a->n_kv_heads;
+    if (pg->max_pages_per_seq > (int64_t(1) << 30) || cap > (int64_t(1) << 30) || a->n_new * grp > (int64_t(1) << 30))
+        return set_error(TQ_ERROR_UNSUPPORTED, "capacity and rows per head must be at most 2^30");
+    if (a->max_kv_len < 0 || a->max_kv_len > cap) return set_error(TQ_ERROR_INVALID_VALUE, "max_kv_len outside [0, capacity]");
+    if (!std::isfinite(a->sm_scale)) return set_error(TQ_ERROR_INVALID_VALUE, "sm_scale is not finite");
+    r->B = a->batch; r->Hq = a->n_q_heads; r->Hkv = a->n_kv_heads; r->grp = (int)grp; r->D = a->head_dim;
+    r->n = a->n_new;
+    r->q = a->q; r->q_dtype = (int)a->q_dtype;
+    r->out = a->out; r->out_dtype = (int)a->out_dtype;
+    for (int i = 0; i < 3; ++i) {
+        r->qs[i] = a->q_stride[i];
+        r->os[i] = a->out_stride[i];
+    }
+    r->k = a->k_codes; r->v = a->v_codes; r->ks = a->k_scale; r->vs = a->v_scale;
+    r->pages = pg->page_table; r->max_pages = pg->max_pages_per_seq; r->num_pages = pg->num_pages; r->page_shift = shift;
+    r->kv_len = a->kv_len; r->q_len = a->q_len;
+    r->sm_scale = a->sm_scale != 0.0f ? a->sm_scale : 1.0f / sqrtf((float)a->head_dim);
+    r->causal = a->causal != 0; r->rotate_q = a->rotate_q != 0; r->v_rotated = a->v_rotated != 0;
+    r->norm = fwht_norm(a->head_dim);
+    r->lse = a->lse; r->status = a->status;
+    *p = q8_plan(a->batch, a->n_kv_heads, (int)grp, a->head_dim, a->n_new, a->max_kv_len > 0 ? a->max_kv_len : cap);
+    return TQ_SUCCESS;
+}
+
+extern "C" size_t tq_attention_q8_workspace_size(const tq_attention_q8_args* a, const tq_kv_pages* pages) {
+    clear_error();
+    Q8Run r;
+    Q8Plan p;
+    if (q8_check(a, pages, &r, &p) != TQ_SUCCESS) return 0;
+    return q8_workspace_bytes(r.B, r.Hkv, r.D, p);
+}
+
+extern "C" tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args* a, const tq_kv_pages* pages, void* stream) {
+    clear_error();
+    Q8Run r;
+    Q8Plan p;
+    tq_status s = q8_check(a, pages, &r, &p);
+    if (s) return s;
+    if (r.B == 0 || r.n == 0) return TQ_SUCCESS;
+    if (!r.q || !r.out || !r.k || !r.v || !r.ks || !r.vs || !r.kv_len) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
+    uintptr_t m = (uintptr_t)r.q | (uintptr_t)r.out | (uintptr_t)r.k | (uintptr_t)r.v;
+    for (int i = 0; i < 3; ++i)
+        m |= (uintptr_t)(r.qs[i] * (int64_t)dtype_bytes(r.q_dtype)) | (uintptr_t)(r.os[i] * (int64_t)dtype_bytes(r.out_dtype));
+    if (m & 15) return set_error(TQ_ERROR_MISALIGNED, "codes and the rows of q and out must start on 16-byte boundaries");
+    if (((uintptr_t)r.ks | (uintptr_t)r.vs | (uintptr_t)r.kv_len | (uintptr_t)r.q_len | (uintptr_t)r.lse | (uintptr_t)r.status) & 3)
+        return set_error(TQ_ERROR_MISALIGNED, "scales, lengths, lse or status not 4-byte aligned");
+    const size_t need = q8_workspace_bytes(r.B, r.Hkv, r.D, p);
+    if (need && (!a->workspace || a->workspace_bytes < need))
+        return set_error(TQ_ERROR_INVALID_VALUE, "workspace of %zu bytes needed", need);
+    if (need && ((uintptr_t)a->workspace & 15)) return set_error(TQ_ERROR_MISALIGNED, "workspace must be 16-byte aligned");
+    return cuda_status(launch_attention_q8(r, p, a->workspace, (cudaStream_t)stream), "attention launch");
 }
