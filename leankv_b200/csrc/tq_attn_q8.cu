@@ -22,16 +22,12 @@
 #include <type_traits>
 #include <utility>
 
-#include "tq_attn_q8.h"
+#include "tq_attn_q8.cuh"
 #include "tq_kernels.h"
-#include "tq_rope.h"
-#include "tq_rows.cuh"
 
 namespace tq {
 
 constexpr int Q8_WARPS = 8, Q8_THREADS = 32 * Q8_WARPS;
-constexpr float Q8_SHIFT = 6.0f, Q8_SLACK = 8.0f;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -43,79 +39,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-template <typename T>
-__device__ __forceinline__ void load16(const void* p, int64_t at, float (&v)[16]) {
-    float a[8], b[8];
-    load8<T>(static_cast<const T*>(p) + at, a);
-    load8<T>(static_cast<const T*>(p) + at + 8, b);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { v[j] = a[j]; v[8 + j] = b[j]; }
-}
-__device__ __forceinline__ void load_row16(int dtype, const void* p, int64_t at, float (&v)[16]) {
-    if (dtype == DT_F32) load16<float>(p, at, v);
-    else if (dtype == DT_F16) load16<__half>(p, at, v);
-    else load16<__nv_bfloat16>(p, at, v);
-}
-template <typename T>
-__device__ __forceinline__ void put16(void* p, int64_t at, const float (&v)[16]) {
-    float a[8], b[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { a[j] = v[j]; b[j] = v[8 + j]; }
-    store8<T>(static_cast<T*>(p) + at, a);
-    store8<T>(static_cast<T*>(p) + at + 8, b);
-}
-__device__ __forceinline__ void store_row16(int dtype, void* p, int64_t at, const float (&v)[16]) {
-    if (dtype == DT_F32) put16<float>(p, at, v);
-    else if (dtype == DT_F16) put16<__half>(p, at, v);
-    else put16<__nv_bfloat16>(p, at, v);
-}
-
-struct SeqLens {
-    int len, q_len;   // cached tokens (this step's included), query tokens
-};
-__device__ __forceinline__ SeqLens seq_lens(const Q8Run& r, int b) {
-    const int64_t cap = r.max_pages << r.page_shift;
-    int64_t len = r.kv_len[b], ql = r.q_len ? r.q_len[b] : r.n;
-    len = len < 0 ? 0 : (len > cap ? cap : len);
-    ql = ql < 0 ? 0 : (ql > r.n ? r.n : ql);
-    return {(int)len, (int)ql};
-}
-// last token that query token i sees (-1: none)
-__device__ __forceinline__ int last_seen(const Q8Run& r, const SeqLens& s, int i) {
-    if (i >= s.q_len) return -1;
-    const int lim = r.causal ? s.len - s.q_len + i : s.len - 1;
-    return lim < 0 ? -1 : lim;
-}
-
-// the 16-token block of a (sequence, KV head): its index in the pool (codes at 16 D times it, scale at it), or
-// -1 for a page outside the pool
-__device__ __forceinline__ int block_at(const Q8Run& r, int b, int h, int block) {
-    const int per = r.page_shift - 4;   // log2 blocks per page
-    const int32_t pg = r.pages[(int64_t)b * r.max_pages + (block >> per)];
-    if (pg < 0 || pg >= r.num_pages) return -1;
-    return (int)((((int64_t)pg * r.Hkv + h) << per) + (block & ((1 << per) - 1)));
-}
-
 template <int D, int MT> struct Q8Cfg {
     static constexpr int ROWS = 16 * MT, NK = D / 16;
     static constexpr int STAGES = D == 256 ? 3 : (MT == 1 ? 3 : 5);
@@ -558,21 +486,24 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int r
 
 // ── plan and launch ────────────────────────────────────────────────────────
 
+constexpr int PROMPT_ROWS = 96;
+
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
     Q8Plan p;
     const int64_t rows = n * grp;
-    p.rows = D == 128 && rows > 16 ? 32 : 16;
+    p.prompt = rows >= PROMPT_ROWS;
+    p.rows = p.prompt ? (D == 128 ? 256 : 128) : (D == 128 && rows > 16 ? 32 : 16);
     p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = (int64_t)B * Hkv * p.row_tiles;
     const int64_t slots = (int64_t)sm_count() * (D == 128 && p.rows == 16 ? 2 : 1);
-    // Splits: a CTA's time is its tokens plus a start and a merge worth about 384 tokens; the grid runs in
-    // waves of `slots` CTAs.  Take the number with the least waves * (tokens + 384).
-    const int64_t len = max_len > 0 ? max_len : 1;
+    // Splits: a CTA's time is its tokens plus a start and a merge worth about `start` tokens; the grid runs in
+    // waves of `slots` CTAs.  Take the number with the least waves * (tokens + start).
+    const int64_t len = max_len > 0 ? max_len : 1, start = p.prompt ? 768 : 384;
     int64_t best = INT64_MAX;
     for (int s = 1; s <= 256; ++s) {
         const int64_t per = ((len + s - 1) / s + 127) / 128 * 128;
         if (s > 1 && (int64_t)(s - 1) * per >= len) continue;   // the last split would be empty
-        const int64_t waves = (units * s + slots - 1) / slots, cost = waves * (per + 384);
+        const int64_t waves = (units * s + slots - 1) / slots, cost = waves * (per + start);
         if (cost < best) { best = cost; p.splits = s; }
     }
     return p;
@@ -598,7 +529,8 @@ cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace
     float* part = static_cast<float*>(workspace);
     float* part_lse = part + (size_t)r.B * r.Hkv * p.row_tiles * p.splits * p.rows * r.D;
     cudaError_t e;
-    if (r.D == 256) e = launch_rows<256, 1>(r, p, part, part_lse, st);
+    if (p.prompt) e = launch_attention_q8_prompt(r, p, part, part_lse, st);
+    else if (r.D == 256) e = launch_rows<256, 1>(r, p, part, part_lse, st);
     else if (p.rows == 32) e = launch_rows<128, 2>(r, p, part, part_lse, st);
     else e = launch_rows<128, 1>(r, p, part, part_lse, st);
     if (e != cudaSuccess || p.splits <= 1) return e;

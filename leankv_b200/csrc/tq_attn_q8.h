@@ -42,6 +42,7 @@ struct Q8Plan {
 
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len);
 size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p);
+cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st);
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st);
 
 }  // namespace tq

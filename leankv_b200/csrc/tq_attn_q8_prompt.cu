@@ -1,0 +1,542 @@
+// tq_attn_q8_prompt.cu — attention over 8-bit pages for prompts, on tcgen05.
+//
+// The mathematics is tq_attn_q8.cu's; with 128 or more query rows per KV head the two products bound it.
+//
+// A CTA takes QT tiles of 128 query rows (tokens x heads of one group) of one (sequence, KV head).  Warps:
+//   4 QT softmax warps   one thread per row: scores from TMEM, weights back to TMEM, the output's rescaling
+//   1 issuing warp       one thread issues all tcgen05.mma
+//   4 converting warps   8-bit codes from the pages to f16 tiles in shared memory
+// Per tile of KT tokens: S = Q K^T (both from shared memory, f16, fp32 sums in TMEM), weights P in f16 written
+// over S, O += P V (P from TMEM, V from shared memory).  D = 128: two row tiles of 128 tokens take turns, so that
+// one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).  D = 256: O alone
+// takes 256 columns and Q 64 KB, so one row tile takes 64 tokens at a time with two buffers for S.
+//
+// Shared tiles are runs of 64 elements: [row][128 bytes], 16-byte chunk c of row x at c ^ (x & 7) (the 128-byte
+// swizzle of the matrix descriptors).  K is read with its elements contiguous, V as the transposed operand from
+// the same layout.  Codes are exact in f16; scales never touch the tiles: they enter with the scores.
+//
+// Every wait gives up after about a second (status TQ_ERROR_TIMEOUT) instead of hanging.
+#include "leankv_tq.h"
+#include "tq_attn_q8.cuh"
+#include "tq_kernels.h"
+
+namespace tq {
+
+// ── tcgen05, mbarriers ─────────────────────────────────────────────────────
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+constexpr uint64_t WAIT_NS = 1000000000ull;
+// waits for the phase of `parity`; false once any wait of the CTA has run out
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int* failed) {
+    const uint64_t until = now_ns() + WAIT_NS;
+    while (!mbar_try(bar, parity)) {
+        if (*failed) return false;
+        if (now_ns() > until) {
+            *failed = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+        if (mbar_try(bar, parity)) return true;
+    return mbar_wait_long(bar, parity, failed);
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 32 consecutive columns of this thread's TMEM lane
+__device__ __forceinline__ void tc_ld32(uint32_t a, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+                   "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+                   "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(a));
+}
+__device__ __forceinline__ void tc_st32(uint32_t a, const uint32_t (&v)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+                   "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+                   "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t a, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Matrix descriptor of a 128-byte-swizzled tile: start and strides in 16-byte units.  stride: 8 rows (1024
+// bytes); lead: from one run of 64 elements to the next (used by the transposed operand only).
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead_bytes) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(lead_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// f16 operands, fp32 sums, M = 128; tb: B is stored with its N dimension contiguous
+constexpr uint32_t mma_idesc(int n, int tb) { return (1u << 4) | ((uint32_t)tb << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
+
+template <int D> struct PromptCfg {
+    static constexpr int QT = D == 128 ? 2 : 1, KT = D == 128 ? 128 : 64, ROWS = 128 * QT;
+    static constexpr int SEGS = D / 64;                    // 64-element runs of a row
+    static constexpr int Q_TILE = 128 * D * 2, KV_TILE = KT * D * 2, SEG = KT * 128;
+    static constexpr int SBUF = 2;                         // S buffers: one per row tile, or two of one
+    static constexpr int SOFT_WARPS = 4 * QT, WARPS = SOFT_WARPS + 5;
+    static constexpr int TILES = QT * Q_TILE + 4 * KV_TILE;   // Q, two K and two V buffers
+    static constexpr int SMEM = TILES + 1024;              // the tiles start on 1024 bytes
+};
+
+template <int D>
+__global__ void __launch_bounds__(PromptCfg<D>::WARPS * 32, 1)
+attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ part, float* __restrict__ part_lse) {
+    using C = PromptCfg<D>;
+    constexpr int QT = C::QT, KT = C::KT, ROWS = C::ROWS, LPR = D / 16, THREADS = C::WARPS * 32;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[16];
+    __shared__ float s_f[ROWS], s_lse[ROWS];
+    __shared__ int s_lim[ROWS];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed;
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t tile0 = smem_u32(tiles);
+    const uint32_t q_at = tile0, k_at = tile0 + QT * C::Q_TILE, v_at = k_at + 2 * C::KV_TILE;
+    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t k_full = bar0, k_empty = bar0 + 16, v_full = bar0 + 32, v_empty = bar0 + 48;   // two each
+    const uint32_t s_full = bar0 + 64, p_full = bar0 + 80, o_done = bar0 + 96, done = bar0 + 104;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // units with the most tokens first: the last row tiles of a causal prompt see the longest prefix
+    const int split = blockIdx.x % splits;
+    const int64_t u = blockIdx.x / splits;
+    const int pairs = r.B * r.Hkv;
+    const int rt = row_tiles - 1 - (int)(u / pairs), pair = (int)(u % pairs), h = pair % r.Hkv, b = pair / r.Hkv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const SeqLens sl = seq_lens(r, b);
+    const int total_rows = (int)r.n * r.grp, row0 = rt * ROWS;
+    int last_i = (row0 + ROWS - 1) / r.grp;
+    if (last_i >= sl.q_len) last_i = sl.q_len - 1;
+    const int first_i = row0 / r.grp;
+    const int kv_end = last_i < first_i ? 0 : last_seen(r, sl, last_i) + 1;
+    const int all_tiles = (kv_end + KT - 1) / KT, per = (all_tiles + splits - 1) / splits;
+    const int t_begin = split * per < all_tiles ? split * per : all_tiles;
+    const int tiles_n = all_tiles - t_begin < per ? all_tiles - t_begin : per;
+    const int64_t unit = (int64_t)pair * row_tiles + rt;
+    if (tiles_n <= 0 && splits > 1) {
+        for (int i = threadIdx.x; i < ROWS; i += THREADS) part_lse[(unit * splits + split) * ROWS + i] = -INFINITY;
+        return;
+    }
+
+    if (threadIdx.x == 0) {
+        s_failed = 0;
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(k_full + 8 * i, 4);     // the converting warps
+            mbar_init(v_full + 8 * i, 4);
+            mbar_init(k_empty + 8 * i, 1);    // commits of the issuing thread
+            mbar_init(v_empty + 8 * i, 1);
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 128);   // the rows' threads
+        }
+        mbar_init(o_done, 1);
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == C::SOFT_WARPS) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+
+    // ── q': Hadamard, row maximum, f16, swizzled tiles ──
+    for (int base = warp * (32 / LPR); base < ROWS; base += C::WARPS * (32 / LPR)) {
+        const int row = base + lane / LPR, e0 = (lane % LPR) * 16, gr = row0 + row, i = gr / r.grp;
+        const bool live = gr < total_rows && i < sl.q_len;
+        float v[16];
+        if (live) {
+            load_row16(r.q_dtype, r.q, b * r.qs[0] + (h * r.grp + gr % r.grp) * r.qs[1] + (int64_t)i * r.qs[2] + e0, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+        }
+        if (r.rotate_q) fwht16<D>(v, r.norm);
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+        for (int o = 1; o < LPR; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = pack_h2(v[2 * j] * inv, v[2 * j + 1] * inv);
+        const int qt = row >> 7, rr = row & 127, c = (e0 & 63) >> 3;
+        uint8_t* at = tiles + qt * C::Q_TILE + (e0 >> 6) * (128 * 128) + rr * 128;
+        *reinterpret_cast<uint4*>(at + ((c ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(at + (((c + 1) ^ (rr & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+        if (lane % LPR == 0) {
+            s_f[row] = top * r.sm_scale * LOG2E;
+            s_lim[row] = live ? last_seen(r, sl, i) : -1;
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const uint32_t o_col = 256;   // S buffers at columns 0 and 128 (0 and 64), O from 256 on
+
+    if (warp < C::SOFT_WARPS) {
+        // ── softmax: thread = row ──
+        const int qt = warp >> 2, row = qt * 128 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t o_at = lanes + o_col + qt * 128;
+        const float f = s_f[row];
+        const int lim = s_lim[row];
+        float m = -INFINITY, l = 0.0f;
+        // scales of the tile's blocks, one per lane (lane & 7), a tile ahead
+        constexpr int BPT = KT / 16;
+        float ks = 0.0f, vs = 0.0f;
+        int blk = -1;
+        auto scales = [&](int t) {
+            const int block = (t_begin + t) * BPT + (lane & (BPT - 1));
+            blk = -1;
+            ks = vs = 0.0f;
+            if (t < tiles_n && block * 16 < kv_end) {
+                blk = block_at(r, b, h, block);
+                if (blk >= 0) { ks = r.ks[blk]; vs = r.vs[blk]; }
+                else if (r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
+            }
+        };
+        scales(0);
+        for (int t = 0; t < tiles_n; ++t) {
+            const int sb = QT == 2 ? qt : (t & 1);
+            const uint32_t s_at = lanes + sb * KT;
+            const float ks_l = ks, vse = vs > 0.0f ? vs : 0x1p-100f;
+            const float lv_l = lg2(vse), iv_l = __frcp_rn(vse);
+            const uint32_t there = __ballot_sync(0xffffffffu, blk >= 0) & ((1u << BPT) - 1);
+            scales(t + 1);
+            const int tok0 = (t_begin + t) * KT;
+            const bool edge = __any_sync(0xffffffffu, tok0 + KT - 1 > lim) || there != (1u << BPT) - 1;
+            const uint32_t par = QT == 2 ? (t & 1) : ((t >> 1) & 1);
+            if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * sb, par, &s_failed))) break;
+            tc_fence_after();
+
+            auto scores = [&](int c, float (&y)[32]) {   // 32 columns: two scale blocks
+                uint32_t raw[32];
+                tc_ld32(s_at + 32 * c, raw);
+                tc_wait_ld();
+#pragma unroll
+                for (int bl = 0; bl < 2; ++bl) {
+                    const float a = f * __shfl_sync(0xffffffffu, ks_l, 2 * c + bl);
+                    const float lv = __shfl_sync(0xffffffffu, lv_l, 2 * c + bl);
+                    const float2 a2 = make_float2(a, a), c2 = make_float2(lv, lv);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[16 * bl + j]), __uint_as_float(raw[16 * bl + j + 1])), a2, c2);
+                        y[16 * bl + j] = x.x;
+                        y[16 * bl + j + 1] = x.y;
+                    }
+                    if (edge) {
+                        const bool gone = !((there >> (2 * c + bl)) & 1);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (gone || tok0 + 32 * c + 16 * bl + j > lim) y[16 * bl + j] = -INFINITY;
+                    }
+                }
+            };
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c) {
+                float y[32];
+                scores(c, y);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) top = fmaxf(top, y[j]);
+            }
+            const bool move = top > m + Q8_SLACK;
+            if (__any_sync(0xffffffffu, move)) {
+                const float now = move ? top : m;
+                const float w = move ? ex2(m - now) : 1.0f;
+                m = now;
+                l *= w;
+                if (t > 0) {
+                    // the products up to the last tile's are done: with two row tiles this tile's scores were
+                    // issued after them, else their own commit says so
+                    if (QT == 1) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(o_done, (t - 1) & 1, &s_failed))) break;
+                        tc_fence_after();
+                    }
+                    // rare after the first tiles: not unrolled
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t x[32];
+                        tc_ld32(o_at + 32 * c, x);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * w);
+                        tc_st32(o_at + 32 * c, x);
+                    }
+                }
+            }
+            const float ref = m == -INFINITY ? 0.0f : Q8_SHIFT - m;
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c) {
+                float y[32];
+                scores(c, y);
+                uint32_t p[16];
+#pragma unroll
+                for (int bl = 0; bl < 2; ++bl) {
+                    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const float2 e = __fadd2_rn(make_float2(y[16 * bl + j], y[16 * bl + j + 1]), make_float2(ref, ref));
+                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
+                        sum = __fadd2_rn(sum, w);
+                        p[8 * bl + j / 2] = pack_h2(w.x, w.y);
+                    }
+                    l = fmaf(sum.x + sum.y, __shfl_sync(0xffffffffu, iv_l, 2 * c + bl), l);
+                }
+                // 32 weights take 16 columns, all left of the columns still to be read
+                tc_st16(s_at + 16 * c, p);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(p_full + 8 * sb);
+        }
+        s_lse[row] = l > 0.0f ? (m - Q8_SHIFT + lg2(l)) * LN2 : -INFINITY;
+        s_f[row] = l > 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
+    } else if (warp == C::SOFT_WARPS) {
+        // ── issue ──
+        if (lane == 0 && tiles_n > 0) {
+            constexpr uint32_t id_s = mma_idesc(KT, 0), id_o = mma_idesc(D, 1);
+            bool ok = true;
+            auto scores = [&](int qt, int t) {
+                const uint32_t q = q_at + qt * C::Q_TILE, k = k_at + (t & 1) * C::KV_TILE;
+                const uint32_t d = tmem + (QT == 2 ? qt : (t & 1)) * KT;
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j)
+                    tc_mma_ss(d, tile_desc(q + (j >> 2) * (128 * 128) + (j & 3) * 32, 16), tile_desc(k + (j >> 2) * C::SEG + (j & 3) * 32, 16),
+                              id_s, j > 0);
+                tc_commit(s_full + 8 * (QT == 2 ? qt : (t & 1)));
+            };
+            auto values = [&](int qt, int t) {
+                const uint32_t p = tmem + (QT == 2 ? qt : (t & 1)) * KT, v = v_at + (t & 1) * C::KV_TILE;
+#pragma unroll
+                for (int j = 0; j < KT / 16; ++j)
+                    tc_mma_ts(tmem + o_col + qt * 128, p + 8 * j, tile_desc(v + j * 2048, C::SEG), id_o, t > 0 || j > 0);
+            };
+            auto full = [&](uint32_t bar, int t) {
+                ok = ok && mbar_wait(bar + 8 * (t & 1), (t >> 1) & 1, &s_failed);
+                tc_fence_after();
+                return ok;
+            };
+            if constexpr (QT == 2) {
+                if (full(k_full, 0)) {
+                    scores(0, 0);
+                    scores(1, 0);
+                    tc_commit(k_empty);
+                }
+                for (int t = 0; ok && t < tiles_n; ++t) {
+                    if (!full(v_full, t)) break;
+                    for (int qt = 0; qt < 2; ++qt) {
+                        ok = ok && mbar_wait(p_full + 8 * qt, t & 1, &s_failed);
+                        if (!ok) break;
+                        tc_fence_after();
+                        values(qt, t);
+                        if (qt == 1) tc_commit(v_empty + 8 * (t & 1));
+                        if (t + 1 < tiles_n) {
+                            if (qt == 0 && !full(k_full, t + 1)) break;
+                            scores(qt, t + 1);
+                            if (qt == 1) tc_commit(k_empty + 8 * ((t + 1) & 1));
+                        }
+                    }
+                }
+            } else {
+                for (int t = 0; t < 2 && t < tiles_n; ++t)
+                    if (full(k_full, t)) {
+                        scores(0, t);
+                        tc_commit(k_empty + 8 * t);
+                    }
+                for (int t = 0; ok && t < tiles_n; ++t) {
+                    if (!full(v_full, t) || !full(p_full, t)) break;
+                    values(0, t);
+                    tc_commit(v_empty + 8 * (t & 1));
+                    tc_commit(o_done);
+                    if (t + 2 < tiles_n) {
+                        if (!full(k_full, t + 2)) break;
+                        scores(0, t + 2);
+                        tc_commit(k_empty + 8 * (t & 1));
+                    }
+                }
+            }
+            tc_commit(done);
+        }
+        __syncwarp();
+    } else {
+        // ── conversion: 8 chunks of 16 codes per thread and tile, two stores of 8 f16 each ──
+        const int cw = warp - C::SOFT_WARPS - 1, sub = lane >> 2, c4 = lane & 3;
+        constexpr int WROWS = KT / 4, GROUPS = WROWS / 8;   // rows per warp, 8-row groups among them
+        auto load = [&](const int8_t* pool, int t, uint4 (&w)[8]) {
+#pragma unroll
+            for (int gi = 0; gi < GROUPS; ++gi) {
+                const int tok = (t_begin + t) * KT + cw * WROWS + 8 * gi;   // group's first token (warp-uniform)
+                const int blk = tok < kv_end ? block_at(r, b, h, tok >> 4) : -1;
+                const int8_t* p = pool + ((int64_t)blk * 16 + (tok & 15) + sub) * D + 16 * c4;
+#pragma unroll
+                for (int s = 0; s < C::SEGS; ++s)
+                    w[gi * C::SEGS + s] = blk >= 0 ? __ldg(reinterpret_cast<const uint4*>(p + 64 * s)) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto store = [&](uint32_t tile, const uint4 (&w)[8]) {
+            const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
+#pragma unroll
+            for (int gi = 0; gi < GROUPS; ++gi) {
+                const int row = cw * WROWS + 8 * gi + sub;   // row & 7 == sub
+#pragma unroll
+                for (int s = 0; s < C::SEGS; ++s) {
+                    const uint4 x = w[gi * C::SEGS + s];
+                    const uint32_t in[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+                    uint32_t o[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t v = __byte_perm(in[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140);
+                        const __half2 hv = __hsub2(*reinterpret_cast<__half2*>(&v), off);
+                        o[j] = *reinterpret_cast<const uint32_t*>(&hv);
+                    }
+                    const uint32_t at = tile + s * C::SEG + row * 128;
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((2 * c4) ^ sub) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((2 * c4 + 1) ^ sub) << 4)), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        uint4 kw[8], vw[8];
+        if (tiles_n > 0) load(r.k, 0, kw);
+        for (int t = 0; t < tiles_n; ++t) {
+            load(r.v, t, vw);
+            const uint32_t par = ((t >> 1) & 1) ^ 1;   // the first pass over the two buffers does not wait
+            if (t >= 2 && !__all_sync(0xffffffffu, mbar_wait(k_empty + 8 * (t & 1), par, &s_failed))) break;
+            store(k_at + (t & 1) * C::KV_TILE, kw);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full + 8 * (t & 1));
+            if (t + 1 < tiles_n) load(r.k, t + 1, kw);
+            if (t >= 2 && !__all_sync(0xffffffffu, mbar_wait(v_empty + 8 * (t & 1), par, &s_failed))) break;
+            store(v_at + (t & 1) * C::KV_TILE, vw);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_full + 8 * (t & 1));
+        }
+    }
+
+    // ── the output rows: O / l through shared memory (the tiles are free once all products are done) ──
+    bool fine = true;
+    if (tiles_n > 0) fine = mbar_wait(done, 0, &s_failed);
+    tc_fence_after();
+    __syncthreads();
+    fine = fine && s_failed == 0;
+    float* rows = reinterpret_cast<float*>(tiles);
+    // chunk c (4 floats) of a row at c ^ (row & 7)
+    if (warp < C::SOFT_WARPS) {
+        const int qt = warp >> 2, row = qt * 128 + (warp & 3) * 32 + lane;
+        const uint32_t o_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + o_col + qt * 128;
+        const float inv = s_f[row];
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t x[32];
+            if (tiles_n > 0 && fine) {
+                tc_ld32(o_at + 32 * c, x);
+                tc_wait_ld();
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float4 y = make_float4(__uint_as_float(x[4 * j]) * inv, __uint_as_float(x[4 * j + 1]) * inv,
+                                       __uint_as_float(x[4 * j + 2]) * inv, __uint_as_float(x[4 * j + 3]) * inv);
+                if (inv == 0.0f) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                reinterpret_cast<float4*>(rows + row * D)[(8 * c + j) ^ (row & 7)] = y;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == C::SOFT_WARPS) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+    if (!fine && threadIdx.x == 0 && r.status) atomicMax(r.status, (int)TQ_ERROR_TIMEOUT);
+    for (int base = warp * (32 / LPR); base < ROWS; base += C::WARPS * (32 / LPR)) {
+        const int row = base + lane / LPR, e0 = (lane % LPR) * 16, gr = row0 + row, i = gr / r.grp;
+        float v[16];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float4 x = reinterpret_cast<const float4*>(rows + row * D)[(e0 / 4 + c) ^ (row & 7)];
+            v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = x.z; v[4 * c + 3] = x.w;
+        }
+        if (splits > 1) {
+            const int64_t at = (unit * splits + split) * ROWS + row;
+            put16<float>(part, at * D + e0, v);
+            if (e0 == 0) part_lse[at] = s_lse[row];
+            continue;
+        }
+        if (r.v_rotated) fwht16<D>(v, r.norm);
+        if (gr < total_rows) {
+            const int hq = h * r.grp + gr % r.grp;
+            store_row16(r.out_dtype, r.out, b * r.os[0] + hq * r.os[1] + (int64_t)i * r.os[2] + e0, v);
+            if (r.lse && e0 == 0) r.lse[((int64_t)b * r.Hq + hq) * r.n + i] = s_lse[row];
+        }
+    }
+}
+
+template <int D>
+static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
+    using C = PromptCfg<D>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t grid = (int64_t)r.B * r.Hkv * p.row_tiles * p.splits;
+    if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
+    attn_q8_prompt_kernel<D><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
+    return r.D == 256 ? launch_prompt_d<256>(r, p, part, part_lse, st) : launch_prompt_d<128>(r, p, part, part_lse, st);
+}
+
+}  // namespace tq

@@ -5,6 +5,10 @@ at the worst, 2^-11 of each element's value while normal), weights to f16 (2^-11
 is off by at most ds = sm_scale * sum_d 2^-12 * max|q'| * |k_d|, a weight by the factor e^(2 ds), so an output
 element by at most (2 ds + 2^-11) * sum_j p_j |v_j| (both computed here in float64 from the test's own
 inputs), with 2^-14 of sum_j p_j |v_j| for the fp32 sums of up to 2^13 terms, and half a step of the output type.
+A weight below f16's normal numbers is off by half its smallest step, 2^-25, of weights held as
+2^6 p_j vs_j / 2^m with 2^m at most the row's largest p_j vs_j: by 2^-31 max_j(p_j vs_j) / vs_j, which is
+2^-31 max_j(p_j vs_j) sum_j |code_j| of an output element (an element whose code is 0 for the one token that a
+row attends to is the sum of such weights alone).
 The log-sum-exp is off by at most ds + 2^-14.
 """
 import math
@@ -70,6 +74,9 @@ def _reference(q, kp, vp, ks, vs, table, kv_len, q_len, causal, rotate_q, v_rota
         p = torch.softmax(s, -1).nan_to_num(0.0)
         o, size = p @ v[:, None], p @ v.abs()[:, None]
         t = (torch.expm1(2 * e) + 2.0 ** -11 + 2.0 ** -14) * size
+        step = vs[pg].double().repeat_interleave(16, -1).transpose(0, 1).flatten(1, 2)[:, :L]
+        codes = vp[pg].double().transpose(0, 1).flatten(1, 2)[:, :L].abs().sum(1)
+        t = t + 2.0 ** -31 * (p * step[:, None, None]).amax(-1, keepdim=True) * codes[:, None, None]
         if v_rotated:
             o, t = o @ had, t @ had.abs()   # each element of the sum may be off by its own tolerance
         out[b, :, :ql], tol[b, :, :ql] = o.flatten(0, 1), t.flatten(0, 1)
@@ -119,6 +126,25 @@ def test_matches_formula(D, grp, n, P, dtype):
     if n > 1:
         ql = torch.tensor([n, 1, 3, 0, n - 1], dtype=torch.int32, device=DEV)
         _check(_q(B, H * grp, n, D, dtype, n), kp, vp, ks, vs, table, lens, q_len=ql)
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("grp,n,top", [(4, 32, 300), (1, 128, 128), (8, 70, 1000), (3, 111, 140), (1, 300, 700), (2, 257, 257), (16, 40, 513)])
+@pytest.mark.parametrize("P,dtype", [(16, torch.bfloat16), (64, torch.float16)])
+def test_prompts_match_formula(D, grp, n, top, P, dtype):
+    """Prompts: row tiles with ragged ends, lengths that end inside tiles, prefixes, sequences shorter than
+    their queries, empty ones, padded batches."""
+    B, H = 4, 2
+    per = -(-top // P)
+    kp, ks = _pools(B * per + 3, H, P, D, 1)
+    vp, vs = _pools(B * per + 3, H, P, D, 2)
+    table = _table(B, per, B * per + 3, 3)
+    lens = torch.tensor([top, n, 0, n // 2 + 1], dtype=torch.int32, device=DEV)
+    q = _q(B, H * grp, n, D, dtype, n)
+    _check(q, kp, vp, ks, vs, table, lens)
+    ql = torch.tensor([n, n // 3, 3, n // 2 + 1], dtype=torch.int32, device=DEV)
+    _check(q, kp, vp, ks, vs, table, lens, q_len=ql)
+    _check(q, kp, vp, ks, vs, table, lens, causal=False, rotate_q=False, v_rotated=False)
 
 
 @pytest.mark.parametrize("D", [128, 256])
