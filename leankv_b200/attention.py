@@ -9,11 +9,13 @@ output rotated back, so the result is attention in the original space.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
 from . import _lib as L
-from .ops import _DTYPES, _check_rows, _need_cuda, _on_device, _same_device, _stream
+from .ops import (_DTYPES, _PAGES, _call, _check_lengths, _check_q8_pools, _check_rows, _check_table, _device_of,
+                  _need_cuda, _stream)
 
 
 class AttnArgs(C.Structure):
@@ -158,19 +160,8 @@ def decode_attention_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     return (out, lse) if return_lse else out
 
 
-class AttnQ8Args(C.Structure):
-    """Mirror of tq_attention_q8_args (include/leankv_tq.h)."""
-    _fields_ = [
-        ("batch", C.c_int), ("n_q_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
-        ("n_new", C.c_int64),
-        ("q", C.c_void_p), ("q_dtype", C.c_int), ("q_stride", C.c_int64 * 3),
-        ("out", C.c_void_p), ("out_dtype", C.c_int), ("out_stride", C.c_int64 * 3),
-        ("k_codes", C.c_void_p), ("k_scale", C.c_void_p), ("v_codes", C.c_void_p), ("v_scale", C.c_void_p),
-        ("kv_len", C.c_void_p), ("q_len", C.c_void_p), ("max_kv_len", C.c_int64), ("sm_scale", C.c_float),
-        ("causal", C.c_int), ("rotate_q", C.c_int), ("v_rotated", C.c_int),
-        ("lse", C.c_void_p), ("status", C.c_void_p),
-        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
-    ]
+# tq_attention_q8_args (include/leankv_tq.h)
+_ATTN_Q8 = struct.Struct("iiiiqPiqqqPiqqqPPPPPPqfiiiPPPN")
 
 
 def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
@@ -192,69 +183,51 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     lse_out (float32 [B, Hq, n]): destinations.  status: int32 CUDA tensor [1], raised to 1 when a page id
     outside the pool is met (its tokens are left out).
     """
-    _need_cuda(q, k_pool, v_pool, k_scale, v_scale, page_table, kv_len)
+    device = _device_of(q, k_pool, v_pool, k_scale, v_scale, page_table, kv_len, q_len, out, lse_out, status)
     single = q.dim() == 3
     if single:
         q = q.unsqueeze(2)
         out = out.unsqueeze(2) if out is not None else None
-    _check_rows(q, "q")
+    qs = _check_rows(q, "q")
     B, Hq, n, D = q.shape
-    if k_pool.dtype != torch.int8 or k_pool.dim() != 4 or k_pool.shape[3] != D or not k_pool.is_contiguous() \
-            or v_pool.dtype != torch.int8 or v_pool.shape != k_pool.shape or not v_pool.is_contiguous():
-        raise ValueError("pools must be contiguous int8 [num_pages, n_kv_heads, page_size, head_dim], both alike")
-    pages, Hkv, page_size, _ = k_pool.shape
-    for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if s.dtype != torch.float32 or s.shape != (pages, Hkv, page_size // 16) or not s.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous float32 [num_pages, n_kv_heads, page_size / 16] tensor")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B \
-            or not page_table.is_contiguous():
-        raise ValueError("page_table must be a contiguous int32 [batch, max_pages_per_seq] tensor")
-    for t, name in ((kv_len, "kv_len"), (q_len, "q_len")):
-        if t is not None:
-            _need_cuda(t)
-            if t.dtype != torch.int32 or t.numel() != B or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous int32 [batch] tensor")
+    Hkv = k_pool.shape[1] if k_pool.dim() == 4 else 0
+    pages, page_size = _check_q8_pools(k_pool, v_pool, k_scale, v_scale, Hkv, D)
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError("n_q_heads must be a multiple of n_kv_heads")
+    _check_table(page_table, B)
+    _check_lengths(kv_len, B, "kv_len")
+    if q_len is not None:
+        _check_lengths(q_len, B, "q_len")
     if out is None:
-        out = torch.empty((B, n, Hq, D), dtype=out_dtype or q.dtype, device=q.device).transpose(1, 2)
-    else:
-        _need_cuda(out)
-        if out.shape != q.shape or out.stride(3) != 1 or (out_dtype is not None and out.dtype != out_dtype):
-            raise ValueError("out must have q's shape, head_dim contiguous")
+        out = torch.empty_strided((B, Hq, n, D), (n * Hq * D, D, Hq * D, 1), dtype=out_dtype or q.dtype, device=q.device)
+    elif out.shape != q.shape or out.stride(3) != 1 or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError("out must have q's shape, head_dim contiguous")
     if out.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {out.dtype}")
-    if lse_out is not None:
-        _need_cuda(lse_out)
-        if lse_out.dtype != torch.float32 or lse_out.numel() != B * Hq * n or not lse_out.is_contiguous():
+    lse = lse_out
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.numel() != B * Hq * n or not lse.is_contiguous():
             raise ValueError("lse_out must be a contiguous float32 [B, Hq, n] tensor")
-        lse = lse_out
-    else:
-        lse = torch.empty((B, Hq, n), dtype=torch.float32, device=q.device) if return_lse else None
-    if status is not None:
-        _need_cuda(status)
-        if status.dtype != torch.int32 or status.numel() < 1:
-            raise ValueError("status must be an int32 tensor")
-    _same_device(q, k_pool, v_pool, k_scale, v_scale, page_table, kv_len, q_len, out, lse, status)
-    qs, os = q.stride(), out.stride()
-    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
-    a = AttnQ8Args(B, Hq, Hkv, D, n, q.data_ptr(), _DTYPES[q.dtype], qs[:3], out.data_ptr(), _DTYPES[out.dtype], os[:3],
-                   k_pool.data_ptr(), k_scale.data_ptr(), v_pool.data_ptr(), v_scale.data_ptr(), kv_len.data_ptr(),
-                   ptr(q_len), int(max_kv_len or 0), float(sm_scale or 0.0), int(causal), int(rotate_q), int(v_rotated),
-                   ptr(lse), ptr(status), None, 0)
-    pg = make_pages(page_table, pages, page_size)
+    elif return_lse:
+        lse = torch.empty((B, Hq, n), dtype=torch.float32, device=q.device)
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError("status must be an int32 tensor")
+    os = out.stride()
+    fields = (B, Hq, Hkv, D, n, q.data_ptr(), _DTYPES[q.dtype], qs[0], qs[1], qs[2], out.data_ptr(), _DTYPES[out.dtype],
+              os[0], os[1], os[2], k_pool.data_ptr(), k_scale.data_ptr(), v_pool.data_ptr(), v_scale.data_ptr(),
+              kv_len.data_ptr(), 0 if q_len is None else q_len.data_ptr(), int(max_kv_len or 0), float(sm_scale or 0.0),
+              int(causal), int(rotate_q), int(v_rotated), 0 if lse is None else lse.data_ptr(),
+              0 if status is None else status.data_ptr())
+    pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
     lib = L.load()
-    with _on_device(q):
-        need = lib.tq_attention_q8_workspace_size(C.byref(a), C.byref(pg))
-        if need:
-            # from the allocator on every call: streams and captured graphs each get their own
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        L.check(lib.tq_attention_q8_paged_cuda(C.byref(a), C.byref(pg), _stream(q)))
-    out = out.squeeze(2) if single else out
-    if return_lse:
-        return out, (lse.squeeze(2) if single and lse.dim() == 3 else lse)
-    return out
+    need = lib.tq_attention_q8_workspace_size(_ATTN_Q8.pack(*fields, 0, 0), pg)
+    # from the allocator on every call: streams and captured graphs each get their own
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _call(device, lib.tq_attention_q8_paged_cuda, _ATTN_Q8.pack(*fields, ws.data_ptr() if need else 0, need), pg)
+    if single:
+        out = out.squeeze(2)
+        lse = lse.squeeze(2) if lse is not None and lse.dim() == 3 else lse
+    return (out, lse) if return_lse else out
 
 
 def _btype(cache: torch.Tensor) -> int:

@@ -505,6 +505,7 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
         if (s > 1 && (int64_t)(s - 1) * per >= len) continue;   // the last split would be empty
         const int64_t waves = (units * s + slots - 1) / slots, cost = waves * (per + start);
         if (cost < best) { best = cost; p.splits = s; }
+        if (waves > 8) break;   // finer splits only add starts
     }
     return p;
 }

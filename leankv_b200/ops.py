@@ -6,8 +6,8 @@ TQ4_0 or (n_blocks, 14) for TQ3_0 — the byte layout of src/ggml-tq.h:131-141.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import struct
 from typing import NamedTuple
 
 import torch
@@ -21,8 +21,13 @@ BLOCK_BYTES = L.BLOCK_BYTES
 _DTYPES = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16}
 
 
+# the current stream's handle without the Stream object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _stream(t: torch.Tensor) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    return C.c_void_p(_raw_stream(t.device.index))
 
 
 def _need_cuda(*ts: torch.Tensor) -> None:
@@ -227,82 +232,96 @@ def rotary_axes(sections, device="cuda", interleaved: bool = False) -> torch.Ten
     return torch.tensor(order, dtype=torch.int32, device=device)
 
 
-class _Rope(C.Structure):
-    """Mirror of tq_rope (include/leankv_tq.h)."""
-    _fields_ = [("inv_freq", C.c_void_p), ("axis", C.c_void_p), ("positions", C.c_void_p), ("n_axes", C.c_int),
-                ("rotary_dim", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int), ("scale", C.c_double)]
+# Argument blocks of include/leankv_tq.h as native struct layouts (packing one takes a fraction of the time of
+# filling ctypes structures, which is most of a small call).
+_ROPE_FMT, _HEADS_FMT = "PPPiiiid", "PPiqqqqqq"
+_ROPE = struct.Struct(_ROPE_FMT)                      # tq_rope
+_HEADS = struct.Struct(_HEADS_FMT)                    # tq_head_rows
+_APPEND = struct.Struct("iiiqi0q" + 3 * _HEADS_FMT + _ROPE_FMT + "PiPPiPPPiP")   # tq_rotary_append_args
+_PAGES = struct.Struct("Pqqi")                        # tq_kv_pages
+_NO_HEADS, _NO_ROPE = (0,) * 9, (0, 0, 0, 0, 0, 0, 0, 0.0)
+
+def _device_of(*ts) -> int:
+    """The CUDA device that holds all tensors (None entries are skipped)."""
+    d = ts[0].get_device()
+    for t in ts:
+        if t is not None and (t.get_device() != d or d < 0):
+            _need_cuda(*(u for u in ts if u is not None))
+            raise ValueError(f"tensors on {ts[0].device} and {t.device}")
+    return d
 
 
-class _HeadRows(C.Structure):
-    """Mirror of tq_head_rows (include/leankv_tq.h)."""
-    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("heads", C.c_int), ("src_stride", C.c_int64 * 3),
-                ("dst_stride", C.c_int64 * 3)]
+def _call(device: int, fn, *args) -> None:
+    """A library call on the device's current stream; launches go to the current device."""
+    if device == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _raw_stream(device))
+    if status:
+        L.check(status)
 
 
-class _RotaryAppendArgs(C.Structure):
-    """Mirror of tq_rotary_append_args (include/leankv_tq.h)."""
-    _fields_ = [("batch", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("n_new", C.c_int64),
-                ("dtype", C.c_int), ("k", _HeadRows), ("v", _HeadRows), ("q", _HeadRows), ("rope", _Rope),
-                ("k_pool", C.c_void_p), ("k_type", C.c_int), ("k_scale", C.c_void_p), ("v_pool", C.c_void_p),
-                ("v_type", C.c_int), ("v_scale", C.c_void_p), ("pos", C.c_void_p), ("new_len", C.c_void_p),
-                ("rotate", C.c_int), ("overflow", C.c_void_p)]
-
-
-def _on_device(t: torch.Tensor):
-    """Launches go to the current device: make it the tensor's."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _same_device(t: torch.Tensor, *others) -> None:
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise ValueError(f"tensors on {t.device} and {o.device}")
-
-
-def _check_rows(t: torch.Tensor, name: str) -> None:
-    if t.dim() != 4 or t.dtype not in _DTYPES or (t.shape[3] > 1 and t.stride(3) != 1):
+def _check_rows(t: torch.Tensor, name: str) -> tuple:
+    """The strides of [batch, heads, tokens, head_dim] rows."""
+    s = t.stride()
+    if len(s) != 4 or t.dtype not in _DTYPES or (s[3] != 1 and t.shape[3] > 1):
         raise ValueError(f"{name} must be a f32/f16/bf16 [batch, heads, tokens, head_dim] tensor, head_dim contiguous")
+    return s
 
 
-def _rows(src: torch.Tensor, dst: torch.Tensor | None = None) -> _HeadRows:
-    s = src.stride()
-    if dst is None:
-        return _HeadRows(src.data_ptr(), None, src.shape[1], (s[0], s[1], s[2]))
-    d = dst.stride()
-    return _HeadRows(src.data_ptr(), dst.data_ptr(), src.shape[1], (s[0], s[1], s[2]), (d[0], d[1], d[2]))
+def _check_lengths(t: torch.Tensor, batch: int, name: str) -> None:
+    if t.dtype != torch.int32 or t.numel() != batch or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 [batch] tensor")
 
 
-def _rope(rope: Rotary, like: torch.Tensor, positions: torch.Tensor | None, inverse: bool) -> _Rope:
-    f, ax = rope.inv_freq, rope.axis
-    _need_cuda(f)
-    if f.dtype != torch.float64 or f.dim() != 1 or not f.is_contiguous():
-        raise ValueError("inv_freq must be a contiguous float64 [rotary_dim / 2] tensor")
-    if ax is not None:
-        _need_cuda(ax)
-        if ax.dtype != torch.int32 or ax.shape != f.shape or not ax.is_contiguous():
-            raise ValueError("axis must be a contiguous int32 tensor of inv_freq's shape")
-    axes = 1
-    if positions is not None:
-        _need_cuda(positions)
-        if positions.dtype != torch.int32 or not positions.is_contiguous() or positions.dim() not in (2, 3) \
-                or positions.shape[-2] != like.shape[0] or positions.shape[-1] != like.shape[2]:
-            raise ValueError("positions must be a contiguous int32 [batch, tokens] or [axes, batch, tokens] tensor")
-        axes = positions.shape[0] if positions.dim() == 3 else 1
-        if axes > 1 and ax is None:
-            raise ValueError("positions of several axes need the axis of each pair")
-    _same_device(like, f, ax, positions)
-    return _Rope(f.data_ptr(), None if ax is None else ax.data_ptr(), None if positions is None else positions.data_ptr(),
-                 axes, 2 * f.shape[0], int(rope.interleaved), int(inverse), float(rope.scale))
+def _check_table(t: torch.Tensor, batch: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != batch or not t.is_contiguous():
+        raise ValueError("page_table must be a contiguous int32 [batch, max_pages_per_seq] tensor")
 
 
-def _rotary_out(t: torch.Tensor, out: torch.Tensor | None, name: str) -> torch.Tensor:
+def _check_q8_pools(k_pool, v_pool, k_scale, v_scale, H: int, D: int) -> tuple:
+    """(pages, page_size) of 8-bit pools and their scales."""
+    shape = k_pool.shape
+    if k_pool.dtype != torch.int8 or len(shape) != 4 or shape[1] != H or shape[3] != D or not k_pool.is_contiguous() \
+            or v_pool.dtype != torch.int8 or v_pool.shape != shape or not v_pool.is_contiguous():
+        raise ValueError("8-bit pools must be contiguous int8 [num_pages, n_kv_heads, page_size, head_dim], both alike")
+    want = (shape[0], H, shape[2] // Q8_BLOCK)
+    for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if s is None or s.dtype != torch.float32 or s.shape != want or not s.is_contiguous():
+            raise ValueError(f"8-bit pools need {name}, a contiguous float32 [num_pages, n_kv_heads, page_size / 16] tensor")
+    return shape[0], shape[2]
+
+
+def _rows_out(t: torch.Tensor, out: torch.Tensor | None, name: str) -> torch.Tensor:
     if out is None:
         # token-major memory, as the projections on either side have it
-        return torch.empty((t.shape[0], t.shape[2], t.shape[1], t.shape[3]), dtype=t.dtype, device=t.device).transpose(1, 2)
-    _need_cuda(out)
+        B, H, n, D = t.shape
+        return torch.empty_strided((B, H, n, D), (n * H * D, D, H * D, 1), dtype=t.dtype, device=t.device)
     if out.shape != t.shape or out.dtype != t.dtype or (out.shape[3] > 1 and out.stride(3) != 1):
         raise ValueError(f"{name} must have the shape and type of its input, head_dim contiguous")
     return out
+
+
+def _rope_fields(rope: Rotary, batch: int, tokens: int, positions: torch.Tensor | None, inverse: bool) -> tuple:
+    """tq_rope's fields, checked (devices apart)."""
+    f, ax, interleaved, scale = rope
+    if f.dtype != torch.float64 or f.dim() != 1 or not f.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float64 [rotary_dim / 2] tensor")
+    if ax is not None and (ax.dtype != torch.int32 or ax.shape != f.shape or not ax.is_contiguous()):
+        raise ValueError("axis must be a contiguous int32 tensor of inv_freq's shape")
+    axes, where = 1, 0
+    if positions is not None:
+        shape = positions.shape
+        if positions.dtype != torch.int32 or not positions.is_contiguous() or len(shape) not in (2, 3) \
+                or shape[-2] != batch or shape[-1] != tokens:
+            raise ValueError("positions must be a contiguous int32 [batch, tokens] or [axes, batch, tokens] tensor")
+        axes = shape[0] if len(shape) == 3 else 1
+        if axes > 1 and ax is None:
+            raise ValueError("positions of several axes need the axis of each pair")
+        where = positions.data_ptr()
+    return (f.data_ptr(), 0 if ax is None else ax.data_ptr(), where, axes, 2 * f.shape[0], int(interleaved), int(inverse),
+            float(scale))
 
 
 def rotary(q: torch.Tensor, positions: torch.Tensor, rope: Rotary, k: torch.Tensor | None = None,
@@ -314,25 +333,26 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, rope: Rotary, k: torch.Tens
     Computed in float32 with angles exact at every position, rounded once.  inverse turns back: the
     gradient of the inputs from that of the outputs.  out / k_out: destinations (may be q / k themselves).
     Returns the rotated q, or (q, k)."""
-    _need_cuda(q)
-    _check_rows(q, "q")
-    if k is not None:
-        _need_cuda(k)
-        _check_rows(k, "k")
-        if k.dtype != q.dtype or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]:
-            raise ValueError("k must have q's type, batch, tokens and head_dim")
     if positions is None:
         raise ValueError("positions are needed")
-    r = _rope(rope, q, positions, inverse)
-    out = _rotary_out(q, out, "out")
-    k_out = _rotary_out(k, k_out, "k_out") if k is not None else None
-    _same_device(q, k, out, k_out)
-    if q.shape[1] == 0 or (k is not None and k.shape[1] == 0):
-        raise ValueError("no heads")
-    with _on_device(q):
-        L.check(L.load().tq_rotary_cuda(C.byref(r), _DTYPES[q.dtype], q.shape[0], q.shape[2], q.shape[3],
-                                        C.byref(_rows(q, out)), C.byref(_rows(k, k_out)) if k is not None else None,
-                                        _stream(q)))
+    device = _device_of(q, positions, rope.inv_freq, rope.axis, k, out, k_out)
+    qs = _check_rows(q, "q")
+    B, H, n, D = q.shape
+    r = _rope_fields(rope, B, n, positions, inverse)
+    out = _rows_out(q, out, "out")
+    os = out.stride()
+    x = _HEADS.pack(q.data_ptr(), out.data_ptr(), H, qs[0], qs[1], qs[2], os[0], os[1], os[2])
+    x2 = None
+    if k is not None:
+        ks = _check_rows(k, "k")
+        if k.dtype != q.dtype or k.shape[0] != B or k.shape[2] != n or k.shape[3] != D:
+            raise ValueError("k must have q's type, batch, tokens and head_dim")
+        k_out = _rows_out(k, k_out, "k_out")
+        os = k_out.stride()
+        x2 = _HEADS.pack(k.data_ptr(), k_out.data_ptr(), k.shape[1], ks[0], ks[1], ks[2], os[0], os[1], os[2])
+    elif k_out is not None:
+        raise ValueError("k_out without k")
+    _call(device, L.load().tq_rotary_cuda, _ROPE.pack(*r), _DTYPES[q.dtype], B, n, D, x, x2)
     return out if k is None else (out, k_out)
 
 
@@ -354,70 +374,53 @@ def kv_append_rotary_paged(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tenso
     a padded batch are not stored.  rotate: the head_dim Hadamard rotation, as the attention expects.
     Rows without a place are counted into overflow, keys and values each.  Returns the rotated q (in q_out
     when given, which may be q), or None without q."""
-    _need_cuda(k, v, k_pool, v_pool, page_table)
-    _check_rows(k, "k")
-    _check_rows(v, "v")
+    device = _device_of(k, v, k_pool, v_pool, page_table, pos, new_len, k_scale, v_scale, q, q_out, overflow, positions,
+                        *((rope.inv_freq, rope.axis) if rope is not None else ()))
+    ks, vs = _check_rows(k, "k"), _check_rows(v, "v")
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError("k and v must have the same shape and type")
     B, H, n_new, D = k.shape
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B \
-            or not page_table.is_contiguous():
-        raise ValueError("page_table must be a contiguous int32 [batch, max_pages_per_seq] tensor")
-    if not k_pool.is_contiguous() or not v_pool.is_contiguous() or k_pool.shape[:3] != v_pool.shape[:3] \
-            or k_pool.dim() < 4 or k_pool.shape[1] != H:
-        raise ValueError("pools must be contiguous, with the same pages, n_kv_heads and page size")
-    pages, _, page_size = k_pool.shape[:3]
+    _check_table(page_table, B)
     if k_pool.dtype == torch.int8:
         kt = vt = Q8
-        if k_pool.shape != (pages, H, page_size, D) or v_pool.shape != k_pool.shape or v_pool.dtype != torch.int8:
-            raise ValueError("8-bit pools must be int8 [num_pages, n_kv_heads, page_size, head_dim], both")
-        for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-            if s is None:
-                raise ValueError(f"8-bit pools need {name}")
-            _need_cuda(s)
-            if s.dtype != torch.float32 or s.shape != (pages, H, page_size // Q8_BLOCK) or not s.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous float32 [num_pages, n_kv_heads, page_size / 16] tensor")
+        pages, page_size = _check_q8_pools(k_pool, v_pool, k_scale, v_scale, H, D)
+        k_sc, v_sc = k_scale.data_ptr(), v_scale.data_ptr()
     else:
-        kt = {n: t for t, n in BLOCK_BYTES.items()}.get(k_pool.shape[-1])
-        vt = TQ4_0
+        kt, vt = {n: t for t, n in BLOCK_BYTES.items()}.get(k_pool.shape[-1]), TQ4_0
+        pages, page_size = (k_pool.shape[0], k_pool.shape[2]) if k_pool.dim() == 5 else (0, 0)
         if k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 or kt is None \
-                or k_pool.shape != (pages, H, page_size, D // QK, BLOCK_BYTES[kt]) \
-                or v_pool.shape != (pages, H, page_size, D // QK, BLOCK_BYTES[TQ4_0]):
-            raise ValueError("pools must be uint8 [num_pages, n_kv_heads, page_size, head_dim/32, bytes] blocks, "
-                             "TQ4_0 for the values")
+                or k_pool.shape != (pages, H, page_size, D // QK, BLOCK_BYTES[kt]) or not k_pool.is_contiguous() \
+                or v_pool.shape != (pages, H, page_size, D // QK, BLOCK_BYTES[TQ4_0]) or not v_pool.is_contiguous():
+            raise ValueError("pools must be contiguous uint8 [num_pages, n_kv_heads, page_size, head_dim/32, bytes] "
+                             "blocks, TQ4_0 for the values")
         if k_scale is not None or v_scale is not None:
             raise ValueError("TQ pools have no scales")
-    for t, name in ((pos, "pos"), (new_len, "new_len")):
-        if t is not None:
-            _need_cuda(t)
-            if t.dtype != torch.int32 or t.numel() != B or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous int32 [batch] tensor")
-    if overflow is not None:
-        _need_cuda(overflow)
-        if overflow.dtype != torch.int32:
-            raise ValueError("overflow must be an int32 tensor")
-    if positions is not None and rope is None:
-        raise ValueError("positions without a rotation")
+        k_sc = v_sc = 0
+    if pos is not None:
+        _check_lengths(pos, B, "pos")
+    if new_len is not None:
+        _check_lengths(new_len, B, "new_len")
+    if overflow is not None and (overflow.dtype != torch.int32 or overflow.numel() < 1):
+        raise ValueError("overflow must be an int32 tensor")
+    if rope is None and (positions is not None or q is not None):
+        raise ValueError("positions or q without a rotation")
+    r = _NO_ROPE if rope is None else _rope_fields(rope, B, n_new, positions, False)
+    heads = _NO_HEADS
     if q is not None:
-        _need_cuda(q)
-        _check_rows(q, "q")
+        qs = _check_rows(q, "q")
         if q.dtype != k.dtype or q.shape[0] != B or q.shape[2] != n_new or q.shape[3] != D or q.shape[1] == 0:
             raise ValueError("q must have k's type, batch, tokens and head_dim")
-        if rope is None:
-            raise ValueError("q without a rotation")
-        q_out = _rotary_out(q, q_out, "q_out")
+        q_out = _rows_out(q, q_out, "q_out")
+        os = q_out.stride()
+        heads = (q.data_ptr(), q_out.data_ptr(), q.shape[1], qs[0], qs[1], qs[2], os[0], os[1], os[2])
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _same_device(k, v, k_pool, v_pool, page_table, pos, new_len, k_scale, v_scale, q, q_out, overflow)
-    from .attention import make_pages
-    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
-    a = _RotaryAppendArgs(B, H, D, n_new, _DTYPES[k.dtype], _rows(k), _rows(v),
-                          _HeadRows() if q is None else _rows(q, q_out),
-                          _Rope() if rope is None else _rope(rope, k, positions, False), ptr(k_pool), kt, ptr(k_scale),
-                          ptr(v_pool), vt, ptr(v_scale), ptr(pos), ptr(new_len), int(rotate), ptr(overflow))
-    with _on_device(k):
-        L.check(L.load().tq_kv_append_rotary_paged_cuda(C.byref(a), C.byref(make_pages(page_table, pages, page_size)),
-                                                        _stream(k)))
+    a = _APPEND.pack(B, H, D, n_new, _DTYPES[k.dtype], k.data_ptr(), 0, H, ks[0], ks[1], ks[2], 0, 0, 0,
+                     v.data_ptr(), 0, H, vs[0], vs[1], vs[2], 0, 0, 0, *heads, *r,
+                     k_pool.data_ptr(), kt, k_sc, v_pool.data_ptr(), vt, v_sc, 0 if pos is None else pos.data_ptr(),
+                     0 if new_len is None else new_len.data_ptr(), int(rotate), 0 if overflow is None else overflow.data_ptr())
+    _call(device, L.load().tq_kv_append_rotary_paged_cuda, a,
+          _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size))
     return q_out
 
 
@@ -425,7 +428,7 @@ def dequantize_q8(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype =
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Values of 8-bit pages: int8 [..., tokens, head_dim] (tokens a multiple of 16, head_dim 128 or 256)
     times float32 [..., tokens / 16], rounded to dtype."""
-    _need_cuda(codes, scale)
+    device = _device_of(codes, scale, out)
     if codes.dtype != torch.int8 or not codes.is_contiguous() or codes.dim() < 2 or codes.shape[-2] % Q8_BLOCK:
         raise ValueError("codes must be a contiguous int8 [..., tokens, head_dim] tensor, tokens a multiple of 16")
     if scale.dtype != torch.float32 or not scale.is_contiguous() \
@@ -433,16 +436,12 @@ def dequantize_q8(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype =
         raise ValueError("scale must be a contiguous float32 [..., tokens / 16] tensor")
     if out is None:
         out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-    else:
-        _need_cuda(out)
-        if out.shape != codes.shape or out.dtype not in _DTYPES or not out.is_contiguous():
-            raise ValueError("out must be a contiguous f32/f16/bf16 tensor of the codes' shape")
+    elif out.shape != codes.shape or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of the codes' shape")
     if out.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {out.dtype}")
-    _same_device(codes, scale, out)
-    with _on_device(codes):
-        L.check(L.load().tq_dequantize_q8_cuda(codes.data_ptr(), scale.data_ptr(), out.data_ptr(), _DTYPES[out.dtype],
-                                               scale.numel(), codes.shape[-1], _stream(codes)))
+    _call(device, L.load().tq_dequantize_q8_cuda, codes.data_ptr(), scale.data_ptr(), out.data_ptr(), _DTYPES[out.dtype],
+          scale.numel(), codes.shape[-1])
     return out
 
 
