@@ -5,7 +5,7 @@
 // A CTA takes QT tiles of 128 query rows (tokens x heads of one group) of one (sequence, KV head).  Warps:
 //   4 QT softmax warps   one thread per row: scores from TMEM, weights back to TMEM, the output's rescaling
 //   1 issuing warp       one thread issues all tcgen05.mma
-//   4 converting warps   8-bit codes from the pages to f16 tiles in shared memory
+//   4 + 3 more warps     8-bit codes of K and V from the pages to f16 tiles in shared memory
 // Per tile of KT tokens: S = Q K^T (both from shared memory, f16, fp32 sums in TMEM), weights P in f16 written
 // over S, O += P V (P from TMEM, V from shared memory).  D = 128: two row tiles of 128 tokens take turns, so that
 // one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).  D = 256: O alone
@@ -44,7 +44,7 @@ __device__ __forceinline__ uint64_t now_ns() {
 }
 constexpr uint64_t WAIT_NS = 1000000000ull;
 // waits for the phase of `parity`; false once any wait of the CTA has run out
-__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int* failed) {
+__device__ __forceinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int* failed) {
     const uint64_t until = now_ns() + WAIT_NS;
     while (!mbar_try(bar, parity)) {
         if (*failed) return false;
@@ -76,35 +76,72 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// 32 consecutive columns of this thread's TMEM lane
-__device__ __forceinline__ void tc_ld32(uint32_t a, uint32_t (&v)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-                   "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-                   "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+// consecutive columns of this thread's TMEM lane; the wait takes the loaded registers, so that nothing that uses
+// them can be moved before it
+__device__ __forceinline__ void tc_ld16(uint32_t a, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+                 "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                 "=r"(v[14]), "=r"(v[15])
                  : "r"(a));
 }
-__device__ __forceinline__ void tc_st32(uint32_t a, const uint32_t (&v)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-                 ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
-                   "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
-                   "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-                 : "memory");
+__device__ __forceinline__ void tc_ld32(uint32_t a, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+                 "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+                 "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                 "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+                 "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+                 "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(a));
+}
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                 "+r"(v[14]), "+r"(v[15])
+                 :: "memory");
+}
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                 "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
+                 "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]),
+                 "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                 :: "memory");
 }
 __device__ __forceinline__ void tc_st16(uint32_t a, const uint32_t (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
                  "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-                 ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_st32(uint32_t a, const uint32_t (&v)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+                 "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+                 "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+                 "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+                 "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
+}
+// ties loaded registers to the place after their wait
+__device__ __forceinline__ void tc_loaded(uint32_t (&v)[32]) {
+    asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Matrix descriptor of a 128-byte-swizzled tile: start and strides in 16-byte units.  stride: 8 rows (1024
@@ -121,10 +158,80 @@ template <int D> struct PromptCfg {
     static constexpr int SEGS = D / 64;                    // 64-element runs of a row
     static constexpr int Q_TILE = 128 * D * 2, KV_TILE = KT * D * 2, SEG = KT * 128;
     static constexpr int SBUF = 2;                         // S buffers: one per row tile, or two of one
-    static constexpr int SOFT_WARPS = 4 * QT, WARPS = SOFT_WARPS + 5;
+    static constexpr int SOFT_WARPS = 4 * QT, CONV = SOFT_WARPS, ISSUE = SOFT_WARPS + 4, WARPS = SOFT_WARPS + 8;
+    // D = 128: 16 warps start with 128 registers; the softmax takes 168 and the others keep 88 (2 x 168 + 2 x 88
+    // = 4 x 128 per warpgroup).  D = 256: 12 warps have 168 from the start.
+    static constexpr bool MOVE_REGS = QT == 2;
     static constexpr int TILES = QT * Q_TILE + 4 * KV_TILE;   // Q, two K and two V buffers
     static constexpr int SMEM = TILES + 1024;              // the tiles start on 1024 bytes
 };
+
+// A converting warp: units [u0, u1) (at most NU) of every tile.  The next tile's codes are loaded while the
+// buffer is waited for, their pages a tile before that.
+template <int D, int NU>
+__device__ __forceinline__ void convert_tiles(const Q8Run& r, const int8_t* __restrict__ pool, int b, int h, int t_begin,
+                                              int tiles_n, int kv_end, int u0, int u1, uint32_t tile_at, uint32_t full,
+                                              uint32_t empty, volatile int* failed) {
+    using C = PromptCfg<D>;
+    constexpr int BPT = C::KT / 16;
+    const int lane = threadIdx.x & 31, sub = lane >> 2, c4 = lane & 3, per_page = r.page_shift - 4;
+    int page = -1;   // of unit u0 + lane
+    auto load_page = [&](int t) {
+        const int block = (t_begin + t) * BPT + (u0 + lane) / C::SEGS;
+        page = -1;
+        if (u0 + lane < u1 && t < tiles_n && block * 16 < kv_end)
+            page = r.pages[(int64_t)b * r.max_pages + (block >> per_page)];
+    };
+    uint4 w[NU][2];
+    auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int pg = __shfl_sync(0xffffffffu, page, i), u = u0 + i;
+            const int block = (t_begin + t) * BPT + u / C::SEGS;
+            w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);   // tokens that are not there
+            if (pg >= 0 && pg < r.num_pages) {
+                const int64_t blk = (((int64_t)pg * r.Hkv + h) << per_page) + (block & ((1 << per_page) - 1));
+                const int8_t* p = pool + (blk * 16 + sub) * D + (u % C::SEGS) * 64 + 16 * c4;
+                w[i][0] = __ldg(reinterpret_cast<const uint4*>(p));
+                w[i][1] = __ldg(reinterpret_cast<const uint4*>(p + 8 * D));
+            }
+        }
+    };
+    load_page(0);
+    load(0);
+    load_page(1);
+    const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1024 + 128
+    for (int t = 0; t < tiles_n; ++t) {
+        // the first pass over the two buffers does not wait
+        if (t >= 2 && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * (t & 1), ((t >> 1) & 1) ^ 1, failed))) break;
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            if (u0 + i >= u1) break;
+            const int u = u0 + i;
+            const uint32_t at = tile_at + (t & 1) * C::KV_TILE + (u % C::SEGS) * C::SEG + (u / C::SEGS) * 2048 + sub * 128;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {   // rows sub and sub + 8 of the block
+                const uint32_t in[4] = {w[i][x].x ^ 0x80808080u, w[i][x].y ^ 0x80808080u, w[i][x].z ^ 0x80808080u, w[i][x].w ^ 0x80808080u};
+                uint32_t o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t v = __byte_perm(in[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140);
+                    const __half2 hv = __hsub2(*reinterpret_cast<__half2*>(&v), off);
+                    o[j] = *reinterpret_cast<const uint32_t*>(&hv);
+                }
+                sts128(at + x * 1024 + (((2 * c4) ^ sub) << 4), o[0], o[1], o[2], o[3]);
+                sts128(at + x * 1024 + (((2 * c4 + 1) ^ sub) << 4), o[4], o[5], o[6], o[7]);
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + 8 * (t & 1));
+        if (t + 1 < tiles_n) {
+            load(t + 1);
+            load_page(t + 2);
+        }
+    }
+}
 
 template <int D>
 __global__ void __launch_bounds__(PromptCfg<D>::WARPS * 32, 1)
@@ -170,7 +277,7 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
         s_failed = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + 8 * i, 4);     // the converting warps
-            mbar_init(v_full + 8 * i, 4);
+            mbar_init(v_full + 8 * i, 3);
             mbar_init(k_empty + 8 * i, 1);    // commits of the issuing thread
             mbar_init(v_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
@@ -180,7 +287,7 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == C::SOFT_WARPS) {
+    if (warp == C::ISSUE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -202,7 +309,8 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
         for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(v[j]));
 #pragma unroll
         for (int o = 1; o < LPR; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
+        float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
+        if (r.sm_scale < 0.0f) inv = -inv;   // the row's factor is not negative
         uint32_t w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = pack_h2(v[2 * j] * inv, v[2 * j + 1] * inv);
@@ -211,7 +319,7 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
         *reinterpret_cast<uint4*>(at + ((c ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         *reinterpret_cast<uint4*>(at + (((c + 1) ^ (rr & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
         if (lane % LPR == 0) {
-            s_f[row] = top * r.sm_scale * LOG2E;
+            s_f[row] = top * fabsf(r.sm_scale) * LOG2E;
             s_lim[row] = live ? last_seen(r, sl, i) : -1;
         }
     }
@@ -222,6 +330,10 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
     const uint32_t tmem = s_tmem;
     const uint32_t o_col = 256;   // S buffers at columns 0 and 128 (0 and 64), O from 256 on
 
+    if constexpr (C::MOVE_REGS) {   // by whole warpgroups, each at one instruction
+        if (warp < C::SOFT_WARPS) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    }
     if (warp < C::SOFT_WARPS) {
         // ── softmax: thread = row ──
         const int qt = warp >> 2, row = qt * 128 + (warp & 3) * 32 + lane;
@@ -230,64 +342,72 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
         const float f = s_f[row];
         const int lim = s_lim[row];
         float m = -INFINITY, l = 0.0f;
-        // scales of the tile's blocks, one per lane (lane & 7), a tile ahead
-        constexpr int BPT = KT / 16;
+        // scales of the tile's blocks, one per lane (lane & 7): loaded a tile ahead, their pages two tiles ahead
+        constexpr int BPT = KT / 16, CH = KT / 32;
+        const int per_page = r.page_shift - 4;
         float ks = 0.0f, vs = 0.0f;
-        int blk = -1;
-        auto scales = [&](int t) {
+        int blk = -1, page = 0;
+        auto load_page = [&](int t) {
+            const int block = (t_begin + t) * BPT + (lane & (BPT - 1));
+            page = -2;   // no block
+            if (t < tiles_n && block * 16 < kv_end) page = r.pages[(int64_t)b * r.max_pages + (block >> per_page)];
+        };
+        auto load_scales = [&](int t) {
             const int block = (t_begin + t) * BPT + (lane & (BPT - 1));
             blk = -1;
             ks = vs = 0.0f;
-            if (t < tiles_n && block * 16 < kv_end) {
-                blk = block_at(r, b, h, block);
-                if (blk >= 0) { ks = r.ks[blk]; vs = r.vs[blk]; }
-                else if (r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
+            if (page >= 0 && page < r.num_pages) {
+                blk = (int)((((int64_t)page * r.Hkv + h) << per_page) + (block & ((1 << per_page) - 1)));
+                ks = r.ks[blk];
+                vs = r.vs[blk];
+            } else if (page != -2 && r.status) {
+                atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
             }
         };
-        scales(0);
+        load_page(0);
+        load_scales(0);
+        load_page(1);
         for (int t = 0; t < tiles_n; ++t) {
             const int sb = QT == 2 ? qt : (t & 1);
             const uint32_t s_at = lanes + sb * KT;
             const float ks_l = ks, vse = vs > 0.0f ? vs : 0x1p-100f;
             const float lv_l = lg2(vse), iv_l = __frcp_rn(vse);
             const uint32_t there = __ballot_sync(0xffffffffu, blk >= 0) & ((1u << BPT) - 1);
-            scales(t + 1);
+            load_scales(t + 1);
+            load_page(t + 2);
             const int tok0 = (t_begin + t) * KT;
             const bool edge = __any_sync(0xffffffffu, tok0 + KT - 1 > lim) || there != (1u << BPT) - 1;
             const uint32_t par = QT == 2 ? (t & 1) : ((t >> 1) & 1);
             if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * sb, par, &s_failed))) break;
             tc_fence_after();
 
-            auto scores = [&](int c, float (&y)[32]) {   // 32 columns: two scale blocks
-                uint32_t raw[32];
-                tc_ld32(s_at + 32 * c, raw);
-                tc_wait_ld();
+            // the row's scores, in registers
+            uint32_t raw[CH][32];
 #pragma unroll
-                for (int bl = 0; bl < 2; ++bl) {
-                    const float a = f * __shfl_sync(0xffffffffu, ks_l, 2 * c + bl);
-                    const float lv = __shfl_sync(0xffffffffu, lv_l, 2 * c + bl);
-                    const float2 a2 = make_float2(a, a), c2 = make_float2(lv, lv);
+            for (int c = 0; c < CH; ++c) tc_ld32(s_at + 32 * c, raw[c]);
+            tc_wait_ld(raw[0]);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[16 * bl + j]), __uint_as_float(raw[16 * bl + j + 1])), a2, c2);
-                        y[16 * bl + j] = x.x;
-                        y[16 * bl + j + 1] = x.y;
+            for (int c = 1; c < CH; ++c) tc_loaded(raw[c]);
+            if (edge) {
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const bool seen = tok0 + 32 * c + j <= lim && ((there >> (2 * c + j / 16)) & 1);
+                        raw[c][j] = seen ? raw[c][j] : 0xff800000u;   // -inf
                     }
-                    if (edge) {
-                        const bool gone = !((there >> (2 * c + bl)) & 1);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (gone || tok0 + 32 * c + 16 * bl + j > lim) y[16 * bl + j] = -INFINITY;
-                    }
-                }
-            };
+            }
+            // the largest exponent, from each scale block's largest sum (f and ks are not negative)
             float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c) {
-                float y[32];
-                scores(c, y);
+            for (int c = 0; c < BPT; ++c) {
+                const uint32_t* x = raw[c >> 1] + 16 * (c & 1);
+                float y = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
 #pragma unroll
-                for (int j = 0; j < 32; ++j) top = fmaxf(top, y[j]);
+                for (int j = 3; j < 15; j += 2) y = max3(y, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+                y = fmaxf(y, __uint_as_float(x[15]));
+                const float a = f * __shfl_sync(0xffffffffu, ks_l, c), lv = __shfl_sync(0xffffffffu, lv_l, c);
+                top = fmaxf(top, y == -INFINITY ? y : fmaf(y, a, lv));
             }
             const bool move = top > m + Q8_SLACK;
             if (__any_sync(0xffffffffu, move)) {
@@ -302,37 +422,41 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
                         if (!__all_sync(0xffffffffu, mbar_wait(o_done, (t - 1) & 1, &s_failed))) break;
                         tc_fence_after();
                     }
-                    // rare after the first tiles: not unrolled
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t x[32];
-                        tc_ld32(o_at + 32 * c, x);
-                        tc_wait_ld();
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t x[16];
+                        tc_ld16(o_at + 16 * c, x);
+                        tc_wait_ld(x);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * w);
-                        tc_st32(o_at + 32 * c, x);
+                        for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * w);
+                        tc_st16(o_at + 16 * c, x);
                     }
                 }
             }
+            // weights 2^(s + log2 vs - m + SHIFT) in f16 over the scores, 32 of them in 16 columns
             const float ref = m == -INFINITY ? 0.0f : Q8_SHIFT - m;
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c) {
-                float y[32];
-                scores(c, y);
+            for (int c = 0; c < CH; ++c) {
                 uint32_t p[16];
 #pragma unroll
                 for (int bl = 0; bl < 2; ++bl) {
+                    const float a = f * __shfl_sync(0xffffffffu, ks_l, 2 * c + bl);
+                    const float lv = __shfl_sync(0xffffffffu, lv_l, 2 * c + bl) + ref;
                     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        const float2 e = __fadd2_rn(make_float2(y[16 * bl + j], y[16 * bl + j + 1]), make_float2(ref, ref));
+                        const float x0 = __uint_as_float(raw[c][16 * bl + j]), x1 = __uint_as_float(raw[c][16 * bl + j + 1]);
+                        float2 e = __ffma2_rn(make_float2(x0, x1), make_float2(a, a), make_float2(lv, lv));
+                        if (edge && a == 0.0f) {   // -inf times a zero factor
+                            e.x = x0 == -INFINITY ? x0 : e.x;
+                            e.y = x1 == -INFINITY ? x1 : e.y;
+                        }
                         const float2 w = make_float2(ex2(e.x), ex2(e.y));
                         sum = __fadd2_rn(sum, w);
                         p[8 * bl + j / 2] = pack_h2(w.x, w.y);
                     }
                     l = fmaf(sum.x + sum.y, __shfl_sync(0xffffffffu, iv_l, 2 * c + bl), l);
                 }
-                // 32 weights take 16 columns, all left of the columns still to be read
                 tc_st16(s_at + 16 * c, p);
             }
             tc_wait_st();
@@ -341,7 +465,7 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
         }
         s_lse[row] = l > 0.0f ? (m - Q8_SHIFT + lg2(l)) * LN2 : -INFINITY;
         s_f[row] = l > 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
-    } else if (warp == C::SOFT_WARPS) {
+    } else if (warp == C::ISSUE) {
         // ── issue ──
         if (lane == 0 && tiles_n > 0) {
             constexpr uint32_t id_s = mma_idesc(KT, 0), id_o = mma_idesc(D, 1);
@@ -409,58 +533,12 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
         }
         __syncwarp();
     } else {
-        // ── conversion: 8 chunks of 16 codes per thread and tile, two stores of 8 f16 each ──
-        const int cw = warp - C::SOFT_WARPS - 1, sub = lane >> 2, c4 = lane & 3;
-        constexpr int WROWS = KT / 4, GROUPS = WROWS / 8;   // rows per warp, 8-row groups among them
-        auto load = [&](const int8_t* pool, int t, uint4 (&w)[8]) {
-#pragma unroll
-            for (int gi = 0; gi < GROUPS; ++gi) {
-                const int tok = (t_begin + t) * KT + cw * WROWS + 8 * gi;   // group's first token (warp-uniform)
-                const int blk = tok < kv_end ? block_at(r, b, h, tok >> 4) : -1;
-                const int8_t* p = pool + ((int64_t)blk * 16 + (tok & 15) + sub) * D + 16 * c4;
-#pragma unroll
-                for (int s = 0; s < C::SEGS; ++s)
-                    w[gi * C::SEGS + s] = blk >= 0 ? __ldg(reinterpret_cast<const uint4*>(p + 64 * s)) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto store = [&](uint32_t tile, const uint4 (&w)[8]) {
-            const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
-#pragma unroll
-            for (int gi = 0; gi < GROUPS; ++gi) {
-                const int row = cw * WROWS + 8 * gi + sub;   // row & 7 == sub
-#pragma unroll
-                for (int s = 0; s < C::SEGS; ++s) {
-                    const uint4 x = w[gi * C::SEGS + s];
-                    const uint32_t in[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
-                    uint32_t o[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        uint32_t v = __byte_perm(in[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140);
-                        const __half2 hv = __hsub2(*reinterpret_cast<__half2*>(&v), off);
-                        o[j] = *reinterpret_cast<const uint32_t*>(&hv);
-                    }
-                    const uint32_t at = tile + s * C::SEG + row * 128;
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((2 * c4) ^ sub) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((2 * c4 + 1) ^ sub) << 4)), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        };
-        uint4 kw[8], vw[8];
-        if (tiles_n > 0) load(r.k, 0, kw);
-        for (int t = 0; t < tiles_n; ++t) {
-            load(r.v, t, vw);
-            const uint32_t par = ((t >> 1) & 1) ^ 1;   // the first pass over the two buffers does not wait
-            if (t >= 2 && !__all_sync(0xffffffffu, mbar_wait(k_empty + 8 * (t & 1), par, &s_failed))) break;
-            store(k_at + (t & 1) * C::KV_TILE, kw);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(k_full + 8 * (t & 1));
-            if (t + 1 < tiles_n) load(r.k, t + 1, kw);
-            if (t >= 2 && !__all_sync(0xffffffffu, mbar_wait(v_empty + 8 * (t & 1), par, &s_failed))) break;
-            store(v_at + (t & 1) * C::KV_TILE, vw);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(v_full + 8 * (t & 1));
-        }
+        // ── conversion: 16 units of a 16-token block and 64 elements per tile; 4 warps for K, 3 for V ──
+        const int vw = warp - C::ISSUE - 1;
+        if (warp < C::ISSUE)
+            convert_tiles<D, 4>(r, r.k, b, h, t_begin, tiles_n, kv_end, 4 * (warp - C::CONV), 4 * (warp - C::CONV) + 4, k_at, k_full, k_empty, &s_failed);
+        else
+            convert_tiles<D, 6>(r, r.v, b, h, t_begin, tiles_n, kv_end, vw == 0 ? 0 : 5 * vw + 1, 5 * vw + 6, v_at, v_full, v_empty, &s_failed);
     }
 
     // ── the output rows: O / l through shared memory (the tiles are free once all products are done) ──
@@ -480,7 +558,7 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
             uint32_t x[32];
             if (tiles_n > 0 && fine) {
                 tc_ld32(o_at + 32 * c, x);
-                tc_wait_ld();
+                tc_wait_ld(x);
             } else {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) x[j] = 0;
@@ -496,7 +574,7 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == C::SOFT_WARPS) {
+    if (warp == C::ISSUE) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
