@@ -31,9 +31,10 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// one attempt, during which the thread may be suspended for up to about 10 us
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 10000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
@@ -56,9 +57,7 @@ __device__ __forceinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, vo
     return true;
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-        if (mbar_try(bar, parity)) return true;
+    if (mbar_try(bar, parity)) return true;
     return mbar_wait_long(bar, parity, failed);
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -341,6 +340,7 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
         const uint32_t o_at = lanes + o_col + qt * 128;
         const float f = s_f[row];
         const int lim = s_lim[row];
+        constexpr float TINY = 1e-38f;   // least factor of a sum: -inf stays -inf where f or ks is zero
         float m = -INFINITY, l = 0.0f;
         // scales of the tile's blocks, one per lane (lane & 7): loaded a tile ahead, their pages two tiles ahead
         constexpr int BPT = KT / 16, CH = KT / 32;
@@ -389,12 +389,16 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
 #pragma unroll
             for (int c = 1; c < CH; ++c) tc_loaded(raw[c]);
             if (edge) {
+                // few tiles: kept a branch (if-converted, these selects would cost every tile 2 instructions a score)
+                asm volatile("" ::: "memory");
 #pragma unroll
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const bool seen = tok0 + 32 * c + j <= lim && ((there >> (2 * c + j / 16)) & 1);
-                        raw[c][j] = seen ? raw[c][j] : 0xff800000u;   // -inf
+                    for (int bl = 0; bl < 2; ++bl) {
+                        const int left = (there >> (2 * c + bl)) & 1 ? lim - (tok0 + 32 * c + 16 * bl) : -1;   // last column seen
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (j > left) raw[c][16 * bl + j] = 0xff800000u;   // -inf
                     }
             }
             // the largest exponent, from each scale block's largest sum (f and ks are not negative)
@@ -406,8 +410,8 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
 #pragma unroll
                 for (int j = 3; j < 15; j += 2) y = max3(y, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
                 y = fmaxf(y, __uint_as_float(x[15]));
-                const float a = f * __shfl_sync(0xffffffffu, ks_l, c), lv = __shfl_sync(0xffffffffu, lv_l, c);
-                top = fmaxf(top, y == -INFINITY ? y : fmaf(y, a, lv));
+                const float a = fmaxf(f * __shfl_sync(0xffffffffu, ks_l, c), TINY), lv = __shfl_sync(0xffffffffu, lv_l, c);
+                top = fmaxf(top, fmaf(y, a, lv));
             }
             const bool move = top > m + Q8_SLACK;
             if (__any_sync(0xffffffffu, move)) {
@@ -440,17 +444,13 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
                 uint32_t p[16];
 #pragma unroll
                 for (int bl = 0; bl < 2; ++bl) {
-                    const float a = f * __shfl_sync(0xffffffffu, ks_l, 2 * c + bl);
+                    const float a = fmaxf(f * __shfl_sync(0xffffffffu, ks_l, 2 * c + bl), TINY);
                     const float lv = __shfl_sync(0xffffffffu, lv_l, 2 * c + bl) + ref;
                     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        const float x0 = __uint_as_float(raw[c][16 * bl + j]), x1 = __uint_as_float(raw[c][16 * bl + j + 1]);
-                        float2 e = __ffma2_rn(make_float2(x0, x1), make_float2(a, a), make_float2(lv, lv));
-                        if (edge && a == 0.0f) {   // -inf times a zero factor
-                            e.x = x0 == -INFINITY ? x0 : e.x;
-                            e.y = x1 == -INFINITY ? x1 : e.y;
-                        }
+                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(raw[c][16 * bl + j]), __uint_as_float(raw[c][16 * bl + j + 1])),
+                                                    make_float2(a, a), make_float2(lv, lv));
                         const float2 w = make_float2(ex2(e.x), ex2(e.y));
                         sum = __fadd2_rn(sum, w);
                         p[8 * bl + j / 2] = pack_h2(w.x, w.y);
