@@ -492,7 +492,7 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
     Q8Plan p;
     const int64_t rows = n * grp;
     p.prompt = rows >= PROMPT_ROWS;
-    p.rows = p.prompt ? (D == 128 ? 256 : 128) : (D == 128 && rows > 16 ? 32 : 16);
+    p.rows = p.prompt ? q8_prompt_rows(D) : (D == 128 && rows > 16 ? 32 : 16);
     p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = (int64_t)B * Hkv * p.row_tiles;
     const int64_t slots = (int64_t)sm_count() * (D == 128 && p.rows == 16 ? 2 : 1);
@@ -507,13 +507,16 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
         if (cost < best) { best = cost; p.splits = s; }
         if (waves > 8) break;   // finer splits only add starts
     }
+    if (p.prompt) q8_prompt_tiles((int64_t)B * Hkv, D, len, &p);
     return p;
 }
 
-size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p) {
+// work memory: the splits' partial rows and their lse, then a prompt's tiles
+static size_t part_bytes(int B, int Hkv, int D, const Q8Plan& p) {
     if (p.splits <= 1) return 0;
-    return (size_t)B * Hkv * p.row_tiles * p.splits * p.rows * (D + 1) * 4;
+    return ((size_t)B * Hkv * p.row_tiles * p.splits * p.rows * (D + 1) * 4 + 255) & ~size_t(255);
 }
+size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p) { return part_bytes(B, Hkv, D, p) + p.tile_bytes; }
 
 template <int D, int MT>
 static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
@@ -530,7 +533,7 @@ cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace
     float* part = static_cast<float*>(workspace);
     float* part_lse = part + (size_t)r.B * r.Hkv * p.row_tiles * p.splits * p.rows * r.D;
     cudaError_t e;
-    if (p.prompt) e = launch_attention_q8_prompt(r, p, part, part_lse, st);
+    if (p.prompt) e = launch_attention_q8_prompt(r, p, part, part_lse, static_cast<uint8_t*>(workspace) + part_bytes(r.B, r.Hkv, r.D, p), st);
     else if (r.D == 256) e = launch_rows<256, 1>(r, p, part, part_lse, st);
     else if (p.rows == 32) e = launch_rows<128, 2>(r, p, part, part_lse, st);
     else e = launch_rows<128, 1>(r, p, part, part_lse, st);

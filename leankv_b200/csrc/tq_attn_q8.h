@@ -25,6 +25,7 @@ struct Q8Run {
     int page_shift = 4;
     const int32_t* kv_len = nullptr;
     const int32_t* q_len = nullptr;   // null: n
+    int max_len = 0;                  // the caller's bound of kv_len
     float sm_scale = 0.0f;
     int causal = 1, rotate_q = 1, v_rotated = 1;
     float norm = 1.0f;             // 1 / sqrt(D) of the Hadamard transform
@@ -37,12 +38,17 @@ struct Q8Plan {
     int rows = 16;                 // query rows per unit
     int row_tiles = 1;             // units per (sequence, KV head)
     int splits = 1;
-    bool prompt = false;           // the tcgen05 kernel
+    bool prompt = false;           // the tcgen05 kernel:
+    int tiles_max = 0;             // tiles of a pair's tokens
+    int pairs_pass = 0;            // (sequence, KV head) pairs whose tiles the work memory holds at a time
+    size_t tile_bytes = 0;
 };
 
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len);
 size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p);
-cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st);
+int q8_prompt_rows(int D);
+void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p);
+cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st);
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st);
 
 }  // namespace tq

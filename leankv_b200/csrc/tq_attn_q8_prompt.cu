@@ -1,17 +1,25 @@
 // tq_attn_q8_prompt.cu — attention over 8-bit pages for prompts, on tcgen05.
 //
-// The mathematics is tq_attn_q8.cu's; with 128 or more query rows per KV head the two products bound it.
+// The mathematics is tq_attn_q8.cu's; with 100 or more query rows per KV head the two products bound it.  Two
+// kernels:
 //
-// A CTA takes QT tiles of 128 query rows (tokens x heads of one group) of one (sequence, KV head).  Warps:
-//   4 QT softmax warps   one thread per row: scores from TMEM, weights back to TMEM, the output's rescaling
-//   1 issuing warp       one thread issues all tcgen05.mma
-//   4 + 3 more warps     8-bit codes of K and V from the pages to f16 tiles in shared memory
+// expand_q8_kernel turns the codes that the rows will see into f16 tiles, once, in work memory: a tile is the image
+// of its shared-memory buffer, so that the second kernel fetches it with one bulk copy.  (Converted by warps of the
+// second kernel, every tile would be converted for each of a prompt's row tiles: 28 % of its instructions, 677
+// instead of XXX us for an 8192-token prompt.)  It also gathers what a block's scales contribute to the scores.
+//
+// attn_q8_prompt_kernel: a CTA takes QT tiles of 128 query rows (tokens x heads of one group) of one (sequence, KV
+// head).  Warps:
+//   8 QT softmax warps   two threads per row, half of a tile's columns each: scores from TMEM, weights back to
+//                        TMEM, the output's rescaling
+//   1 issuing warp       one elected lane issues all tcgen05.mma
+//   1 loading warp       one lane issues the bulk copies of K and V tiles
 // Per tile of KT tokens: S = Q K^T (both from shared memory, f16, fp32 sums in TMEM), weights P in f16 written
 // over S, O += P V (P from TMEM, V from shared memory).  D = 128: two row tiles of 128 tokens take turns, so that
 // one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).  D = 256: O alone
 // takes 256 columns and Q 64 KB, so one row tile takes 64 tokens at a time with two buffers for S.
 //
-// Shared tiles are runs of 64 elements: [row][128 bytes], 16-byte chunk c of row x at c ^ (x & 7) (the 128-byte
+// Tiles are runs of 64 elements: [row][128 bytes], 16-byte chunk c of row x at c ^ (x & 7) (the 128-byte
 // swizzle of the matrix descriptors).  K is read with its elements contiguous, V as the transposed operand from
 // the same layout.  Codes are exact in f16; scales never touch the tiles: they enter with the scores.
 //
@@ -60,20 +68,35 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     if (mbar_try(bar, parity)) return true;
     return mbar_wait_long(bar, parity, failed);
 }
+// waits for a bulk copy (at most the same time), whether or not another wait has run out
+__device__ __forceinline__ void mbar_wait_copy(uint32_t bar, uint32_t parity) {
+    const uint64_t until = now_ns() + WAIT_NS;
+    while (!mbar_try(bar, parity) && now_ns() < until) {
+    }
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The issuing warp runs converged and one elected lane issues: the operands then stay in uniform registers
+// (issued from a branch of one thread, each product waits for its operands to be moved there, 94 cycles a
+// product instead of the 64 that it takes).
+__device__ __forceinline__ uint32_t tc_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void tc_commit(uint32_t one, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %0, 0;\n\t"
+                 "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(one), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void tc_mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
 }
 // consecutive columns of this thread's TMEM lane; the wait takes the loaded registers, so that nothing that uses
 // them can be moved before it
@@ -143,6 +166,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// one thread: `bytes` from global to shared memory, counted by the barrier (with the thread's own arrival)
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 // Matrix descriptor of a 128-byte-swizzled tile: start and strides in 16-byte units.  stride: 8 rows (1024
 // bytes); lead: from one run of 64 elements to the next (used by the transposed operand only).
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead_bytes) {
@@ -157,89 +187,83 @@ template <int D> struct PromptCfg {
     static constexpr int SEGS = D / 64;                    // 64-element runs of a row
     static constexpr int Q_TILE = 128 * D * 2, KV_TILE = KT * D * 2, SEG = KT * 128;
     static constexpr int SBUF = 2;                         // S buffers: one per row tile, or two of one
-    static constexpr int SOFT_WARPS = 4 * QT, CONV = SOFT_WARPS, ISSUE = SOFT_WARPS + 4, WARPS = SOFT_WARPS + 8;
-    // D = 128: 16 warps start with 128 registers; the softmax takes 168 and the others keep 88 (2 x 168 + 2 x 88
-    // = 4 x 128 per warpgroup).  D = 256: 12 warps have 168 from the start.
-    static constexpr bool MOVE_REGS = QT == 2;
+    static constexpr int TPR = 2;                          // softmax threads per row
+    static constexpr int SOFT_WARPS = 4 * TPR * QT, ISSUE = SOFT_WARPS, LOAD = SOFT_WARPS + 1, WARPS = SOFT_WARPS + 2;
+    static constexpr int COLS = KT / TPR;                  // columns of a softmax thread
+    static constexpr int BPT = KT / 16;                    // scale blocks of a tile
     static constexpr int TILES = QT * Q_TILE + 4 * KV_TILE;   // Q, two K and two V buffers
     static constexpr int SMEM = TILES + 1024;              // the tiles start on 1024 bytes
 };
 
-// A converting warp: units [u0, u1) (at most NU) of every tile.  The next tile's codes are loaded while the
-// buffer is waited for, their pages a tile before that.
-template <int D, int NU>
-__device__ __forceinline__ void convert_tiles(const Q8Run& r, const int8_t* __restrict__ pool, int b, int h, int t_begin,
-                                              int tiles_n, int kv_end, int u0, int u1, uint32_t tile_at, uint32_t full,
-                                              uint32_t empty, volatile int* failed) {
+// ── codes to tiles ─────────────────────────────────────────────────────────
+// Work memory of the pairs (sequence, KV head) of one pass: K and V tiles [pair][tile][2][KV_TILE bytes], then the
+// blocks' factors [pair][tile][BPT] as float4 (K scale, log2 and reciprocal of the V scale): a score enters the
+// softmax as s * factor.x + factor.y, its weight counts factor.z.  Blocks that are not there (behind the last
+// token, pages outside the pool) get a log2 of -inf: their weights are 0.
+template <int D>
+__global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t pair0, int tiles_max, uint8_t* __restrict__ tiles,
+                                                        float4* __restrict__ factors) {
     using C = PromptCfg<D>;
-    constexpr int BPT = C::KT / 16;
-    const int lane = threadIdx.x & 31, sub = lane >> 2, c4 = lane & 3, per_page = r.page_shift - 4;
-    int page = -1;   // of unit u0 + lane
-    auto load_page = [&](int t) {
-        const int block = (t_begin + t) * BPT + (u0 + lane) / C::SEGS;
-        page = -1;
-        if (u0 + lane < u1 && t < tiles_n && block * 16 < kv_end)
-            page = r.pages[(int64_t)b * r.max_pages + (block >> per_page)];
-    };
-    uint4 w[NU][2];
-    auto load = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            const int pg = __shfl_sync(0xffffffffu, page, i), u = u0 + i;
-            const int block = (t_begin + t) * BPT + u / C::SEGS;
-            w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);   // tokens that are not there
-            if (pg >= 0 && pg < r.num_pages) {
-                const int64_t blk = (((int64_t)pg * r.Hkv + h) << per_page) + (block & ((1 << per_page) - 1));
-                const int8_t* p = pool + (blk * 16 + sub) * D + (u % C::SEGS) * 64 + 16 * c4;
-                w[i][0] = __ldg(reinterpret_cast<const uint4*>(p));
-                w[i][1] = __ldg(reinterpret_cast<const uint4*>(p + 8 * D));
-            }
-        }
-    };
-    load_page(0);
-    load(0);
-    load_page(1);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tile = blockIdx.x % tiles_max;
+    const int64_t slot = blockIdx.x / tiles_max, pair = pair0 + slot;
+    const int h = (int)(pair % r.Hkv), b = (int)(pair / r.Hkv);
+    const SeqLens sl = seq_lens(r, b);
+    if (tile * C::KT >= sl.len || sl.q_len == 0) return;   // tile < tiles_max by the grid
+    uint8_t* image = tiles + (slot * tiles_max + tile) * (2 * C::KV_TILE);
     const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1024 + 128
-    for (int t = 0; t < tiles_n; ++t) {
-        // the first pass over the two buffers does not wait
-        if (t >= 2 && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * (t & 1), ((t >> 1) & 1) ^ 1, failed))) break;
+    // a warp takes 8 rows x 64 elements (four lanes a row, 16 codes a lane) at a time
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane >> 2, c4 = lane & 3;
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            if (u0 + i >= u1) break;
-            const int u = u0 + i;
-            const uint32_t at = tile_at + (t & 1) * C::KV_TILE + (u % C::SEGS) * C::SEG + (u / C::SEGS) * 2048 + sub * 128;
+    for (int i = 0; i < C::KT / 8 * C::SEGS / 8; ++i) {
+        const int u = warp + 8 * i, seg = u % C::SEGS, row = u / C::SEGS * 8 + sub;
+        const int tok = tile * C::KT + row;
+        const int blk = (tok & ~15) < sl.len ? block_at(r, b, h, tok >> 4) : -1;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {   // rows sub and sub + 8 of the block
-                const uint32_t in[4] = {w[i][x].x ^ 0x80808080u, w[i][x].y ^ 0x80808080u, w[i][x].z ^ 0x80808080u, w[i][x].w ^ 0x80808080u};
-                uint32_t o[8];
+        for (int x = 0; x < 2; ++x) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (blk >= 0)
+                w = __ldg(reinterpret_cast<const uint4*>((x ? r.v : r.k) + ((int64_t)blk * 16 + (tok & 15)) * D + seg * 64 + 16 * c4));
+            const uint32_t in[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+            uint32_t o[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t v = __byte_perm(in[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140);
-                    const __half2 hv = __hsub2(*reinterpret_cast<__half2*>(&v), off);
-                    o[j] = *reinterpret_cast<const uint32_t*>(&hv);
-                }
-                sts128(at + x * 1024 + (((2 * c4) ^ sub) << 4), o[0], o[1], o[2], o[3]);
-                sts128(at + x * 1024 + (((2 * c4 + 1) ^ sub) << 4), o[4], o[5], o[6], o[7]);
+            for (int j = 0; j < 8; ++j) {
+                uint32_t v = __byte_perm(in[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140);
+                const __half2 hv = __hsub2(*reinterpret_cast<__half2*>(&v), off);
+                o[j] = *reinterpret_cast<const uint32_t*>(&hv);
+            }
+            uint8_t* to = image + x * C::KV_TILE + seg * C::SEG + row * 128;
+            *reinterpret_cast<uint4*>(to + (((2 * c4) ^ sub) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(to + (((2 * c4 + 1) ^ sub) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+    }
+    if (threadIdx.x < C::BPT) {
+        const int block = tile * C::BPT + threadIdx.x;
+        float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+        if (block * 16 < sl.len) {
+            const int blk = block_at(r, b, h, block);
+            if (blk >= 0) {
+                const float vs = r.vs[blk], vse = vs > 0.0f ? vs : 0x1p-100f;   // zero values: their weights still count
+                f = make_float4(r.ks[blk], lg2(vse), __frcp_rn(vse), 0.0f);
+            } else if (r.status) {
+                atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full + 8 * (t & 1));
-        if (t + 1 < tiles_n) {
-            load(t + 1);
-            load_page(t + 2);
-        }
+        factors[(slot * tiles_max + tile) * C::BPT + threadIdx.x] = f;
     }
 }
 
 template <int D>
 __global__ void __launch_bounds__(PromptCfg<D>::WARPS * 32, 1)
-attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ part, float* __restrict__ part_lse) {
+attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, const uint8_t* __restrict__ kv_tiles,
+                      const float4* __restrict__ factors, int row_tiles, int splits, float* __restrict__ part,
+                      float* __restrict__ part_lse) {
     using C = PromptCfg<D>;
-    constexpr int QT = C::QT, KT = C::KT, ROWS = C::ROWS, LPR = D / 16, THREADS = C::WARPS * 32;
+    constexpr int QT = C::QT, KT = C::KT, TPR = C::TPR, ROWS = C::ROWS, LPR = D / 16, THREADS = C::WARPS * 32;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[16];
-    __shared__ float s_f[ROWS], s_lse[ROWS];
+    __shared__ __align__(8) uint64_t bars[18];
+    __shared__ float s_f[ROWS], s_lse[ROWS], s_top[TPR == 2 ? 2 : 1][TPR == 2 ? ROWS : 1], s_sum[TPR == 2 ? 2 : 1][TPR == 2 ? ROWS : 1];
+    __shared__ __align__(16) float4 s_fac[4][C::BPT];   // blocks' factors of four tiles
     __shared__ int s_lim[ROWS];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
@@ -249,24 +273,30 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
     const uint32_t bar0 = smem_u32(bars);
     const uint32_t k_full = bar0, k_empty = bar0 + 16, v_full = bar0 + 32, v_empty = bar0 + 48;   // two each
     const uint32_t s_full = bar0 + 64, p_full = bar0 + 80, o_done = bar0 + 96, done = bar0 + 104;
+    const uint32_t f_full = bar0 + 112;   // four
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // units with the most tokens first: the last row tiles of a causal prompt see the longest prefix
     const int split = blockIdx.x % splits;
     const int64_t u = blockIdx.x / splits;
-    const int pairs = r.B * r.Hkv;
-    const int rt = row_tiles - 1 - (int)(u / pairs), pair = (int)(u % pairs), h = pair % r.Hkv, b = pair / r.Hkv;
+    const int rt = row_tiles - 1 - (int)(u / pairs), slot = (int)(u % pairs);
+    const int64_t pair = pair0 + slot;
+    const int h = (int)(pair % r.Hkv), b = (int)(pair / r.Hkv);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const SeqLens sl = seq_lens(r, b);
     const int total_rows = (int)r.n * r.grp, row0 = rt * ROWS;
     int last_i = (row0 + ROWS - 1) / r.grp;
     if (last_i >= sl.q_len) last_i = sl.q_len - 1;
     const int first_i = row0 / r.grp;
-    const int kv_end = last_i < first_i ? 0 : last_seen(r, sl, last_i) + 1;
+    int kv_end = last_i < first_i ? 0 : last_seen(r, sl, last_i) + 1;
+    if (kv_end > r.max_len) {   // longer than the caller's bound: the work memory has no tiles for it
+        kv_end = r.max_len;
+        if (threadIdx.x == 0 && r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
+    }
     const int all_tiles = (kv_end + KT - 1) / KT, per = (all_tiles + splits - 1) / splits;
     const int t_begin = split * per < all_tiles ? split * per : all_tiles;
     const int tiles_n = all_tiles - t_begin < per ? all_tiles - t_begin : per;
-    const int64_t unit = (int64_t)pair * row_tiles + rt;
+    const int64_t unit = pair * row_tiles + rt;
     if (tiles_n <= 0 && splits > 1) {
         for (int i = threadIdx.x; i < ROWS; i += THREADS) part_lse[(unit * splits + split) * ROWS + i] = -INFINITY;
         return;
@@ -275,13 +305,14 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
     if (threadIdx.x == 0) {
         s_failed = 0;
         for (int i = 0; i < 2; ++i) {
-            mbar_init(k_full + 8 * i, 4);     // the converting warps
-            mbar_init(v_full + 8 * i, 3);
+            mbar_init(k_full + 8 * i, 1);     // the loading lane, and the bytes of its copy
+            mbar_init(v_full + 8 * i, 1);
             mbar_init(k_empty + 8 * i, 1);    // commits of the issuing thread
             mbar_init(v_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 128);   // the rows' threads
+            mbar_init(p_full + 8 * i, 4 * TPR);   // the warps of a row tile
         }
+        for (int i = 0; i < 4; ++i) mbar_init(f_full + 8 * i, 1);
         mbar_init(o_done, 1);
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -324,61 +355,33 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the tiles are there
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     const uint32_t o_col = 256;   // S buffers at columns 0 and 128 (0 and 64), O from 256 on
 
-    if constexpr (C::MOVE_REGS) {   // by whole warpgroups, each at one instruction
-        if (warp < C::SOFT_WARPS) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    }
     if (warp < C::SOFT_WARPS) {
-        // ── softmax: thread = row ──
-        const int qt = warp >> 2, row = qt * 128 + (warp & 3) * 32 + lane;
+        // ── softmax: thread = half a row ──
+        const int qt = warp / (4 * TPR), half = TPR == 2 ? (warp >> 2) & 1 : 0, row = qt * 128 + (warp & 3) * 32 + lane;
+        const int pair_bar = 1 + qt * 4 + (warp & 3);   // barrier of the two warps of the same rows
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t o_at = lanes + o_col + qt * 128;
+        const uint32_t o_at = lanes + o_col + qt * 128 + half * (D / TPR);
         const float f = s_f[row];
         const int lim = s_lim[row];
         constexpr float TINY = 1e-38f;   // least factor of a sum: -inf stays -inf where f or ks is zero
         float m = -INFINITY, l = 0.0f;
-        // scales of the tile's blocks, one per lane (lane & 7): loaded a tile ahead, their pages two tiles ahead
-        constexpr int BPT = KT / 16, CH = KT / 32;
-        const int per_page = r.page_shift - 4;
-        float ks = 0.0f, vs = 0.0f;
-        int blk = -1, page = 0;
-        auto load_page = [&](int t) {
-            const int block = (t_begin + t) * BPT + (lane & (BPT - 1));
-            page = -2;   // no block
-            if (t < tiles_n && block * 16 < kv_end) page = r.pages[(int64_t)b * r.max_pages + (block >> per_page)];
-        };
-        auto load_scales = [&](int t) {
-            const int block = (t_begin + t) * BPT + (lane & (BPT - 1));
-            blk = -1;
-            ks = vs = 0.0f;
-            if (page >= 0 && page < r.num_pages) {
-                blk = (int)((((int64_t)page * r.Hkv + h) << per_page) + (block & ((1 << per_page) - 1)));
-                ks = r.ks[blk];
-                vs = r.vs[blk];
-            } else if (page != -2 && r.status) {
-                atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
-            }
-        };
-        load_page(0);
-        load_scales(0);
-        load_page(1);
+        bool ok = true;
+        constexpr int BPH = C::BPT / TPR, CH = C::COLS / 32;
         for (int t = 0; t < tiles_n; ++t) {
             const int sb = QT == 2 ? qt : (t & 1);
-            const uint32_t s_at = lanes + sb * KT;
-            const float ks_l = ks, vse = vs > 0.0f ? vs : 0x1p-100f;
-            const float lv_l = lg2(vse), iv_l = __frcp_rn(vse);
-            const uint32_t there = __ballot_sync(0xffffffffu, blk >= 0) & ((1u << BPT) - 1);
-            load_scales(t + 1);
-            load_page(t + 2);
-            const int tok0 = (t_begin + t) * KT;
-            const bool edge = __any_sync(0xffffffffu, tok0 + KT - 1 > lim) || there != (1u << BPT) - 1;
+            const uint32_t s_at = lanes + sb * KT + half * C::COLS, p_at = lanes + sb * KT + half * (C::COLS / 2);
+            const float4* fac = s_fac[t & 3] + half * BPH;   // factors of this thread's blocks
+            const int tok0 = (t_begin + t) * KT + half * C::COLS;
+            const bool edge = __any_sync(0xffffffffu, tok0 + C::COLS - 1 > lim);
             const uint32_t par = QT == 2 ? (t & 1) : ((t >> 1) & 1);
-            if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * sb, par, &s_failed))) break;
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(f_full + 8 * (t & 3), (t >> 2) & 1, &s_failed));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(s_full + 8 * sb, par, &s_failed));
             tc_fence_after();
 
             // the row's scores, in registers
@@ -395,7 +398,7 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
                     for (int bl = 0; bl < 2; ++bl) {
-                        const int left = (there >> (2 * c + bl)) & 1 ? lim - (tok0 + 32 * c + 16 * bl) : -1;   // last column seen
+                        const int left = lim - (tok0 + 32 * c + 16 * bl);   // last column seen
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
                             if (j > left) raw[c][16 * bl + j] = 0xff800000u;   // -inf
@@ -404,15 +407,27 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
             // the largest exponent, from each scale block's largest sum (f and ks are not negative)
             float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < BPT; ++c) {
+            for (int c = 0; c < BPH; ++c) {
                 const uint32_t* x = raw[c >> 1] + 16 * (c & 1);
                 float y = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
 #pragma unroll
                 for (int j = 3; j < 15; j += 2) y = max3(y, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
                 y = fmaxf(y, __uint_as_float(x[15]));
-                const float a = fmaxf(f * __shfl_sync(0xffffffffu, ks_l, c), TINY), lv = __shfl_sync(0xffffffffu, lv_l, c);
-                top = fmaxf(top, fmaf(y, a, lv));
+                const float2 fl = *reinterpret_cast<const float2*>(fac + c);
+                top = fmaxf(top, fmaf(y, fmaxf(f * fl.x, TINY), fl.y));
             }
+            if constexpr (TPR == 2) {
+                // The row's other half has its own maximum (never NaN: that says that a wait ran out there, and
+                // both halves leave here).  Past the barrier the other half has read its scores, too.
+                s_top[half][row] = ok ? top : NAN;
+                tc_fence_before();
+                asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+                tc_fence_after();
+                const float other = s_top[half ^ 1][row];
+                ok = !__any_sync(0xffffffffu, !ok || other != other);
+                top = fmaxf(top, other);
+            }
+            if (!ok) break;
             const bool move = top > m + Q8_SLACK;
             if (__any_sync(0xffffffffu, move)) {
                 const float now = move ? top : m;
@@ -423,11 +438,11 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
                     // the products up to the last tile's are done: with two row tiles this tile's scores were
                     // issued after them, else their own commit says so
                     if (QT == 1) {
-                        if (!__all_sync(0xffffffffu, mbar_wait(o_done, (t - 1) & 1, &s_failed))) break;
+                        ok = __all_sync(0xffffffffu, mbar_wait(o_done, (t - 1) & 1, &s_failed));   // false: out by next tile
                         tc_fence_after();
                     }
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
+                    for (int c = 0; c < D / TPR / 16; ++c) {   // this thread's columns of O
                         uint32_t x[16];
                         tc_ld16(o_at + 16 * c, x);
                         tc_wait_ld(x);
@@ -444,49 +459,60 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
                 uint32_t p[16];
 #pragma unroll
                 for (int bl = 0; bl < 2; ++bl) {
-                    const float a = fmaxf(f * __shfl_sync(0xffffffffu, ks_l, 2 * c + bl), TINY);
-                    const float lv = __shfl_sync(0xffffffffu, lv_l, 2 * c + bl) + ref;
+                    const float4 fl = fac[2 * c + bl];
+                    const float a = fmaxf(f * fl.x, TINY), y = fl.y + ref;
                     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         const float2 e = __ffma2_rn(make_float2(__uint_as_float(raw[c][16 * bl + j]), __uint_as_float(raw[c][16 * bl + j + 1])),
-                                                    make_float2(a, a), make_float2(lv, lv));
+                                                    make_float2(a, a), make_float2(y, y));
                         const float2 w = make_float2(ex2(e.x), ex2(e.y));
                         sum = __fadd2_rn(sum, w);
                         p[8 * bl + j / 2] = pack_h2(w.x, w.y);
                     }
-                    l = fmaf(sum.x + sum.y, __shfl_sync(0xffffffffu, iv_l, 2 * c + bl), l);
+                    l = fmaf(sum.x + sum.y, fl.z, l);
                 }
-                tc_st16(s_at + 16 * c, p);
+                tc_st16(p_at + 16 * c, p);
             }
             tc_wait_st();
             tc_fence_before();
-            mbar_arrive(p_full + 8 * sb);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 8 * sb);
         }
-        s_lse[row] = l > 0.0f ? (m - Q8_SHIFT + lg2(l)) * LN2 : -INFINITY;
-        s_f[row] = l > 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
+        if constexpr (TPR == 2) {
+            s_sum[half][row] = l;
+            asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+            l = s_sum[0][row] + s_sum[1][row];
+        }
+        if (half == 0) {
+            s_lse[row] = l > 0.0f ? (m - Q8_SHIFT + lg2(l)) * LN2 : -INFINITY;
+            s_f[row] = l > 0.0f ? __fdiv_rn(1.0f, l) : 0.0f;
+        }
     } else if (warp == C::ISSUE) {
         // ── issue ──
-        if (lane == 0 && tiles_n > 0) {
+        if (tiles_n > 0) {
             constexpr uint32_t id_s = mma_idesc(KT, 0), id_o = mma_idesc(D, 1);
+            const uint32_t one = tc_elect();
+            // descriptors count in 16 bytes; no tile crosses the address field's end
+            const uint64_t q_desc = tile_desc(q_at, 16), k_desc = tile_desc(k_at, 16), v_desc = tile_desc(v_at, C::SEG);
             bool ok = true;
             auto scores = [&](int qt, int t) {
-                const uint32_t q = q_at + qt * C::Q_TILE, k = k_at + (t & 1) * C::KV_TILE;
+                const uint64_t q = q_desc + qt * (C::Q_TILE >> 4), k = k_desc + (t & 1) * (C::KV_TILE >> 4);
                 const uint32_t d = tmem + (QT == 2 ? qt : (t & 1)) * KT;
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)
-                    tc_mma_ss(d, tile_desc(q + (j >> 2) * (128 * 128) + (j & 3) * 32, 16), tile_desc(k + (j >> 2) * C::SEG + (j & 3) * 32, 16),
-                              id_s, j > 0);
-                tc_commit(s_full + 8 * (QT == 2 ? qt : (t & 1)));
+                    tc_mma_ss(one, d, q + ((j >> 2) * (128 * 128 >> 4) + (j & 3) * 2), k + ((j >> 2) * (C::SEG >> 4) + (j & 3) * 2), id_s, j > 0);
+                tc_commit(one, s_full + 8 * (QT == 2 ? qt : (t & 1)));
             };
             auto values = [&](int qt, int t) {
-                const uint32_t p = tmem + (QT == 2 ? qt : (t & 1)) * KT, v = v_at + (t & 1) * C::KV_TILE;
+                const uint32_t p = tmem + (QT == 2 ? qt : (t & 1)) * KT;
+                const uint64_t v = v_desc + (t & 1) * (C::KV_TILE >> 4);
 #pragma unroll
                 for (int j = 0; j < KT / 16; ++j)
-                    tc_mma_ts(tmem + o_col + qt * 128, p + 8 * j, tile_desc(v + j * 2048, C::SEG), id_o, t > 0 || j > 0);
+                    tc_mma_ts(one, tmem + o_col + qt * 128, p + 8 * j, v + j * 128, id_o, t > 0 || j > 0);
             };
             auto full = [&](uint32_t bar, int t) {
-                ok = ok && mbar_wait(bar + 8 * (t & 1), (t >> 1) & 1, &s_failed);
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar + 8 * (t & 1), (t >> 1) & 1, &s_failed));
                 tc_fence_after();
                 return ok;
             };
@@ -494,20 +520,20 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
                 if (full(k_full, 0)) {
                     scores(0, 0);
                     scores(1, 0);
-                    tc_commit(k_empty);
+                    tc_commit(one, k_empty);
                 }
                 for (int t = 0; ok && t < tiles_n; ++t) {
                     if (!full(v_full, t)) break;
                     for (int qt = 0; qt < 2; ++qt) {
-                        ok = ok && mbar_wait(p_full + 8 * qt, t & 1, &s_failed);
+                        ok = ok && __all_sync(0xffffffffu, mbar_wait(p_full + 8 * qt, t & 1, &s_failed));
                         if (!ok) break;
                         tc_fence_after();
                         values(qt, t);
-                        if (qt == 1) tc_commit(v_empty + 8 * (t & 1));
+                        if (qt == 1) tc_commit(one, v_empty + 8 * (t & 1));
                         if (t + 1 < tiles_n) {
                             if (qt == 0 && !full(k_full, t + 1)) break;
                             scores(qt, t + 1);
-                            if (qt == 1) tc_commit(k_empty + 8 * ((t + 1) & 1));
+                            if (qt == 1) tc_commit(one, k_empty + 8 * ((t + 1) & 1));
                         }
                     }
                 }
@@ -515,30 +541,50 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
                 for (int t = 0; t < 2 && t < tiles_n; ++t)
                     if (full(k_full, t)) {
                         scores(0, t);
-                        tc_commit(k_empty + 8 * t);
+                        tc_commit(one, k_empty + 8 * t);
                     }
                 for (int t = 0; ok && t < tiles_n; ++t) {
                     if (!full(v_full, t) || !full(p_full, t)) break;
                     values(0, t);
-                    tc_commit(v_empty + 8 * (t & 1));
-                    tc_commit(o_done);
+                    tc_commit(one, v_empty + 8 * (t & 1));
+                    tc_commit(one, o_done);
                     if (t + 2 < tiles_n) {
                         if (!full(k_full, t + 2)) break;
                         scores(0, t + 2);
-                        tc_commit(k_empty + 8 * (t & 1));
+                        tc_commit(one, k_empty + 8 * (t & 1));
                     }
                 }
             }
-            tc_commit(done);
+            tc_commit(one, done);
         }
         __syncwarp();
     } else {
-        // ── conversion: 16 units of a 16-token block and 64 elements per tile; 4 warps for K, 3 for V ──
-        const int vw = warp - C::ISSUE - 1;
-        if (warp < C::ISSUE)
-            convert_tiles<D, 4>(r, r.k, b, h, t_begin, tiles_n, kv_end, 4 * (warp - C::CONV), 4 * (warp - C::CONV) + 4, k_at, k_full, k_empty, &s_failed);
-        else
-            convert_tiles<D, 6>(r, r.v, b, h, t_begin, tiles_n, kv_end, vw == 0 ? 0 : 5 * vw + 1, 5 * vw + 6, v_at, v_full, v_empty, &s_failed);
+        // ── load ──
+        if (lane == 0) {
+            const uint8_t* from = kv_tiles + ((int64_t)slot * tiles_max + t_begin) * (2 * C::KV_TILE);
+            const float4* fac = factors + ((int64_t)slot * tiles_max + t_begin) * C::BPT;
+            int nk = 0, nv = 0;   // copies begun
+            for (int t = 0; t < tiles_n; ++t, from += 2 * C::KV_TILE) {
+                const int buf = t & 1, par = ((t >> 1) & 1) ^ 1;   // the first pass over the two buffers does not wait
+                if (t >= 2 && !mbar_wait(k_empty + 8 * buf, par, &s_failed)) break;
+                // The factors' ring of four: a K buffer is free again when both row tiles' softmax is three tiles
+                // back, so the factors of four tiles back have been used.
+                bulk_load(smem_u32(s_fac[t & 3]), fac + t * C::BPT, C::BPT * 16, f_full + 8 * (t & 3));
+                bulk_load(k_at + buf * C::KV_TILE, from, C::KV_TILE, k_full + 8 * buf);
+                ++nk;
+                if (t >= 2 && !mbar_wait(v_empty + 8 * buf, par, &s_failed)) break;
+                bulk_load(v_at + buf * C::KV_TILE, from + C::KV_TILE, C::KV_TILE, v_full + 8 * buf);
+                ++nv;
+            }
+            // no copy is in flight when the CTA ends, whatever became of the other warps
+            for (int i = nk - 2; i < nk; ++i)
+                if (i >= 0) mbar_wait_copy(k_full + 8 * (i & 1), (i >> 1) & 1);
+            for (int i = nk - 4; i < nk; ++i)
+                if (i >= 0) mbar_wait_copy(f_full + 8 * (i & 3), (i >> 2) & 1);
+            for (int i = nv - 2; i < nv; ++i)
+                if (i >= 0) mbar_wait_copy(v_full + 8 * (i & 1), (i >> 1) & 1);
+        }
+        __syncwarp();
     }
 
     // ── the output rows: O / l through shared memory (the tiles are free once all products are done) ──
@@ -550,11 +596,11 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
     float* rows = reinterpret_cast<float*>(tiles);
     // chunk c (4 floats) of a row at c ^ (row & 7)
     if (warp < C::SOFT_WARPS) {
-        const int qt = warp >> 2, row = qt * 128 + (warp & 3) * 32 + lane;
+        const int qt = warp / (4 * TPR), half = TPR == 2 ? (warp >> 2) & 1 : 0, row = qt * 128 + (warp & 3) * 32 + lane;
         const uint32_t o_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + o_col + qt * 128;
         const float inv = s_f[row];
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = half * (D / TPR / 32); c < (half + 1) * (D / TPR / 32); ++c) {
             uint32_t x[32];
             if (tiles_n > 0 && fine) {
                 tc_ld32(o_at + 32 * c, x);
@@ -602,19 +648,52 @@ attn_q8_prompt_kernel(const Q8Run r, int row_tiles, int splits, float* __restric
     }
 }
 
+// Work memory: partial sums of split units, then the tiles and factors of one pass's pairs.
 template <int D>
-static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
+static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, uint8_t* tiles, cudaStream_t st) {
     using C = PromptCfg<D>;
     cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
-    const int64_t grid = (int64_t)r.B * r.Hkv * p.row_tiles * p.splits;
-    if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    attn_q8_prompt_kernel<D><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
-    return cudaGetLastError();
+    float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * p.tiles_max * (2 * C::KV_TILE));
+    const int64_t pairs = (int64_t)r.B * r.Hkv;
+    for (int64_t pair0 = 0; pair0 < pairs; pair0 += p.pairs_pass) {
+        const int now = (int)(pairs - pair0 < p.pairs_pass ? pairs - pair0 : p.pairs_pass);
+        const int64_t grid = (int64_t)now * p.row_tiles * p.splits, expand = (int64_t)now * p.tiles_max;
+        if (grid >= (int64_t(1) << 31) || expand >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
+        expand_q8_kernel<D><<<(unsigned)expand, 256, 0, st>>>(r, pair0, p.tiles_max, tiles, factors);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3(C::WARPS * 32);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
+                               (const float4*)factors, p.row_tiles, p.splits, part, part_lse);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
-cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
-    return r.D == 256 ? launch_prompt_d<256>(r, p, part, part_lse, st) : launch_prompt_d<128>(r, p, part, part_lse, st);
+cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st) {
+    uint8_t* t = static_cast<uint8_t*>(tiles);
+    return r.D == 256 ? launch_prompt_d<256>(r, p, part, part_lse, t, st) : launch_prompt_d<128>(r, p, part, part_lse, t, st);
+}
+
+int q8_prompt_rows(int D) { return D == 128 ? PromptCfg<128>::ROWS : PromptCfg<256>::ROWS; }
+
+// tiles of one pass: all pairs, or as many as 1 GiB holds
+void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p) {
+    const int kt = D == 128 ? PromptCfg<128>::KT : PromptCfg<256>::KT;
+    p->tiles_max = (int)((max_len + kt - 1) / kt);
+    const int64_t bytes = (int64_t)p->tiles_max * (4 * kt * D + kt);   // two f16 tiles, 16 bytes per 16 tokens
+    const int64_t most = bytes > 0 ? (int64_t(1) << 30) / bytes : pairs;
+    p->pairs_pass = (int)(most < 1 ? 1 : (most < pairs ? most : pairs));
+    p->tile_bytes = (size_t)bytes * p->pairs_pass;
 }
 
 }  // namespace tq

@@ -187,6 +187,7 @@ static tq_status q8_check(const tq_attention_q8_args* a, const tq_kv_pages* pg, 
     r->causal = a->causal != 0; r->rotate_q = a->rotate_q != 0; r->v_rotated = a->v_rotated != 0;
     r->norm = fwht_norm(a->head_dim);
     r->lse = a->lse; r->status = a->status;
+    r->max_len = (int)(a->max_kv_len > 0 ? a->max_kv_len : cap);
     *p = q8_plan(a->batch, a->n_kv_heads, (int)grp, a->head_dim, a->n_new, a->max_kv_len > 0 ? a->max_kv_len : cap);
     return TQ_SUCCESS;
 }
