@@ -49,12 +49,12 @@ template <int D, int MT> struct Q8Cfg {
     static constexpr int STAGES = D == 256 ? 3 : (MT == 1 ? 3 : 5);
     static constexpr int BLOCK = 16 * D;                       // bytes of one tensor's block
     static constexpr int RING = STAGES * 2 * BLOCK;            // per warp
-    static constexpr bool QREG = D == 128 && MT == 1;          // q' fragments stay in registers
+    static constexpr bool QREG = false;
     static constexpr int QBYTES = MT * NK * 512;
     static constexpr int MERGE = Q8_WARPS * ROWS * D * 4;      // the warps' sums, over the rings
     static constexpr int RINGS = Q8_WARPS * RING > MERGE ? Q8_WARPS * RING : MERGE;
     static constexpr int SMEM = RINGS + QBYTES + (2 * Q8_WARPS * ROWS + 4 * ROWS) * 4;
-    static constexpr int CTAS = QREG ? 2 : 1;
+    static constexpr int CTAS = D == 128 && MT == 1 ? 2 : 1;
 };
 
 // Four 8-bit codes of a word, biased by 128, as f16 subnormals (c + 128) 2^-24: elements 0, 1 and 2, 3.
@@ -106,7 +106,7 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
     const int mine = nblk_all > warp ? (nblk_all - warp + Q8_WARPS - 1) / Q8_WARPS : 0;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * C::RING;
     int nx_blk = -1, cu_blk = -1;                             // windows of 32 blocks, one per lane
-    float nx_ks = 0.0f, nx_vs = 0.0f, cu_ks = 0.0f, cu_vs = 0.0f;
+    float nx_ks = 0.0f, nx_vs = 0.0f, cu_ks = 0.0f, cu_lv = 0.0f, cu_iv = 0.0f;
     auto window = [&](int i) {                                // blocks i .. i + 31 of this warp
         nx_blk = -1;
         nx_ks = nx_vs = 0.0f;
@@ -120,26 +120,29 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
             }
         }
     };
+    // A block's 16-byte chunk c of token x in a 128-byte half is copied to chunk c ^ (x & 7) of half * 2048 + x * 128.
+    // A lane takes every 32nd chunk of the block; its places differ by constants and by the xor of constants.
+    const uint32_t to0 = D == 128 ? (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4)
+                                  : ((lane >> 3) & 1) * 2048 + (lane >> 4) * 128 + (((lane & 7) ^ (lane >> 4)) << 4);
+    uint32_t fill = ring;                                     // the stage that the next copies go to
     auto issue = [&](int i) {
         if (i < mine) {
             if ((i & 31) == 0) window(i);
             const int blk = __shfl_sync(0xffffffffu, nx_blk, i & 31);
             if (blk >= 0) {
-                const uint32_t dst = ring + (i % C::STAGES) * (2 * C::BLOCK);
-                const int8_t* kp = r.k + (int64_t)blk * C::BLOCK;
-                const int8_t* vp = r.v + (int64_t)blk * C::BLOCK;
-                // 16-byte chunk c of row (token) x of a 128-byte half lies at chunk c ^ (x & 7)
+                const int8_t* kp = r.k + (int64_t)blk * C::BLOCK + lane * 16;
+                const int8_t* vp = r.v + (int64_t)blk * C::BLOCK + lane * 16;
 #pragma unroll
                 for (int e = 0; e < C::BLOCK / 512; ++e) {
-                    const int id = lane + 32 * e, half = id >> 7, x = (id >> 3) & 15, c = id & 7;
-                    const uint32_t at = half * 2048 + x * 128 + ((c ^ (x & 7)) << 4);
-                    const int64_t from = (int64_t)x * D + half * 128 + c * 16;
-                    cp16(dst + at, kp + from);
-                    cp16(dst + C::BLOCK + at, vp + from);
+                    const uint32_t to = fill + e * (D == 128 ? 512 : 256) + (to0 ^ (D == 128 ? (e & 1) << 6 : ((2 * e) & 7) << 4));
+                    cp16(to, kp + e * 512);
+                    cp16(to + C::BLOCK, vp + e * 512);
                 }
             }
         }
         cp_commit();
+        fill += 2 * C::BLOCK;
+        if (fill == ring + C::RING) fill = ring;
     };
 #pragma unroll
     for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
@@ -223,14 +226,25 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
             for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
 
     // ── blocks of 16 tokens ──
+    uint32_t kt = ring - 2 * C::BLOCK;
     for (int i = 0; i < mine; ++i) {
         cp_wait<C::STAGES - 2>();
         __syncwarp();
-        if ((i & 31) == 0) { cu_blk = nx_blk; cu_ks = nx_ks; cu_vs = nx_vs; }
+        if ((i & 31) == 0) {
+            // a block of zero values takes the smallest scale: its weights still count
+            const float vse = nx_vs > 0.0f ? nx_vs : 0x1p-100f;
+            cu_blk = nx_blk;
+            cu_ks = nx_ks;
+            cu_lv = lg2(vse);
+            cu_iv = __frcp_rn(vse);
+        }
         issue(i + C::STAGES - 1);   // into the stage that was read in the last turn
+        kt += 2 * C::BLOCK;
+        if (kt == ring + C::RING) kt = ring;
         if (__shfl_sync(0xffffffffu, cu_blk, i & 31) < 0) continue;   // a page outside the pool holds nothing
-        const float ks = __shfl_sync(0xffffffffu, cu_ks, i & 31), vs = __shfl_sync(0xffffffffu, cu_vs, i & 31);
-        const uint32_t kt = ring + (i % C::STAGES) * (2 * C::BLOCK), vt = kt + C::BLOCK;
+        const float ks = __shfl_sync(0xffffffffu, cu_ks, i & 31), lv = __shfl_sync(0xffffffffu, cu_lv, i & 31);
+        const float iv = __shfl_sync(0xffffffffu, cu_iv, i & 31);
+        const uint32_t vt = kt + C::BLOCK;
 
         // scores: columns are tokens, n-tile 0 tokens 0..7, n-tile 1 tokens 8..15 (lane row g)
         float s[MT][2][4];
@@ -270,11 +284,8 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
             }
         }
 
-        // y = s * f ks + log2 vs (a block of zero values takes the smallest scale: its weights still count)
-        const float vse = vs > 0.0f ? vs : 0x1p-100f, lv = lg2(vse), iv = __frcp_rn(vse);
+        // y = s * f ks + log2 vs
         const int tok0 = (blk0 + warp + i * Q8_WARPS) << 4;
-        const bool edge = tok0 + 15 > lim_min;
-        bool over = false;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -283,22 +294,40 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float y = fmaf(s[mt][nt][2 * k + e], a, c);
-                        if (edge && tok0 + nt * 8 + 2 * t + e > lim[mt][k]) y = -INFINITY;
-                        s[mt][nt][2 * k + e] = y;
-                        over |= y > m[mt][k] + Q8_SLACK;
-                    }
+                    for (int e = 0; e < 2; ++e) s[mt][nt][2 * k + e] = fmaf(s[mt][nt][2 * k + e], a, c);
+            }
+        if (tok0 + 15 > lim_min) {
+            // the last blocks only: kept a branch
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int left = lim[mt][k] - tok0 - 2 * t;   // last column seen, from this lane's first
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (nt * 8 + e > left) s[mt][nt][2 * k + e] = -INFINITY;
+                }
+        }
+        float top[MT][2];
+        bool over = false;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                top[mt][k] = fmaxf(max3(s[mt][0][2 * k], s[mt][0][2 * k + 1], s[mt][1][2 * k]), s[mt][1][2 * k + 1]);
+                over |= top[mt][k] > m[mt][k] + Q8_SLACK;
             }
         if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    float top = fmaxf(fmaxf(s[mt][0][2 * k], s[mt][0][2 * k + 1]), fmaxf(s[mt][1][2 * k], s[mt][1][2 * k + 1]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float now = fmaxf(m[mt][k], top);
+                    float now = fmaxf(top[mt][k], __shfl_xor_sync(0xffffffffu, top[mt][k], 1));
+                    now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
+                    now = fmaxf(m[mt][k], now);
                     const float w = now == -INFINITY ? 1.0f : ex2(m[mt][k] - now);
                     m[mt][k] = now;
                     l[mt][k] *= w;
