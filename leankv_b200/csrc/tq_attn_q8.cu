@@ -4,12 +4,15 @@
 //   q' = H q (rotate_q),  s_j = sm_scale * sum_d q'_d c_jd * ks[j / 16],  p = softmax over the tokens it sees,
 //   o = sum_j p_j c'_jd * vs[j / 16],  out = H o (v_rotated).
 //
-// Work.  A unit is 16 or 32 query rows (tokens x heads of one group) of one (sequence, KV head); its tokens are
-// split over CTAs, and within a CTA over 8 warps that never wait for one another: a warp takes every 8th block
-// of 16 tokens (one scale block of K and V, 2 KB each at D = 128), which it copies into its own ring of
-// shared memory (cp.async, 16 bytes a lane).  Products are mma.sync m16n8k16 in f16 with fp32 accumulators:
-// with 1 to 40 rows per KV head the cache is read at memory speed, a tcgen05 tile (128 rows) would be mostly
-// empty, and its operands would have to go through shared memory once more after the conversion from 8 bits.
+// Work.  A unit is up to 40 (D = 256: 16) query rows (tokens x heads of one group) of one (sequence, KV head); its
+// tokens are split over CTAs, and within a CTA over 8 warps that never wait for one another: a warp takes every 8th
+// block of 16 tokens (one scale block of K and V, 2 KB each at D = 128), which it copies into its own ring of
+// shared memory (cp.async, 16 bytes a lane), converts once and multiplies with all rows of the unit.  Products are
+// mma.sync m16n8k16 in f16 with fp32 accumulators, the cache as the A operand (16 tokens x 16 elements of K, 16
+// elements x 16 tokens of V) and 8 rows as B: with the rows as A (16 of them), a decode step's 1 to 8 rows would
+// leave half or more of every product empty, and accumulators, weights and query fragments would take twice the
+// registers.  A tcgen05 tile (128 rows) would be emptier still, and its operands would have to go through shared
+// memory once more after the conversion from 8 bits.
 //
 // Numbers.  A row of q' is scaled by its largest element and rounded to f16.  Codes are integers of 8 bits and
 // exact in f16.  K codes enter the product as subnormals (c + 128) 2^-24: one byte permute for two values;
@@ -44,17 +47,16 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <int D, int MT> struct Q8Cfg {
-    static constexpr int ROWS = 16 * MT, NK = D / 16;
-    static constexpr int STAGES = D == 256 ? 3 : (MT == 1 ? 3 : 5);
+template <int D, int NT> struct Q8Cfg {
+    static constexpr int ROWS = 8 * NT, NK = D / 16;
+    static constexpr int CTAS = D == 128 && NT == 1 ? 2 : 1;   // per SM
+    static constexpr int STAGES = D == 256 || CTAS == 2 ? 3 : 5;
     static constexpr int BLOCK = 16 * D;                       // bytes of one tensor's block
     static constexpr int RING = STAGES * 2 * BLOCK;            // per warp
-    static constexpr bool QREG = false;
-    static constexpr int QBYTES = MT * NK * 512;
+    static constexpr int QBYTES = NT * NK * 256;
     static constexpr int MERGE = Q8_WARPS * ROWS * D * 4;      // the warps' sums, over the rings
     static constexpr int RINGS = Q8_WARPS * RING > MERGE ? Q8_WARPS * RING : MERGE;
     static constexpr int SMEM = RINGS + QBYTES + (2 * Q8_WARPS * ROWS + 4 * ROWS) * 4;
-    static constexpr int CTAS = D == 128 && MT == 1 ? 2 : 1;
 };
 
 // Four 8-bit codes of a word, biased by 128, as f16 subnormals (c + 128) 2^-24: elements 0, 1 and 2, 3.
@@ -64,11 +66,18 @@ __device__ __forceinline__ void bytes_sub(uint32_t w, uint32_t& lo, uint32_t& hi
     hi = __byte_perm(u, 0u, 0x4342);
 }
 
+// an 8 x 8 matrix of f16 pairs, transposed across the warp
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // One unit's share of tokens.  Partial results go to part / part_lse (splits > 1), else to out / lse.
-template <int D, int MT>
-__global__ void __launch_bounds__(Q8_THREADS, Q8Cfg<D, MT>::CTAS)
+template <int D, int NT>
+__global__ void __launch_bounds__(Q8_THREADS, Q8Cfg<D, NT>::CTAS)
 attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ part, float* __restrict__ part_lse) {
-    using C = Q8Cfg<D, MT>;
+    using C = Q8Cfg<D, NT>;
     constexpr int ROWS = C::ROWS, NK = C::NK, HALVES = D / 128, LPR = D / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* s_q = smem + C::RINGS;
@@ -147,9 +156,9 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
 #pragma unroll
     for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
 
-    // ── q': Hadamard, row maximum, f16, in the order of the mma's A fragments ──
+    // ── q': Hadamard, row maximum, f16, in the order of the mma's B fragments ──
     // k-step j = 8 half + jj of lane t covers elements 128 half + 32 t + 4 jj .. + 3 (so that a lane's K bytes
-    // are one run of 32), words a0, a2 = elements 0..1, 2..3 of row g; a1, a3 of row g + 8
+    // are one run of 32), words b0, b1 = elements 0..1, 2..3 of row g; two k-steps in 16 bytes
     for (int base = warp * (32 / LPR); base < ROWS; base += Q8_WARPS * (32 / LPR)) {
         const int row = base + lane / LPR, e0 = (lane % LPR) * 16;
         const int gr = row0 + row, i = gr / r.grp;
@@ -178,13 +187,10 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         }
 #pragma unroll
         for (int o = 1; o < LPR; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const int mt = row >> 4, rr = row & 15, half = e0 >> 7, tt = (e0 & 127) >> 5, jj0 = (e0 & 31) >> 2;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t* f = reinterpret_cast<uint32_t*>(s_q + ((mt * NK + half * 8 + jj0 + j) * 32 + (rr & 7) * 4 + tt) * 16);
-            f[rr >> 3] = w[2 * j];
-            f[2 + (rr >> 3)] = w[2 * j + 1];
-        }
+        const int half = e0 >> 7, tt = (e0 & 127) >> 5, j0 = half * 8 + ((e0 & 31) >> 2);
+        uint4* to = reinterpret_cast<uint4*>(s_q) + ((row >> 3) * (NK / 2) + j0 / 2) * 32 + (row & 7) * 4 + tt;
+        to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        to[32] = make_uint4(w[4], w[5], w[6], w[7]);
         if (lane % LPR == 0) {
             s_f[row] = top * r.sm_scale * LOG2E;
             s_s[row] = 128.0f * sum;
@@ -193,37 +199,29 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
     }
     __syncthreads();
 
-    uint32_t qf[C::QREG ? NK : 1][4];
     const uint32_t sq = (uint32_t)__cvta_generic_to_shared(s_q) + lane * 16;
-    if constexpr (C::QREG) {
+    // this lane's rows: columns 2t and 2t + 1 of each n-tile
+    float f[NT][2], fs[NT][2], m[NT][2], l[NT][2];
+    int lim_min = 0x7fffffff;
 #pragma unroll
-        for (int j = 0; j < NK; ++j) {
-            const uint4 w = lds128(sq + j * 512);
-            qf[j][0] = w.x; qf[j][1] = w.y; qf[j][2] = w.z; qf[j][3] = w.w;
-        }
-    }
-    float f[MT][2], fs[MT][2], m[MT][2], l[MT][2];
-    int lim[MT][2], lim_min = 0x7fffffff;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int row = mt * 16 + 8 * k + g;
-            f[mt][k] = s_f[row];
-            fs[mt][k] = s_f[row] * s_s[row];
-            lim[mt][k] = s_lim[row];
-            lim_min = lim[mt][k] < lim_min ? lim[mt][k] : lim_min;
-            m[mt][k] = -INFINITY;
-            l[mt][k] = 0.0f;
+        for (int e = 0; e < 2; ++e) {
+            const int row = nt * 8 + 2 * t + e;
+            f[nt][e] = s_f[row] * 0x1p24f;
+            fs[nt][e] = s_f[row] * s_s[row];
+            lim_min = s_lim[row] < lim_min ? s_lim[row] : lim_min;
+            m[nt][e] = -INFINITY;
+            l[nt][e] = 0.0f;
         }
     lim_min = __reduce_min_sync(0xffffffffu, lim_min);
-    float o[MT][2 * NK][4];
+    float o[NT][NK][4];   // m-tile i: elements 16 g + 2 i (words 0, 1) and 16 g + 2 i + 1 (words 2, 3) of each half
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 2 * NK; ++j)
+        for (int j = 0; j < NK; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) o[nt][j][e] = 0.0f;
 
     // ── blocks of 16 tokens ──
     uint32_t kt = ring - 2 * C::BLOCK;
@@ -246,40 +244,34 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         const float iv = __shfl_sync(0xffffffffu, cu_iv, i & 31);
         const uint32_t vt = kt + C::BLOCK;
 
-        // scores: columns are tokens, n-tile 0 tokens 0..7, n-tile 1 tokens 8..15 (lane row g)
-        float s[MT][2][4];
+        // scores: words 0, 1 of token g, words 2, 3 of token g + 8, for this lane's rows
+        float s[NT][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
 #pragma unroll
         for (int half = 0; half < HALVES; ++half) {
             uint32_t kw[2][8];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                const uint32_t row = kt + half * 2048 + (nt * 8 + g) * 128;
-                const uint4 x = lds128(row + (((2 * t) ^ g) << 4)), y = lds128(row + (((2 * t + 1) ^ g) << 4));
-                kw[nt][0] = x.x; kw[nt][1] = x.y; kw[nt][2] = x.z; kw[nt][3] = x.w;
-                kw[nt][4] = y.x; kw[nt][5] = y.y; kw[nt][6] = y.z; kw[nt][7] = y.w;
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t row = kt + half * 2048 + (x * 8 + g) * 128;
+                const uint4 u = lds128(row + (((2 * t) ^ g) << 4)), w = lds128(row + (((2 * t + 1) ^ g) << 4));
+                kw[x][0] = u.x; kw[x][1] = u.y; kw[x][2] = u.z; kw[x][3] = u.w;
+                kw[x][4] = w.x; kw[x][5] = w.y; kw[x][6] = w.z; kw[x][7] = w.w;
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t b0[2], b1[2];
-                bytes_sub(kw[0][j], b0[0], b1[0]);
-                bytes_sub(kw[1][j], b0[1], b1[1]);
+            for (int j = 0; j < 8; j += 2) {
+                uint32_t a0[4], a1[4];
+                bytes_sub(kw[0][j], a0[0], a0[2]);
+                bytes_sub(kw[1][j], a0[1], a0[3]);
+                bytes_sub(kw[0][j + 1], a1[0], a1[2]);
+                bytes_sub(kw[1][j + 1], a1[1], a1[3]);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    uint32_t a[4];
-                    if constexpr (C::QREG) {
-                        a[0] = qf[j][0]; a[1] = qf[j][1]; a[2] = qf[j][2]; a[3] = qf[j][3];
-                    } else {
-                        const uint4 w = lds128(sq + (mt * NK + half * 8 + j) * 512);
-                        a[0] = w.x; a[1] = w.y; a[2] = w.z; a[3] = w.w;
-                    }
-                    mma16816(s[mt][0], a, b0[0], b1[0]);
-                    mma16816(s[mt][1], a, b0[1], b1[1]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint4 q = lds128(sq + (nt * (NK / 2) + half * 4 + j / 2) * 512);
+                    mma16816(s[nt], a0, q.x, q.y);
+                    mma16816(s[nt], a1, q.z, q.w);
                 }
             }
         }
@@ -287,71 +279,65 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         // y = s * f ks + log2 vs
         const int tok0 = (blk0 + warp + i * Q8_WARPS) << 4;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const float a = f[mt][k] * ks * 0x1p24f, c = lv - fs[mt][k] * ks;
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) s[mt][nt][2 * k + e] = fmaf(s[mt][nt][2 * k + e], a, c);
+            for (int e = 0; e < 2; ++e) {
+                const float a = f[nt][e] * ks, c = fmaf(-fs[nt][e], ks, lv);
+                s[nt][e] = fmaf(s[nt][e], a, c);
+                s[nt][2 + e] = fmaf(s[nt][2 + e], a, c);
             }
         if (tok0 + 15 > lim_min) {
             // the last blocks only: kept a branch
             asm volatile("" ::: "memory");
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int left = lim[mt][k] - tok0 - 2 * t;   // last column seen, from this lane's first
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (nt * 8 + e > left) s[mt][nt][2 * k + e] = -INFINITY;
+                for (int e = 0; e < 2; ++e) {
+                    const int left = s_lim[nt * 8 + 2 * t + e] - tok0 - g;   // last token seen, from this lane's first
+                    if (left < 0) s[nt][e] = -INFINITY;
+                    if (left < 8) s[nt][2 + e] = -INFINITY;
                 }
         }
-        float top[MT][2];
         bool over = false;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                top[mt][k] = fmaxf(max3(s[mt][0][2 * k], s[mt][0][2 * k + 1], s[mt][1][2 * k]), s[mt][1][2 * k + 1]);
-                over |= top[mt][k] > m[mt][k] + Q8_SLACK;
-            }
+            for (int e = 0; e < 2; ++e) over |= fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + Q8_SLACK;
         if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float now = fmaxf(top[mt][k], __shfl_xor_sync(0xffffffffu, top[mt][k], 1));
-                    now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 2));
-                    now = fmaxf(m[mt][k], now);
-                    const float w = now == -INFINITY ? 1.0f : ex2(m[mt][k] - now);
-                    m[mt][k] = now;
-                    l[mt][k] *= w;
+                for (int e = 0; e < 2; ++e) {
+                    float now = fmaxf(s[nt][e], s[nt][2 + e]);
 #pragma unroll
-                    for (int j = 0; j < 2 * NK; ++j) {
-                        o[mt][j][2 * k] *= w;
-                        o[mt][j][2 * k + 1] *= w;
+                    for (int x = 4; x < 32; x *= 2) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, x));
+                    now = fmaxf(m[nt][e], now);
+                    const float w = now == -INFINITY ? 1.0f : ex2(m[nt][e] - now);
+                    m[nt][e] = now;
+                    l[nt][e] *= w;
+#pragma unroll
+                    for (int j = 0; j < NK; ++j) {
+                        o[nt][j][e] *= w;
+                        o[nt][j][2 + e] *= w;
                     }
                 }
         }
-        uint32_t pf[MT][4];
+        uint32_t pf[NT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const float ref = m[mt][k] == -INFINITY ? 0.0f : m[mt][k] - Q8_SHIFT;
-                const float p0 = ex2(s[mt][0][2 * k] - ref), p1 = ex2(s[mt][0][2 * k + 1] - ref);
-                const float p2 = ex2(s[mt][1][2 * k] - ref), p3 = ex2(s[mt][1][2 * k + 1] - ref);
-                l[mt][k] = fmaf((p0 + p1) + (p2 + p3), iv, l[mt][k]);
-                pf[mt][k] = pack_h2(p0, p1);
-                pf[mt][2 + k] = pack_h2(p2, p3);
+            for (int e = 0; e < 2; ++e) {
+                const float ref = m[nt][e] == -INFINITY ? 0.0f : m[nt][e] - Q8_SHIFT;
+                p[e] = ex2(s[nt][e] - ref);
+                p[2 + e] = ex2(s[nt][2 + e] - ref);
+                l[nt][e] = fmaf(p[e] + p[2 + e], iv, l[nt][e]);
             }
+            pf[nt][0] = transposed(pack_h2(p[0], p[1]));   // row g, tokens 2t, 2t + 1
+            pf[nt][1] = transposed(pack_h2(p[2], p[3]));   // tokens 2t + 8, 2t + 9
+        }
 
-        // out += P V: lane g's elements 16 g + j of each half (n-tile j), tokens 2t, 2t + 1, 2t + 8, 2t + 9
+        // out += V^T P: the lane's elements 16 g .. 16 g + 15 of each half, tokens 2t, 2t + 1, 2t + 8, 2t + 9
         const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
 #pragma unroll
         for (int half = 0; half < HALVES; ++half) {
@@ -365,20 +351,19 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
             }
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                uint32_t pr[4];   // byte pairs (token 2t, 2t + 1): elements 0, 1 | 2, 3; then tokens + 8
-                pr[0] = __byte_perm(vw[0][w], vw[1][w], 0x5140);
-                pr[1] = __byte_perm(vw[0][w], vw[1][w], 0x7362);
-                pr[2] = __byte_perm(vw[2][w], vw[3][w], 0x5140);
-                pr[3] = __byte_perm(vw[2][w], vw[3][w], 0x7362);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t sel = (e & 1) ? 0x4342 : 0x4140;
-                    uint32_t b0 = __byte_perm(pr[e >> 1], 0x64646464u, sel), b1 = __byte_perm(pr[2 + (e >> 1)], 0x64646464u, sel);
-                    const __half2 h0 = __hsub2(*reinterpret_cast<__half2*>(&b0), off), h1 = __hsub2(*reinterpret_cast<__half2*>(&b1), off);
-                    b0 = *reinterpret_cast<const uint32_t*>(&h0);
-                    b1 = *reinterpret_cast<const uint32_t*>(&h1);
+                for (int x = 0; x < 2; ++x) {   // elements 4 w + 2 x and the next
+                    const uint32_t sel = x ? 0x7362 : 0x5140;   // byte pairs (token 2t, 2t + 1) of two elements
+                    const uint32_t lo = __byte_perm(vw[0][w], vw[1][w], sel), hi = __byte_perm(vw[2][w], vw[3][w], sel);
+                    uint32_t a[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342),
+                                     __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][half * 16 + 4 * w + e], pf[mt], b0, b1);
+                    for (int e = 0; e < 4; ++e) {
+                        const __half2 hv = __hsub2(*reinterpret_cast<__half2*>(&a[e]), off);
+                        a[e] = *reinterpret_cast<const uint32_t*>(&hv);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][half * 8 + 2 * w + x], a, pf[nt][0], pf[nt][1]);
                 }
             }
         }
@@ -387,37 +372,35 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
 
     // ── the 8 warps' sums ──
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float x = l[mt][k];
-            x += __shfl_xor_sync(0xffffffffu, x, 1);
-            x += __shfl_xor_sync(0xffffffffu, x, 2);
-            if (t == 0) {
-                s_m[warp * ROWS + mt * 16 + 8 * k + g] = m[mt][k];
-                s_l[warp * ROWS + mt * 16 + 8 * k + g] = x;
+        for (int e = 0; e < 2; ++e) {
+            float x = l[nt][e];
+#pragma unroll
+            for (int y = 4; y < 32; y *= 2) x += __shfl_xor_sync(0xffffffffu, x, y);
+            if (g == 0) {
+                s_m[warp * ROWS + nt * 8 + 2 * t + e] = m[nt][e];
+                s_l[warp * ROWS + nt * 8 + 2 * t + e] = x;
             }
         }
     __syncthreads();   // every warp is done with its ring
-    // chunk c (4 floats) of a row at (c & ~7) | ((c ^ (4 row + (c >> 3))) & 7): no bank conflicts
+    // chunk c (4 floats) of a row at (c & ~7) | ((c ^ (row >> 1)) & 7): no bank conflicts
     float* sums = reinterpret_cast<float*>(smem);
     auto cell = [&](int w, int row, int c) {
-        return sums + ((w * ROWS + row) * (D / 4) + ((c & ~7) | ((c ^ (4 * row + (c >> 3))) & 7))) * 4;
+        return sums + ((w * ROWS + row) * (D / 4) + ((c & ~7) | ((c ^ (row >> 1)) & 7))) * 4;
     };
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int half = 0; half < HALVES; ++half)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)   // column 2t + e of n-tile j is element 16 (2t + e) + j
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int j = half * 16 + 4 * c;
-                        *reinterpret_cast<float4*>(cell(warp, mt * 16 + 8 * k + g, half * 32 + 8 * t + 4 * e + c)) =
-                            make_float4(o[mt][j][2 * k + e], o[mt][j + 1][2 * k + e], o[mt][j + 2][2 * k + e], o[mt][j + 3][2 * k + e]);
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    const int j = half * 8 + 2 * c;
+                    *reinterpret_cast<float4*>(cell(warp, nt * 8 + 2 * t + e, half * 32 + 4 * g + c)) =
+                        make_float4(o[nt][j][e], o[nt][j][2 + e], o[nt][j + 1][e], o[nt][j + 1][2 + e]);
+                }
     __syncthreads();
     for (int id = threadIdx.x; id < ROWS * (D / 4); id += Q8_THREADS) {
         const int row = id / (D / 4), c = id % (D / 4);
@@ -520,11 +503,18 @@ constexpr int PROMPT_ROWS = 96;
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
     Q8Plan p;
     const int64_t rows = n * grp;
+    if (rows == 0 || B == 0) return p;
     p.prompt = rows >= PROMPT_ROWS;
-    p.rows = p.prompt ? q8_prompt_rows(D) : (D == 128 && rows > 16 ? 32 : 16);
-    p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
+    if (p.prompt) {
+        p.rows = q8_prompt_rows(D);
+        p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
+    } else {   // as few units as the accumulators' registers allow, alike in size
+        const int most = D == 128 ? 40 : 16;
+        p.row_tiles = (int)((rows + most - 1) / most);
+        p.rows = (int)((rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles)) * 8;
+    }
     const int64_t units = (int64_t)B * Hkv * p.row_tiles;
-    const int64_t slots = (int64_t)sm_count() * (D == 128 && p.rows == 16 ? 2 : 1);
+    const int64_t slots = (int64_t)sm_count() * (D == 128 && p.rows == 8 ? 2 : 1);
     // Splits: a CTA's time is its tokens plus a start and a merge worth about `start` tokens; the grid runs in
     // waves of `slots` CTAs.  Take the number with the least waves * (tokens + start).
     const int64_t len = max_len > 0 ? max_len : 1, start = p.prompt ? 768 : 384;
@@ -547,14 +537,14 @@ static size_t part_bytes(int B, int Hkv, int D, const Q8Plan& p) {
 }
 size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p) { return part_bytes(B, Hkv, D, p) + p.tile_bytes; }
 
-template <int D, int MT>
+template <int D, int NT>
 static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
-    using C = Q8Cfg<D, MT>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    using C = Q8Cfg<D, NT>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)r.B * r.Hkv * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    attn_q8_kernel<D, MT><<<(unsigned)grid, Q8_THREADS, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
+    attn_q8_kernel<D, NT><<<(unsigned)grid, Q8_THREADS, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
     return cudaGetLastError();
 }
 
@@ -563,9 +553,12 @@ cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace
     float* part_lse = part + (size_t)r.B * r.Hkv * p.row_tiles * p.splits * p.rows * r.D;
     cudaError_t e;
     if (p.prompt) e = launch_attention_q8_prompt(r, p, part, part_lse, static_cast<uint8_t*>(workspace) + part_bytes(r.B, r.Hkv, r.D, p), st);
-    else if (r.D == 256) e = launch_rows<256, 1>(r, p, part, part_lse, st);
-    else if (p.rows == 32) e = launch_rows<128, 2>(r, p, part, part_lse, st);
-    else e = launch_rows<128, 1>(r, p, part, part_lse, st);
+    else if (r.D == 256) e = p.rows == 8 ? launch_rows<256, 1>(r, p, part, part_lse, st) : launch_rows<256, 2>(r, p, part, part_lse, st);
+    else if (p.rows == 8) e = launch_rows<128, 1>(r, p, part, part_lse, st);
+    else if (p.rows == 16) e = launch_rows<128, 2>(r, p, part, part_lse, st);
+    else if (p.rows == 24) e = launch_rows<128, 3>(r, p, part, part_lse, st);
+    else if (p.rows == 32) e = launch_rows<128, 4>(r, p, part, part_lse, st);
+    else e = launch_rows<128, 5>(r, p, part, part_lse, st);
     if (e != cudaSuccess || p.splits <= 1) return e;
     const int64_t rows = (int64_t)r.B * r.Hq * r.n, rpc = 128 / (r.D / 16);
     cudaLaunchConfig_t cfg = {};
