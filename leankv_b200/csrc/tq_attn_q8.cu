@@ -83,9 +83,9 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
     uint8_t* s_q = smem + C::RINGS;
     float* s_m = reinterpret_cast<float*>(s_q + C::QBYTES);   // [warp][row]
     float* s_l = s_m + Q8_WARPS * ROWS;
-    float* s_f = s_l + Q8_WARPS * ROWS;                       // row's factor of the scores (log2 domain)
-    float* s_s = s_f + ROWS;                                  // 128 * sum of the row's f16 q'
-    int* s_lim = reinterpret_cast<int*>(s_s + ROWS);          // last token seen
+    // a row's factor of the scores (log2 domain, for sums of codes times 2^-24), and that of 128 * sum of its q'
+    float2* s_f = reinterpret_cast<float2*>(s_l + Q8_WARPS * ROWS);
+    int* s_lim = reinterpret_cast<int*>(s_f + ROWS);          // last token seen
     float* s_lse = reinterpret_cast<float*>(s_lim + ROWS);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -192,8 +192,8 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         to[0] = make_uint4(w[0], w[1], w[2], w[3]);
         to[32] = make_uint4(w[4], w[5], w[6], w[7]);
         if (lane % LPR == 0) {
-            s_f[row] = top * r.sm_scale * LOG2E;
-            s_s[row] = 128.0f * sum;
+            const float fr = top * r.sm_scale * LOG2E;
+            s_f[row] = make_float2(fr * 0x1p24f, fr * 128.0f * sum);
             s_lim[row] = live ? last_seen(r, sl, i) : -1;
         }
     }
@@ -201,15 +201,13 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
 
     const uint32_t sq = (uint32_t)__cvta_generic_to_shared(s_q) + lane * 16;
     // this lane's rows: columns 2t and 2t + 1 of each n-tile
-    float f[NT][2], fs[NT][2], m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2];
     int lim_min = 0x7fffffff;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int row = nt * 8 + 2 * t + e;
-            f[nt][e] = s_f[row] * 0x1p24f;
-            fs[nt][e] = s_f[row] * s_s[row];
             lim_min = s_lim[row] < lim_min ? s_lim[row] : lim_min;
             m[nt][e] = -INFINITY;
             l[nt][e] = 0.0f;
@@ -279,13 +277,14 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         // y = s * f ks + log2 vs
         const int tok0 = (blk0 + warp + i * Q8_WARPS) << 4;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float a = f[nt][e] * ks, c = fmaf(-fs[nt][e], ks, lv);
-                s[nt][e] = fmaf(s[nt][e], a, c);
-                s[nt][2 + e] = fmaf(s[nt][2 + e], a, c);
-            }
+        for (int nt = 0; nt < NT; ++nt) {
+            const float4 fr = *reinterpret_cast<const float4*>(s_f + nt * 8 + 2 * t);   // rows 2t and 2t + 1
+            const float a0 = fr.x * ks, c0 = fmaf(-fr.y, ks, lv), a1 = fr.z * ks, c1 = fmaf(-fr.w, ks, lv);
+            s[nt][0] = fmaf(s[nt][0], a0, c0);
+            s[nt][1] = fmaf(s[nt][1], a1, c1);
+            s[nt][2] = fmaf(s[nt][2], a0, c0);
+            s[nt][3] = fmaf(s[nt][3], a1, c1);
+        }
         if (tok0 + 15 > lim_min) {
             // the last blocks only: kept a branch
             asm volatile("" ::: "memory");
