@@ -4,7 +4,7 @@
 //   q' = H q (rotate_q),  s_j = sm_scale * sum_d q'_d c_jd * ks[j / 16],  p = softmax over the tokens it sees,
 //   o = sum_j p_j c'_jd * vs[j / 16],  out = H o (v_rotated).
 //
-// Work.  A unit is up to 40 (D = 256: 16) query rows (tokens x heads of one group) of one (sequence, KV head); its
+// Work.  A unit is up to 24 (D = 256: 16) query rows (tokens x heads of one group) of one (sequence, KV head); its
 // tokens are split over CTAs, and within a CTA over 8 warps that never wait for one another: a warp takes every 8th
 // block of 16 tokens (one scale block of K and V, 2 KB each at D = 128), which it copies into its own ring of
 // shared memory (cp.async, 16 bytes a lane), converts once and multiplies with all rows of the unit.  Products are
@@ -507,16 +507,20 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
     if (p.prompt) {
         p.rows = q8_prompt_rows(D);
         p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
-    } else {   // as few units as the accumulators' registers allow, alike in size
-        const int most = D == 128 ? 40 : 16;
+    } else {
+        // As few units as the registers allow, alike in size.  More rows share a conversion, but 40 of them leave
+        // registers for 8 warps per SM only: 24 sequences of 5 x 8 rows, up to 9000 tokens: 131 us with 40, 118 to
+        // 128 us with 24, 130 us with 16.
+        const int most = D == 128 ? 24 : 16;
         p.row_tiles = (int)((rows + most - 1) / most);
         p.rows = (int)((rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles)) * 8;
     }
     const int64_t units = (int64_t)B * Hkv * p.row_tiles;
     const int64_t slots = (int64_t)sm_count() * (D == 128 && p.rows == 8 ? 2 : 1);
     // Splits: a CTA's time is its tokens plus a start and a merge worth about `start` tokens; the grid runs in
-    // waves of `slots` CTAs.  Take the number with the least waves * (tokens + start).
-    const int64_t len = max_len > 0 ? max_len : 1, start = p.prompt ? 768 : 384;
+    // waves of `slots` CTAs.  Take the number with the least waves * (tokens + start).  (16 x 32768 tokens, one
+    // row group each: 172 us with start = 1024, 179 us with 384.)
+    const int64_t len = max_len > 0 ? max_len : 1, start = p.prompt ? 768 : 1024;
     int64_t best = INT64_MAX;
     for (int s = 1; s <= 256; ++s) {
         const int64_t per = ((len + s - 1) / s + 127) / 128 * 128;
@@ -555,9 +559,7 @@ cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace
     else if (r.D == 256) e = p.rows == 8 ? launch_rows<256, 1>(r, p, part, part_lse, st) : launch_rows<256, 2>(r, p, part, part_lse, st);
     else if (p.rows == 8) e = launch_rows<128, 1>(r, p, part, part_lse, st);
     else if (p.rows == 16) e = launch_rows<128, 2>(r, p, part, part_lse, st);
-    else if (p.rows == 24) e = launch_rows<128, 3>(r, p, part, part_lse, st);
-    else if (p.rows == 32) e = launch_rows<128, 4>(r, p, part, part_lse, st);
-    else e = launch_rows<128, 5>(r, p, part, part_lse, st);
+    else e = launch_rows<128, 3>(r, p, part, part_lse, st);
     if (e != cudaSuccess || p.splits <= 1) return e;
     const int64_t rows = (int64_t)r.B * r.Hq * r.n, rpc = 128 / (r.D / 16);
     cudaLaunchConfig_t cfg = {};
