@@ -20,6 +20,7 @@
 
 #include "tq_common.cuh"
 #include "tq_kernels.h"
+#include "tq_near.cuh"
 #include "tq_rope.h"
 #include "tq_rows.cuh"
 
@@ -148,53 +149,97 @@ __device__ __forceinline__ void turn_neighbours(float (&v)[8], const float2* __r
     }
 }
 
-// Rotates token rows [r0, r1) of one head: an item is one row's pair of 8-element runs that turn into each
-// other (c and c + R / 16 runs on), or two runs that are only copied.  Every element is read and written by
-// one thread, so dst may be src.
-template <typename T>
-__device__ __forceinline__ void rope_rows(const T* __restrict__ src, int64_t src_tok, T* dst, int64_t dst_tok, int D,
-                                          const Rope& rope, const float2* __restrict__ tab, int64_t t0, int r0, int r1,
-                                          int lane, int lanes) {
+// Rotates `count` rows, `src_step` elements apart, row k by the angles of table row tab_row + k * tab_step: the
+// tokens of one head (tab_step 1) or the heads of one token (0).  An item is one row's pair of 8-element runs that
+// turn into each other (c and c + R / 16 runs on), or two runs that are only copied.  Every element is read and
+// written by one thread, so dst may be src.
+template <typename T, int BATCH>
+__device__ __forceinline__ void rope_rows(const T* __restrict__ src, int64_t src_step, T* dst, int64_t dst_step, int D,
+                                          const Rope& rope, const float2* __restrict__ tab, int count, int tab_row,
+                                          int tab_step, int lane, int lanes) {
     const int R = rope.rotary_dim, n8 = ((R >> 1) + 7) >> 3, half8 = R >> 4;
     const int per = (D + 15) >> 4;   // items per row
-    for (int it = lane; it < (r1 - r0) * per; it += lanes) {
-        const int row = r0 + it / per, c = it % per;
-        const T* s = src + (t0 + row) * src_tok;
-        T* d = dst + (t0 + row) * dst_tok;
-        float a[8], b[8];
-        if (c < half8 && !rope.interleaved) {
-            load8<T>(s + 8 * c, a);
-            load8<T>(s + 8 * c + (R >> 1), b);
-            float cs[8], sn[8];
-            angles8(tab, row, c, n8, cs, sn);
+    const int items = count * per;
+    // items of a lane: BATCH at a time, so that their loads are under way together
+    for (int first = lane; first < items; first += BATCH * lanes) {
+        Raw8<T> a[BATCH], b[BATCH];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = a[j], y = b[j];
-                a[j] = rot_lo(x, y, cs[j], sn[j]);
-                b[j] = rot_hi(x, y, cs[j], sn[j]);
+        for (int i = 0; i < BATCH; ++i) {
+            const int it = first + i * lanes;
+            if (it >= items) break;
+            const int k = it / per, c = it % per;
+            const T* s = src + k * src_step;
+            const T* d = dst + k * dst_step;
+            const bool apart = c < half8 && !rope.interleaved;
+            if (c >= half8 && s == d) continue;
+            const int lo = apart ? 8 * c : 16 * c, hi = apart ? 8 * c + (R >> 1) : 16 * c + 8;
+            a[i] = load_raw8<T>(s + lo);
+            if (hi < D) b[i] = load_raw8<T>(s + hi);
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int it = first + i * lanes;
+            if (it >= items) break;
+            const int k = it / per, c = it % per, row = tab_row + k * tab_step;
+            const T* s = src + k * src_step;
+            T* d = dst + k * dst_step;
+            if (c >= half8 && s == d) continue;
+            const bool apart = c < half8 && !rope.interleaved;
+            const int lo = apart ? 8 * c : 16 * c, hi = apart ? 8 * c + (R >> 1) : 16 * c + 8;
+            if (c >= half8) {
+                store_raw8<T>(d + lo, a[i]);
+                if (hi < D) store_raw8<T>(d + hi, b[i]);
+                continue;
             }
-            store8<T>(d + 8 * c, a);
-            store8<T>(d + 8 * c + (R >> 1), b);
-        } else if (c < half8) {
-            load8<T>(s + 16 * c, a);
-            load8<T>(s + 16 * c + 8, b);
-            turn_neighbours(a, tab, row, 2 * c, n8);
-            turn_neighbours(b, tab, row, 2 * c + 1, n8);
-            store8<T>(d + 16 * c, a);
-            store8<T>(d + 16 * c + 8, b);
-        } else if (s != d) {
-            load8<T>(s + 16 * c, a);
-            store8<T>(d + 16 * c, a);
-            if (16 * c + 8 < D) {
-                load8<T>(s + 16 * c + 8, b);
-                store8<T>(d + 16 * c + 8, b);
+            float x[8], y[8];
+            unpack8(a[i], x);
+            unpack8(b[i], y);
+            if (apart) {
+                float cs[8], sn[8];
+                angles8(tab, row, c, n8, cs, sn);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float u = x[j], w = y[j];
+                    x[j] = rot_lo(u, w, cs[j], sn[j]);
+                    y[j] = rot_hi(u, w, cs[j], sn[j]);
+                }
+            } else {
+                turn_neighbours(x, tab, row, 2 * c, n8);
+                turn_neighbours(y, tab, row, 2 * c + 1, n8);
             }
+            store8<T>(d + lo, x);
+            store8<T>(d + hi, y);
         }
     }
 }
 
+// The warp's share of a tile's rows [r0, r1) of `heads` heads: whole heads, or whole tokens where a token's heads
+// lie together in memory (a warp then reads a run of heads * D elements).
+template <typename T, int BATCH>
+__device__ __forceinline__ void rope_heads(const HeadRows& x, int b, int64_t t0, int r0, int r1, int h0, int h1, bool by_token,
+                                           int D, const Rope& rope, const float2* __restrict__ tab, int part, int parts) {
+    const int lane = threadIdx.x & 31;
+    const T* src = static_cast<const T*>(x.src) + b * x.ss[0] + t0 * x.ss[2];
+    T* dst = static_cast<T*>(x.dst) + b * x.ds[0] + t0 * x.ds[2];
+    if (by_token) {
+        for (int row = r0 + part; row < r1; row += parts)
+            rope_rows<T, BATCH>(src + row * x.ss[2] + h0 * x.ss[1], x.ss[1], dst + row * x.ds[2] + h0 * x.ds[1], x.ds[1], D, rope, tab,
+                                h1 - h0, row, 0, lane, 32);
+    } else {
+        for (int h = h0 + part; h < h1; h += parts)
+            rope_rows<T, BATCH>(src + r0 * x.ss[2] + h * x.ss[1], x.ss[2], dst + r0 * x.ds[2] + h * x.ds[1], x.ds[2], D, rope, tab,
+                                r1 - r0, r0, 1, lane, 32);
+    }
+}
+// tokens of one head lie further apart than the heads of one token
+__device__ __forceinline__ bool token_major(const HeadRows& x) { return x.ss[1] < x.ss[2] && x.ss[1] > 0; }
+
+// CTAs per SM: 64 registers are enough for bf16 (8192 tokens of 40 heads: 65 us, with 80 registers 73 us); the
+// conversions of f16 spill there (4551 tokens of 18 wide heads: 34 us, with 80 registers 25 us)
+template <typename T> constexpr int ROTARY_CTAS = std::is_same<T, __nv_bfloat16>::value ? 4 : 3;
+
 template <typename T>
-__global__ void __launch_bounds__(ROPE_THREADS) rotary_kernel(const RotaryRun r, int tiles, int groups, int per_group) {
+__global__ void __launch_bounds__(ROPE_THREADS, ROTARY_CTAS<T>) rotary_kernel(const RotaryRun r, int tiles, int groups, int per_group) {
     extern __shared__ __align__(16) uint8_t smem[];
     float2* tab = reinterpret_cast<float2*>(smem);
     const int g = blockIdx.x % groups, tile = (blockIdx.x / groups) % tiles, b = blockIdx.x / groups / tiles;
@@ -202,78 +247,140 @@ __global__ void __launch_bounds__(ROPE_THREADS) rotary_kernel(const RotaryRun r,
     const int rows = (int)(r.n_new - t0 < ROPE_TOKENS ? r.n_new - t0 : ROPE_TOKENS);
     fill_angles(tab, r.rope, b, r.batch, t0, r.n_new, 0);
     __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h0 = r.x[0].heads, total = h0 + r.x[1].heads;
-    const int end = (g + 1) * per_group < total ? (g + 1) * per_group : total;
-    for (int u = g * per_group + warp; u < end; u += ROPE_WARPS) {
-        const HeadRows& x = r.x[u >= h0];
-        const int h = u >= h0 ? u - h0 : u;
-        rope_rows<T>(static_cast<const T*>(x.src) + b * x.ss[0] + h * x.ss[1], x.ss[2],
-                     static_cast<T*>(x.dst) + b * x.ds[0] + h * x.ds[1], x.ds[2], r.head_dim, r.rope, tab, t0, 0, rows,
-                     lane, 32);
+    const int warp = threadIdx.x >> 5;
+    // heads [g per_group, ...) of the list x[0] | x[1]
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int first = i ? r.x[0].heads : 0;
+        int h0 = g * per_group - first, h1 = h0 + per_group;
+        h0 = h0 < 0 ? 0 : h0;
+        h1 = h1 > r.x[i].heads ? r.x[i].heads : h1;
+        if (h0 < h1)
+            rope_heads<T, 2>(r.x[i], b, t0, 0, rows, h0, h1, rows >= ROPE_WARPS && token_major(r.x[i]), r.head_dim,
+                                                  r.rope, tab, warp, ROPE_WARPS);
     }
 }
 
 // ── append ─────────────────────────────────────────────────────────────────
 
-// elements e .. e + 7 of a key row, turned: the partners are read from the row again (they sit in the L1)
-template <typename T>
-__device__ __forceinline__ void turned8(const T* __restrict__ row_ptr, int e, const Rope& rope,
-                                        const float2* __restrict__ tab, int row, int n8, float (&v)[8]) {
-    load8<T>(row_ptr + e, v);
-    const int R = rope.rotary_dim;
-    if (e >= R) return;
-    if (rope.interleaved) {
-        turn_neighbours(v, tab, row, e >> 3, n8);
-        return;
-    }
-    const int hi = e >= (R >> 1);
-    const int c = (hi ? e - (R >> 1) : e) >> 3;
-    float p[8], cs[8], sn[8];
-    load8<T>(row_ptr + (hi ? e - (R >> 1) : e + (R >> 1)), p);
-    angles8(tab, row, c, n8, cs, sn);
+// A lane holds elements 8 i .. 8 i + 7 and D / 2 + 8 i .. of a row (v[0 .. 7], v[8 .. 15]), so that the halves of a
+// pair (i, i + D / 2) meet in one lane.  Hadamard stages in the reference's order: h = 1, 2, 4 within 8 elements,
+// h = 8 .. D / 4 between lanes, h = D / 2 between the two runs; each a correctly rounded sum and difference, then
+// the factor 1 / sqrt(D).
+template <int D>
+__device__ __forceinline__ void fwht_halves(float (&v)[16], float norm) {
+    const float2 m1 = make_float2(-1.0f, -1.0f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = hi ? rot_hi(p[j], v[j], cs[j], sn[j]) : rot_lo(v[j], p[j], cs[j], sn[j]);
+    for (int j = 0; j < 16; j += 2) {
+        const float a = v[j], b = v[j + 1];
+        v[j] = __fadd_rn(a, b);
+        v[j + 1] = __fsub_rn(a, b);
+    }
+#pragma unroll
+    for (int h = 2; h < 8; h *= 2) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            if (j & h) continue;
+            const float2 a = make_float2(v[j], v[j + 1]), b = make_float2(v[j + h], v[j + h + 1]);
+            const float2 s = __fadd2_rn(a, b), d = __ffma2_rn(b, m1, a);
+            v[j] = s.x; v[j + 1] = s.y; v[j + h] = d.x; v[j + h + 1] = d.y;
+        }
+    }
+#pragma unroll
+    for (int bit = 1; bit < D / 16; bit *= 2) {
+        const float sg = (threadIdx.x & bit) ? -1.0f : 1.0f;   // lower: self + other, upper: other - self
+        const float2 sg2 = make_float2(sg, sg);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float p0 = __shfl_xor_sync(0xffffffffu, v[j], bit), p1 = __shfl_xor_sync(0xffffffffu, v[j + 1], bit);
+            const float2 s = __ffma2_rn(make_float2(v[j], v[j + 1]), sg2, make_float2(p0, p1));
+            v[j] = s.x; v[j + 1] = s.y;
+        }
+    }
+    const float2 n2 = make_float2(norm, norm);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const float2 a = make_float2(v[j], v[j + 1]), b = make_float2(v[j + 8], v[j + 9]);
+        const float2 s = __fmul2_rn(__fadd2_rn(a, b), n2), d = __fmul2_rn(__ffma2_rn(b, m1, a), n2);
+        v[j] = s.x; v[j + 1] = s.y; v[j + 8] = d.x; v[j + 9] = d.y;
+    }
 }
 
-// Packs the 16 codes of a lane (half `odd` of a 32-element block) into the staged block at blk.
+// elements e .. e + 7 of a key row, turned (any rotary_dim and pairing); a partner run is read from the row again
+template <typename T>
+__device__ __forceinline__ void turned8(const T* __restrict__ row_ptr, int e, const Rope& rope,
+                                        const float2* __restrict__ tab, int row, int n8, float* v8) {
+    float v[8];
+    load8<T>(row_ptr + e, v);
+    const int R = rope.rotary_dim;
+    if (e < R && rope.interleaved) {
+        turn_neighbours(v, tab, row, e >> 3, n8);
+    } else if (e < R) {
+        const int hi = e >= (R >> 1);
+        const int c = (hi ? e - (R >> 1) : e) >> 3;
+        float p[8], cs[8], sn[8];
+        load8<T>(row_ptr + (hi ? e - (R >> 1) : e + (R >> 1)), p);
+        angles8(tab, row, c, n8, cs, sn);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = hi ? rot_hi(p[j], v[j], cs[j], sn[j]) : rot_lo(v[j], p[j], cs[j], sn[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v8[j] = v[j];
+}
+
+// Packs this lane's 8 codes (elements 8 a .. 8 a + 7 of a 32-element block, a = lane & 3) into the staged block.
 template <int QT>
-__device__ __forceinline__ void stage_half_block(uint8_t* __restrict__ blk, const uint32_t (&code)[16], int odd,
-                                                 uint16_t d) {
-    if (!odd) *reinterpret_cast<uint16_t*>(blk) = d;
-    if constexpr (QT == 4) {   // byte j = code j | code j + 16 << 4: the even lane packs bytes 0..7, the odd 8..15
-        uint32_t lo = 0, hi = 0;
+__device__ __forceinline__ void stage_quarter_block(uint8_t* __restrict__ blk, const uint32_t* code, int a, uint16_t d) {
+    if (a == 0) *reinterpret_cast<uint16_t*>(blk) = d;
+    if constexpr (QT == 4) {
+        // byte j = code j | code j + 16 << 4: lanes a and a + 2 hold the nibbles of bytes 8 a .. 8 a + 7; the lower
+        // lane writes the first four of them, the upper lane the others
+        uint32_t own = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            lo |= code[j] << (4 * j);
-            hi |= code[8 + j] << (4 * j);
-        }
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
-        const uint32_t a = odd ? other : lo, b = odd ? hi : other;   // nibbles of elements j and j + 16
-        uint16_t* w = reinterpret_cast<uint16_t*>(blk + 2 + 8 * odd);
+        for (int j = 0; j < 8; ++j) own |= code[j] << (4 * j);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 2);
+        const uint32_t lo = (a < 2 ? own : other >> 16) & 0xFFFFu, hi = (a < 2 ? other : own >> 16) & 0xFFFFu;
+        uint16_t* w = reinterpret_cast<uint16_t*>(blk + 2 + 8 * (a & 1) + 4 * (a >> 1));
+        // nibbles n0 .. n3 of each to the low and high halves of four bytes
+        const uint32_t l0 = lo & 0xFFu, l1 = lo >> 8, h0 = hi & 0xFFu, h1 = hi >> 8;
+        w[0] = (uint16_t)((l0 & 15u) | ((h0 & 15u) << 4) | ((l0 >> 4) << 8) | ((h0 >> 4) << 12));
+        w[1] = (uint16_t)((l1 & 15u) | ((h1 & 15u) << 4) | ((l1 >> 4) << 8) | ((h1 >> 4) << 12));
+    } else if constexpr (QT == 3) {
+        // 24 bits at byte 3 a: an even lane writes its first two bytes and its last with the odd lane's first
+        uint32_t g = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t x = (a >> (8 * i)) & 0xFFu, y = (b >> (8 * i)) & 0xFFu;
-            w[i] = (uint16_t)((x & 15u) | ((y & 15u) << 4) | ((x >> 4) << 8) | ((y >> 4) << 12));
+        for (int j = 0; j < 8; ++j) g |= code[j] << (3 * j);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, g, 1);
+        uint16_t* w = reinterpret_cast<uint16_t*>(blk + 2 + 6 * (a >> 1));
+        if (a & 1) {
+            w[2] = (uint16_t)(g >> 8);
+        } else {
+            w[0] = (uint16_t)g;
+            w[1] = (uint16_t)((g >> 16) | ((other & 0xFFu) << 8));
         }
-    } else if constexpr (QT == 3) {   // two 24-bit groups of 8 codes
-        uint32_t g[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            g[0] |= code[j] << (3 * j);
-            g[1] |= code[8 + j] << (3 * j);
-        }
-        uint16_t* w = reinterpret_cast<uint16_t*>(blk + 2 + 6 * odd);
-        w[0] = (uint16_t)g[0];
-        w[1] = (uint16_t)((g[0] >> 16) | (g[1] << 8));
-        w[2] = (uint16_t)(g[1] >> 8);
     } else {
         uint32_t g = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) g |= code[j] << (2 * j);
-        uint16_t* w = reinterpret_cast<uint16_t*>(blk + 2 + 4 * odd);
-        w[0] = (uint16_t)g;
-        w[1] = (uint16_t)(g >> 16);
+        for (int j = 0; j < 8; ++j) g |= code[j] << (2 * j);
+        reinterpret_cast<uint16_t*>(blk + 2)[a] = (uint16_t)g;
+    }
+}
+
+// codes of 8 elements of a block whose maximum is amax; near: shared address of the level table, or 0 (few rows: the
+// comparisons cost less than the table)
+template <int QT>
+__device__ __forceinline__ void nearest8(const float* v, float amax, uint32_t near, uint32_t* code) {
+    const float inv = amax > 0.0f ? __fdiv_rn(1.0f, amax) : 0.0f;
+    if (near != 0 && inv != INFINITY) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+            near_pair(__fmul2_rn(make_float2(v[j], v[j + 1]), make_float2(inv, inv)), near, code[j], code[j + 1]);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float xn = __fmul_rn(v[j], inv);
+        code[j] = (uint32_t)(QT == 4 ? tq4_nearest(xn) : QT == 3 ? tq3_nearest(xn) : tq2_nearest(xn));
     }
 }
 
@@ -293,9 +400,9 @@ template <int D, typename T, int QT>
 __device__ __forceinline__ void append_unit(const RotaryAppendRun& r, const HeadRows& x, const PoolDst& dst, bool turn,
                                             int b, int h, int64_t slot0, int64_t t0, int ra, int rb, int older,
                                             const float2* __restrict__ tab, uint8_t* __restrict__ stage,
-                                            float* __restrict__ s_amax, int sub, int bar) {
+                                            float* __restrict__ s_amax, uint32_t near, int sub, int bar) {
     constexpr int LPR = D / 16, RPP = 32 / LPR, WPU = D / 128, RPW = 16 / WPU, PASSES = RPW / RPP;
-    const int lane = threadIdx.x & 31, lr = lane / LPR, le = (lane % LPR) * 16;
+    const int lane = threadIdx.x & 31, lr = lane / LPR, li = lane % LPR;
     const int64_t at = tile_rows_at(r, b, h, slot0);
     if (at < 0) {
         if (r.overflow && lane == 0 && sub == 0) atomicAdd(r.overflow, rb - ra);
@@ -303,41 +410,67 @@ __device__ __forceinline__ void append_unit(const RotaryAppendRun& r, const Head
     }
     const T* src = static_cast<const T*>(x.src) + b * x.ss[0] + h * x.ss[1] + t0 * x.ss[2];
     const int n8 = ((r.rope.rotary_dim >> 1) + 7) >> 3;
-
-    auto row_values = [&](int row, float (&v)[16]) {
-        float a[8], c[8];
+    // halves of the whole head turn into each other: the lane has both; else their runs are read where they lie
+    const bool halves = !turn || (r.rope.rotary_dim == D && !r.rope.interleaved);
+    auto has_rows = [&](int p) {   // the same for all lanes
+        const int base = sub * RPW + p * RPP;
+        return base + RPP > ra && base < rb;
+    };
+    auto load = [&](int p, Raw8<T>& lo, Raw8<T>& hi) {
+        const int row = sub * RPW + p * RPP + lr;
         if (row >= ra && row < rb) {
-            const T* p = src + row * x.ss[2];
-            if (turn) {
-                turned8<T>(p, le, r.rope, tab, row, n8, a);
-                turned8<T>(p, le + 8, r.rope, tab, row, n8, c);
-            } else {
-                load8<T>(p + le, a);
-                load8<T>(p + le + 8, c);
-            }
+            const T* q = src + row * x.ss[2] + 8 * li;
+            lo = load_raw8<T>(q);
+            hi = load_raw8<T>(q + D / 2);
+        }
+    };
+    auto values = [&](int p, const Raw8<T>& lo, const Raw8<T>& hi, float (&v)[16]) {
+        const int row = sub * RPW + p * RPP + lr;
+        if (row >= ra && row < rb) {
+            if (halves) {
+                float a[8], c[8];
+                unpack8(lo, a);
+                unpack8(hi, c);
+                if (turn) {
+                    float cs[8], sn[8];
+                    angles8(tab, row, li, n8, cs, sn);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { v[j] = a[j]; v[8 + j] = c[j]; }
+                    for (int j = 0; j < 8; ++j) {
+                        v[j] = rot_lo(a[j], c[j], cs[j], sn[j]);
+                        v[8 + j] = rot_hi(a[j], c[j], cs[j], sn[j]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) { v[j] = a[j]; v[8 + j] = c[j]; }
+                }
+            } else {
+                turned8<T>(src + row * x.ss[2], 8 * li, r.rope, tab, row, n8, v);
+                turned8<T>(src + row * x.ss[2], D / 2 + 8 * li, r.rope, tab, row, n8, v + 8);
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] = 0.0f;
         }
-        if (r.rotate) fwht16<D>(v, r.norm);
+        if (r.rotate) fwht_halves<D>(v, r.norm);
     };
 
     if constexpr (QT == 8) {
         float v[PASSES][16];
         float amax = 0.0f;
+        {
 #pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            const int base = sub * RPW + p * RPP;
-            if (base + RPP <= ra || base >= rb) {   // no new row in this pass (the same for all lanes)
+            for (int p = 0; p < PASSES; ++p) {
+                Raw8<T> lo, hi;
+                if (has_rows(p)) load(p, lo, hi);
+                if (!has_rows(p)) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[p][j] = 0.0f;
-                continue;
+                    for (int j = 0; j < 16; ++j) v[p][j] = 0.0f;
+                    continue;
+                }
+                values(p, lo, hi, v[p]);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(v[p][j]));
             }
-            row_values(base + lr, v[p]);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(v[p][j]));
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -361,67 +494,70 @@ __device__ __forceinline__ void append_unit(const RotaryAppendRun& r, const Head
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
             const int row = sub * RPW + p * RPP + lr;
-            uint4* cell = reinterpret_cast<uint4*>(pool + row * D + le);
-            if (row >= ra && row < rb) {
-                uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t acc = 0;
+            for (int half = 0; half < 2; ++half) {
+                uint2* cell = reinterpret_cast<uint2*>(pool + row * D + half * (D / 2) + 8 * li);
+                uint32_t w[2];
+                if (row >= ra && row < rb) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        int c = __float2int_rn(__fmul_rn(v[p][4 * i + j], inv));
-                        c = c < -127 ? -127 : (c > 127 ? 127 : c);
-                        acc |= (uint32_t)(c & 0xFF) << (8 * j);
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t acc = 0;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            int c = __float2int_rn(__fmul_rn(v[p][8 * half + 4 * i + j], inv));
+                            c = c < -127 ? -127 : (c > 127 ? 127 : c);
+                            acc |= (uint32_t)(c & 0xFF) << (8 * j);
+                        }
+                        w[i] = acc;
                     }
-                    w[i] = acc;
-                }
-                *cell = make_uint4(w[0], w[1], w[2], w[3]);
-            } else if (grow && row < older) {
-                const uint4 o = *cell;
-                const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
-                uint32_t w[4];
+                    *cell = make_uint2(w[0], w[1]);
+                } else if (grow && row < older) {
+                    const uint2 o = *cell;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t acc = 0;
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t acc = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int c = (int)(int8_t)(ow[i] >> (8 * j));
-                        acc |= (uint32_t)(__float2int_rn(__fmul_rn((float)c, ratio)) & 0xFF) << (8 * j);
+                        for (int j = 0; j < 4; ++j) {
+                            const int c = (int)(int8_t)((i ? o.y : o.x) >> (8 * j));
+                            acc |= (uint32_t)(__float2int_rn(__fmul_rn((float)c, ratio)) & 0xFF) << (8 * j);
+                        }
+                        w[i] = acc;
                     }
-                    w[i] = acc;
+                    *cell = make_uint2(w[0], w[1]);
                 }
-                *cell = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
-        if (lane == 0 && sub == 0 && s != s_old) *sp = s;
-        else if (lane == 0 && sub == 0 && older == 0) *sp = s;
+        if (lane == 0 && sub == 0 && (older == 0 || s != s_old)) *sp = s;
     } else {
         constexpr int BB = BlockBytes<QT>::value, ROWB = D / 32 * BB;
+        Raw8<T> lo, hi;
+        if (has_rows(0)) load(0, lo, hi);
 #pragma unroll 1
         for (int p = 0; p < PASSES; ++p) {
-            const int base = sub * RPW + p * RPP, row = base + lr;
-            if (base + RPP <= ra || base >= rb) continue;
             float v[16];
-            row_values(row, v);
-            float amax = 0.0f;
+            const bool some = has_rows(p);
+            if (some) values(p, lo, hi, v);
+            if (p + 1 < PASSES && has_rows(p + 1)) load(p + 1, lo, hi);   // the next rows, under this pass's search
+            if (!some) continue;
+            const int row = p * RPP + lr;   // staged row
 #pragma unroll
-            for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(v[j]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            const float inv = amax > 0.0f ? __fdiv_rn(1.0f, amax) : 0.0f;
-            uint32_t code[16];
+            for (int half = 0; half < 2; ++half) {
+                float amax = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float xn = __fmul_rn(v[j], inv);
-                code[j] = (uint32_t)(QT == 4 ? tq4_nearest(xn) : QT == 3 ? tq3_nearest(xn) : tq2_nearest(xn));
+                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[8 * half + j]));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                uint32_t code[8];
+                nearest8<QT>(v + 8 * half, amax, near, code);
+                stage_quarter_block<QT>(stage + row * ROWB + (half * (LPR / 4) + (li >> 2)) * BB, code, li & 3, half_trunc(amax));
             }
-            stage_half_block<QT>(stage + (row - sub * RPW) * ROWB + (le >> 5) * BB, code, (le >> 4) & 1, half_trunc(amax));
         }
         __syncwarp();
         // the new rows are consecutive slots of one page: one run of 8-byte words
-        const int lo = ra > sub * RPW ? ra : sub * RPW, hi = rb < (sub + 1) * RPW ? rb : (sub + 1) * RPW;
-        const uint2* from = reinterpret_cast<const uint2*>(stage + (lo - sub * RPW) * ROWB);
-        uint2* to = reinterpret_cast<uint2*>(dst.pool + (at + lo) * ROWB);
-        for (int i = lane; i < (hi - lo) * (ROWB / 8); i += 32) to[i] = from[i];
+        const int first = ra > sub * RPW ? ra : sub * RPW, last = rb < (sub + 1) * RPW ? rb : (sub + 1) * RPW;
+        const uint2* from = reinterpret_cast<const uint2*>(stage + (first - sub * RPW) * ROWB);
+        uint2* to = reinterpret_cast<uint2*>(dst.pool + (at + first) * ROWB);
+        for (int i = lane; i < (last - first) * (ROWB / 8); i += 32) to[i] = from[i];
         __syncwarp();
     }
 }
@@ -430,7 +566,7 @@ __device__ __forceinline__ void append_unit(const RotaryAppendRun& r, const Head
 // K heads | V heads | query heads.  The slot alignment gives an 8-bit scale block to one unit.
 template <int D, typename T, int KT>
 __global__ void __launch_bounds__(ROPE_THREADS, 2)
-rotary_append_kernel(const RotaryAppendRun r, int tiles, int groups, int per_group) {
+rotary_append_kernel(const RotaryAppendRun r, int tiles, int groups, int per_group, int tables) {
     constexpr int WPU = D / 128, VT = KT == 8 ? 8 : 4;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) uint8_t s_stage[KT == 8 ? 16 : ROPE_WARPS * STAGE_BYTES];
@@ -443,30 +579,40 @@ rotary_append_kernel(const RotaryAppendRun r, int tiles, int groups, int per_gro
     int64_t len = r.new_len ? r.new_len[b] : r.n_new;
     len = len < 0 ? 0 : (len > r.n_new ? r.n_new : len);
     const bool turn = r.rope.inv_freq != nullptr;
-    if (turn) {
-        fill_angles(tab, r.rope, b, r.batch, t0, r.n_new, pos);
-        __syncthreads();
+    if (turn) fill_angles(tab, r.rope, b, r.batch, t0, r.n_new, pos);
+    // level tables of the key and the value type behind the angles
+    uint32_t near_k = 0, near_v = 0;
+    if (KT != 8 && tables) {
+        uint2* t = reinterpret_cast<uint2*>(smem + tables);
+        near_table_init<KT == 8 ? 4 : KT, ROPE_THREADS>(t);
+        if (KT != 4) near_table_init<4, ROPE_THREADS>(t + NEAR_ROWS * NEAR_REP);
+        near_k = (uint32_t)__cvta_generic_to_shared(t) + 8u * (threadIdx.x & (NEAR_REP - 1));
+        near_v = near_k + (KT != 4 ? NEAR_ROWS * NEAR_REP * (uint32_t)sizeof(uint2) : 0u);
     }
+    __syncthreads();
     const int ra = t0 < 0 ? (int)-t0 : 0;
     const int rb = len - t0 < ROPE_TOKENS ? (int)(len - t0) : ROPE_TOKENS;        // stored rows of the tile
     const int rq = r.n_new - t0 < ROPE_TOKENS ? (int)(r.n_new - t0) : ROPE_TOKENS;   // query rows
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPU;
+    const int warp = threadIdx.x >> 5, sub = warp % WPU;
+    // heads [g per_group, ...) of the list K | V | queries
     const int Hkv = r.n_kv_heads, total = 2 * Hkv + r.q.heads;
-    const int end = (g + 1) * per_group < total ? (g + 1) * per_group : total;
-    for (int u = g * per_group + warp / WPU; u < end; u += ROPE_WARPS / WPU) {
+    const int first = g * per_group, end = first + per_group < total ? first + per_group : total;
+    const int slots = ROPE_WARPS / WPU, slot = warp / WPU;
+    for (int u = first + slot; u < end && u < 2 * Hkv; u += slots) {
         uint8_t* stage = s_stage + (KT == 8 ? 0 : warp * STAGE_BYTES);
         float* am = s_amax + (warp - sub);
-        const int bar = 1 + warp / WPU;
-        if (u < Hkv) {
-            if (ra < rb) append_unit<D, T, KT>(r, r.k, r.kd, turn, b, u, slot0, t0, ra, rb, ra, tab, stage, am, sub, bar);
-        } else if (u < 2 * Hkv) {
-            if (ra < rb) append_unit<D, T, VT>(r, r.v, r.vd, false, b, u - Hkv, slot0, t0, ra, rb, ra, tab, stage, am, sub, bar);
-        } else {
-            const int h = u - 2 * Hkv;
-            rope_rows<T>(static_cast<const T*>(r.q.src) + b * r.q.ss[0] + h * r.q.ss[1], r.q.ss[2],
-                         static_cast<T*>(r.q.dst) + b * r.q.ds[0] + h * r.q.ds[1], r.q.ds[2], D, r.rope, tab, t0, ra, rq,
-                         lane + 32 * sub, 32 * WPU);
-        }
+        const int bar = 1 + slot;
+        if (ra >= rb) continue;
+        if (u < Hkv) append_unit<D, T, KT>(r, r.k, r.kd, turn, b, u, slot0, t0, ra, rb, ra, tab, stage, am, near_k, sub, bar);
+        else append_unit<D, T, VT>(r, r.v, r.vd, false, b, u - Hkv, slot0, t0, ra, rb, ra, tab, stage, am, near_v, sub, bar);
+    }
+    const int h0 = first > 2 * Hkv ? first - 2 * Hkv : 0, h1 = end - 2 * Hkv;
+    if (h0 < h1) {
+        // the warps that have taken one K or V head fewer begin
+        const int taken = first < 2 * Hkv ? (2 * Hkv - first) % slots * WPU : 0;
+        const int part = (warp + ROPE_WARPS - taken) % ROPE_WARPS;
+        rope_heads<T, sizeof(T) == 2 ? 2 : 1>(r.q, b, t0, ra, rq, h0, h1, rq - ra >= ROPE_WARPS && token_major(r.q), D, r.rope, tab, part,
+                                              ROPE_WARPS);
     }
 }
 
@@ -526,13 +672,18 @@ static cudaError_t launch_append(const RotaryAppendRun& r, cudaStream_t st) {
     split_heads(tiles * r.batch, 2 * r.n_kv_heads + r.q.heads, ROPE_WARPS / (D / 128), groups, per);
     const int64_t grid = tiles * r.batch * groups;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    const size_t sm = angle_bytes(r.rope);
+    // The level tables (8 KB each) pay when a warp has units of full tiles to search: a 16384-token prompt of 8 + 8
+    // heads and 32 query heads took 119 us with them and 126 us without.  Steps of a few tokens take comparisons.
+    const size_t angles = (angle_bytes(r.rope) + 127) & ~size_t(127);
+    const bool table = r.kd.type != 8 && r.n_new >= ROPE_TOKENS;
+    const int at = table ? (int)(angles > 0 ? angles : 128) : 0;
+    const size_t sm = table ? at + (size_t)NEAR_ROWS * NEAR_REP * sizeof(uint2) * (r.kd.type == 4 ? 1 : 2) : angles;
     const unsigned gr = (unsigned)grid;
     switch (r.kd.type) {
-        case 2: rotary_append_kernel<D, T, 2><<<gr, ROPE_THREADS, sm, st>>>(r, (int)tiles, groups, per); break;
-        case 3: rotary_append_kernel<D, T, 3><<<gr, ROPE_THREADS, sm, st>>>(r, (int)tiles, groups, per); break;
-        case 4: rotary_append_kernel<D, T, 4><<<gr, ROPE_THREADS, sm, st>>>(r, (int)tiles, groups, per); break;
-        default: rotary_append_kernel<D, T, 8><<<gr, ROPE_THREADS, sm, st>>>(r, (int)tiles, groups, per); break;
+        case 2: rotary_append_kernel<D, T, 2><<<gr, ROPE_THREADS, sm, st>>>(r, (int)tiles, groups, per, at); break;
+        case 3: rotary_append_kernel<D, T, 3><<<gr, ROPE_THREADS, sm, st>>>(r, (int)tiles, groups, per, at); break;
+        case 4: rotary_append_kernel<D, T, 4><<<gr, ROPE_THREADS, sm, st>>>(r, (int)tiles, groups, per, at); break;
+        default: rotary_append_kernel<D, T, 8><<<gr, ROPE_THREADS, sm, st>>>(r, (int)tiles, groups, per, at); break;
     }
     return cudaGetLastError();
 }

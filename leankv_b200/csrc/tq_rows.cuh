@@ -6,23 +6,34 @@
 
 namespace tq {
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// 8 elements as loaded
+template <typename T> struct Raw8 { uint4 w[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+    return r;
 }
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+template <typename T>
+__device__ __forceinline__ void store_raw8(T* p, const Raw8<T>& r) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
+}
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&v)[8]) {
+    v[0] = __uint_as_float(r.w[0].x); v[1] = __uint_as_float(r.w[0].y); v[2] = __uint_as_float(r.w[0].z); v[3] = __uint_as_float(r.w[0].w);
+    v[4] = __uint_as_float(r.w[1].x); v[5] = __uint_as_float(r.w[1].y); v[6] = __uint_as_float(r.w[1].z); v[7] = __uint_as_float(r.w[1].w);
+}
+__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& r, float (&v)[8]) {
+    const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         v[2 * i] = __uint_as_float(u[i] << 16);
         v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
     }
 }
-template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void unpack8(const Raw8<__half>& r, float (&v)[8]) {
+    const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
@@ -30,6 +41,8 @@ template <> __device__ __forceinline__ void load8<__half>(const __half* p, float
         v[2 * i + 1] = f.y;
     }
 }
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) { unpack8(load_raw8<T>(p), v); }
 template <typename T> __device__ __forceinline__ void store8(T* p, const float (&v)[8]);
 template <> __device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
