@@ -517,15 +517,18 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
     }
     const int64_t units = (int64_t)B * Hkv * p.row_tiles;
     const int64_t slots = (int64_t)sm_count() * (D == 128 && p.rows == 8 ? 2 : 1);
-    // Splits: a CTA's time is its tokens plus a start and a merge worth about `start` tokens; the grid runs in
-    // waves of `slots` CTAs.  Take the number with the least waves * (tokens + start).  (16 x 32768 tokens, one
-    // row group each: 172 us with start = 1024, 179 us with 384.)
-    const int64_t len = max_len > 0 ? max_len : 1, start = p.prompt ? 768 : 1024;
+    // Splits: a CTA's time is its tokens plus a start worth `start` tokens and, when split, the writing and merging of
+    // its partial rows worth `join`; the grid runs in waves of `slots` CTAs.  Take the number with the least
+    // waves * (tokens + start).  Two CTAs share an SM and hide each other's starts where units have 8 rows
+    // (16 x 32768 tokens: 172 us with 1024, 179 us with 384); with one CTA per SM, lengths that differ want more and
+    // shorter splits (24 sequences of up to 9000 tokens, 40 rows: 118 us with 384, 129 us with 1024).
+    const int64_t len = max_len > 0 ? max_len : 1;
+    const int64_t start = p.prompt ? 768 : (slots > sm_count() ? 1024 : 384), join = p.prompt ? 512 : 0;
     int64_t best = INT64_MAX;
     for (int s = 1; s <= 256; ++s) {
         const int64_t per = ((len + s - 1) / s + 127) / 128 * 128;
         if (s > 1 && (int64_t)(s - 1) * per >= len) continue;   // the last split would be empty
-        const int64_t waves = (units * s + slots - 1) / slots, cost = waves * (per + start);
+        const int64_t waves = (units * s + slots - 1) / slots, cost = waves * (per + start + (s > 1 ? join : 0));
         if (cost < best) { best = cost; p.splits = s; }
         if (waves > 8) break;   // finer splits only add starts
     }

@@ -256,7 +256,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     using C = PromptCfg<D>;
     constexpr int QT = C::QT, KT = C::KT, TPR = C::TPR, ROWS = C::ROWS, LPR = D / 16, THREADS = C::WARPS * 32;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[18];
+    __shared__ __align__(8) uint64_t bars[20];
     __shared__ float s_f[ROWS], s_lse[ROWS], s_top[TPR == 2 ? 2 : 1][TPR == 2 ? ROWS : 1], s_sum[TPR == 2 ? 2 : 1][TPR == 2 ? ROWS : 1];
     __shared__ __align__(16) float4 s_fac[4][C::BPT];   // blocks' factors of four tiles
     __shared__ int s_lim[ROWS];
@@ -268,7 +268,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     const uint32_t bar0 = smem_u32(bars);
     const uint32_t k_full = bar0, k_empty = bar0 + 16, v_full = bar0 + 32, v_empty = bar0 + 48;   // two each
     const uint32_t s_full = bar0 + 64, p_full = bar0 + 80, o_done = bar0 + 96, done = bar0 + 104;
-    const uint32_t f_full = bar0 + 112;   // four
+    const uint32_t f_full = bar0 + 112, turn = bar0 + 144;   // four, two
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // units with the most tokens first: the last row tiles of a causal prompt see the longest prefix
@@ -306,6 +306,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
             mbar_init(v_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_full + 8 * i, 4 * TPR);   // the warps of a row tile
+            mbar_init(turn + 8 * i, 4 * TPR);     // the other tile's warps
         }
         for (int i = 0; i < 4; ++i) mbar_init(f_full + 8 * i, 1);
         mbar_init(o_done, 1);
@@ -447,27 +448,49 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
                     }
                 }
             }
-            // weights 2^(s + log2 vs - m + SHIFT) in f16 over the scores, 32 of them in 16 columns
+            // Weights 2^(s + log2 vs - m + SHIFT) in f16 over the scores, 32 of them in 16 columns.  The two row tiles
+            // make theirs in turn: the special function unit, which bounds them, then works for one while the other
+            // one's products run (left to themselves, both tiles fall into step and wait for each unit together).
+            if constexpr (QT == 2) {
+                if (qt == 1 || t > 0)
+                    ok = __all_sync(0xffffffffu, mbar_wait(turn + 8 * qt, qt == 1 ? t & 1 : (t - 1) & 1, &s_failed));   // false: out by next tile
+            }
             const float ref = m == -INFINITY ? 0.0f : Q8_SHIFT - m;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 uint32_t p[16];
+                float e[32];
 #pragma unroll
                 for (int bl = 0; bl < 2; ++bl) {
                     const float4 fl = fac[2 * c + bl];
                     const float a = fmaxf(f * fl.x, TINY), y = fl.y + ref;
-                    float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(raw[c][16 * bl + j]), __uint_as_float(raw[c][16 * bl + j + 1])),
+                    for (int j = 16 * bl; j < 16 * bl + 16; j += 2) {
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[c][j]), __uint_as_float(raw[c][j + 1])),
                                                     make_float2(a, a), make_float2(y, y));
-                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
-                        sum = __fadd2_rn(sum, w);
-                        p[8 * bl + j / 2] = pack_h2(w.x, w.y);
+                        e[j] = x.x;
+                        e[j + 1] = x.y;
                     }
-                    l = fmaf(sum.x + sum.y, fl.z, l);
                 }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) e[j] = ex2(e[j]);
+#pragma unroll
+                for (int bl = 0; bl < 2; ++bl) {
+                    float2 s0 = make_float2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+                    for (int j = 16 * bl; j < 16 * bl + 16; j += 4) {
+                        s0 = __fadd2_rn(s0, make_float2(e[j], e[j + 1]));
+                        s1 = __fadd2_rn(s1, make_float2(e[j + 2], e[j + 3]));
+                    }
+                    l = fmaf((s0.x + s0.y) + (s1.x + s1.y), fac[2 * c + bl].z, l);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) p[j] = pack_h2(e[2 * j], e[2 * j + 1]);
                 tc_st16(p_at + 16 * c, p);
+            }
+            if constexpr (QT == 2) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(turn + 8 * (qt ^ 1));
             }
             tc_wait_st();
             tc_fence_before();
