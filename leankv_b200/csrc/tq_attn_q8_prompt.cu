@@ -293,6 +293,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     const int tiles_n = all_tiles - t_begin < per ? all_tiles - t_begin : per;
     const int64_t unit = pair * row_tiles + rt;
     if (tiles_n <= 0 && splits > 1) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");   // this grid does not end before the tiles' kernel
         for (int i = threadIdx.x; i < ROWS; i += THREADS) part_lse[(unit * splits + split) * ROWS + i] = -INFINITY;
         return;
     }
