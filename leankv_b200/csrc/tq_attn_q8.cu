@@ -497,15 +497,16 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int r
 
 // ── plan and launch ────────────────────────────────────────────────────────
 
-constexpr int PROMPT_ROWS = 96;
+constexpr int DIRECT_ROWS = 25, PROMPT_ROWS = 129;
 
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
     Q8Plan p;
     const int64_t rows = n * grp;
     if (rows == 0 || B == 0) return p;
-    p.prompt = rows >= PROMPT_ROWS;
+    p.prompt = rows >= DIRECT_ROWS;
+    p.direct = rows < PROMPT_ROWS;
     if (p.prompt) {
-        p.rows = q8_prompt_rows(D);
+        p.rows = q8_prompt_rows(D, p.direct);
         p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     } else {
         // As few units as the registers allow, alike in size.  More rows share a conversion, but 40 of them leave
@@ -532,7 +533,7 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
         if (cost < best) { best = cost; p.splits = s; }
         if (waves > 8) break;   // finer splits only add starts
     }
-    if (p.prompt) q8_prompt_tiles((int64_t)B * Hkv, D, len, &p);
+    if (p.prompt && !p.direct) q8_prompt_tiles((int64_t)B * Hkv, D, len, &p);
     return p;
 }
 

@@ -39,6 +39,7 @@ struct Q8Plan {
     int row_tiles = 1;             // units per (sequence, KV head)
     int splits = 1;
     bool prompt = false;           // the tcgen05 kernel:
+    bool direct = false;           // which converts codes itself, or reads tiles from the work memory:
     int tiles_max = 0;             // tiles of a pair's tokens
     int pairs_pass = 0;            // (sequence, KV head) pairs whose tiles the work memory holds at a time
     size_t tile_bytes = 0;
@@ -46,7 +47,7 @@ struct Q8Plan {
 
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len);
 size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p);
-int q8_prompt_rows(int D);
+int q8_prompt_rows(int D, bool direct);
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p);
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st);
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st);

@@ -152,6 +152,12 @@ __device__ __forceinline__ void tc_st32(uint32_t a, const uint32_t (&v)[32]) {
                  "r"(v[29]), "r"(v[30]), "r"(v[31])
                  : "memory");
 }
+// a read-only load that stays where it is written
+__device__ __forceinline__ uint4 ldg_now(const int8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 // ties loaded registers to the place after their wait
 __device__ __forceinline__ void tc_loaded(uint32_t (&v)[32]) {
     asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
@@ -177,18 +183,38 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead_bytes
 // f16 operands, fp32 sums, M = 128; tb: B is stored with its N dimension contiguous
 constexpr uint32_t mma_idesc(int n, int tb) { return (1u << 4) | ((uint32_t)tb << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
 
-template <int D> struct PromptCfg {
-    static constexpr int QT = D == 128 ? 2 : 1, KT = D == 128 ? 128 : 64, ROWS = 128 * QT;
+// DIRECT: codes are converted by warps of the kernel itself
+template <int D, bool DIRECT> struct PromptCfg {
+    static constexpr int QT = D == 128 && !DIRECT ? 2 : 1, KT = D == 128 ? 128 : 64, ROWS = 128 * QT;
     static constexpr int SEGS = D / 64;                    // 64-element runs of a row
     static constexpr int Q_TILE = 128 * D * 2, KV_TILE = KT * D * 2, SEG = KT * 128;
     static constexpr int SBUF = 2;                         // S buffers: one per row tile, or two of one
     static constexpr int TPR = 2;                          // softmax threads per row
-    static constexpr int SOFT_WARPS = 4 * TPR * QT, ISSUE = SOFT_WARPS, LOAD = SOFT_WARPS + 1, WARPS = SOFT_WARPS + 2;
+    static constexpr int SOFT_WARPS = 4 * TPR * QT, ISSUE = SOFT_WARPS, LOAD = SOFT_WARPS + 1;
+    static constexpr int CONV_WARPS = 7, WARPS = LOAD + (DIRECT ? CONV_WARPS : 1);
     static constexpr int COLS = KT / TPR;                  // columns of a softmax thread
     static constexpr int BPT = KT / 16;                    // scale blocks of a tile
     static constexpr int TILES = QT * Q_TILE + 4 * KV_TILE;   // Q, two K and two V buffers
     static constexpr int SMEM = TILES + 1024;              // the tiles start on 1024 bytes
 };
+
+// 16 codes as f16: bytes of 1024 + (c + 128), minus 1152
+__device__ __forceinline__ void codes_to_f16(uint4 w, uint32_t (&o)[8]) {
+    const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));
+    const uint32_t in[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        uint32_t v = __byte_perm(in[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140);
+        const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&v), off);
+        o[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+// a block's factors from its scales (blk -1: not there)
+__device__ __forceinline__ float4 block_factors(int blk, float ks, float vs) {
+    if (blk < 0) return make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+    const float vse = vs > 0.0f ? vs : 0x1p-100f;   // zero values: their weights still count
+    return make_float4(ks, lg2(vse), __frcp_rn(vse), 0.0f);
+}
 
 // ── codes to tiles ─────────────────────────────────────────────────────────
 // Work memory of the pairs (sequence, KV head) of one pass: K and V tiles [pair][tile][2][KV_TILE bytes], then the
@@ -198,7 +224,7 @@ template <int D> struct PromptCfg {
 template <int D>
 __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t pair0, int tiles_max, uint8_t* __restrict__ tiles,
                                                         float4* __restrict__ factors) {
-    using C = PromptCfg<D>;
+    using C = PromptCfg<D, false>;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tile = blockIdx.x % tiles_max;
     const int64_t slot = blockIdx.x / tiles_max, pair = pair0 + slot;
@@ -206,7 +232,6 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t p
     const SeqLens sl = seq_lens(r, b);
     if (tile * C::KT >= sl.len || sl.q_len == 0) return;   // tile < tiles_max by the grid
     uint8_t* image = tiles + (slot * tiles_max + tile) * (2 * C::KV_TILE);
-    const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1024 + 128
     // a warp takes 8 rows x 64 elements (four lanes a row, 16 codes a lane) at a time
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane >> 2, c4 = lane & 3;
 #pragma unroll
@@ -219,14 +244,8 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t p
             uint4 w = make_uint4(0, 0, 0, 0);
             if (blk >= 0)
                 w = __ldg(reinterpret_cast<const uint4*>((x ? r.v : r.k) + ((int64_t)blk * 16 + (tok & 15)) * D + seg * 64 + 16 * c4));
-            const uint32_t in[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
             uint32_t o[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t v = __byte_perm(in[j >> 1], 0x64646464u, (j & 1) ? 0x4342 : 0x4140);
-                const __half2 hv = __hsub2(*reinterpret_cast<__half2*>(&v), off);
-                o[j] = *reinterpret_cast<const uint32_t*>(&hv);
-            }
+            codes_to_f16(w, o);
             uint8_t* to = image + x * C::KV_TILE + seg * C::SEG + row * 128;
             *reinterpret_cast<uint4*>(to + (((2 * c4) ^ sub) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
             *reinterpret_cast<uint4*>(to + (((2 * c4 + 1) ^ sub) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
@@ -234,26 +253,117 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t p
     }
     if (threadIdx.x < C::BPT) {
         const int block = tile * C::BPT + threadIdx.x;
-        float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
+        int blk = -1;
         if (block * 16 < sl.len) {
-            const int blk = block_at(r, b, h, block);
-            if (blk >= 0) {
-                const float vs = r.vs[blk], vse = vs > 0.0f ? vs : 0x1p-100f;   // zero values: their weights still count
-                f = make_float4(r.ks[blk], lg2(vse), __frcp_rn(vse), 0.0f);
-            } else if (r.status) {
-                atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
-            }
+            blk = block_at(r, b, h, block);
+            if (blk < 0 && r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
         }
+        const float4 f = block_factors(blk, blk < 0 ? 0.0f : r.ks[blk], blk < 0 ? 0.0f : r.vs[blk]);
         factors[(slot * tiles_max + tile) * C::BPT + threadIdx.x] = f;
     }
 }
 
+// ── conversion by warps of the attention kernel (DIRECT) ────────────────────
+// A tile of K or V is 16 units of a 16-token block and 64 elements (1 KB of codes, two 16-byte loads and four
+// stores a lane); warp cw takes units cw, cw + 7, cw + 14.  K and V of a tile follow one another; codes are loaded
+// one tensor ahead, pages two tiles ahead.  Warp 0 also provides the blocks' factors.
 template <int D>
-__global__ void __launch_bounds__(PromptCfg<D>::WARPS * 32, 1)
+__device__ __forceinline__ void convert_tiles(const Q8Run& r, int b, int h, int t_begin, int tiles_n, int kv_end, int cw,
+                                              uint32_t k_at, uint32_t v_at, uint32_t k_full, uint32_t k_empty,
+                                              uint32_t v_full, uint32_t v_empty, float4 (*s_fac)[PromptCfg<D, true>::BPT],
+                                              uint32_t f_full, volatile int* failed) {
+    using C = PromptCfg<D, true>;
+    constexpr int NU = 3;
+    const int lane = threadIdx.x & 31, sub = lane >> 2, c4 = lane & 3, per_page = r.page_shift - 4;
+    const int32_t* pages = r.pages + (int64_t)b * r.max_pages;
+    // lanes 0 .. 2: the page of unit cw + 7 lane; lanes 8 .. : that of block lane - 8 (for the factors)
+    int page = -1;
+    auto lane_block = [&](int t) { return (t_begin + t) * C::BPT + (lane < 8 ? (cw + 7 * lane) / C::SEGS : lane - 8); };
+    auto load_page = [&](int t) {
+        const int block = lane_block(t);
+        page = -2;   // none
+        if ((lane < 8 ? cw + 7 * lane < 16 : cw == 0 && lane - 8 < C::BPT) && t < tiles_n && block * 16 < kv_end)
+            page = pages[block >> per_page];
+    };
+    int at[NU], fac_blk = -1;      // blocks of the units (-1: no tokens there) and of the lane's factors
+    float fac_ks = 0.0f, fac_vs = 0.0f;
+    auto locate = [&](int t) {
+        const int block = lane_block(t);
+        int blk = -1;
+        if (page >= 0 && page < r.num_pages) blk = ((page * r.Hkv + h) << per_page) + (block & ((1 << per_page) - 1));
+        else if (page != -2 && r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
+#pragma unroll
+        for (int i = 0; i < NU; ++i) at[i] = __shfl_sync(0xffffffffu, blk, i);
+        if (cw == 0 && lane >= 8) {
+            fac_blk = blk;
+            if (blk >= 0) {
+                fac_ks = r.ks[blk];
+                fac_vs = r.vs[blk];
+            }
+        }
+    };
+    auto load = [&](const int8_t* __restrict__ pool, uint4 (&w)[NU][2]) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            w[i][0] = w[i][1] = make_uint4(0, 0, 0, 0);
+            if (at[i] >= 0) {
+                const int8_t* p = pool + (int64_t)at[i] * (16 * D) + ((cw + 7 * i) % C::SEGS) * 64 + sub * D + 16 * c4;
+                w[i][0] = ldg_now(p);
+                w[i][1] = ldg_now(p + 8 * D);
+            }
+        }
+    };
+    auto store = [&](uint32_t tile, const uint4 (&w)[NU][2]) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int u = cw + 7 * i;
+            if (u >= 16) break;
+            const uint32_t to = tile + (u % C::SEGS) * C::SEG + (u / C::SEGS) * 2048 + sub * 128;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {   // rows sub and sub + 8 of the block
+                uint32_t o[8];
+                codes_to_f16(w[i][x], o);
+                sts128(to + x * 1024 + (((2 * c4) ^ sub) << 4), o[0], o[1], o[2], o[3]);
+                sts128(to + x * 1024 + (((2 * c4 + 1) ^ sub) << 4), o[4], o[5], o[6], o[7]);
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+    };
+    uint4 kw[NU][2], vw[NU][2];
+    load_page(0);
+    locate(0);
+    load_page(1);
+    load(r.k, kw);
+    for (int t = 0; t < tiles_n; ++t) {
+        const int buf = t & 1, par = ((t >> 1) & 1) ^ 1;   // the first pass over the two buffers does not wait
+        load(r.v, vw);
+        if (t >= 2 && !__all_sync(0xffffffffu, mbar_wait(k_empty + 8 * buf, par, failed))) break;
+        if (cw == 0) {
+            // ring of four: a K buffer is free again when the softmax is three tiles back
+            if (lane >= 8 && lane < 8 + C::BPT) s_fac[t & 3][lane - 8] = block_factors(fac_blk, fac_ks, fac_vs);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(f_full + 8 * (t & 3));
+        }
+        store(k_at + buf * C::KV_TILE, kw);
+        if (lane == 0) mbar_arrive(k_full + 8 * buf);
+        if (t + 1 < tiles_n) {
+            locate(t + 1);
+            load_page(t + 2);
+            load(r.k, kw);
+        }
+        if (t >= 2 && !__all_sync(0xffffffffu, mbar_wait(v_empty + 8 * buf, par, failed))) break;
+        store(v_at + buf * C::KV_TILE, vw);
+        if (lane == 0) mbar_arrive(v_full + 8 * buf);
+    }
+}
+
+template <int D, bool DIRECT>
+__global__ void __launch_bounds__(PromptCfg<D, DIRECT>::WARPS * 32, 1)
 attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, const uint8_t* __restrict__ kv_tiles,
                       const float4* __restrict__ factors, int row_tiles, int splits, float* __restrict__ part,
                       float* __restrict__ part_lse) {
-    using C = PromptCfg<D>;
+    using C = PromptCfg<D, DIRECT>;
     constexpr int QT = C::QT, KT = C::KT, TPR = C::TPR, ROWS = C::ROWS, LPR = D / 16, THREADS = C::WARPS * 32;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[20];
@@ -284,7 +394,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     if (last_i >= sl.q_len) last_i = sl.q_len - 1;
     const int first_i = row0 / r.grp;
     int kv_end = last_i < first_i ? 0 : last_seen(r, sl, last_i) + 1;
-    if (kv_end > r.max_len) {   // longer than the caller's bound: the work memory has no tiles for it
+    if (!DIRECT && kv_end > r.max_len) {   // longer than the caller's bound: the work memory has no tiles for it
         kv_end = r.max_len;
         if (threadIdx.x == 0 && r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
     }
@@ -301,8 +411,8 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     if (threadIdx.x == 0) {
         s_failed = 0;
         for (int i = 0; i < 2; ++i) {
-            mbar_init(k_full + 8 * i, 1);     // the loading lane, and the bytes of its copy
-            mbar_init(v_full + 8 * i, 1);
+            mbar_init(k_full + 8 * i, DIRECT ? C::CONV_WARPS : 1);   // converting warps; or the loading lane (and bytes)
+            mbar_init(v_full + 8 * i, DIRECT ? C::CONV_WARPS : 1);
             mbar_init(k_empty + 8 * i, 1);    // commits of the issuing thread
             mbar_init(v_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
@@ -578,8 +688,11 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
         }
         __syncwarp();
     } else {
-        // ── load ──
-        if (lane == 0) {
+        // ── tiles ──
+        if constexpr (DIRECT) {
+            convert_tiles<D>(r, b, h, t_begin, tiles_n, kv_end, warp - C::LOAD, k_at, v_at, k_full, k_empty, v_full, v_empty, s_fac,
+                             f_full, &s_failed);
+        } else if (lane == 0) {
             const uint8_t* from = kv_tiles + ((int64_t)slot * tiles_max + t_begin) * (2 * C::KV_TILE);
             const float4* fac = factors + ((int64_t)slot * tiles_max + t_begin) * C::BPT;
             int nk = 0, nv = 0;   // copies begun
@@ -670,8 +783,8 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
 // Work memory: partial sums of split units, then the tiles and factors of one pass's pairs.
 template <int D>
 static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, uint8_t* tiles, cudaStream_t st) {
-    using C = PromptCfg<D>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    using C = PromptCfg<D, false>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * p.tiles_max * (2 * C::KV_TILE));
     const int64_t pairs = (int64_t)r.B * r.Hkv;
@@ -691,23 +804,39 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
+        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
                                (const float4*)factors, p.row_tiles, p.splits, part, part_lse);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
 }
 
+template <int D>
+static cudaError_t launch_direct_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
+    using C = PromptCfg<D, true>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t pairs = (int64_t)r.B * r.Hkv, grid = pairs * p.row_tiles * p.splits;
+    if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
+    attn_q8_prompt_kernel<D, true><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, 0, (int)pairs, 0, nullptr, nullptr, p.row_tiles,
+                                                                                   p.splits, part, part_lse);
+    return cudaGetLastError();
+}
+
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st) {
     uint8_t* t = static_cast<uint8_t*>(tiles);
+    if (p.direct) return r.D == 256 ? launch_direct_d<256>(r, p, part, part_lse, st) : launch_direct_d<128>(r, p, part, part_lse, st);
     return r.D == 256 ? launch_prompt_d<256>(r, p, part, part_lse, t, st) : launch_prompt_d<128>(r, p, part, part_lse, t, st);
 }
 
-int q8_prompt_rows(int D) { return D == 128 ? PromptCfg<128>::ROWS : PromptCfg<256>::ROWS; }
+int q8_prompt_rows(int D, bool direct) {
+    if (direct) return D == 128 ? PromptCfg<128, true>::ROWS : PromptCfg<256, true>::ROWS;
+    return D == 128 ? PromptCfg<128, false>::ROWS : PromptCfg<256, false>::ROWS;
+}
 
 // tiles of one pass: all pairs, or as many as 1 GiB holds
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p) {
-    const int kt = D == 128 ? PromptCfg<128>::KT : PromptCfg<256>::KT;
+    const int kt = D == 128 ? PromptCfg<128, false>::KT : PromptCfg<256, false>::KT;
     p->tiles_max = (int)((max_len + kt - 1) / kt);
     const int64_t bytes = (int64_t)p->tiles_max * (4 * kt * D + kt);   // two f16 tiles, 16 bytes per 16 tokens
     const int64_t most = bytes > 0 ? (int64_t(1) << 30) / bytes : pairs;
