@@ -497,13 +497,21 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int r
 
 // ── plan and launch ────────────────────────────────────────────────────────
 
-constexpr int DIRECT_ROWS = 25, PROMPT_ROWS = 129;
+// Which kernel, by the query rows of a KV head (us at 8 sequences x 8 KV heads x 16000 tokens, D = 128 | 256):
+//   rows         24          48          64         128          256         384         512
+//   few       80 | 186   139 | 263   210 | 356   400 | 647   683 | 1243  947 | 1922  1345 | 2447
+//   direct   121 | 233   130 | 239   124 | 238   129 | 241   226 |  439   349 | 668   446 |  874
+//   tiles    303 | 470   305 | 470   303 | 471   306 | 475   290 |  577   433 | 831   399 |  868
+// few: this file's kernel (a conversion for 24 or 16 rows); direct: tcgen05, a conversion for 128 rows; tiles:
+// tcgen05 from tiles expanded once.
+constexpr int DIRECT_ROWS_128 = 49, DIRECT_ROWS_256 = 33, PROMPT_ROWS = 449;
+
 
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
     Q8Plan p;
     const int64_t rows = n * grp;
     if (rows == 0 || B == 0) return p;
-    p.prompt = rows >= DIRECT_ROWS;
+    p.prompt = rows >= (D == 128 ? DIRECT_ROWS_128 : DIRECT_ROWS_256);
     p.direct = rows < PROMPT_ROWS;
     if (p.prompt) {
         p.rows = q8_prompt_rows(D, p.direct);

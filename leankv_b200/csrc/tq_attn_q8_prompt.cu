@@ -479,6 +479,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
         constexpr float TINY = 1e-38f;   // least factor of a sum: -inf stays -inf where f or ks is zero
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
+        const bool idle = __all_sync(0xffffffffu, lim < 0);
         constexpr int BPH = C::BPT / TPR, CH = C::COLS / 32;
         for (int t = 0; t < tiles_n; ++t) {
             const int sb = QT == 2 ? qt : (t & 1);
@@ -490,6 +491,16 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
             ok = ok && __all_sync(0xffffffffu, mbar_wait(f_full + 8 * (t & 3), (t >> 2) & 1, &s_failed));
             ok = ok && __all_sync(0xffffffffu, mbar_wait(s_full + 8 * sb, par, &s_failed));
             tc_fence_after();
+            if (idle) {   // no row of the warp sees anything: whatever the products make of them is not read
+                if constexpr (QT == 2) {   // the turns are kept all the same: a tile that runs ahead would use up two of them
+                    if (qt == 1 || t > 0)
+                        ok = ok && __all_sync(0xffffffffu, mbar_wait(turn + 8 * qt, qt == 1 ? t & 1 : (t - 1) & 1, &s_failed));
+                    if (ok && lane == 0) mbar_arrive(turn + 8 * (qt ^ 1));
+                }
+                if (!ok) break;
+                if (lane == 0) mbar_arrive(p_full + 8 * sb);
+                continue;
+            }
 
             // the row's scores, in registers
             uint32_t raw[CH][32];
