@@ -448,7 +448,8 @@ tq_status tq_dequantize_q8_cuda(const int8_t *codes, const float *scale, void *y
  * rounded to f16, codes are exact, weights are rounded to f16, statistics are fp32.  q must be finite.
  * head_dim 128 or 256, any n_q_heads / n_kv_heads, page_size a power of two in 16 .. 65536.  A page id
  * outside the pool that holds tokens a row would see is treated as holding none, and TQ_ERROR_INVALID_VALUE is
- * stored in *status.  Work memory: tq_attention_q8_workspace_size() bytes, written before they are read; calls
+ * stored in *status; so it is when a sequence is longer than max_kv_len and tokens behind that bound are left out
+ * (kernels for many rows).  A wait inside a kernel that runs out (about a second) stores TQ_ERROR_TIMEOUT.  Work memory: tq_attention_q8_workspace_size() bytes, written before they are read; calls
  * that can overlap need their own.
  */
 typedef struct {
@@ -460,11 +461,11 @@ typedef struct {
     const int8_t *v_codes;      const float *v_scale;
     const int32_t *kv_len;      /* device [batch] */
     const int32_t *q_len;       /* device [batch], or NULL */
-    int64_t max_kv_len;         /* about the largest kv_len: sizes the work split, not the result; 0 = capacity */
+    int64_t max_kv_len;         /* upper bound of kv_len (0 = capacity): sizes the work split and the work memory */
     float sm_scale;             /* 0 = 1/sqrt(head_dim) */
     int causal, rotate_q, v_rotated;
     float *lse;                 /* optional [batch][n_q_heads][n_new], natural log */
-    int32_t *status;            /* optional device word, raised to TQ_ERROR_INVALID_VALUE by a bad page id */
+    int32_t *status;            /* optional device word, raised as above (never lowered: clear it before) */
     void *workspace;            size_t workspace_bytes;
 } tq_attention_q8_args;
 size_t tq_attention_q8_workspace_size(const tq_attention_q8_args *a, const tq_kv_pages *pages);

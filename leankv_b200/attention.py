@@ -15,7 +15,7 @@ import torch
 
 from . import _lib as L
 from .ops import (_DTYPES, _PAGES, _call, _check_lengths, _check_q8_pools, _check_rows, _check_table, _device_of,
-                  _need_cuda, _stream)
+                  _need_cuda, _own_rows, _stream)
 
 
 class AttnArgs(C.Structure):
@@ -178,8 +178,9 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     ops.kv_append_rotary_paged writes them; page_table int32 [B, max_pages_per_seq]; kv_len int32 [B], the
     cached tokens with this step's.  Query token i of the q_len[b] (default n) of sequence b is cached token
     kv_len[b] - q_len[b] + i and sees the tokens up to itself (causal) or all.  Rows that see nothing, those
-    of a padded batch (i >= q_len[b]) among them, give zeros and a log-sum-exp of -inf.  max_kv_len: about the largest
-    length, for splitting the work (default: the capacity).  out_dtype: q's by default; out [like q] /
+    of a padded batch (i >= q_len[b]) among them, give zeros and a log-sum-exp of -inf.  max_kv_len: an upper bound
+    of kv_len that sizes the work and, for many rows, the work memory (default: the capacity; up to 1 GiB, or what
+    one sequence and head needs): tokens behind it may be left out, with status raised.  out_dtype: q's by default; out [like q] /
     lse_out (float32 [B, Hq, n]): destinations.  status: int32 CUDA tensor [1], raised to 1 when a page id
     outside the pool is met (its tokens are left out).
     """
@@ -200,8 +201,8 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
         _check_lengths(q_len, B, "q_len")
     if out is None:
         out = torch.empty_strided((B, Hq, n, D), (n * Hq * D, D, Hq * D, 1), dtype=out_dtype or q.dtype, device=q.device)
-    elif out.shape != q.shape or out.stride(3) != 1 or (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError("out must have q's shape, head_dim contiguous")
+    elif out.shape != q.shape or not _own_rows(out) or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError("out must have q's shape, head_dim contiguous, every row its own memory")
     if out.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {out.dtype}")
     lse = lse_out

@@ -293,13 +293,18 @@ def _check_q8_pools(k_pool, v_pool, k_scale, v_scale, H: int, D: int) -> tuple:
     return shape[0], shape[2]
 
 
+def _own_rows(t: torch.Tensor) -> bool:
+    """head_dim contiguous, and no dimension expanded (rows written over one another)."""
+    return all(n <= 1 or (s == 1 if i == 3 else s != 0) for i, (n, s) in enumerate(zip(t.shape, t.stride())))
+
+
 def _rows_out(t: torch.Tensor, out: torch.Tensor | None, name: str) -> torch.Tensor:
     if out is None:
         # token-major memory, as the projections on either side have it
         B, H, n, D = t.shape
         return torch.empty_strided((B, H, n, D), (n * H * D, D, H * D, 1), dtype=t.dtype, device=t.device)
-    if out.shape != t.shape or out.dtype != t.dtype or (out.shape[3] > 1 and out.stride(3) != 1):
-        raise ValueError(f"{name} must have the shape and type of its input, head_dim contiguous")
+    if out.shape != t.shape or out.dtype != t.dtype or not _own_rows(out):
+        raise ValueError(f"{name} must have the shape and type of its input, head_dim contiguous, every row its own memory")
     return out
 
 

@@ -10,6 +10,12 @@ A weight below f16's normal numbers is off by half its smallest step, 2^-25, of 
 2^-31 max_j(p_j vs_j) sum_j |code_j| of an output element (an element whose code is 0 for the one token that a
 row attends to is the sum of such weights alone).
 The log-sum-exp is off by at most ds + 2^-14.
+
+That bound is for the worst signs.  The error's size is held to three times what independent roundings give: a
+rounding is evenly spread over +- half a step, at most 2^-11 of the value, so its variance is at most 2^-22 / 3 of the
+value's square.  Those of q' move an output by sum_d e_d q'_d c_d with c_d = sm_scale sum_j p_j k_jd (v_j - o), those
+of the weights by sum_j e_j p_j v_j; to first order the squares add up, over rows and elements (the Hadamard matrix
+keeps them).
 """
 import math
 
@@ -43,7 +49,8 @@ def _table(B, per, pages, seed):
 
 
 def _reference(q, kp, vp, ks, vs, table, kv_len, q_len, causal, rotate_q, v_rotated, sm_scale):
-    """out, lse, and the tolerances of both (before the output's own rounding), float64."""
+    """out, lse, and the tolerances of both (before the output's own rounding), float64, and the expected square of
+    the whole error."""
     B, Hq, n, D = q.shape
     H = kp.shape[1]
     grp = Hq // H
@@ -52,6 +59,7 @@ def _reference(q, kp, vp, ks, vs, table, kv_len, q_len, causal, rotate_q, v_rota
     tol = torch.zeros_like(out)
     lse = torch.full((B, Hq, n), -math.inf, dtype=torch.float64, device=DEV)
     ltol = torch.zeros_like(lse)
+    square = 0.0
     for b in range(B):
         L = int(kv_len[b])
         ql = n if q_len is None else int(q_len[b])
@@ -73,16 +81,25 @@ def _reference(q, kp, vp, ks, vs, table, kv_len, q_len, causal, rotate_q, v_rota
         e = ds.amax(-1, keepdim=True)
         p = torch.softmax(s, -1).nan_to_num(0.0)
         o, size = p @ v[:, None], p @ v.abs()[:, None]
+        square_at = 0
         t = (torch.expm1(2 * e) + 2.0 ** -11 + 2.0 ** -14) * size
         step = vs[pg].double().repeat_interleave(16, -1).transpose(0, 1).flatten(1, 2)[:, :L]
         codes = vp[pg].double().transpose(0, 1).flatten(1, 2)[:, :L].abs().sum(1)
         t = t + 2.0 ** -31 * (p * step[:, None, None]).amax(-1, keepdim=True) * codes[:, None, None]
+        for h in range(H):
+            for some in p[h].flatten(0, 1).split(64):
+                c = sm_scale * (torch.einsum("rt,td,te->rde", some, k[h], v[h]) - (some @ k[h])[..., None] * (some @ v[h])[:, None])
+                rows = slice(square_at, square_at + len(some))
+                square += float((x[h].flatten(0, 1)[rows].square()[..., None] * c.square()).sum()) * 2.0 ** -22 / 3
+                square += float((some.square() @ v[h].square()).sum()) * 2.0 ** -22 / 3
+                square_at += len(some)
+            square_at = 0
         if v_rotated:
             o, t = o @ had, t @ had.abs()   # each element of the sum may be off by its own tolerance
         out[b, :, :ql], tol[b, :, :ql] = o.flatten(0, 1), t.flatten(0, 1)
         lse[b, :, :ql] = torch.logsumexp(s, -1).flatten(0, 1)
         ltol[b, :, :ql] = (e.squeeze(-1) + 2.0 ** -14).flatten(0, 1)
-    return out, lse, tol, ltol
+    return out, lse, tol, ltol, square
 
 
 def _check(q, kp, vp, ks, vs, table, kv_len, q_len=None, causal=True, rotate_q=True, v_rotated=True, sm_scale=None,
@@ -91,7 +108,7 @@ def _check(q, kp, vp, ks, vs, table, kv_len, q_len=None, causal=True, rotate_q=T
     got, lse = attention.attention_q8_paged(q, kp, vp, ks, vs, table, kv_len, q_len=q_len, causal=causal, rotate_q=rotate_q,
                                             v_rotated=v_rotated, sm_scale=sm_scale, out_dtype=out_dtype, return_lse=True,
                                             max_kv_len=max_kv_len)
-    want, wlse, tol, ltol = _reference(q, kp, vp, ks, vs, table, kv_len, q_len, causal, rotate_q, v_rotated, sm_scale or D ** -0.5)
+    want, wlse, tol, ltol, square = _reference(q, kp, vp, ks, vs, table, kv_len, q_len, causal, rotate_q, v_rotated, sm_scale or D ** -0.5)
     half = torch.finfo(got.dtype).eps / 2
     err = (got.double() - want).abs()
     assert bool((err <= tol * (1 + half) + half * want.abs() + 1e-30).all()), (err - tol).max()
@@ -99,9 +116,8 @@ def _check(q, kp, vp, ks, vs, table, kv_len, q_len=None, causal=True, rotate_q=T
     assert torch.equal(lse == -math.inf, empty)
     assert bool((got[empty] == 0).all())
     assert bool(((lse.double() - wlse).abs()[~empty] <= ltol[~empty]).all())
-    # the bound is for the worst signs; the error's size is far below it
-    if float(want.norm()) > 0:
-        assert float((got.double() - want).norm() / want.norm()) < 2 * half + 2e-3
+    # 2^-14 of the output for the fp32 sums, as above
+    assert float((got.double() - want).norm()) <= 3 * square ** 0.5 + (half + 2.0 ** -14) * float(want.norm()) + 1e-30
     return got, lse
 
 
@@ -174,9 +190,11 @@ def test_long_context_and_splits(n):
         assert float((a[0].float() - b[0].float()).abs().max()) <= 2.0 ** -7 * float(a[0].float().abs().max())
 
 
-def test_scales_of_all_sizes():
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("n", [2, 20, 130])   # rows for each of the three kernels
+def test_scales_of_all_sizes(n, D):
     """Blocks whose scales differ by many orders, zero blocks (scale 0) and very large scores."""
-    B, H, grp, D, P = 2, 2, 4, 128, 16
+    B, H, grp, P = 2, 2, 4, 16
     kp, ks = _pools(40, H, P, D, 12)
     vp, vs = _pools(40, H, P, D, 13, spread=6.0)
     vp[::5] = 0
@@ -186,19 +204,21 @@ def test_scales_of_all_sizes():
     table = _table(B, 20, 40, 14)
     lens = torch.tensor([320, 201], dtype=torch.int32, device=DEV)
     for size in (0.0, 1e-3, 1.0, 30.0):
-        _check(_q(B, H * grp, 2, D, torch.float32, 15, size), kp, vp, ks, vs, table, lens, out_dtype=torch.float32)
+        _check(_q(B, H * grp, n, D, torch.float32, 15, size), kp, vp, ks, vs, table, lens, out_dtype=torch.float32)
     # only zero values
-    got = attention.attention_q8_paged(_q(B, H * grp, 1, D, torch.float32, 1), kp, vp * 0, ks, vs * 0, table, lens)
+    got = attention.attention_q8_paged(_q(B, H * grp, n, D, torch.float32, 1), kp, vp * 0, ks, vs * 0, table, lens)
     assert bool((got == 0).all())
 
 
-def test_garbage_behind_the_sequence_is_not_seen():
-    B, H, grp, D, P = 2, 2, 4, 128, 32
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("n", [3, 25, 130])
+def test_garbage_behind_the_sequence_is_not_seen(n, D):
+    B, H, grp, P = 2, 2, 4, 32
     kp, ks = _pools(20, H, P, D, 16)
     vp, vs = _pools(20, H, P, D, 17)
     table = _table(B, 10, 20, 18)
     lens = torch.tensor([50, 161], dtype=torch.int32, device=DEV)
-    q = _q(B, H * grp, 3, D, torch.bfloat16, 19)
+    q = _q(B, H * grp, n, D, torch.bfloat16, 19)
     a = attention.attention_q8_paged(q, kp, vp, ks, vs, table, lens)
     for b in range(B):
         L = int(lens[b])
@@ -213,23 +233,26 @@ def test_garbage_behind_the_sequence_is_not_seen():
     assert torch.equal(a, attention.attention_q8_paged(q, kp, vp, ks, vs, table, lens))
 
 
-def test_bad_page_is_reported_and_left_out():
-    B, H, D, P = 1, 1, 128, 16
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_bad_page_is_reported_and_left_out(n, D):
+    B, H, P = 1, 1, 16
     kp, ks = _pools(8, H, P, D, 20)
     vp, vs = _pools(8, H, P, D, 21)
     table = torch.arange(8, dtype=torch.int32, device=DEV).view(1, 8)
     lens = torch.tensor([128], dtype=torch.int32, device=DEV)
-    q = _q(B, 2, 1, D, torch.float32, 22)
+    q = _q(B, 2, n, D, torch.float32, 22)
     status = torch.zeros(1, dtype=torch.int32, device=DEV)
-    attention.attention_q8_paged(q, kp, vp, ks, vs, table, lens, status=status)
+    run = lambda t: attention.attention_q8_paged(q, kp, vp, ks, vs, t, lens, status=status, causal=False)   # noqa: E731
+    run(table)
     assert int(status.item()) == 0
     bad = table.clone()
     bad[0, 3] = 8
     bad[0, 7] = -1
-    got = attention.attention_q8_paged(q, kp, vp, ks, vs, bad, lens, status=status)
+    got = run(bad)
     assert int(status.item()) == 1
     keep = torch.tensor([[0, 1, 2, 4, 5, 6]], dtype=torch.int32, device=DEV)
-    want, _, tol, _ = _reference(q, kp, vp, ks, vs, keep, torch.tensor([96]), None, True, True, True, D ** -0.5)
+    want, _, tol, _, _ = _reference(q, kp, vp, ks, vs, keep, torch.tensor([96]), None, False, True, True, D ** -0.5)
     assert bool(((got.double() - want).abs() <= tol + 1e-6).all())
 
 
@@ -314,6 +337,53 @@ def test_append_then_attend_with_rotary():
                 rel = float((out[b, :, :new[b]].double() - want).norm() / want.norm())
                 assert rel < 0.03, rel
             assert bool((out[b, :, new[b]:] == 0).all())
+
+
+def test_bound_of_the_lengths():
+    """A sequence longer than max_kv_len: reported where the work memory is sized by it (many rows)."""
+    B, H, grp, D, P, n = 2, 1, 8, 128, 64, 64
+    kp, ks = _pools(32, H, P, D, 1)
+    vp, vs = _pools(32, H, P, D, 2)
+    table = _table(B, 16, 32, 3)
+    lens = torch.tensor([700, 900], dtype=torch.int32, device=DEV)
+    q = _q(B, H * grp, n, D, torch.bfloat16, 4)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    want = attention.attention_q8_paged(q, kp, vp, ks, vs, table, lens, status=status)
+    got = attention.attention_q8_paged(q, kp, vp, ks, vs, table, lens, max_kv_len=900, status=status)
+    assert int(status.item()) == 0 and torch.equal(got, want)
+    got = attention.attention_q8_paged(q, kp, vp, ks, vs, table, lens, max_kv_len=800, status=status)
+    assert int(status.item()) == 1 and torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize("n", [1, 8, 64])
+def test_prompts_on_two_streams_and_replayed(n):
+    """Each call has work memory of its own: overlapping calls and two graphs replayed in turn keep their results."""
+    B, H, grp, D, P = 3, 2, 8, 128, 64
+    kp, ks = _pools(60, H, P, D, 36)
+    vp, vs = _pools(60, H, P, D, 37)
+    table = _table(B, 20, 60, 38)
+    lens = torch.tensor([1280, 333, 700], dtype=torch.int32, device=DEV)
+    qs = [_q(B, H * grp, n, D, torch.bfloat16, 40 + i) for i in range(2)]
+    call = lambda i, **kw: attention.attention_q8_paged(qs[i], kp, vp, ks, vs, table, lens, **kw)   # noqa: E731
+    want = [call(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], [torch.empty_like(w) for w in want]
+    for i in range(2):
+        with torch.cuda.graph(graphs[i]):
+            call(i, out=outs[i])
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i]) and torch.equal(outs[i], want[i])
 
 
 def test_refusals():

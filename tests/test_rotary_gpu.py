@@ -171,7 +171,7 @@ def test_rotary_empty_and_refusals():
     bad = [dict(q=x.double()), dict(q=x[0]), dict(q=x.transpose(2, 3)), dict(positions=pos.long()),
            dict(positions=pos[:1]), dict(positions=pos.expand(3, 2, 4).contiguous()), dict(positions=None),
            dict(rope=ops.Rotary(freq.float())), dict(rope=ops.Rotary(freq, axis=freq)), dict(k=x[:, :, :2]),
-           dict(k=x.float()), dict(out=x.float()), dict(q=x.cpu()), dict(rope=ops.Rotary(freq.cpu()))]
+           dict(k=x.float()), dict(out=x.float()), dict(out=x[:1].expand(2, 2, 4, 64)), dict(q=x.cpu()), dict(rope=ops.Rotary(freq.cpu()))]
     for change in bad:
         with pytest.raises(ValueError):
             ops.rotary(**{**dict(q=x, positions=pos, rope=rope), **change})
