@@ -14,7 +14,8 @@
 // registers.  A tcgen05 tile (128 rows) would be emptier still, and its operands would have to go through shared
 // memory once more after the conversion from 8 bits.
 //
-// Numbers.  A row of q' is scaled by its largest element and rounded to f16.  Codes are integers of 8 bits and
+// Numbers.  A row of q' is scaled by its largest element and rounded to f16 (for outputs of more than 8 bits as the
+// sum of two f16 terms: scores are then off by fp32 sums only).  Codes are integers of 8 bits and
 // exact in f16.  K codes enter the product as subnormals (c + 128) 2^-24: one byte permute for two values;
 // 128 times the row's sum of q' is taken off in fp32.  V codes are made from 1024 + (c + 128) minus 1152
 // (the offset left in would cost up to 5 bits of the sum).  The V scale goes into the exponent:
@@ -47,13 +48,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <int D, int NT> struct Q8Cfg {
+template <int D, int NT, bool LO> struct Q8Cfg {
     static constexpr int ROWS = 8 * NT, NK = D / 16;
     static constexpr int CTAS = D == 128 && NT == 1 ? 2 : 1;   // per SM
     static constexpr int STAGES = D == 256 || CTAS == 2 ? 3 : 5;
     static constexpr int BLOCK = 16 * D;                       // bytes of one tensor's block
     static constexpr int RING = STAGES * 2 * BLOCK;            // per warp
-    static constexpr int QBYTES = NT * NK * 256;
+    static constexpr int QPART = NT * NK * 256, QBYTES = LO ? 2 * QPART : QPART;
     static constexpr int MERGE = Q8_WARPS * ROWS * D * 4;      // the warps' sums, over the rings
     static constexpr int RINGS = Q8_WARPS * RING > MERGE ? Q8_WARPS * RING : MERGE;
     static constexpr int SMEM = RINGS + QBYTES + (2 * Q8_WARPS * ROWS + 4 * ROWS) * 4;
@@ -74,10 +75,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 
 // One unit's share of tokens.  Partial results go to part / part_lse (splits > 1), else to out / lse.
-template <int D, int NT>
-__global__ void __launch_bounds__(Q8_THREADS, Q8Cfg<D, NT>::CTAS)
+template <int D, int NT, bool LO>
+__global__ void __launch_bounds__(Q8_THREADS, Q8Cfg<D, NT, LO>::CTAS)
 attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ part, float* __restrict__ part_lse) {
-    using C = Q8Cfg<D, NT>;
+    using C = Q8Cfg<D, NT, LO>;
     constexpr int ROWS = C::ROWS, NK = C::NK, HALVES = D / 128, LPR = D / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* s_q = smem + C::RINGS;
@@ -178,12 +179,18 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         for (int o = 1; o < LPR; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
         float sum = 0.0f;
-        uint32_t w[8];
+        uint32_t w[8], wl[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const __half2 p = __floats2half2_rn(v[2 * j] * inv, v[2 * j + 1] * inv);
-            sum += __low2float(p) + __high2float(p);
+            const float x = v[2 * j] * inv, y = v[2 * j + 1] * inv;
+            const __half2 p = __floats2half2_rn(x, y);
             w[j] = *reinterpret_cast<const uint32_t*>(&p);
+            sum += __low2float(p) + __high2float(p);
+            if constexpr (LO) {   // what the rounding left, as a second term
+                const __half2 q = __floats2half2_rn(x - __low2float(p), y - __high2float(p));
+                wl[j] = *reinterpret_cast<const uint32_t*>(&q);
+                sum += __low2float(q) + __high2float(q);
+            }
         }
 #pragma unroll
         for (int o = 1; o < LPR; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -191,6 +198,10 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         uint4* to = reinterpret_cast<uint4*>(s_q) + ((row >> 3) * (NK / 2) + j0 / 2) * 32 + (row & 7) * 4 + tt;
         to[0] = make_uint4(w[0], w[1], w[2], w[3]);
         to[32] = make_uint4(w[4], w[5], w[6], w[7]);
+        if constexpr (LO) {
+            to[C::QPART / 16] = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+            to[C::QPART / 16 + 32] = make_uint4(wl[4], wl[5], wl[6], wl[7]);
+        }
         if (lane % LPR == 0) {
             const float fr = top * r.sm_scale * LOG2E;
             s_f[row] = make_float2(fr * 0x1p24f, fr * 128.0f * sum);
@@ -270,6 +281,11 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
                     const uint4 q = lds128(sq + (nt * (NK / 2) + half * 4 + j / 2) * 512);
                     mma16816(s[nt], a0, q.x, q.y);
                     mma16816(s[nt], a1, q.z, q.w);
+                    if constexpr (LO) {
+                        const uint4 ql = lds128(sq + C::QPART + (nt * (NK / 2) + half * 4 + j / 2) * 512);
+                        mma16816(s[nt], a0, ql.x, ql.y);
+                        mma16816(s[nt], a1, ql.z, ql.w);
+                    }
                 }
             }
         }
@@ -552,15 +568,22 @@ static size_t part_bytes(int B, int Hkv, int D, const Q8Plan& p) {
 }
 size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p) { return part_bytes(B, Hkv, D, p) + p.tile_bytes; }
 
-template <int D, int NT>
-static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
-    using C = Q8Cfg<D, NT>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+template <int D, int NT, bool LO>
+static cudaError_t launch_one(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
+    using C = Q8Cfg<D, NT, LO>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<D, NT, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)r.B * r.Hkv * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    attn_q8_kernel<D, NT><<<(unsigned)grid, Q8_THREADS, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
+    attn_q8_kernel<D, NT, LO><<<(unsigned)grid, Q8_THREADS, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
     return cudaGetLastError();
+}
+
+// The second term of q' costs 8 to 16 more products a block; where the output has bf16's 8 bits nothing of it would
+// be seen.
+template <int D, int NT>
+static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
+    return r.out_dtype == DT_BF16 ? launch_one<D, NT, false>(r, p, part, part_lse, st) : launch_one<D, NT, true>(r, p, part, part_lse, st);
 }
 
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st) {
