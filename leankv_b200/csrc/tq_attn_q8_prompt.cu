@@ -1,23 +1,38 @@
-// tq_attn_q8_prompt.cu — attention over 8-bit pages for prompts, on tcgen05.
+// tq_attn_q8_prompt.cu — attention over 8-bit pages for prompts and long drafts, on tcgen05.
 //
-// The mathematics is tq_attn_q8.cu's; with 100 or more query rows per KV head the two products bound it.  Two
-// kernels:
+// The mathematics is tq_attn_q8.cu's.  With many query rows per KV head the two products and the exponentials bound
+// it, not the cache: an 8192-token causal prompt of 32 heads of 128 (550 Gflop with the masked half left out) takes
+// 563 to 597 us, 920 to 977 Tflop/s; the products alone would take 337 us at the measured bf16 rate, the
+// exponentials (16 a cycle and SM) about as long, and a row's softmax waits for its scores and its values for its
+// weights.  ncu on that case: tensor pipe 44 %, special function unit 45 %, issue 46 %.  Two ways of getting f16 tiles
+// from codes, chosen by rows (q8_plan in tq_attn_q8.cu has both sides' times):
 //
-// expand_q8_kernel turns the codes that the rows will see into f16 tiles, once, in work memory: a tile is the image
-// of its shared-memory buffer, so that the second kernel fetches it with one bulk copy.  (Converted by warps of the
-// second kernel, every tile would be converted for each of a prompt's row tiles: 28 % of its instructions, 677
-// instead of XXX us for an 8192-token prompt.)  It also gathers what a block's scales contribute to the scores.
+// tiles (DIRECT = false), many rows: expand_q8_kernel turns the codes that the rows will see into f16 tiles, once,
+// in work memory: a tile is the image of its shared-memory buffer, so that the second kernel fetches it with one bulk
+// copy.  (Converted by warps of the second kernel, every tile would be converted for each of a prompt's row tiles:
+// 28 % of its instructions, 677 instead of 606 us for the 8192-token prompt when that was changed.)  It also gathers
+// what a block's scales contribute to the scores.
+//
+// DIRECT, up to a few row tiles: seven warps of the attention kernel convert the codes on their way into shared
+// memory (convert_tiles), with no work memory and no first pass over the cache.
 //
 // attn_q8_prompt_kernel: a CTA takes QT tiles of 128 query rows (tokens x heads of one group) of one (sequence, KV
-// head).  Warps:
+// head), or one split of their tokens.  Warps:
 //   8 QT softmax warps   two threads per row, half of a tile's columns each: scores from TMEM, weights back to
 //                        TMEM, the output's rescaling
 //   1 issuing warp       one elected lane issues all tcgen05.mma
-//   1 loading warp       one lane issues the bulk copies of K and V tiles
+//   1 loading warp       one lane issues the bulk copies of K and V tiles; DIRECT: 7 converting warps in its place
 // Per tile of KT tokens: S = Q K^T (both from shared memory, f16, fp32 sums in TMEM), weights P in f16 written
-// over S, O += P V (P from TMEM, V from shared memory).  D = 128: two row tiles of 128 tokens take turns, so that
-// one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).  D = 256: O alone
-// takes 256 columns and Q 64 KB, so one row tile takes 64 tokens at a time with two buffers for S.
+// over S, O += P V (P from TMEM, V from shared memory).  D = 128 from tiles: two row tiles take turns, so that
+// one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).  Otherwise one row tile
+// has two buffers for S: D = 256, whose O alone takes 256 columns and Q 64 KB, takes 64 tokens at a time.
+//
+// Roundings: a row of q' is scaled by its largest element and rounded to f16, for outputs of more than bf16's 8 bits
+// (LO) to the sum of two f16 terms; the second one is read from TMEM.  With one term the float16 answer of 700 rows
+// was off by 4.3e-4 of its norm, with two by 2.8e-4 (2.1e-4 is float16's own rounding); the time rises by the
+// products, 118 -> 136 us for pieces of prompts of heads of 256, 597 -> 783 us for the 8192-token prompt (whose tiles
+// shrink to 64 tokens to make room).  In bfloat16, off by 1.7e-3 either way, the second term is left out.  Weights
+// are f16, off by up to 2^-12 of each, which averages out over the tokens.
 //
 // Tiles are runs of 64 elements: [row][128 bytes], 16-byte chunk c of row x at c ^ (x & 7) (the 128-byte
 // swizzle of the matrix descriptors).  K is read with its elements contiguous, V as the transposed operand from
@@ -27,6 +42,8 @@
 #include "leankv_tq.h"
 #include "tq_attn_q8.cuh"
 #include "tq_kernels.h"
+
+#include <type_traits>
 
 namespace tq {
 
@@ -184,8 +201,11 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead_bytes
 constexpr uint32_t mma_idesc(int n, int tb) { return (1u << 4) | ((uint32_t)tb << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
 
 // DIRECT: codes are converted by warps of the kernel itself
-template <int D, bool DIRECT> struct PromptCfg {
-    static constexpr int QT = D == 128 && !DIRECT ? 2 : 1, KT = D == 128 ? 128 : 64, ROWS = 128 * QT;
+// LO: q' as the sum of two f16 terms, the second one in TMEM (D / 2 columns a row tile: with two row tiles of D = 128
+// they are the columns that scores of 64 instead of 128 tokens leave)
+template <int D, bool DIRECT, bool LO> struct PromptCfg {
+    static constexpr int QT = D == 128 && !DIRECT ? 2 : 1, KT = D == 128 && (DIRECT || !LO) ? 128 : 64, ROWS = 128 * QT;
+    static constexpr int LO_COL = D == 128 && DIRECT ? 384 : 128;
     static constexpr int SEGS = D / 64;                    // 64-element runs of a row
     static constexpr int Q_TILE = 128 * D * 2, KV_TILE = KT * D * 2, SEG = KT * 128;
     static constexpr int SBUF = 2;                         // S buffers: one per row tile, or two of one
@@ -221,10 +241,10 @@ __device__ __forceinline__ float4 block_factors(int blk, float ks, float vs) {
 // blocks' factors [pair][tile][BPT] as float4 (K scale, log2 and reciprocal of the V scale): a score enters the
 // softmax as s * factor.x + factor.y, its weight counts factor.z.  Blocks that are not there (behind the last
 // token, pages outside the pool) get a log2 of -inf: their weights are 0.
-template <int D>
+template <int D, bool LO>
 __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t pair0, int tiles_max, uint8_t* __restrict__ tiles,
                                                         float4* __restrict__ factors) {
-    using C = PromptCfg<D, false>;
+    using C = PromptCfg<D, false, LO>;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tile = blockIdx.x % tiles_max;
     const int64_t slot = blockIdx.x / tiles_max, pair = pair0 + slot;
@@ -270,9 +290,9 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t p
 template <int D>
 __device__ __forceinline__ void convert_tiles(const Q8Run& r, int b, int h, int t_begin, int tiles_n, int kv_end, int cw,
                                               uint32_t k_at, uint32_t v_at, uint32_t k_full, uint32_t k_empty,
-                                              uint32_t v_full, uint32_t v_empty, float4 (*s_fac)[PromptCfg<D, true>::BPT],
+                                              uint32_t v_full, uint32_t v_empty, float4 (*s_fac)[PromptCfg<D, true, false>::BPT],
                                               uint32_t f_full, volatile int* failed) {
-    using C = PromptCfg<D, true>;
+    using C = PromptCfg<D, true, false>;   // the same with LO
     constexpr int NU = 3;
     const int lane = threadIdx.x & 31, sub = lane >> 2, c4 = lane & 3, per_page = r.page_shift - 4;
     const int32_t* pages = r.pages + (int64_t)b * r.max_pages;
@@ -358,12 +378,12 @@ __device__ __forceinline__ void convert_tiles(const Q8Run& r, int b, int h, int 
     }
 }
 
-template <int D, bool DIRECT>
-__global__ void __launch_bounds__(PromptCfg<D, DIRECT>::WARPS * 32, 1)
+template <int D, bool DIRECT, bool LO>
+__global__ void __launch_bounds__(PromptCfg<D, DIRECT, LO>::WARPS * 32, 1)
 attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, const uint8_t* __restrict__ kv_tiles,
                       const float4* __restrict__ factors, int row_tiles, int splits, float* __restrict__ part,
                       float* __restrict__ part_lse) {
-    using C = PromptCfg<D, DIRECT>;
+    using C = PromptCfg<D, DIRECT, LO>;
     constexpr int QT = C::QT, KT = C::KT, TPR = C::TPR, ROWS = C::ROWS, LPR = D / 16, THREADS = C::WARPS * 32;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[20];
@@ -450,11 +470,24 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
         if (r.sm_scale < 0.0f) inv = -inv;   // the row's factor is not negative
         uint32_t w[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = pack_h2(v[2 * j] * inv, v[2 * j + 1] * inv);
+        for (int j = 0; j < 16; ++j) v[j] *= inv;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = pack_h2(v[2 * j], v[2 * j + 1]);
         const int qt = row >> 7, rr = row & 127, c = (e0 & 63) >> 3;
         uint8_t* at = tiles + qt * C::Q_TILE + (e0 >> 6) * (128 * 128) + rr * 128;
         *reinterpret_cast<uint4*>(at + ((c ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         *reinterpret_cast<uint4*>(at + (((c + 1) ^ (rr & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+        if constexpr (LO) {   // what the rounding left goes to TMEM by way of the K and V buffers
+            static_assert(QT * C::Q_TILE <= 4 * C::KV_TILE, "the second terms' way into TMEM");
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                w[j] = pack_h2(v[2 * j] - hi.x, v[2 * j + 1] - hi.y);
+            }
+            at += QT * C::Q_TILE;
+            *reinterpret_cast<uint4*>(at + ((c ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(at + (((c + 1) ^ (rr & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
         if (lane % LPR == 0) {
             s_f[row] = top * fabsf(r.sm_scale) * LOG2E;
             s_lim[row] = live ? last_seen(r, sl, i) : -1;
@@ -466,7 +499,29 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    const uint32_t o_col = 256;   // S buffers at columns 0 and 128 (0 and 64), O from 256 on
+    const uint32_t o_col = 256;   // S buffers at columns 0 and KT, O from 256 on
+    if constexpr (LO) {
+        if (warp < C::SOFT_WARPS) {   // a thread takes half a row, a run of 64 elements at a time
+            const int qt = warp / (4 * TPR), half = (warp >> 2) & 1, rr = (warp & 3) * 32 + lane;
+            const uint8_t* from = tiles + QT * C::Q_TILE + qt * C::Q_TILE + rr * 128;
+            const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::LO_COL + qt * (D / 2);
+#pragma unroll
+            for (int seg = half * (C::SEGS / 2); seg < (half + 1) * (C::SEGS / 2); ++seg) {
+                uint32_t x[32];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(from + seg * (128 * 128) + ((c ^ (rr & 7)) << 4));
+                    x[4 * c] = y.x; x[4 * c + 1] = y.y; x[4 * c + 2] = y.z; x[4 * c + 3] = y.w;
+                }
+                tc_st32(to + 32 * seg, x);
+            }
+            tc_wait_st();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // copies into these buffers come after
+        }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    }
 
     if (warp < C::SOFT_WARPS) {
         // ── softmax: thread = half a row ──
@@ -642,6 +697,11 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)
                     tc_mma_ss(one, d, q + ((j >> 2) * (128 * 128 >> 4) + (j & 3) * 2), k + ((j >> 2) * (C::SEG >> 4) + (j & 3) * 2), id_s, j > 0);
+                if constexpr (LO) {
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j)
+                        tc_mma_ts(one, d, tmem + C::LO_COL + qt * (D / 2) + 8 * j, k + ((j >> 2) * (C::SEG >> 4) + (j & 3) * 2), id_s, 1);
+                }
                 tc_commit(one, s_full + 8 * (QT == 2 ? qt : (t & 1)));
             };
             auto values = [&](int qt, int t) {
@@ -792,18 +852,19 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
 }
 
 // Work memory: partial sums of split units, then the tiles and factors of one pass's pairs.
-template <int D>
+template <int D, bool LO>
 static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, uint8_t* tiles, cudaStream_t st) {
-    using C = PromptCfg<D, false>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    using C = PromptCfg<D, false, LO>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, false, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
-    float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * p.tiles_max * (2 * C::KV_TILE));
+    const int tiles_max = p.tiles_max * (PromptCfg<D, false, false>::KT / C::KT);   // counted in the larger tiles
+    float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * tiles_max * (2 * C::KV_TILE));
     const int64_t pairs = (int64_t)r.B * r.Hkv;
     for (int64_t pair0 = 0; pair0 < pairs; pair0 += p.pairs_pass) {
         const int now = (int)(pairs - pair0 < p.pairs_pass ? pairs - pair0 : p.pairs_pass);
-        const int64_t grid = (int64_t)now * p.row_tiles * p.splits, expand = (int64_t)now * p.tiles_max;
+        const int64_t grid = (int64_t)now * p.row_tiles * p.splits, expand = (int64_t)now * tiles_max;
         if (grid >= (int64_t(1) << 31) || expand >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-        expand_q8_kernel<D><<<(unsigned)expand, 256, 0, st>>>(r, pair0, p.tiles_max, tiles, factors);
+        expand_q8_kernel<D, LO><<<(unsigned)expand, 256, 0, st>>>(r, pair0, tiles_max, tiles, factors);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)grid);
@@ -815,39 +876,44 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
+        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false, LO>, r, pair0, now, tiles_max, (const uint8_t*)tiles,
                                (const float4*)factors, p.row_tiles, p.splits, part, part_lse);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
 }
 
-template <int D>
+template <int D, bool LO>
 static cudaError_t launch_direct_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
-    using C = PromptCfg<D, true>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    using C = PromptCfg<D, true, LO>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, true, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t pairs = (int64_t)r.B * r.Hkv, grid = pairs * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    attn_q8_prompt_kernel<D, true><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, 0, (int)pairs, 0, nullptr, nullptr, p.row_tiles,
+    attn_q8_prompt_kernel<D, true, LO><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, 0, (int)pairs, 0, nullptr, nullptr, p.row_tiles,
                                                                                    p.splits, part, part_lse);
     return cudaGetLastError();
 }
 
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st) {
     uint8_t* t = static_cast<uint8_t*>(tiles);
-    if (p.direct) return r.D == 256 ? launch_direct_d<256>(r, p, part, part_lse, st) : launch_direct_d<128>(r, p, part, part_lse, st);
-    return r.D == 256 ? launch_prompt_d<256>(r, p, part, part_lse, t, st) : launch_prompt_d<128>(r, p, part, part_lse, t, st);
+    const auto run = [&](auto lo) {
+        constexpr bool LO = decltype(lo)::value;
+        if (p.direct) return r.D == 256 ? launch_direct_d<256, LO>(r, p, part, part_lse, st) : launch_direct_d<128, LO>(r, p, part, part_lse, st);
+        return r.D == 256 ? launch_prompt_d<256, LO>(r, p, part, part_lse, t, st) : launch_prompt_d<128, LO>(r, p, part, part_lse, t, st);
+    };
+    // q' as one f16 term where the output has bf16's 8 bits, as two where it has more
+    return r.out_dtype == DT_BF16 ? run(std::false_type()) : run(std::true_type());
 }
 
 int q8_prompt_rows(int D, bool direct) {
-    if (direct) return D == 128 ? PromptCfg<128, true>::ROWS : PromptCfg<256, true>::ROWS;
-    return D == 128 ? PromptCfg<128, false>::ROWS : PromptCfg<256, false>::ROWS;
+    if (direct) return D == 128 ? PromptCfg<128, true, false>::ROWS : PromptCfg<256, true, false>::ROWS;
+    return D == 128 ? PromptCfg<128, false, false>::ROWS : PromptCfg<256, false, false>::ROWS;
 }
 
 // tiles of one pass: all pairs, or as many as 1 GiB holds
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p) {
-    const int kt = D == 128 ? PromptCfg<128, false>::KT : PromptCfg<256, false>::KT;
+    const int kt = D == 128 ? PromptCfg<128, false, false>::KT : PromptCfg<256, false, false>::KT;
     p->tiles_max = (int)((max_len + kt - 1) / kt);
     const int64_t bytes = (int64_t)p->tiles_max * (4 * kt * D + kt);   // two f16 tiles, 16 bytes per 16 tokens
     const int64_t most = bytes > 0 ? (int64_t(1) << 30) / bytes : pairs;
