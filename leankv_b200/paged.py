@@ -246,13 +246,16 @@ class PagedKVCache:
 
     def attention(self, step: Batch, layer: int, q, sm_scale: float | None = None, out_dtype=None, out=None):
         """Attention over each sequence's tokens, this step's included: q [B, n_q_heads, head_dim], one token per
-        sequence, or, with k_bits=8, [B, n_q_heads, n_new, head_dim], each row seeing the tokens up to its own."""
+        sequence (its last), or, with k_bits=8, [B, n_q_heads, n_new, head_dim], each row seeing the tokens up to its
+        own; rows of padding give zeros."""
         from . import attention as A
         if self.k_bits == 8:
             if q.dim() == 4 and q.shape[2] != step.n_new:
                 raise ValueError(f"q must have the step's {step.n_new} tokens")
+            # one row per sequence out of several is the last one; where the step has one row each, some may be padding
+            counts = step.new_len if q.dim() == 4 or step.n_new == 1 else None
             return A.attention_q8_paged(q, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
-                                        step.table, step.kv_len, q_len=step.new_len if q.dim() == 4 else None,
+                                        step.table, step.kv_len, q_len=counts,
                                         max_kv_len=step.max_kv_len, sm_scale=sm_scale, out_dtype=out_dtype or q.dtype, out=out)
         return A.decode_attention_paged(q.contiguous(), self.k[layer], self.v[layer], step.table, step.kv_len,
                                         max_kv_len=step.max_kv_len, sm_scale=sm_scale,

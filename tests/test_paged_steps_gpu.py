@@ -118,3 +118,28 @@ def test_q8_cache_refusals():
     q, k, v = _rows(2, 2, 4, 2, 128, 1)
     with pytest.raises(ValueError):
         opt.append(step, 0, k, v)
+
+
+def test_q8_one_row_each_and_padding():
+    """A step of one row or none for each sequence: a row of padding gives zeros in either shape of q; one row out of a
+    step of several is each sequence's last."""
+    D, hk, grp = 128, 2, 4
+    cache = PagedKVCache(1, hk, D, num_pages=16, page_size=16, max_seqs=2, k_bits=8)
+    rope = ops.Rotary(ops.rotary_frequencies(D, device=DEV))
+    seqs = [cache.add_sequence(), cache.add_sequence()]
+    for seed, counts in enumerate([[20, 33], [1, 0]]):
+        step = cache.batch(seqs, counts)
+        q, k, v = _rows(2, step.n_new, hk * grp, hk, D, seed)
+        q = cache.append(step, 0, k, v, rope=rope, q=q)
+        every = cache.attention(step, 0, q)
+        if step.n_new == 1:
+            one = cache.attention(step, 0, q[:, :, 0])
+            assert torch.equal(one, every[:, :, 0])
+            assert not one[1].any() and one[0].any()
+        else:
+            last = torch.stack([q[b, :, n - 1] for b, n in enumerate(counts)])
+            one = cache.attention(step, 0, last)
+            for b, n in enumerate(counts):   # the same scores in other sums: both are within 2^-8 of the true values' norm
+                x, y = one[b].double(), every[b, :, n - 1].double()
+                assert (x - y).norm() <= 2 * 2.0 ** -8 * y.norm()
+        cache.commit(step)
