@@ -24,6 +24,8 @@ _DTYPES = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16, torch.bfloat1
 # the current stream's handle without the Stream object around it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda device: torch.cuda.current_stream(device).cuda_stream)
+# the current device, without the lazy-initialization check that a CUDA tensor has made already (0.1 instead of 1 us)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream(t: torch.Tensor) -> C.c_void_p:
@@ -253,7 +255,7 @@ def _device_of(*ts) -> int:
 
 def _call(device: int, fn, *args) -> None:
     """A library call on the device's current stream; launches go to the current device."""
-    if device == torch.cuda.current_device():
+    if device == _current_device():
         status = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
