@@ -562,10 +562,16 @@ __device__ __forceinline__ void append_unit(const RotaryAppendRun& r, const Head
     }
 }
 
+// CTAs per SM: 80 registers spill a few bytes of the TQ encoders' for 16-bit rows, and the third CTA hides more of
+// their chains (16384 tokens of 8 + 8 and 32 query heads: 100 us, 111 with two CTAs, 107 with four; a token of 64
+// sequences 10.4, 11.5 and 11.9 us).  32-bit rows (8192 tokens: 102 us with three, 83 with two) and the 8-bit pages'
+// kernels (4 x 2000 tokens: 46.7 and 44.9 us) spill too much.
+template <typename T, int KT> constexpr int APPEND_CTAS = KT != 8 && sizeof(T) == 2 ? 3 : 2;
+
 // Work of a CTA: 16 slot-aligned tokens of one sequence, heads [g * per_group, ...) of the list
 // K heads | V heads | query heads.  The slot alignment gives an 8-bit scale block to one unit.
 template <int D, typename T, int KT>
-__global__ void __launch_bounds__(ROPE_THREADS, 2)
+__global__ void __launch_bounds__(ROPE_THREADS, APPEND_CTAS<T, KT>)
 rotary_append_kernel(const RotaryAppendRun r, int tiles, int groups, int per_group, int tables) {
     constexpr int WPU = D / 128, VT = KT == 8 ? 8 : 4;
     extern __shared__ __align__(16) uint8_t smem[];
