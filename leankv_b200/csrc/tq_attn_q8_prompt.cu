@@ -32,7 +32,7 @@
 // was off by 4.3e-4 of its norm, with two by 2.8e-4 (2.1e-4 is float16's own rounding); the time rises by the
 // products, 118 -> 136 us for pieces of prompts of heads of 256, 597 -> 783 us for the 8192-token prompt (whose tiles
 // shrink to 64 tokens to make room).  In bfloat16, off by 1.7e-3 either way, the second term is left out.  Weights
-// are f16, off by up to 2^-12 of each, which averages out over the tokens.
+// are f16, off by up to 2^-11 of each, which averages out over the tokens.
 //
 // Tiles are runs of 64 elements: [row][128 bytes], 16-byte chunk c of row x at c ^ (x & 7) (the 128-byte
 // swizzle of the matrix descriptors).  K is read with its elements contiguous, V as the transposed operand from

@@ -642,7 +642,9 @@ __global__ void __launch_bounds__(256) dequantize_q8_kernel(const uint4* __restr
 // ── launches ───────────────────────────────────────────────────────────────
 
 // Heads per CTA.  One CTA for all heads of a tile computes the tile's angles once; a batch of few tokens
-// spreads its heads over CTAs instead (down to one unit per warp) until the grid covers the SMs twice.
+// spreads its heads over CTAs instead (down to one unit per warp) until the grid covers the SMs twice.  Where the tiles
+// cover them once, a split that leaves the last CTA under half of the others' heads only adds angles and an uneven
+// end (285 tiles of 18 heads of 256: 30 us as 16 + 2, 20 us whole; 188 tiles: 23 and 19 us).
 static void split_heads(int64_t tiles, int total, int slots, int& groups, int& per_group) {
     const int64_t want = 2 * (int64_t)sm_count();
     int64_t g = (want + tiles - 1) / tiles;
@@ -652,6 +654,10 @@ static void split_heads(int64_t tiles, int total, int slots, int& groups, int& p
     per_group = (int)((total + g - 1) / g);
     per_group = (per_group + slots - 1) / slots * slots;
     groups = (total + per_group - 1) / per_group;
+    if (tiles >= sm_count() && 2 * (total - (groups - 1) * per_group) < per_group) {
+        groups = 1;
+        per_group = total;
+    }
 }
 
 static size_t angle_bytes(const Rope& r) {
@@ -679,7 +685,7 @@ static cudaError_t launch_append(const RotaryAppendRun& r, cudaStream_t st) {
     const int64_t grid = tiles * r.batch * groups;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
     // The level tables (8 KB each) pay when a warp has units of full tiles to search: a 16384-token prompt of 8 + 8
-    // heads and 32 query heads took 119 us with them and 126 us without.  Steps of a few tokens take comparisons.
+    // heads and 32 query heads took 100 us with them and 115 us without.  Steps of a few tokens take comparisons.
     const size_t angles = (angle_bytes(r.rope) + 127) & ~size_t(127);
     const bool table = r.kd.type != 8 && r.n_new >= ROPE_TOKENS;
     const int at = table ? (int)(angles > 0 ? angles : 128) : 0;
