@@ -706,7 +706,10 @@ def run_ours(args, ws, rank, local):
     if rank == 0 and peer_error is None:
         cpu = None
         if ws == 1 and not args.no_cpu_baseline:
-            cpu = time_cpu_sample(args.workload, os.cpu_count() or 1)
+            try:
+                cpu = time_cpu_sample(args.workload, os.cpu_count() or 1)
+            except RuntimeError as e:   # without the reference's C library the sample is left out, not the line
+                cpu = {"unavailable": str(e)}
         is_codec = isinstance(wl, Codec)
         out = {
             "metric": METRIC, "value": round(value, 3), "unit": "GB/s", "n_gpus": ws, "steps": args.steps,
@@ -750,7 +753,10 @@ def run_reference(args, ws, rank):
         return None
     n = os.cpu_count() or 1
     wl = args.workload
-    fn, nbytes, kind, sample = cpu_sample(wl, n)
+    try:
+        fn, nbytes, kind, sample = cpu_sample(wl, n)
+    except RuntimeError as e:
+        return {"impl": "reference", "unavailable": str(e)}
     config = {"workload": WORKLOAD[wl]}
     if wl in ("attn", "c4", "c5"):
         config["shape"] = {"attn": "B=16 Hq=32 Hkv=8 D=128 ctx=32768, fp16 q/out",
