@@ -529,14 +529,16 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int r
 // tcgen05 from tiles expanded once.
 constexpr int DIRECT_ROWS_128 = 49, DIRECT_ROWS_256 = 33, PROMPT_ROWS = 449;
 
-Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
+// lo: q' as the sum of two f16 terms
+Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo) {
     Q8Plan p;
+    p.lo = lo;
     const int64_t rows = n * grp;
     if (rows == 0 || B == 0) return p;
     p.prompt = rows >= (D == 128 ? DIRECT_ROWS_128 : DIRECT_ROWS_256);
     p.direct = rows < PROMPT_ROWS;
     if (p.prompt) {
-        p.rows = q8_prompt_rows(D, p.direct);
+        p.rows = q8_prompt_rows(D, p.direct, lo);
         p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     } else {
         // As few units as the registers allow, alike in size.  More rows share a conversion, but 40 of them leave
@@ -585,11 +587,9 @@ static cudaError_t launch_one(const Q8Run& r, const Q8Plan& p, float* part, floa
     return cudaGetLastError();
 }
 
-// The second term of q' costs 8 to 16 more products a block; where the output has bf16's 8 bits nothing of it would
-// be seen.
 template <int D, int NT>
 static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
-    return r.out_dtype == DT_BF16 ? launch_one<D, NT, false>(r, p, part, part_lse, st) : launch_one<D, NT, true>(r, p, part, part_lse, st);
+    return p.lo ? launch_one<D, NT, true>(r, p, part, part_lse, st) : launch_one<D, NT, false>(r, p, part, part_lse, st);
 }
 
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st) {

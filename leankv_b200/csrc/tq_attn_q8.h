@@ -38,6 +38,7 @@ struct Q8Plan {
     int rows = 16;                 // query rows per unit
     int row_tiles = 1;             // units per (sequence, KV head)
     int splits = 1;
+    bool lo = false;               // q' as two f16 terms
     bool prompt = false;           // the tcgen05 kernel:
     bool direct = false;           // which converts codes itself, or reads tiles from the work memory:
     int tiles_max = 0;             // tiles of a pair's tokens
@@ -45,9 +46,9 @@ struct Q8Plan {
     size_t tile_bytes = 0;
 };
 
-Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len);
+Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo);
 size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p);
-int q8_prompt_rows(int D, bool direct);
+int q8_prompt_rows(int D, bool direct, bool lo);
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p);
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st);
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st);

@@ -23,15 +23,14 @@
 //   1 issuing warp       one elected lane issues all tcgen05.mma
 //   1 loading warp       one lane issues the bulk copies of K and V tiles; DIRECT: 7 converting warps in its place
 // Per tile of KT tokens: S = Q K^T (both from shared memory, f16, fp32 sums in TMEM), weights P in f16 written
-// over S, O += P V (P from TMEM, V from shared memory).  D = 128 from tiles: two row tiles take turns, so that
+// over S, O += P V (P from TMEM, V from shared memory).  D = 128 from tiles, without LO: two row tiles take turns, so that
 // one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).  Otherwise one row tile
 // has two buffers for S: D = 256, whose O alone takes 256 columns and Q 64 KB, takes 64 tokens at a time.
 //
 // Roundings: a row of q' is scaled by its largest element and rounded to f16, for outputs of more than bf16's 8 bits
 // (LO) to the sum of two f16 terms; the second one is read from TMEM.  With one term the float16 answer of 700 rows
 // was off by 4.3e-4 of its norm, with two by 2.8e-4 (2.1e-4 is float16's own rounding); the time rises by the
-// products, 118 -> 136 us for pieces of prompts of heads of 256, 597 -> 783 us for the 8192-token prompt (whose tiles
-// shrink to 64 tokens to make room).  In bfloat16, off by 1.7e-3 either way, the second term is left out.  Weights
+// products, 118 -> 136 us for pieces of prompts of heads of 256, 597 -> 753 us for the 8192-token prompt.  In bfloat16, off by 1.7e-3 either way, the second term is left out.  Weights
 // are f16, off by up to 2^-11 of each, which averages out over the tokens.
 //
 // Tiles are runs of 64 elements: [row][128 bytes], 16-byte chunk c of row x at c ^ (x & 7) (the 128-byte
@@ -201,11 +200,11 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead_bytes
 constexpr uint32_t mma_idesc(int n, int tb) { return (1u << 4) | ((uint32_t)tb << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
 
 // DIRECT: codes are converted by warps of the kernel itself
-// LO: q' as the sum of two f16 terms, the second one in TMEM (D / 2 columns a row tile: with two row tiles of D = 128
-// they are the columns that scores of 64 instead of 128 tokens leave)
+// LO: q' as the sum of two f16 terms, the second one in TMEM (D / 2 columns).  Two row tiles of D = 128 leave no room
+// for it: one takes its place (8192-token prompt 753 us; two of them, 64 tokens at a time, 783 us)
 template <int D, bool DIRECT, bool LO> struct PromptCfg {
-    static constexpr int QT = D == 128 && !DIRECT ? 2 : 1, KT = D == 128 && (DIRECT || !LO) ? 128 : 64, ROWS = 128 * QT;
-    static constexpr int LO_COL = D == 128 && DIRECT ? 384 : 128;
+    static constexpr int QT = D == 128 && !DIRECT && !LO ? 2 : 1, KT = D == 128 ? 128 : 64, ROWS = 128 * QT;
+    static constexpr int LO_COL = D == 128 ? 384 : 128;
     static constexpr int SEGS = D / 64;                    // 64-element runs of a row
     static constexpr int Q_TILE = 128 * D * 2, KV_TILE = KT * D * 2, SEG = KT * 128;
     static constexpr int SBUF = 2;                         // S buffers: one per row tile, or two of one
@@ -241,10 +240,10 @@ __device__ __forceinline__ float4 block_factors(int blk, float ks, float vs) {
 // blocks' factors [pair][tile][BPT] as float4 (K scale, log2 and reciprocal of the V scale): a score enters the
 // softmax as s * factor.x + factor.y, its weight counts factor.z.  Blocks that are not there (behind the last
 // token, pages outside the pool) get a log2 of -inf: their weights are 0.
-template <int D, bool LO>
+template <int D>
 __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t pair0, int tiles_max, uint8_t* __restrict__ tiles,
                                                         float4* __restrict__ factors) {
-    using C = PromptCfg<D, false, LO>;
+    using C = PromptCfg<D, false, false>;   // the same with LO
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tile = blockIdx.x % tiles_max;
     const int64_t slot = blockIdx.x / tiles_max, pair = pair0 + slot;
@@ -502,9 +501,10 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     const uint32_t o_col = 256;   // S buffers at columns 0 and KT, O from 256 on
     if constexpr (LO) {
         if (warp < C::SOFT_WARPS) {   // a thread takes half a row, a run of 64 elements at a time
-            const int qt = warp / (4 * TPR), half = (warp >> 2) & 1, rr = (warp & 3) * 32 + lane;
-            const uint8_t* from = tiles + QT * C::Q_TILE + qt * C::Q_TILE + rr * 128;
-            const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::LO_COL + qt * (D / 2);
+            static_assert(QT == 1, "one row tile's second term has room");
+            const int half = (warp >> 2) & 1, rr = (warp & 3) * 32 + lane;
+            const uint8_t* from = tiles + C::Q_TILE + rr * 128;
+            const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::LO_COL;
 #pragma unroll
             for (int seg = half * (C::SEGS / 2); seg < (half + 1) * (C::SEGS / 2); ++seg) {
                 uint32_t x[32];
@@ -700,7 +700,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
                 if constexpr (LO) {
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j)
-                        tc_mma_ts(one, d, tmem + C::LO_COL + qt * (D / 2) + 8 * j, k + ((j >> 2) * (C::SEG >> 4) + (j & 3) * 2), id_s, 1);
+                        tc_mma_ts(one, d, tmem + C::LO_COL + 8 * j, k + ((j >> 2) * (C::SEG >> 4) + (j & 3) * 2), id_s, 1);
                 }
                 tc_commit(one, s_full + 8 * (QT == 2 ? qt : (t & 1)));
             };
@@ -857,14 +857,13 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
     using C = PromptCfg<D, false, LO>;
     cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, false, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
-    const int tiles_max = p.tiles_max * (PromptCfg<D, false, false>::KT / C::KT);   // counted in the larger tiles
-    float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * tiles_max * (2 * C::KV_TILE));
+    float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * p.tiles_max * (2 * C::KV_TILE));
     const int64_t pairs = (int64_t)r.B * r.Hkv;
     for (int64_t pair0 = 0; pair0 < pairs; pair0 += p.pairs_pass) {
         const int now = (int)(pairs - pair0 < p.pairs_pass ? pairs - pair0 : p.pairs_pass);
-        const int64_t grid = (int64_t)now * p.row_tiles * p.splits, expand = (int64_t)now * tiles_max;
+        const int64_t grid = (int64_t)now * p.row_tiles * p.splits, expand = (int64_t)now * p.tiles_max;
         if (grid >= (int64_t(1) << 31) || expand >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-        expand_q8_kernel<D, LO><<<(unsigned)expand, 256, 0, st>>>(r, pair0, tiles_max, tiles, factors);
+        expand_q8_kernel<D><<<(unsigned)expand, 256, 0, st>>>(r, pair0, p.tiles_max, tiles, factors);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)grid);
@@ -876,7 +875,7 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false, LO>, r, pair0, now, tiles_max, (const uint8_t*)tiles,
+        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false, LO>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
                                (const float4*)factors, p.row_tiles, p.splits, part, part_lse);
         if (e != cudaSuccess) return e;
     }
@@ -902,14 +901,10 @@ cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* p
         if (p.direct) return r.D == 256 ? launch_direct_d<256, LO>(r, p, part, part_lse, st) : launch_direct_d<128, LO>(r, p, part, part_lse, st);
         return r.D == 256 ? launch_prompt_d<256, LO>(r, p, part, part_lse, t, st) : launch_prompt_d<128, LO>(r, p, part, part_lse, t, st);
     };
-    // q' as one f16 term where the output has bf16's 8 bits, as two where it has more
-    return r.out_dtype == DT_BF16 ? run(std::false_type()) : run(std::true_type());
+    return p.lo ? run(std::true_type()) : run(std::false_type());
 }
 
-int q8_prompt_rows(int D, bool direct) {
-    if (direct) return D == 128 ? PromptCfg<128, true, false>::ROWS : PromptCfg<256, true, false>::ROWS;
-    return D == 128 ? PromptCfg<128, false, false>::ROWS : PromptCfg<256, false, false>::ROWS;
-}
+int q8_prompt_rows(int D, bool direct, bool lo) { return D == 128 && !direct && !lo ? PromptCfg<128, false, false>::ROWS : 128; }
 
 // tiles of one pass: all pairs, or as many as 1 GiB holds
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p) {

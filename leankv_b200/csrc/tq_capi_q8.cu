@@ -188,7 +188,8 @@ static tq_status q8_check(const tq_attention_q8_args* a, const tq_kv_pages* pg, 
     r->norm = fwht_norm(a->head_dim);
     r->lse = a->lse; r->status = a->status;
     r->max_len = (int)(a->max_kv_len > 0 ? a->max_kv_len : cap);
-    *p = q8_plan(a->batch, a->n_kv_heads, (int)grp, a->head_dim, a->n_new, a->max_kv_len > 0 ? a->max_kv_len : cap);
+    *p = q8_plan(a->batch, a->n_kv_heads, (int)grp, a->head_dim, a->n_new, a->max_kv_len > 0 ? a->max_kv_len : cap,
+                 a->out_dtype != TQ_DTYPE_BF16);   // a bf16 output has 8 bits: one term of 11 does
     return TQ_SUCCESS;
 }
 
