@@ -538,7 +538,7 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool 
     p.prompt = rows >= (D == 128 ? DIRECT_ROWS_128 : DIRECT_ROWS_256);
     p.direct = rows < PROMPT_ROWS;
     if (p.prompt) {
-        p.rows = q8_prompt_rows(D, p.direct, lo);
+        p.rows = q8_prompt_rows((int64_t)B * Hkv, rows, D, p.direct, lo);
         p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     } else {
         // As few units as the registers allow, alike in size.  More rows share a conversion, but 40 of them leave

@@ -48,7 +48,7 @@ struct Q8Plan {
 
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo);
 size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p);
-int q8_prompt_rows(int D, bool direct, bool lo);
+int q8_prompt_rows(int64_t pairs, int64_t rows, int D, bool direct, bool lo);
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p);
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st);
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st);

@@ -23,7 +23,7 @@
 //   1 issuing warp       one elected lane issues all tcgen05.mma
 //   1 loading warp       one lane issues the bulk copies of K and V tiles; DIRECT: 7 converting warps in its place
 // Per tile of KT tokens: S = Q K^T (both from shared memory, f16, fp32 sums in TMEM), weights P in f16 written
-// over S, O += P V (P from TMEM, V from shared memory).  D = 128 from tiles, without LO: two row tiles take turns, so that
+// over S, O += P V (P from TMEM, V from shared memory).  D = 128 from tiles, where there are enough rows: two row tiles take turns, so that
 // one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).  Otherwise one row tile
 // has two buffers for S: D = 256, whose O alone takes 256 columns and Q 64 KB, takes 64 tokens at a time.
 //
@@ -200,10 +200,9 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lead_bytes
 constexpr uint32_t mma_idesc(int n, int tb) { return (1u << 4) | ((uint32_t)tb << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
 
 // DIRECT: codes are converted by warps of the kernel itself
-// LO: q' as the sum of two f16 terms, the second one in TMEM (D / 2 columns).  Two row tiles of D = 128 leave no room
-// for it: one takes its place (8192-token prompt 753 us; two of them, 64 tokens at a time, 783 us)
-template <int D, bool DIRECT, bool LO> struct PromptCfg {
-    static constexpr int QT = D == 128 && !DIRECT && !LO ? 2 : 1, KT = D == 128 ? 128 : 64, ROWS = 128 * QT;
+// QTILES: row tiles of a CTA; two only with D = 128 from tiles
+template <int D, bool DIRECT, int QTILES> struct PromptCfg {
+    static constexpr int QT = QTILES, KT = D == 128 ? 128 : 64, ROWS = 128 * QT;
     static constexpr int LO_COL = D == 128 ? 384 : 128;
     static constexpr int SEGS = D / 64;                    // 64-element runs of a row
     static constexpr int Q_TILE = 128 * D * 2, KV_TILE = KT * D * 2, SEG = KT * 128;
@@ -243,7 +242,7 @@ __device__ __forceinline__ float4 block_factors(int blk, float ks, float vs) {
 template <int D>
 __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t pair0, int tiles_max, uint8_t* __restrict__ tiles,
                                                         float4* __restrict__ factors) {
-    using C = PromptCfg<D, false, false>;   // the same with LO
+    using C = PromptCfg<D, false, 1>;   // the same with two row tiles
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tile = blockIdx.x % tiles_max;
     const int64_t slot = blockIdx.x / tiles_max, pair = pair0 + slot;
@@ -289,9 +288,9 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const Q8Run r, int64_t p
 template <int D>
 __device__ __forceinline__ void convert_tiles(const Q8Run& r, int b, int h, int t_begin, int tiles_n, int kv_end, int cw,
                                               uint32_t k_at, uint32_t v_at, uint32_t k_full, uint32_t k_empty,
-                                              uint32_t v_full, uint32_t v_empty, float4 (*s_fac)[PromptCfg<D, true, false>::BPT],
+                                              uint32_t v_full, uint32_t v_empty, float4 (*s_fac)[PromptCfg<D, true, 1>::BPT],
                                               uint32_t f_full, volatile int* failed) {
-    using C = PromptCfg<D, true, false>;   // the same with LO
+    using C = PromptCfg<D, true, 1>;
     constexpr int NU = 3;
     const int lane = threadIdx.x & 31, sub = lane >> 2, c4 = lane & 3, per_page = r.page_shift - 4;
     const int32_t* pages = r.pages + (int64_t)b * r.max_pages;
@@ -377,12 +376,13 @@ __device__ __forceinline__ void convert_tiles(const Q8Run& r, int b, int h, int 
     }
 }
 
-template <int D, bool DIRECT, bool LO>
-__global__ void __launch_bounds__(PromptCfg<D, DIRECT, LO>::WARPS * 32, 1)
+// LO: q' as the sum of two f16 terms, the second one in TMEM (D / 2 columns, for which two row tiles leave no room)
+template <int D, bool DIRECT, int QTILES, bool LO>
+__global__ void __launch_bounds__(PromptCfg<D, DIRECT, QTILES>::WARPS * 32, 1)
 attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, const uint8_t* __restrict__ kv_tiles,
                       const float4* __restrict__ factors, int row_tiles, int splits, float* __restrict__ part,
                       float* __restrict__ part_lse) {
-    using C = PromptCfg<D, DIRECT, LO>;
+    using C = PromptCfg<D, DIRECT, QTILES>;
     constexpr int QT = C::QT, KT = C::KT, TPR = C::TPR, ROWS = C::ROWS, LPR = D / 16, THREADS = C::WARPS * 32;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[20];
@@ -852,10 +852,10 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
 }
 
 // Work memory: partial sums of split units, then the tiles and factors of one pass's pairs.
-template <int D, bool LO>
+template <int D, int QTILES, bool LO>
 static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, uint8_t* tiles, cudaStream_t st) {
-    using C = PromptCfg<D, false, LO>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, false, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    using C = PromptCfg<D, false, QTILES>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, false, QTILES, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * p.tiles_max * (2 * C::KV_TILE));
     const int64_t pairs = (int64_t)r.B * r.Hkv;
@@ -875,7 +875,7 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false, LO>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
+        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false, QTILES, LO>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
                                (const float4*)factors, p.row_tiles, p.splits, part, part_lse);
         if (e != cudaSuccess) return e;
     }
@@ -884,12 +884,12 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
 
 template <int D, bool LO>
 static cudaError_t launch_direct_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
-    using C = PromptCfg<D, true, LO>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, true, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    using C = PromptCfg<D, true, 1>;
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, true, 1, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t pairs = (int64_t)r.B * r.Hkv, grid = pairs * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    attn_q8_prompt_kernel<D, true, LO><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, 0, (int)pairs, 0, nullptr, nullptr, p.row_tiles,
+    attn_q8_prompt_kernel<D, true, 1, LO><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, 0, (int)pairs, 0, nullptr, nullptr, p.row_tiles,
                                                                                    p.splits, part, part_lse);
     return cudaGetLastError();
 }
@@ -899,16 +899,24 @@ cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* p
     const auto run = [&](auto lo) {
         constexpr bool LO = decltype(lo)::value;
         if (p.direct) return r.D == 256 ? launch_direct_d<256, LO>(r, p, part, part_lse, st) : launch_direct_d<128, LO>(r, p, part, part_lse, st);
-        return r.D == 256 ? launch_prompt_d<256, LO>(r, p, part, part_lse, t, st) : launch_prompt_d<128, LO>(r, p, part, part_lse, t, st);
+        return r.D == 256 ? launch_prompt_d<256, 1, LO>(r, p, part, part_lse, t, st) : launch_prompt_d<128, 1, LO>(r, p, part, part_lse, t, st);
     };
+    if (p.rows == 256) return launch_prompt_d<128, 2, false>(r, p, part, part_lse, t, st);
     return p.lo ? run(std::true_type()) : run(std::false_type());
 }
 
-int q8_prompt_rows(int D, bool direct, bool lo) { return D == 128 && !direct && !lo ? PromptCfg<128, false, false>::ROWS : 128; }
+// Query rows of a CTA.  Two row tiles of D = 128 hide each other's softmax and products (8192-token prompt 597 us, with
+// one 734 us), where there are enough of them: under half of the SMs, more and smaller CTAs end sooner (256 tokens of 32
+// heads 15 us, with two 22 us; 512: 18 and 26 us; from 80 CTAs of two on two are faster: 300 tokens of two sequences
+// behind 4000 103 and 115 us, 1024 tokens 35 and 37 us).  With q' as two terms there is no room for a second one in TMEM
+// (with 64 tokens at a time there is: 783 us for the 8192-token prompt, with one row tile 750 us).
+int q8_prompt_rows(int64_t pairs, int64_t rows, int D, bool direct, bool lo) {
+    return D == 128 && !direct && !lo && 2 * pairs * ((rows + 255) / 256) >= sm_count() ? 256 : 128;
+}
 
 // tiles of one pass: all pairs, or as many as 1 GiB holds
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p) {
-    const int kt = D == 128 ? PromptCfg<128, false, false>::KT : PromptCfg<256, false, false>::KT;
+    const int kt = D == 128 ? PromptCfg<128, false, 1>::KT : PromptCfg<256, false, 1>::KT;
     p->tiles_max = (int)((max_len + kt - 1) / kt);
     const int64_t bytes = (int64_t)p->tiles_max * (4 * kt * D + kt);   // two f16 tiles, 16 bytes per 16 tokens
     const int64_t most = bytes > 0 ? (int64_t(1) << 30) / bytes : pairs;
