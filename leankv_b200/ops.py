@@ -241,6 +241,7 @@ _ROPE = struct.Struct(_ROPE_FMT)                      # tq_rope
 _HEADS = struct.Struct(_HEADS_FMT)                    # tq_head_rows
 _APPEND = struct.Struct("iiiqi0q" + 3 * _HEADS_FMT + _ROPE_FMT + "PiPPiPPPiP")   # tq_rotary_append_args
 _PAGES = struct.Struct("Pqqi")                        # tq_kv_pages
+_TYPE_OF_BYTES = {n: t for t, n in BLOCK_BYTES.items()}
 _NO_HEADS, _NO_ROPE = (0,) * 9, (0, 0, 0, 0, 0, 0, 0, 0.0)
 
 def _device_of(*ts) -> int:
@@ -393,7 +394,7 @@ def kv_append_rotary_paged(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tenso
         pages, page_size = _check_q8_pools(k_pool, v_pool, k_scale, v_scale, H, D)
         k_sc, v_sc = k_scale.data_ptr(), v_scale.data_ptr()
     else:
-        kt, vt = {n: t for t, n in BLOCK_BYTES.items()}.get(k_pool.shape[-1]), TQ4_0
+        kt, vt = _TYPE_OF_BYTES.get(k_pool.shape[-1]), TQ4_0
         pages, page_size = (k_pool.shape[0], k_pool.shape[2]) if k_pool.dim() == 5 else (0, 0)
         if k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 or kt is None \
                 or k_pool.shape != (pages, H, page_size, D // QK, BLOCK_BYTES[kt]) or not k_pool.is_contiguous() \
