@@ -22,16 +22,18 @@
 //                        TMEM, the output's rescaling
 //   1 issuing warp       one elected lane issues all tcgen05.mma
 //   1 loading warp       one lane issues the bulk copies of K and V tiles; DIRECT: 7 converting warps in its place
-// Per tile of KT tokens: S = Q K^T (both from shared memory, f16, fp32 sums in TMEM), weights P in f16 written
-// over S, O += P V (P from TMEM, V from shared memory).  D = 128 from tiles, where there are enough rows: two row tiles take turns, so that
-// one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).  Otherwise one row tile
-// has two buffers for S: D = 256, whose O alone takes 256 columns and Q 64 KB, takes 64 tokens at a time.
+// Per tile of KT tokens: S = Q K^T (both from shared memory, f16, fp32 sums in TMEM), weights P in f16 written over
+// S, O += P V (P from TMEM, V from shared memory).  D = 128 from tiles, where there are enough rows: two row tiles
+// take turns, so that one's softmax runs while the other's products do; TMEM holds S and O of both (512 columns).
+// Otherwise one row tile has two buffers for S: D = 256, whose O alone takes 256 columns and Q 64 KB, takes 64
+// tokens at a time.
 //
-// Roundings: a row of q' is scaled by its largest element and rounded to f16, for outputs of more than bf16's 8 bits
-// (LO) to the sum of two f16 terms; the second one is read from TMEM.  With one term the float16 answer of 700 rows
-// was off by 4.3e-4 of its norm, with two by 2.8e-4 (2.1e-4 is float16's own rounding); the time rises by the
-// products, 118 -> 136 us for pieces of prompts of heads of 256, 597 -> 753 us for the 8192-token prompt.  In bfloat16, off by 1.7e-3 either way, the second term is left out.  Weights
-// are f16, off by up to 2^-11 of each, which averages out over the tokens.
+// Roundings: a row of q' is scaled by its largest element and rounded to f16, for outputs of more than bf16's 8
+// bits (LO) to the sum of two f16 terms; the second one is read from TMEM.  With one term the float16 answer of 700
+// rows was off by 4.3e-4 of its norm, with two by 2.8e-4 (2.1e-4 is float16's own rounding); the time rises by the
+// products, 118 -> 136 us for pieces of prompts of heads of 256, 597 -> 753 us for the 8192-token prompt.  In
+// bfloat16, off by 1.7e-3 either way, the second term is left out.  Weights are f16, off by up to 2^-11 of each,
+// which averages out over the tokens.
 //
 // Tiles are runs of 64 elements: [row][128 bytes], 16-byte chunk c of row x at c ^ (x & 7) (the 128-byte
 // swizzle of the matrix descriptors).  K is read with its elements contiguous, V as the transposed operand from
