@@ -366,8 +366,8 @@ tq_status tq_kv_append_paged_cuda(tq_type type, const void *src, tq_dtype src_dt
  * angle p * inv_freq[i], p the token's position on axis axis[i]:
  *   (a, b) -> (a cos - b sin, b cos + a sin),   cos and sin times scale;
  * elements from rotary_dim on stay as they are.  inverse turns back, which is also the rotation's gradient
- * (scale included).  Angles are exact for every int32 position: the cosines and sines are those of 64-bit
- * arithmetic rounded to float32.  inv_freq is float64 device memory: any frequencies (a base, a scaling
+ * (scale included).  Angles keep 64 bits of a turn at every int32 position (within 3e-13 at a million radians, where
+ * a 64-bit product p * inv_freq is off by up to 1e-10): cosines and sines are the true values rounded to float32.  inv_freq is float64 device memory: any frequencies (a base, a scaling
  * rule, one set per axis) come as values.  |inv_freq| must be below 2^31.  axis entries outside
  * [0, n_axes) read the nearest axis.
  */
