@@ -477,7 +477,10 @@ __device__ __forceinline__ void append_unit(const RotaryAppendRun& r, const Head
 #pragma unroll
         for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         float* sp = dst.scale + (at >> 4);
-        const float s_old = older > 0 ? *sp : 0.0f;
+        // read by the lane that stores the new scale below, so that no lane can meet the new one
+        float s_old = 0.0f;
+        if (older > 0 && lane == 0) s_old = *sp;
+        s_old = __shfl_sync(0xffffffffu, s_old, 0);
         if constexpr (WPU == 2) {
             // the two warps of the unit exchange their maxima; the old scale has been read by both
             if (lane == 0) s_amax[sub] = amax;
