@@ -39,10 +39,12 @@
 // swizzle of the matrix descriptors).  K is read with its elements contiguous, V as the transposed operand from
 // the same layout.  Codes are exact in f16; scales never touch the tiles: they enter with the scores.
 //
-// Every wait gives up after about a second (status TQ_ERROR_TIMEOUT) instead of hanging.
+// Every wait gives up after about a second (status TQ_ERROR_TIMEOUT) instead of hanging; copies and products that were
+// issued before are waited for (tq_wait.h).
 #include "leankv_tq.h"
 #include "tq_attn_q8.cuh"
 #include "tq_kernels.h"
+#include "tq_wait.h"
 
 #include <type_traits>
 
@@ -69,28 +71,17 @@ __device__ __forceinline__ uint64_t now_ns() {
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-constexpr uint64_t WAIT_NS = 1000000000ull;
 // waits for the phase of `parity`; false once any wait of the CTA has run out
 __device__ __forceinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int* failed) {
-    const uint64_t until = now_ns() + WAIT_NS;
-    while (!mbar_try(bar, parity)) {
-        if (*failed) return false;
-        if (now_ns() > until) {
-            *failed = 1;
-            return false;
-        }
-    }
-    return true;
+    return wait_turn([=] { return mbar_try(bar, parity); }, [] { return now_ns(); }, failed);
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* failed) {
     if (mbar_try(bar, parity)) return true;
     return mbar_wait_long(bar, parity, failed);
 }
-// waits for a bulk copy (at most the same time), whether or not another wait has run out
-__device__ __forceinline__ void mbar_wait_copy(uint32_t bar, uint32_t parity) {
-    const uint64_t until = now_ns() + WAIT_NS;
-    while (!mbar_try(bar, parity) && now_ns() < until) {
-    }
+// waits for a bulk copy or for products that have been issued, whether or not another wait has run out
+__device__ __forceinline__ bool mbar_wait_issued(uint32_t bar, uint32_t parity) {
+    return wait_issued([=] { return mbar_try(bar, parity); }, [] { return now_ns(); });
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -783,21 +774,21 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
             }
             // no copy is in flight when the CTA ends, whatever became of the other warps
             for (int i = nk - 2; i < nk; ++i)
-                if (i >= 0) mbar_wait_copy(k_full + 8 * (i & 1), (i >> 1) & 1);
+                if (i >= 0) mbar_wait_issued(k_full + 8 * (i & 1), (i >> 1) & 1);
             for (int i = nk - 4; i < nk; ++i)
-                if (i >= 0) mbar_wait_copy(f_full + 8 * (i & 3), (i >> 2) & 1);
+                if (i >= 0) mbar_wait_issued(f_full + 8 * (i & 3), (i >> 2) & 1);
             for (int i = nv - 2; i < nv; ++i)
-                if (i >= 0) mbar_wait_copy(v_full + 8 * (i & 1), (i >> 1) & 1);
+                if (i >= 0) mbar_wait_issued(v_full + 8 * (i & 1), (i >> 1) & 1);
         }
         __syncwarp();
     }
 
-    // ── the output rows: O / l through shared memory (the tiles are free once all products are done) ──
-    bool fine = true;
-    if (tiles_n > 0) fine = mbar_wait(done, 0, &s_failed);
+    // ── the output rows: O / l through shared memory (the tiles are free once all products are done, which is waited
+    // for after a failed wait, too: the products that were issued before it still read the tiles and write TMEM) ──
+    if (tiles_n > 0 && !mbar_wait_issued(done, 0)) s_failed = 1;
     tc_fence_after();
     __syncthreads();
-    fine = fine && s_failed == 0;
+    const bool fine = s_failed == 0;
     float* rows = reinterpret_cast<float*>(tiles);
     // chunk c (4 floats) of a row at c ^ (row & 7)
     if (warp < C::SOFT_WARPS) {
