@@ -450,7 +450,8 @@ tq_status tq_dequantize_q8_cuda(const int8_t *codes, const float *scale, void *y
  * head_dim 128 or 256, any n_q_heads / n_kv_heads, page_size a power of two in 16 .. 65536.  A page id
  * outside the pool that holds tokens a row would see is treated as holding none, and TQ_ERROR_INVALID_VALUE is
  * stored in *status; so it is when a sequence is longer than max_kv_len and tokens behind that bound are left out
- * (kernels for many rows).  A wait inside a kernel that runs out (about a second) stores TQ_ERROR_TIMEOUT.  Work
+ * (kernels for many rows).  A wait inside a kernel that runs out (about a second) stores TQ_ERROR_TIMEOUT and makes NaN
+ * of the rows and log-sum-exps that it was for.  Work
  * memory: tq_attention_q8_workspace_size() bytes, written before they are read; calls that can overlap need their own.
  */
 typedef struct {

@@ -794,6 +794,9 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     if (warp < C::SOFT_WARPS) {
         const int qt = warp / (4 * TPR), half = TPR == 2 ? (warp >> 2) & 1 : 0, row = qt * 128 + (warp & 3) * 32 + lane;
         const uint32_t o_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + o_col + qt * 128;
+        // a failed wait's rows are NaN, and the log-sum-exp of a split's is +inf, which makes NaN of what the merge joins
+        // with it: nothing that a caller could take for an answer
+        if (!fine && half == 0) s_lse[row] = splits > 1 ? INFINITY : NAN;
         const float inv = s_f[row];
 #pragma unroll 1
         for (int c = half * (D / TPR / 32); c < (half + 1) * (D / TPR / 32); ++c) {
@@ -810,6 +813,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
                 float4 y = make_float4(__uint_as_float(x[4 * j]) * inv, __uint_as_float(x[4 * j + 1]) * inv,
                                        __uint_as_float(x[4 * j + 2]) * inv, __uint_as_float(x[4 * j + 3]) * inv);
                 if (inv == 0.0f) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (!fine) y = make_float4(NAN, NAN, NAN, NAN);
                 reinterpret_cast<float4*>(rows + row * D)[(8 * c + j) ^ (row & 7)] = y;
             }
         }
