@@ -447,7 +447,8 @@ tq_status tq_dequantize_q8_cuda(const int8_t *codes, const float *scale, void *y
  * token), rows on 16-byte boundaries.  Products are f16 with fp32 sums: q' is scaled by its row's maximum and
  * rounded to f16 (to the sum of two f16 terms when out_dtype is not bf16), codes are exact, weights are rounded to
  * f16, statistics are fp32; a float32 output is exact to about 2e-4 of its norm.  q must be finite.
- * head_dim 128 or 256, any n_q_heads / n_kv_heads, page_size a power of two in 16 .. 65536.  A page id
+ * head_dim 128 or 256, any n_q_heads / n_kv_heads, page_size a power of two in 16 .. 65536; capacity and
+ * n_new * n_q_heads / n_kv_heads at most 2^30, batch * n_kv_heads below 2^31, query rows at most 2^40.  A page id
  * outside the pool that holds tokens a row would see is treated as holding none, and TQ_ERROR_INVALID_VALUE is
  * stored in *status; so it is when a sequence is longer than max_kv_len and tokens behind that bound are left out
  * (kernels for many rows).  A wait inside a kernel that runs out (about a second) stores TQ_ERROR_TIMEOUT and makes NaN

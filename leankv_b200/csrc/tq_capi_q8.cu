@@ -168,8 +168,13 @@ static tq_status q8_check(const tq_attention_q8_args* a, const tq_kv_pages* pg, 
     tq_status s = pages_check(pg, a->batch, &shift);
     if (s) return s;
     const int64_t cap = pg->max_pages_per_seq << shift, grp = a->n_q_heads / a->n_kv_heads;
-    if (pg->max_pages_per_seq > (int64_t(1) << 30) || cap > (int64_t(1) << 30) || a->n_new * grp > (int64_t(1) << 30))
+    constexpr int64_t MOST = int64_t(1) << 30, MOST_ROWS = int64_t(1) << 40;
+    if (pg->max_pages_per_seq > MOST || cap > MOST || a->n_new > MOST || a->n_new * grp > MOST)
         return set_error(TQ_ERROR_UNSUPPORTED, "capacity and rows per head must be at most 2^30");
+    // the grid has a CTA for each pair, and the work split's products of rows stay within 64 bits
+    const int64_t pairs = (int64_t)a->batch * a->n_kv_heads;
+    if (pairs > INT32_MAX || (a->n_new > 0 && pairs > MOST_ROWS / (a->n_new * grp)))
+        return set_error(TQ_ERROR_UNSUPPORTED, "batch * n_kv_heads must be below 2^31, query rows at most 2^40");
     if (a->max_kv_len < 0 || a->max_kv_len > cap) return set_error(TQ_ERROR_INVALID_VALUE, "max_kv_len outside [0, capacity]");
     if (!std::isfinite(a->sm_scale)) return set_error(TQ_ERROR_INVALID_VALUE, "sm_scale is not finite");
     r->B = a->batch; r->Hq = a->n_q_heads; r->Hkv = a->n_kv_heads; r->grp = (int)grp; r->D = a->head_dim;
