@@ -390,7 +390,7 @@ typedef struct {
 } tq_head_rows;
 
 /* Rotates x (and x2, optional: e.g. queries and keys) in one launch; dst may be src (with its strides).
- * head_dim: a multiple of 8, at most 512. */
+ * head_dim: a multiple of 8, at most 512; at most 2^24 heads together. */
 tq_status tq_rotary_cuda(const tq_rope *rope, tq_dtype dtype, int batch, int64_t n_new, int head_dim,
                          const tq_head_rows *x, const tq_head_rows *x2, void *stream);
 
@@ -411,7 +411,8 @@ tq_status tq_rotary_cuda(const tq_rope *rope, tq_dtype dtype, int batch, int64_t
  * max |x| / 127 over the rows stored in the block.  It starts anew when slot 0 of the block is written and
  * grows when a later row needs it; then the block's earlier codes are rounded to the new scale.  Slots
  * behind the last row keep their codes.  Scales below 2^-100 are stored as 0.  Inputs must be finite.
- * head_dim 128 or 256.  Two sequences of a call must not share a page that they write.
+ * head_dim 128 or 256; at most 2^24 key, value and query heads together.  Two sequences of a call must not share a
+ * page that they write.
  */
 #define TQ_Q8_BLOCK 16
 typedef struct {
@@ -431,7 +432,7 @@ typedef struct {
 } tq_rotary_append_args;
 tq_status tq_kv_append_rotary_paged_cuda(const tq_rotary_append_args *a, const tq_kv_pages *pages, void *stream);
 /* values of n_blocks 16-token blocks of 8-bit pages: y[i] = codes[i] * scale[i / (16 head_dim)], rounded to
- * y_dtype; head_dim 128 or 256 */
+ * y_dtype; head_dim 128 or 256, n_blocks at most 2^40 */
 tq_status tq_dequantize_q8_cuda(const int8_t *codes, const float *scale, void *y, tq_dtype y_dtype,
                                 int64_t n_blocks, int head_dim, void *stream);
 

@@ -9,6 +9,9 @@
 
 using namespace tq;
 
+// heads of all tensors of a call: their sums and the work split's stay within 32 bits
+constexpr int64_t MOST_HEADS = int64_t(1) << 24;
+
 // rows of 8 elements at a time: base and strides on 16-byte boundaries
 static tq_status rows_check(const tq_head_rows* x, bool has_dst, size_t eb, const char* name) {
     if (x->heads <= 0) return set_error(TQ_ERROR_INVALID_VALUE, "%s: bad head count", name);
@@ -67,6 +70,7 @@ extern "C" tq_status tq_rotary_cuda(const tq_rope* rope, tq_dtype dtype, int bat
     tq_status s = rope_check(rope, head_dim, batch > 0 && n_new > 0, &r.rope);
     if (s) return s;
     if (batch == 0 || n_new == 0) return TQ_SUCCESS;
+    if ((int64_t)x->heads + (x2 ? x2->heads : 0) > MOST_HEADS) return set_error(TQ_ERROR_UNSUPPORTED, "more than 2^24 heads");
     if ((s = rows_check(x, true, dtype_bytes(dtype), "x"))) return s;
     if (x2 && (s = rows_check(x2, true, dtype_bytes(dtype), "x2"))) return s;
     r.batch = batch;
@@ -108,6 +112,7 @@ extern "C" tq_status tq_kv_append_rotary_paged_cuda(const tq_rotary_append_args*
     if (a->k.heads != a->n_kv_heads || a->v.heads != a->n_kv_heads)
         return set_error(TQ_ERROR_INVALID_VALUE, "k and v must have n_kv_heads heads");
     if (a->q.heads < 0) return set_error(TQ_ERROR_INVALID_VALUE, "bad query head count");
+    if (2 * (int64_t)a->n_kv_heads + a->q.heads > MOST_HEADS) return set_error(TQ_ERROR_UNSUPPORTED, "more than 2^24 heads");
     if ((s = rows_check(&a->k, false, eb, "k")) || (s = rows_check(&a->v, false, eb, "v"))) return s;
     if (a->q.heads > 0 && (s = rows_check(&a->q, true, eb, "q"))) return s;
     if (!a->k_pool || !a->v_pool || (q8 && (!a->k_scale || !a->v_scale))) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
@@ -146,6 +151,7 @@ extern "C" tq_status tq_dequantize_q8_cuda(const int8_t* codes, const float* sca
     if (!dtype_ok(y_dtype)) return set_error(TQ_ERROR_INVALID_VALUE, "unknown output dtype %d", (int)y_dtype);
     if (head_dim != 128 && head_dim != 256) return set_error(TQ_ERROR_UNSUPPORTED, "head_dim %d (supported: 128, 256)", head_dim);
     if (n_blocks < 0) return set_error(TQ_ERROR_INVALID_VALUE, "n_blocks=%lld", (long long)n_blocks);
+    if (n_blocks > (int64_t(1) << 40)) return set_error(TQ_ERROR_UNSUPPORTED, "n_blocks=%lld (at most 2^40)", (long long)n_blocks);
     if (n_blocks == 0) return TQ_SUCCESS;
     if (!codes || !scale || !y) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
     if ((((uintptr_t)codes | (uintptr_t)y) & 15) || ((uintptr_t)scale & 3))
