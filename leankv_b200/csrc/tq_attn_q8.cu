@@ -473,20 +473,20 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
 }
 
 // Merge of the splits' normalized partial rows by their log-sum-exp, in split order, then the Hadamard
-// transform and the output type.  D / 16 lanes take a row.
+// transform and the output type, for `pairs` pairs from pair0 on.  D / 16 lanes take a row.
 template <int D>
-__global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int rows, int row_tiles, int splits,
-                                                            const float* __restrict__ part,
+__global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int64_t pair0, int pairs, int rows, int row_tiles,
+                                                            int splits, const float* __restrict__ part,
                                                             const float* __restrict__ part_lse) {
     constexpr int LPR = D / 16, RPC = 128 / LPR;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int total_rows = (int)r.n * r.grp;
-    const int64_t all = (int64_t)r.B * r.Hkv * total_rows;
+    const int64_t all = (int64_t)pairs * total_rows;
     const int64_t id = (int64_t)blockIdx.x * RPC + threadIdx.x / LPR;
     const int e0 = (threadIdx.x % LPR) * 16;
-    const int64_t pair = id < all ? id / total_rows : 0;
-    const int gr = id < all ? (int)(id - pair * total_rows) : 0;
-    const int64_t unit = pair * row_tiles + gr / rows;
+    const int64_t slot = id < all ? id / total_rows : 0, pair = pair0 + slot;
+    const int gr = id < all ? (int)(id - slot * total_rows) : 0;
+    const int64_t unit = slot * row_tiles + gr / rows;
     const float* pl = part_lse + unit * splits * rows + gr % rows;
     float top = -INFINITY;
     for (int s = 0; s < splits; ++s) top = fmaxf(top, pl[(int64_t)s * rows]);
@@ -533,12 +533,17 @@ constexpr int DIRECT_ROWS_128 = 49, DIRECT_ROWS_256 = 33, PROMPT_ROWS = 449;
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo) {
     Q8Plan p;
     p.lo = lo;
-    const int64_t rows = n * grp;
+    const int64_t rows = n * grp, len = max_len > 0 ? max_len : 1;
     if (rows == 0 || B == 0) return p;
     p.prompt = rows >= (D == 128 ? DIRECT_ROWS_128 : DIRECT_ROWS_256);
     p.direct = rows < PROMPT_ROWS;
+    // pairs that run at a time: where the work memory does not hold all pairs' tiles, the passes follow one another,
+    // and rows and splits have to fill the SMs in each (72 pairs of 480 rows behind up to 131072 tokens run 15 at a
+    // time: planned for all 72 at once they were 5 passes of 30 CTAs)
+    p.pairs_pass = B * Hkv;
+    if (p.prompt && !p.direct) q8_prompt_tiles((int64_t)B * Hkv, D, len, &p);
     if (p.prompt) {
-        p.rows = q8_prompt_rows((int64_t)B * Hkv, rows, D, p.direct, lo);
+        p.rows = q8_prompt_rows(p.pairs_pass, rows, D, p.direct, lo);
         p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     } else {
         // As few units as the registers allow, alike in size.  More rows share a conversion, but 40 of them leave
@@ -548,14 +553,13 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool 
         p.row_tiles = (int)((rows + most - 1) / most);
         p.rows = (int)((rows + 8 * p.row_tiles - 1) / (8 * p.row_tiles)) * 8;
     }
-    const int64_t units = (int64_t)B * Hkv * p.row_tiles;
+    const int64_t units = (int64_t)p.pairs_pass * p.row_tiles;
     const int64_t slots = (int64_t)sm_count() * (D == 128 && p.rows == 8 ? 2 : 1);
     // Splits: a CTA's time is its tokens plus a start worth `start` tokens and, when split, the writing and merging of
     // its partial rows worth `join`; the grid runs in waves of `slots` CTAs.  Take the number with the least
     // waves * (tokens + start).  Two CTAs share an SM and hide each other's starts where units have 8 rows
     // (16 x 32768 tokens: 172 us with 1024, 179 us with 384); with one CTA per SM, lengths that differ want more and
     // shorter splits (24 sequences of up to 9000 tokens, 40 rows: 118 us with 384, 129 us with 1024).
-    const int64_t len = max_len > 0 ? max_len : 1;
     const int64_t start = p.prompt ? 768 : (slots > sm_count() ? 1024 : 384), join = p.prompt ? 512 : 0;
     int64_t best = INT64_MAX;
     for (int s = 1; s <= 256; ++s) {
@@ -565,16 +569,16 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool 
         if (cost < best) { best = cost; p.splits = s; }
         if (waves > 8) break;   // finer splits only add starts
     }
-    if (p.prompt && !p.direct) q8_prompt_tiles((int64_t)B * Hkv, D, len, &p);
     return p;
 }
 
-// work memory: the splits' partial rows and their lse, then a prompt's tiles
-static size_t part_bytes(int B, int Hkv, int D, const Q8Plan& p) {
+// work memory of one pass: the splits' partial rows and their lse, then a prompt's tiles
+static size_t part_rows(const Q8Plan& p) { return (size_t)p.pairs_pass * p.row_tiles * p.splits * p.rows; }
+static size_t part_bytes(int D, const Q8Plan& p) {
     if (p.splits <= 1) return 0;
-    return ((size_t)B * Hkv * p.row_tiles * p.splits * p.rows * (D + 1) * 4 + 255) & ~size_t(255);
+    return (part_rows(p) * (D + 1) * 4 + 255) & ~size_t(255);
 }
-size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p) { return part_bytes(B, Hkv, D, p) + p.tile_bytes; }
+size_t q8_workspace_bytes(int D, const Q8Plan& p) { return part_bytes(D, p) + p.tile_bytes; }
 
 template <int D, int NT, bool LO>
 static cudaError_t launch_one(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
@@ -592,17 +596,9 @@ static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, flo
     return p.lo ? launch_one<D, NT, true>(r, p, part, part_lse, st) : launch_one<D, NT, false>(r, p, part, part_lse, st);
 }
 
-cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st) {
-    float* part = static_cast<float*>(workspace);
-    float* part_lse = part + (size_t)r.B * r.Hkv * p.row_tiles * p.splits * p.rows * r.D;
-    cudaError_t e;
-    if (p.prompt) e = launch_attention_q8_prompt(r, p, part, part_lse, static_cast<uint8_t*>(workspace) + part_bytes(r.B, r.Hkv, r.D, p), st);
-    else if (r.D == 256) e = p.rows == 8 ? launch_rows<256, 1>(r, p, part, part_lse, st) : launch_rows<256, 2>(r, p, part, part_lse, st);
-    else if (p.rows == 8) e = launch_rows<128, 1>(r, p, part, part_lse, st);
-    else if (p.rows == 16) e = launch_rows<128, 2>(r, p, part, part_lse, st);
-    else e = launch_rows<128, 3>(r, p, part, part_lse, st);
-    if (e != cudaSuccess || p.splits <= 1) return e;
-    const int64_t rows = (int64_t)r.B * r.Hq * r.n, rpc = 128 / (r.D / 16);
+cudaError_t launch_q8_merge(const Q8Run& r, const Q8Plan& p, int64_t pair0, int pairs, const float* part, const float* part_lse,
+                            cudaStream_t st) {
+    const int64_t rows = (int64_t)pairs * r.grp * r.n, rpc = 128 / (r.D / 16);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((rows + rpc - 1) / rpc));
     cfg.blockDim = dim3(128);
@@ -612,8 +608,21 @@ cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (r.D == 256) return cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<256>, r, p.rows, p.row_tiles, p.splits, (const float*)part, (const float*)part_lse);
-    return cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<128>, r, p.rows, p.row_tiles, p.splits, (const float*)part, (const float*)part_lse);
+    if (r.D == 256) return cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<256>, r, pair0, pairs, p.rows, p.row_tiles, p.splits, part, part_lse);
+    return cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<128>, r, pair0, pairs, p.rows, p.row_tiles, p.splits, part, part_lse);
+}
+
+cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st) {
+    float* part = static_cast<float*>(workspace);
+    float* part_lse = part + part_rows(p) * r.D;
+    cudaError_t e;
+    if (p.prompt) return launch_attention_q8_prompt(r, p, part, part_lse, static_cast<uint8_t*>(workspace) + part_bytes(r.D, p), st);
+    if (r.D == 256) e = p.rows == 8 ? launch_rows<256, 1>(r, p, part, part_lse, st) : launch_rows<256, 2>(r, p, part, part_lse, st);
+    else if (p.rows == 8) e = launch_rows<128, 1>(r, p, part, part_lse, st);
+    else if (p.rows == 16) e = launch_rows<128, 2>(r, p, part, part_lse, st);
+    else e = launch_rows<128, 3>(r, p, part, part_lse, st);
+    if (e != cudaSuccess || p.splits <= 1) return e;
+    return launch_q8_merge(r, p, 0, p.pairs_pass, part, part_lse, st);
 }
 
 }  // namespace tq

@@ -42,15 +42,17 @@ struct Q8Plan {
     bool prompt = false;           // the tcgen05 kernel:
     bool direct = false;           // which converts codes itself, or reads tiles from the work memory:
     int tiles_max = 0;             // tiles of a pair's tokens
-    int pairs_pass = 0;            // (sequence, KV head) pairs whose tiles the work memory holds at a time
+    int pairs_pass = 0;            // (sequence, KV head) pairs that run at a time: all, or as many as have tiles in the work memory
     size_t tile_bytes = 0;
 };
 
 Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo);
-size_t q8_workspace_bytes(int B, int Hkv, int D, const Q8Plan& p);
+size_t q8_workspace_bytes(int D, const Q8Plan& p);
 int q8_prompt_rows(int64_t pairs, int64_t rows, int D, bool direct, bool lo);
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p);
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st);
+cudaError_t launch_q8_merge(const Q8Run& r, const Q8Plan& p, int64_t pair0, int pairs, const float* part, const float* part_lse,
+                            cudaStream_t st);
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st);
 
 }  // namespace tq

@@ -413,7 +413,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     const int all_tiles = (kv_end + KT - 1) / KT, per = (all_tiles + splits - 1) / splits;
     const int t_begin = split * per < all_tiles ? split * per : all_tiles;
     const int tiles_n = all_tiles - t_begin < per ? all_tiles - t_begin : per;
-    const int64_t unit = pair * row_tiles + rt;
+    const int64_t unit = (int64_t)slot * row_tiles + rt;   // its partial rows in the work memory of this pass
     if (tiles_n <= 0 && splits > 1) {
         asm volatile("griddepcontrol.wait;" ::: "memory");   // this grid does not end before the tiles' kernel
         for (int i = threadIdx.x; i < ROWS; i += THREADS) part_lse[(unit * splits + split) * ROWS + i] = -INFINITY;
@@ -848,7 +848,8 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     }
 }
 
-// Work memory: partial sums of split units, then the tiles and factors of one pass's pairs.
+// Work memory: partial sums of split units, then tiles and factors, each of one pass's pairs.  A pass begins when the
+// one before has ended (its first kernel is launched in stream order), so they share it.
 template <int D, int QTILES, bool LO>
 static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, uint8_t* tiles, cudaStream_t st) {
     using C = PromptCfg<D, false, QTILES>;
@@ -874,6 +875,7 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
         cfg.numAttrs = 1;
         e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false, QTILES, LO>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
                                (const float4*)factors, p.row_tiles, p.splits, part, part_lse);
+        if (e == cudaSuccess && p.splits > 1) e = launch_q8_merge(r, p, pair0, now, part, part_lse, st);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -888,7 +890,8 @@ static cudaError_t launch_direct_d(const Q8Run& r, const Q8Plan& p, float* part,
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
     attn_q8_prompt_kernel<D, true, 1, LO><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, 0, (int)pairs, 0, nullptr, nullptr, p.row_tiles,
                                                                                    p.splits, part, part_lse);
-    return cudaGetLastError();
+    e = cudaGetLastError();
+    return e == cudaSuccess && p.splits > 1 ? launch_q8_merge(r, p, 0, (int)pairs, part, part_lse, st) : e;
 }
 
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st) {

@@ -209,7 +209,7 @@ extern "C" size_t tq_attention_q8_workspace_size(const tq_attention_q8_args* a, 
     Q8Run r;
     Q8Plan p;
     if (q8_check(a, pages, &r, &p) != TQ_SUCCESS) return 0;
-    return q8_workspace_bytes(r.B, r.Hkv, r.D, p);
+    return q8_workspace_bytes(r.D, p);
 }
 
 extern "C" tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args* a, const tq_kv_pages* pages, void* stream) {
@@ -226,7 +226,7 @@ extern "C" tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args* a, c
     if (m & 15) return set_error(TQ_ERROR_MISALIGNED, "codes and the rows of q and out must start on 16-byte boundaries");
     if (((uintptr_t)r.ks | (uintptr_t)r.vs | (uintptr_t)r.kv_len | (uintptr_t)r.q_len | (uintptr_t)r.lse | (uintptr_t)r.status) & 3)
         return set_error(TQ_ERROR_MISALIGNED, "scales, lengths, lse or status not 4-byte aligned");
-    const size_t need = q8_workspace_bytes(r.B, r.Hkv, r.D, p);
+    const size_t need = q8_workspace_bytes(r.D, p);
     if (need && (!a->workspace || a->workspace_bytes < need))
         return set_error(TQ_ERROR_INVALID_VALUE, "workspace of %zu bytes needed", need);
     if (need && ((uintptr_t)a->workspace & 15)) return set_error(TQ_ERROR_MISALIGNED, "workspace must be 16-byte aligned");
