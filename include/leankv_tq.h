@@ -469,11 +469,15 @@ typedef struct {
     float sm_scale;             /* 0 = 1/sqrt(head_dim) */
     int causal, rotate_q, v_rotated;
     float *lse;                 /* optional [batch][n_q_heads][n_new], natural log */
-    int32_t *status;            /* optional device word, raised as above (never lowered: clear it before) */
+    int32_t *status;            /* device word, raised as above (never lowered: clear it before), or NULL: the device's
+                                 * own, which tq_attention_q8_last_status() reads */
     void *workspace;            size_t workspace_bytes;
 } tq_attention_q8_args;
 size_t tq_attention_q8_workspace_size(const tq_attention_q8_args *a, const tq_kv_pages *pages);
 tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args *a, const tq_kv_pages *pages, void *stream);
+/* *status: what the calls without a status word have raised on the current device since this was last asked, 0 if
+ * nothing.  Waits for the stream (calls on other streams have to be waited for before) and clears the word. */
+tq_status tq_attention_q8_last_status(int32_t *status, void *stream);
 
 /* log-sum-exp merge of n_parts partial results o[n_parts][n_rows][head_dim] with
  * natural-log lse[n_parts][n_rows] into out[n_rows][head_dim] (+ lse_out, optional):

@@ -110,6 +110,7 @@ SIGNATURES = {
     "tq_dequantize_q8_cuda": (_i32, [_v, _v, _v, _i32, _i64, _i32, _v]),
     "tq_attention_q8_workspace_size": (C.c_size_t, [_v, _v]),
     "tq_attention_q8_paged_cuda": (_i32, [_v, _v, _v]),
+    "tq_attention_q8_last_status": (_i32, [_v, _v]),
     # split-sequence merge over peer memory (exchange handles are opaque pointers)
     "tq_peer_exchange_create": (_i32, [_i32, _i32, _i64, _i32, C.c_uint32, _v, _v]),
     "tq_peer_exchange_connect": (_i32, [_v, _v]),

@@ -183,8 +183,9 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     one sequence and head needs): tokens behind it may be left out, with status raised.  out_dtype: q's by default
     (queries enter the products in 11 bits for a bfloat16 output, in 22 for others; weights in 11: a float32 output is
     exact to about 2e-4 of its norm); out [like q] /
-    lse_out (float32 [B, Hq, n]): destinations.  status: int32 CUDA tensor [1], raised to 1 when a page id
-    outside the pool is met (its tokens are left out).
+    lse_out (float32 [B, Hq, n]): destinations.  status: int32 CUDA tensor [1], raised to 1 (TQ_ERROR_INVALID_VALUE)
+    when a page id outside the pool is met or tokens behind max_kv_len are (they are left out), to 7 (TQ_ERROR_TIMEOUT)
+    when a wait inside a kernel ran out (its rows are NaN); without one, last_status() tells.
     """
     device = _device_of(q, k_pool, v_pool, k_scale, v_scale, page_table, kv_len, q_len, out, lse_out, status)
     single = q.dim() == 3
@@ -269,18 +270,22 @@ def _outputs(q, out_dtype, out, lse_out, return_lse):
 
 
 def last_status(device: torch.device | str | int | None = None) -> int:
-    """Kernel-side status of the last decode_attention on `device` (synchronizes its stream).
+    """Kernel-side status on `device` (synchronizes its current stream): that of the last decode_attention, or, if that
+    is 0, what attention_q8_paged calls without a status tensor have raised since this was last asked (asking clears it).
 
-    0 (TQ_SUCCESS), 7 (TQ_ERROR_TIMEOUT: a bulk copy never completed) or 2
-    (TQ_ERROR_UNSUPPORTED: a block scale of magnitude >= 2^15).
+    0 (TQ_SUCCESS), 7 (TQ_ERROR_TIMEOUT: a bulk copy or a wait never completed), 2 (TQ_ERROR_UNSUPPORTED: a block
+    scale of magnitude >= 2^15) or 1 (TQ_ERROR_INVALID_VALUE: a page id outside the pool, or tokens behind max_kv_len).
     """
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if dev.type == "cuda" and dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
     ws = _workspaces.get((dev.type, dev.index))
-    if ws is None:
-        return 0
-    return int(ws[:4].view(torch.int32).item())
+    status = 0 if ws is None else int(ws[:4].view(torch.int32).item())
+    if status == 0:
+        word = C.c_int32()
+        _call(dev.index, L.load().tq_attention_q8_last_status, C.byref(word))
+        status = word.value
+    return status
 
 
 def merge_partials(parts: torch.Tensor, n_parts: int, n_rows: int, head_dim: int, out: torch.Tensor,

@@ -30,6 +30,7 @@
 // of f16 numbers near their row's largest, whatever the scales of other blocks; the sum of weights l takes
 // p_j / vs in fp32.  m is the largest s + log2 vs seen up to a slack of 8: rows are rescaled only when a score
 // exceeds m by more than that (p stays below 2^14, and is exact to f16's 11 bits down to 2^-20 of the largest).
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -594,6 +595,28 @@ static cudaError_t launch_one(const Q8Run& r, const Q8Plan& p, float* part, floa
 template <int D, int NT>
 static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
     return p.lo ? launch_one<D, NT, true>(r, p, part, part_lse, st) : launch_one<D, NT, false>(r, p, part, part_lse, st);
+}
+
+// raised by calls that bring no status word of their own; zero when the module is loaded
+__device__ int32_t q8_status_word;
+
+// its address on the current device (asked for once a device; the first call may be a captured one)
+cudaError_t q8_default_status(int32_t** word) {
+    static std::atomic<int32_t*> known[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const bool keep = dev >= 0 && dev < 64;
+    if (keep && (*word = known[dev].load(std::memory_order_relaxed)) != nullptr) return cudaSuccess;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if ((e = cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) return e;
+    void* at = nullptr;
+    e = cudaGetSymbolAddress(&at, q8_status_word);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess || back != cudaSuccess) return e != cudaSuccess ? e : back;
+    *word = static_cast<int32_t*>(at);
+    if (keep) known[dev].store(*word, std::memory_order_relaxed);
+    return cudaSuccess;
 }
 
 cudaError_t launch_q8_merge(const Q8Run& r, const Q8Plan& p, int64_t pair0, int pairs, const float* part, const float* part_lse,

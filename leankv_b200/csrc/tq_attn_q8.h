@@ -51,6 +51,7 @@ size_t q8_workspace_bytes(int D, const Q8Plan& p);
 int q8_prompt_rows(int64_t pairs, int64_t rows, int D, bool direct, bool lo);
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p);
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st);
+cudaError_t q8_default_status(int32_t** word);   // of the current device, for calls without a status word
 cudaError_t launch_q8_merge(const Q8Run& r, const Q8Plan& p, int64_t pair0, int pairs, const float* part, const float* part_lse,
                             cudaStream_t st);
 cudaError_t launch_attention_q8(const Q8Run& r, const Q8Plan& p, void* workspace, cudaStream_t st);

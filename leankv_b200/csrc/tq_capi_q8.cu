@@ -230,5 +230,19 @@ extern "C" tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args* a, c
     if (need && (!a->workspace || a->workspace_bytes < need))
         return set_error(TQ_ERROR_INVALID_VALUE, "workspace of %zu bytes needed", need);
     if (need && ((uintptr_t)a->workspace & 15)) return set_error(TQ_ERROR_MISALIGNED, "workspace must be 16-byte aligned");
+    if (!r.status && (s = cuda_status(q8_default_status(&r.status), "status word"))) return s;
     return cuda_status(launch_attention_q8(r, p, a->workspace, (cudaStream_t)stream), "attention launch");
+}
+
+extern "C" tq_status tq_attention_q8_last_status(int32_t* status, void* stream) {
+    clear_error();
+    if (!status) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
+    *status = 0;
+    int32_t* word = nullptr;
+    tq_status s = cuda_status(q8_default_status(&word), "status word");
+    if (s) return s;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if ((s = cuda_status(cudaMemcpyAsync(status, word, sizeof *word, cudaMemcpyDeviceToHost, st), "status copy"))) return s;
+    if ((s = cuda_status(cudaStreamSynchronize(st), "status copy"))) return s;
+    return *status ? cuda_status(cudaMemsetAsync(word, 0, sizeof *word, st), "status clear") : TQ_SUCCESS;
 }

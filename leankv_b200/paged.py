@@ -247,7 +247,8 @@ class PagedKVCache:
     def attention(self, step: Batch, layer: int, q, sm_scale: float | None = None, out_dtype=None, out=None):
         """Attention over each sequence's tokens, this step's included: q [B, n_q_heads, head_dim], one token per
         sequence (its last), or, with k_bits=8, [B, n_q_heads, n_new, head_dim], each row seeing the tokens up to its
-        own; rows of padding give zeros."""
+        own; rows of padding give zeros.  attention.last_status() tells whether a kernel met a page id outside the
+        pool or gave up a wait."""
         from . import attention as A
         if self.k_bits == 8:
             if q.dim() == 4 and q.shape[2] != step.n_new:
