@@ -15,7 +15,7 @@ import torch
 
 from . import _lib as L
 from .ops import (_DTYPES, _PAGES, _call, _check_lengths, _check_q8_pools, _check_rows, _check_table, _device_of,
-                  _need_cuda, _own_rows, _stream)
+                  _need_cuda, _on, _own_rows, _stream)
 
 
 class AttnArgs(C.Structure):
@@ -224,7 +224,7 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
               0 if status is None else status.data_ptr())
     pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
     lib = L.load()
-    need = lib.tq_attention_q8_workspace_size(_ATTN_Q8.pack(*fields, 0, 0), pg)
+    need = _on(device, lib.tq_attention_q8_workspace_size, _ATTN_Q8.pack(*fields, 0, 0), pg)
     # from the allocator on every call: streams and captured graphs each get their own
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _call(device, lib.tq_attention_q8_paged_cuda, _ATTN_Q8.pack(*fields, ws.data_ptr() if need else 0, need), pg)

@@ -254,13 +254,17 @@ def _device_of(*ts) -> int:
     return d
 
 
-def _call(device: int, fn, *args) -> None:
-    """A library call on the device's current stream; launches go to the current device."""
+def _on(device: int, fn, *args):
+    """A library function with `device` the current one: work is planned for it and launched on it."""
     if device == _current_device():
-        status = fn(*args, _raw_stream(device))
-    else:
-        with torch.cuda.device(device):
-            status = fn(*args, _raw_stream(device))
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+def _call(device: int, fn, *args) -> None:
+    """A library call on the device's current stream."""
+    status = _on(device, fn, *args, _raw_stream(device))
     if status:
         L.check(status)
 
