@@ -440,7 +440,8 @@ tq_status tq_dequantize_q8_cuda(const int8_t *codes, const float *scale, void *y
  * Attention over 8-bit pages (TQ_TYPE_Q8 pools as tq_kv_append_rotary_paged_cuda writes them), for one query
  * token per sequence, a few drafted tokens, or a prompt.  Query token i of sequence b's q_len[b] (NULL: n_new)
  * is the cached token kv_len[b] - q_len[b] + i and, when causal, sees the tokens up to itself; else all
- * kv_len[b] tokens (kv_len counts this step's rows, appended before).
+ * kv_len[b] tokens (kv_len counts this step's rows, appended before).  Lengths outside 0 .. capacity and 0 .. n_new
+ * are taken as the nearest.
  *   q' = H q when rotate_q, s_j = sm_scale * q' . (code_j * scale), p = softmax(s),
  *   out = sum_j p_j (code_j * scale), followed by H when v_rotated.
  * Rows that see no token (empty sequences, tokens before the cache's first, rows i >= q_len[b]) give zeros and

@@ -176,7 +176,7 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     q [B, Hq, n, D] of any batch, head and token strides, or [B, Hq, D] for one token; pools int8
     [num_pages, n_kv_heads, page_size, D] with float32 scales [num_pages, n_kv_heads, page_size / 16] as
     ops.kv_append_rotary_paged writes them; page_table int32 [B, max_pages_per_seq]; kv_len int32 [B], the
-    cached tokens with this step's.  Query token i of the q_len[b] (default n) of sequence b is cached token
+    cached tokens with this step's.  Query token i of the q_len[b] (default and at most n) of sequence b is cached token
     kv_len[b] - q_len[b] + i and sees the tokens up to itself (causal) or all.  Rows that see nothing, those
     of a padded batch (i >= q_len[b]) among them, give zeros and a log-sum-exp of -inf.  max_kv_len: an upper bound
     of kv_len that sizes the work and, for many rows, the work memory (default: the capacity; up to 1 GiB, or what

@@ -146,6 +146,7 @@ class Batch:
     max_kv_len: int
     counts: "object" = None    # new tokens of each sequence where they differ (else n_new each)
     new_len: "object" = None   # int32 [B]: the same on the device
+    seen_len: "object" = None  # int32 [B]: kv_len, 0 where a sequence has only padding (None: none has)
 
 
 class PagedKVCache:
@@ -208,9 +209,10 @@ class PagedKVCache:
         rows = max(counts, default=0)
         alike = all(n == rows for n in counts)
         new_len = None if alike else torch.tensor(counts, dtype=torch.int32, device=self.device)
-        return Batch(seqs, rows, self._table.index_select(0, idx).contiguous(), pos.contiguous(),
-                     (pos + (rows if alike else new_len)).contiguous(), int(lens.max()) if len(seqs) else 0,
-                     None if alike else counts, new_len)
+        kv_len = (pos + (rows if alike else new_len)).contiguous()
+        return Batch(seqs, rows, self._table.index_select(0, idx).contiguous(), pos.contiguous(), kv_len,
+                     int(lens.max()) if len(seqs) else 0, None if alike else counts, new_len,
+                     None if alike or min(counts) else kv_len * (new_len > 0))
 
     def append(self, step: Batch, layer: int, k, v, rope=None, positions=None, q=None):
         """Quantize-on-write of the step's new rows k, v [B, n_kv_heads, n_new, head_dim].
@@ -247,18 +249,18 @@ class PagedKVCache:
     def attention(self, step: Batch, layer: int, q, sm_scale: float | None = None, out_dtype=None, out=None):
         """Attention over each sequence's tokens, this step's included: q [B, n_q_heads, head_dim], one token per
         sequence (its last), or, with k_bits=8, [B, n_q_heads, n_new, head_dim], each row seeing the tokens up to its
-        own; rows of padding give zeros.  attention.last_status() tells whether a kernel met a page id outside the
-        pool or gave up a wait."""
+        own; rows of padding, in the first form those of sequences without a token in a step of unequal counts, give
+        zeros.  attention.last_status() tells whether a kernel met a page id outside the pool or gave up a wait."""
         from . import attention as A
         if self.k_bits == 8:
             if q.dim() == 4 and q.shape[2] != step.n_new:
                 raise ValueError(f"q must have the step's {step.n_new} tokens")
-            # one row per sequence out of several is the last one; where the step has one row each, some may be padding
-            counts = step.new_len if q.dim() == 4 or step.n_new == 1 else None
+            # one row per sequence out of several is the last one: a count above q's rows is taken as their number
             return A.attention_q8_paged(q, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
-                                        step.table, step.kv_len, q_len=counts,
+                                        step.table, step.kv_len, q_len=step.new_len,
                                         max_kv_len=step.max_kv_len, sm_scale=sm_scale, out_dtype=out_dtype or q.dtype, out=out)
-        return A.decode_attention_paged(q.contiguous(), self.k[layer], self.v[layer], step.table, step.kv_len,
+        lens = step.kv_len if step.seen_len is None else step.seen_len
+        return A.decode_attention_paged(q.contiguous(), self.k[layer], self.v[layer], step.table, lens,
                                         max_kv_len=step.max_kv_len, sm_scale=sm_scale,
                                         out_dtype=out_dtype or q.dtype, out=out)
 
