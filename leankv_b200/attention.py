@@ -15,7 +15,7 @@ import torch
 
 from . import _lib as L
 from .ops import (_DTYPES, _PAGES, _call, _check_lengths, _check_q8_pools, _check_rows, _check_table, _device_of,
-                  _need_cuda, _on, _own_rows, _stream)
+                  _need_cuda, _on, _own_rows, _row_strides, _stream)
 
 
 class AttnArgs(C.Structure):
@@ -203,9 +203,12 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     if q_len is not None:
         _check_lengths(q_len, B, "q_len")
     if out is None:
-        out = torch.empty_strided((B, Hq, n, D), (n * Hq * D, D, Hq * D, 1), dtype=out_dtype or q.dtype, device=q.device)
+        os = (n * Hq * D, D, Hq * D, 1)
+        out = torch.empty_strided((B, Hq, n, D), os, dtype=out_dtype or q.dtype, device=q.device)
     elif out.shape != q.shape or not _own_rows(out) or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError("out must have q's shape, head_dim contiguous, every row its own memory")
+    else:
+        os = _row_strides(out)
     if out.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {out.dtype}")
     lse = lse_out
@@ -216,7 +219,6 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
         lse = torch.empty((B, Hq, n), dtype=torch.float32, device=q.device)
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise ValueError("status must be an int32 tensor")
-    os = out.stride()
     fields = (B, Hq, Hkv, D, n, q.data_ptr(), _DTYPES[q.dtype], qs[0], qs[1], qs[2], out.data_ptr(), _DTYPES[out.dtype],
               os[0], os[1], os[2], k_pool.data_ptr(), k_scale.data_ptr(), v_pool.data_ptr(), v_scale.data_ptr(),
               kv_len.data_ptr(), 0 if q_len is None else q_len.data_ptr(), int(max_kv_len or 0), float(sm_scale or 0.0),

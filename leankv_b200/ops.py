@@ -269,12 +269,20 @@ def _call(device: int, fn, *args) -> None:
         L.check(status)
 
 
+def _row_strides(t: torch.Tensor) -> tuple:
+    """Batch, head and token strides; those of dimensions of one, which lead nowhere and may be anything (odd ones would
+    be refused as misaligned, unequal ones in place), as a packed tensor has them."""
+    B, H, n, D = t.shape
+    s = t.stride()
+    return (s[0] if B > 1 else 0, s[1] if H > 1 else D, s[2] if n > 1 else 0)
+
+
 def _check_rows(t: torch.Tensor, name: str) -> tuple:
     """The strides of [batch, heads, tokens, head_dim] rows."""
     s = t.stride()
     if len(s) != 4 or t.dtype not in _DTYPES or (s[3] != 1 and t.shape[3] > 1):
         raise ValueError(f"{name} must be a f32/f16/bf16 [batch, heads, tokens, head_dim] tensor, head_dim contiguous")
-    return s
+    return _row_strides(t) if (s[0] | s[1] | s[2]) & 7 else s   # the usual strides are fine as they are
 
 
 def _check_lengths(t: torch.Tensor, batch: int, name: str) -> None:
@@ -305,14 +313,16 @@ def _own_rows(t: torch.Tensor) -> bool:
     return all(n <= 1 or (s == 1 if i == 3 else s != 0) for i, (n, s) in enumerate(zip(t.shape, t.stride())))
 
 
-def _rows_out(t: torch.Tensor, out: torch.Tensor | None, name: str) -> torch.Tensor:
+def _rows_out(t: torch.Tensor, strides: tuple, out: torch.Tensor | None, name: str) -> tuple:
+    """The destination of t's rows, and the strides of both (in place: the same ones)."""
     if out is None:
         # token-major memory, as the projections on either side have it
         B, H, n, D = t.shape
-        return torch.empty_strided((B, H, n, D), (n * H * D, D, H * D, 1), dtype=t.dtype, device=t.device)
+        s = (n * H * D, D, H * D, 1)
+        return torch.empty_strided((B, H, n, D), s, dtype=t.dtype, device=t.device), strides, s
     if out.shape != t.shape or out.dtype != t.dtype or not _own_rows(out):
         raise ValueError(f"{name} must have the shape and type of its input, head_dim contiguous, every row its own memory")
-    return out
+    return out, _row_strides(t), _row_strides(out)
 
 
 def _rope_fields(rope: Rotary, batch: int, tokens: int, positions: torch.Tensor | None, inverse: bool) -> tuple:
@@ -351,16 +361,14 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, rope: Rotary, k: torch.Tens
     qs = _check_rows(q, "q")
     B, H, n, D = q.shape
     r = _rope_fields(rope, B, n, positions, inverse)
-    out = _rows_out(q, out, "out")
-    os = out.stride()
+    out, qs, os = _rows_out(q, qs, out, "out")
     x = _HEADS.pack(q.data_ptr(), out.data_ptr(), H, qs[0], qs[1], qs[2], os[0], os[1], os[2])
     x2 = None
     if k is not None:
         ks = _check_rows(k, "k")
         if k.dtype != q.dtype or k.shape[0] != B or k.shape[2] != n or k.shape[3] != D:
             raise ValueError("k must have q's type, batch, tokens and head_dim")
-        k_out = _rows_out(k, k_out, "k_out")
-        os = k_out.stride()
+        k_out, ks, os = _rows_out(k, ks, k_out, "k_out")
         x2 = _HEADS.pack(k.data_ptr(), k_out.data_ptr(), k.shape[1], ks[0], ks[1], ks[2], os[0], os[1], os[2])
     elif k_out is not None:
         raise ValueError("k_out without k")
@@ -422,8 +430,7 @@ def kv_append_rotary_paged(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tenso
         qs = _check_rows(q, "q")
         if q.dtype != k.dtype or q.shape[0] != B or q.shape[2] != n_new or q.shape[3] != D or q.shape[1] == 0:
             raise ValueError("q must have k's type, batch, tokens and head_dim")
-        q_out = _rows_out(q, q_out, "q_out")
-        os = q_out.stride()
+        q_out, qs, os = _rows_out(q, qs, q_out, "q_out")
         heads = (q.data_ptr(), q_out.data_ptr(), q.shape[1], qs[0], qs[1], qs[2], os[0], os[1], os[2])
     elif q_out is not None:
         raise ValueError("q_out without q")
