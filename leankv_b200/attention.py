@@ -180,7 +180,8 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     kv_len[b] - q_len[b] + i and sees the tokens up to itself (causal) or all.  Rows that see nothing, those
     of a padded batch (i >= q_len[b]) among them, give zeros and a log-sum-exp of -inf.  max_kv_len: an upper bound
     of kv_len that sizes the work and, for many rows, the work memory (default: the capacity; up to 1 GiB, or what
-    one sequence and head needs): tokens behind it may be left out, with status raised.  out_dtype: q's by default
+    one sequence and head needs): tokens behind it may be left out, with status raised.  sm_scale: None or 0 for
+    1 / sqrt(D).  out_dtype: q's by default
     (queries enter the products in 11 bits for a bfloat16 output, in 22 for others; weights in 11: a float32 output is
     exact to about 2e-4 of its norm); out [like q] /
     lse_out (float32 [B, Hq, n]): destinations.  status: int32 CUDA tensor [1], raised to 1 (TQ_ERROR_INVALID_VALUE)

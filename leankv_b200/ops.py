@@ -202,8 +202,9 @@ class Rotary(NamedTuple):
 
     inv_freq: float64 CUDA tensor [rotary_dim / 2], the angle of each pair per position step
     (rotary_frequencies() gives the usual ones; scaling rules come as values).  axis: int32 CUDA tensor
-    [rotary_dim / 2], the position axis of each pair (rotary_axes()), None for one axis.  Pairs are the
-    elements (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; scale multiplies the turned part.
+    [rotary_dim / 2], the position axis of each pair (rotary_axes()), None for one axis; entries outside the
+    positions' axes take the nearest one (device data, not checked).  Pairs are the elements
+    (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; scale, not 0, multiplies the turned part.
     """
     inv_freq: torch.Tensor
     axis: torch.Tensor | None = None
@@ -332,6 +333,8 @@ def _rope_fields(rope: Rotary, batch: int, tokens: int, positions: torch.Tensor 
         raise ValueError("inv_freq must be a contiguous float64 [rotary_dim / 2] tensor")
     if ax is not None and (ax.dtype != torch.int32 or ax.shape != f.shape or not ax.is_contiguous()):
         raise ValueError("axis must be a contiguous int32 tensor of inv_freq's shape")
+    if scale == 0:   # the argument block's 0 stands for 1
+        raise ValueError("scale must not be 0")
     axes, where = 1, 0
     if positions is not None:
         shape = positions.shape
