@@ -35,6 +35,14 @@ With k_bits=8 a step may have any number of tokens, and sequences of different n
     q = cache.append(step, layer, k, v, rope=rope, q=q)
     out = cache.attention(step, layer, q)        # [2, n_q_heads, 300, head_dim]
 
+Drafted tokens of which some are rejected: instead of the drafts' step a batch of the accepted
+counts is committed (their rows are in the pages already); later rows take the rejected ones'
+slots.  8-bit blocks that held a rejected row keep a scale that is large enough for it.
+
+    drafts = cache.batch([a, b], 5)
+    ...                                          # append, attention, acceptance
+    cache.commit(cache.batch([a, b], [2, 4]))
+
 Page bookkeeping (PageTable) is host-side and needs no GPU.
 """
 from __future__ import annotations
