@@ -366,10 +366,11 @@ tq_status tq_kv_append_paged_cuda(tq_type type, const void *src, tq_dtype src_dt
  * angle p * inv_freq[i], p the token's position on axis axis[i]:
  *   (a, b) -> (a cos - b sin, b cos + a sin),   cos and sin times scale;
  * elements from rotary_dim on stay as they are.  inverse turns back, which is also the rotation's gradient
- * (scale included).  Angles keep 64 bits of a turn at every int32 position (within 3e-13 at a million radians, where
- * a 64-bit product p * inv_freq is off by up to 1e-10): cosines and sines are the true values rounded to float32.  inv_freq is float64 device memory: any frequencies (a base, a scaling
- * rule, one set per axis) come as values.  |inv_freq| must be below 2^31.  axis entries outside
- * [0, n_axes) read the nearest axis.
+ * (scale included).  An angle is within |p| 2^-64 turns of p * inv_freq: 3.4e-13 radians at a million positions,
+ * 7.3e-10 at the last int32 one, whatever the frequency (the 64-bit product rounds to 2^-53 of itself, which is nearer
+ * below 0.003 radians a position and farther above).  Its cosine and sine are taken in 64 bits and rounded to float32
+ * once.  inv_freq is float64 device memory: any frequencies (a base, a scaling rule, one set per axis) come as values.
+ * |inv_freq| must be below 2^31.  axis entries outside [0, n_axes) read the nearest axis.
  */
 typedef struct {
     const double *inv_freq;     /* device [rotary_dim / 2] */

@@ -527,7 +527,9 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int64
 //   direct   121 | 233   130 | 239   124 | 238   129 | 241   226 |  439   349 | 668   446 |  874
 //   tiles    303 | 470   305 | 470   303 | 471   306 | 475   290 |  577   433 | 831   399 |  868
 // few: this file's kernel (a conversion for 24 or 16 rows); direct: tcgen05, a conversion for 128 rows; tiles:
-// tcgen05 from tiles expanded once.
+// tcgen05 from tiles expanded once.  The bounds look at rows alone, so they lie between the crossings of different
+// batches: at 48 rows of 128 the table has direct 7 % ahead, with 40 rows in 24 sequences of up to 9000 tokens few is
+// (119 and 147 us).
 constexpr int DIRECT_ROWS_128 = 49, DIRECT_ROWS_256 = 33, PROMPT_ROWS = 449;
 
 // lo: q' as the sum of two f16 terms

@@ -7,14 +7,15 @@
 //   dequantize_q8_kernel<T>           values of 8-bit pages
 //
 // Angles.  A pair turns by p * f with p an integer position, so only the fraction of p * f / 2 pi matters.  F =
-// floor(f / (2 pi) * 2^64) is within 2^-64 of a turn, and p * F mod 2^64 is that fraction within p 2^-64 (3e-13
-// radians at a million positions; nothing is lost to p itself).  The fraction is folded to an eighth of a turn and
-// its sine and cosine are Taylor sums in 64 bits (the next term is below 2^-54), rounded once to 32 bits: the true
-// values' rounding but for one in some 10^5 that lie that near to a border.  64-bit library functions of the 64-bit
-// product p * f give the same but where the product's own rounding (1e-10 at a million) shows: of 41537 random
-// calls, 35 had an element of a rotated row one step of its 16-bit type apart, and none a quantized code.  They
-// cost about 60 instructions for a pair; a CTA takes 16 tokens and keeps their angles in shared memory for all its
-// heads.
+// floor(f / (2 pi) * 2^64) is within 2^-64 of a turn, and p * F mod 2^64 is that fraction within p 2^-64: 3.4e-13
+// radians at a million positions, 7.3e-10 at 2^31, for every f.  (The 64-bit product p * f rounds to 2^-53 of itself:
+// 1.2e-10 at a million radians, and less than p 2^-64 turns where f is below 2 pi 2^-11 = 0.003.)  The fraction is
+// folded to an eighth of a turn and its sine and cosine are Taylor sums in 64 bits (the next term is below 2^-54),
+// rounded once to 32 bits: at a million positions, values near 1 are the true ones' rounding but for one in some 10^5
+// that lie that near to a border.  64-bit library functions of the 64-bit product differ where either's error shows:
+// of 41537 random calls, 35 had an element of a rotated row one step of its 16-bit type apart, and none a quantized
+// code.  They cost about 60 instructions for a pair; a CTA takes 16 tokens and keeps their angles in shared memory for
+// all its heads.
 //
 // Bit-exactness: rotation, Hadamard stages and quantization are single fp32 operations, each correctly
 // rounded, in the order of the separate operations (x c - y s with three roundings, stages h = 1, 2, 4, ...).

@@ -355,8 +355,8 @@ def rotary(q: torch.Tensor, positions: torch.Tensor, rope: Rotary, k: torch.Tens
     [batch, heads, tokens, head_dim] of any batch, head and token strides.
 
     positions: int32 [batch, tokens], or [axes, batch, tokens] with rope.axis naming each pair's axis.
-    Computed in float32, rounded once; angles keep 64 bits of a turn at every position.  inverse turns back: the
-    gradient of the inputs from that of the outputs.  out / k_out: destinations (may be q / k themselves).
+    Computed in float32, rounded once; angles are within 2^-64 turns times the position (3.4e-13 radians at a
+    million).  inverse turns back: the gradient of the inputs from that of the outputs.  out / k_out: destinations (may be q / k themselves).
     Returns the rotated q, or (q, k)."""
     if positions is None:
         raise ValueError("positions are needed")
