@@ -246,8 +246,7 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         cp_wait<C::STAGES - 2>();
         __syncwarp();
         if ((i & 31) == 0) {
-            // a block of zero values takes the smallest scale: its weights still count
-            const float vse = nx_vs > 0.0f ? nx_vs : 0x1p-100f;
+            const float vse = nx_vs > 0.0f ? nx_vs : Q8_ZERO_SCALE;
             cu_blk = nx_blk;
             cu_ks = nx_ks;
             cu_lv = lg2(vse);

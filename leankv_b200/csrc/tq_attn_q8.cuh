@@ -8,6 +8,11 @@ namespace tq {
 
 // weights are 2^(s + log2 vs - m + Q8_SHIFT); a row's m moves when a score exceeds it by more than Q8_SLACK
 constexpr float Q8_SHIFT = 6.0f, Q8_SLACK = 8.0f;
+// What stands in for the scale of a block of zero values, whose weights still count: 1 / vs times weights of up to
+// 2^(Q8_SHIFT + Q8_SLACK) is summed in fp32, so 2^26 tokens of such blocks stay below 2^128 (with 2^-100 it was 2^14
+// tokens: a head of zero values behind 131072 tokens could give NaN).  Not larger: a block of zero values that has
+// nearly all of a row's weight lifts the row's maximum, and the other blocks' weights with it towards f16's end.
+constexpr float Q8_ZERO_SCALE = 0x1p-88f;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float ex2(float x) {

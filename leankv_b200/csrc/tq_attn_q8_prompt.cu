@@ -223,7 +223,7 @@ __device__ __forceinline__ void codes_to_f16(uint4 w, uint32_t (&o)[8]) {
 // a block's factors from its scales (blk -1: not there)
 __device__ __forceinline__ float4 block_factors(int blk, float ks, float vs) {
     if (blk < 0) return make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
-    const float vse = vs > 0.0f ? vs : 0x1p-100f;   // zero values: their weights still count
+    const float vse = vs > 0.0f ? vs : Q8_ZERO_SCALE;
     return make_float4(ks, lg2(vse), __frcp_rn(vse), 0.0f);
 }
 
