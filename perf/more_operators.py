@@ -298,7 +298,7 @@ def _hadamard(x):
     return functools.reduce(_stage, [1 << i for i in range(d.bit_length() - 1)], x) * norm
 
 
-def _unpacked(blocks, bits, kind=torch.float32):
+def _unpacked(blocks, bits):
     """Values [..., head_dim] of TurboQuant blocks [..., head_dim / 32, bytes]."""
     by = blocks[..., 2:].int()
     if bits == 4:
@@ -308,8 +308,8 @@ def _unpacked(blocks, bits, kind=torch.float32):
     else:
         word = (by.unflatten(-1, (4, 3)) << torch.tensor([0, 8, 16], device=DEV)).sum(-1)
         code = (word[..., None] >> 3 * torch.arange(8, device=DEV) & 7).flatten(-2)
-    d = blocks[..., :2].contiguous().view(torch.float16).to(kind)
-    return (torch.tensor(LEVELS[bits], dtype=torch.float32, device=DEV).to(kind)[code] * d).flatten(-2)
+    d = blocks[..., :2].contiguous().view(torch.float16).float()
+    return (torch.tensor(LEVELS[bits], device=DEV)[code] * d).flatten(-2)
 
 
 def _pages(pool, scale, table):
@@ -508,12 +508,23 @@ def _hadamard_matrix(d):
     return (1 - 2 * odd).double() / math.sqrt(d)
 
 
+def _exact_blocks(blocks, bits):
+    """Values of TurboQuant blocks in 64 bits: codes as a stream of bits, the lowest first; 4-bit codes lie in the order
+    0, 16, 1, 17, ...; the scale's exponent and fraction are taken apart."""
+    stream = (blocks[..., 2:, None].int() >> torch.arange(8, device=DEV) & 1).flatten(-2).unflatten(-1, (32, bits))
+    code = (stream << torch.arange(bits, device=DEV)).sum(-1)
+    code = torch.cat((code[..., 0::2], code[..., 1::2]), -1) if bits == 4 else code
+    half = blocks[..., 0:1].long() + 256 * blocks[..., 1:2].long()
+    size = (1024 + half % 1024).double() * torch.exp2((half // 1024 - 25).double())
+    return (torch.tensor(LEVELS[bits], device=DEV).double()[code] * size).flatten(-2)
+
+
 def _exact_rows(s, b, h, total, name="k"):
     """The first rows of one sequence and head, in 64 bits."""
     pages = s["table"][b].long()
     got = s[name + "_pool"][pages, h]
     if s[name + "_scale"] is None:
-        return _unpacked(got, s["case"]["bits"] if name == "k" else 4, torch.float64).flatten(0, 1)[:total]
+        return _exact_blocks(got, s["case"]["bits"] if name == "k" else 4).flatten(0, 1)[:total]
     return (got.double() * s[name + "_scale"][pages, h].double().repeat_interleave(BLOCK, -1)[..., None]).flatten(0, 1)[:total]
 
 
@@ -580,7 +591,7 @@ def _exact_move(s):
     wide = 8 if c["bits"] == 8 else 0
     w = None if s["weights"] is None else s["weights"].double()
     k, v = ((s[t + "_pool"].double() * s[t + "_scale"].double().repeat_interleave(BLOCK, -1)[..., None])[:n] if wide
-            else _unpacked(s[t + "_pool"][:n], c["bits"] if t == "k" else 4, torch.float64) for t in ("k", "v"))
+            else _exact_blocks(s[t + "_pool"][:n], c["bits"] if t == "k" else 4) for t in ("k", "v"))
     heads = torch.arange(h, device=DEV)[:, None]
     for b in range(c["batch"]):
         first, table = int(s["first"][b]), s["table"][b].long()
@@ -598,7 +609,7 @@ def _exact_move(s):
         for out, name in ((k, "k"), (v, "v")):
             pool, scale = s[name + "_pool"], s[name + "_scale"]
             if not wide:
-                got = _unpacked(pool[table[where // p], heads, where % p], c["bits"] if name == "k" else 4, torch.float64)
+                got = _exact_blocks(pool[table[where // p], heads, where % p], c["bits"] if name == "k" else 4)
                 out[table[every // p], :, every % p] = got.transpose(0, 1)
                 continue
             code = pool[table[where // p], heads, where % p].double()
