@@ -481,6 +481,111 @@ tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args *a, const tq_kv_
  * nothing.  Waits for the stream (calls on other streams have to be waited for before) and clears the word. */
 tq_status tq_attention_q8_last_status(int32_t *status, void *stream);
 
+/* ── trees of drafted tokens ─────────────────────────────────────────────────
+ *
+ * A tree of n drafted nodes of a sequence is cached like n more tokens, node i in slot kv_len - q_len + i.  Node i sees all
+ * tokens before the nodes, and those nodes whose bit its mask has: bit j & 31 of word j >> 5 of the node's ceil(n / 32)
+ * words.  tq_draft_tree_cuda makes the masks of trees (itself and its ancestors) and the nodes' depths, 0 for a root; a node's
+ * position for the rotation is that of the first token behind the cached ones plus its depth.  parents: device
+ * [batch][n] at parents_stride words a sequence; parents come before their children, -1 (and whatever does not come before
+ * its child) stands for the cached tokens.  mask: device [batch][n][ceil(n / 32)], depth: device [batch][n], either may be
+ * NULL.  n at most TQ_DRAFT_NODES, batch at most 65535.  No counterpart in the reference.
+ */
+#define TQ_DRAFT_NODES 4096
+tq_status tq_draft_tree_cuda(const int32_t *parents, int64_t parents_stride, int batch, int n, uint32_t *mask, int32_t *depth,
+                             void *stream);
+typedef struct {
+    const uint32_t *mask;       /* device [n_new][ceil(n_new / 32)] words a sequence */
+    int64_t batch_stride;       /* words from one sequence's masks to the next one's; 0: one tree for all */
+} tq_draft_mask;
+/* tq_attention_q8_paged_cuda with the rows of q as nodes of a tree.  a->causal must be set (the tokens before the nodes are seen
+ * whole); bits of nodes i >= q_len[b] are ignored.  Rows that see nothing, padding and nodes before the cache's first token among
+ * them, give zeros and -inf.  Work memory as for tq_attention_q8_paged_cuda. */
+tq_status tq_attention_q8_tree_paged_cuda(const tq_attention_q8_args *a, const tq_kv_pages *pages, const tq_draft_mask *tree,
+                                          void *stream);
+
+/* ── eviction from paged caches ──────────────────────────────────────────────
+ *
+ * Three steps: sums of the attention weights that cached tokens get, kept beside the pages as
+ *   weights  float [num_pages][n_kv_heads][page_size]
+ * the selection of the tokens of each (sequence, KV head) that stay, and moving their rows together.  No counterpart in the
+ * reference.  Page ids outside the pool are treated as holding nothing (TQ_ERROR_INVALID_VALUE in *status).
+ *
+ * tq_attention_weights_paged_cuda: for the tokens t < kv_len[b] of sequence b and KV head h
+ *   w[t] <- (t < fresh[b] ? decay * w[t] : 0) + sum exp(s_it - lse_i),   s_it = sm_scale * q'_i . k_t,
+ * over the group's query heads and those of the last `window` rows i of the sequence's q_len[b] that see t; q' = H q when
+ * rotate_q.  q, lengths, causal, pages and status are those of tq_attention_q8_paged_cuda, lse the log-sum-exps that the
+ * attention of these rows has left (after an accepted path of a tree has moved, its rows see what they saw).  Rows of -inf
+ * add nothing.  With decay 0, and from fresh[b] on, w is not read.  Slots from kv_len[b] on stay as they are.  Keys: TQ_TYPE_Q8 with
+ * k_scale, or TQ2_0 / TQ3_0 / TQ4_0 blocks.  Sums are fp32; a weight is off by about 2^-20 of itself for each unit of its score.
+ * Sequences of a call must not share pages.  Work memory: tq_attention_weights_workspace_size() bytes.
+ */
+typedef struct {
+    int batch, n_q_heads, n_kv_heads, head_dim;
+    int64_t n_new;              /* query tokens per sequence */
+    const void *q;              tq_dtype q_dtype;     int64_t q_stride[3];
+    const void *k_pool;         tq_type k_type;       const float *k_scale;
+    const int32_t *kv_len;      /* device [batch] */
+    const int32_t *q_len;       /* device [batch], or NULL */
+    const float *lse;           /* device [batch][n_q_heads][n_new], natural log */
+    int64_t max_kv_len;         /* upper bound of kv_len (0 = capacity): sizes the work split */
+    int64_t window;             /* 0: all rows */
+    float sm_scale;             /* 0 = 1/sqrt(head_dim) */
+    int causal, rotate_q;
+    float decay;
+    const int32_t *fresh;       /* device [batch], or NULL: no slot begins anew */
+    float *weights;
+    int32_t *status;            /* as in tq_attention_q8_args */
+    void *workspace;            size_t workspace_bytes;
+} tq_attention_weights_args;
+size_t tq_attention_weights_workspace_size(const tq_attention_weights_args *a, const tq_kv_pages *pages);
+tq_status tq_attention_weights_paged_cuda(const tq_attention_weights_args *a, const tq_kv_pages *pages, void *stream);
+
+/* Of the tokens of each (sequence, KV head) those that stay, k = min(keep[b], kv_len[b], width) of them: the last
+ * min(recent, k), then the first min(sinks, k - recent), then those of the largest weights; ties go to the lowest slot.
+ * slots: device [batch][n_kv_heads][width], rising, -1 behind the last.  A weight of NaN counts as -inf; tokens of pages
+ * outside the pool go first.  max_kv_len (0 = capacity) sizes the work; tokens behind it are left out, with TQ_ERROR_INVALID_VALUE
+ * in *status.  Capacity at most 2^30. */
+typedef struct {
+    int batch, n_kv_heads;
+    const float *weights;
+    const int32_t *kv_len;      /* device [batch] */
+    const int32_t *keep;        /* device [batch], or NULL: width for all */
+    int64_t width, sinks, recent;
+    int64_t max_kv_len;
+    int32_t *slots;
+    int32_t *status;            /* as in tq_attention_q8_args */
+} tq_select_args;
+tq_status tq_select_tokens_cuda(const tq_select_args *a, const tq_kv_pages *pages, void *stream);
+
+/* Moves rows between token slots: row j < min(n_rows, count[b]) of (sequence b, KV head h) from slot src[b][h][j] to slot
+ * first[b] + j, keys, values, their scales and, if given, weights.  Negative entries of src move nothing.  TQ rows are
+ * copied.  A destination block of 8-bit rows (TQ_Q8_BLOCK slots) whose rows had one scale all keeps codes and scale; else its scale becomes
+ * max |code| * scale / 127 over the rows that are moved into it and those in it before slot first[b], and codes are rounded to it;
+ * codes of the block's other slots stay as they are, under its new scale.
+ * to_table NULL: in place; a row may only move down (src >= first + j), and the rows of a call may come in any
+ * order.  Otherwise destination slots are looked up in to_table, whose pages must be none that the call reads.  Rows that
+ * would move up, from or to slots without a page, are left and counted in *overflow, one per head.  Two sequences of a
+ * call must not share a page that is written.  Work memory: tq_kv_move_workspace_size() bytes. */
+typedef struct {
+    int batch, n_kv_heads, head_dim;
+    int64_t n_rows;
+    const int32_t *src;         /* device [batch][src_heads][n_rows] */
+    int src_heads;              /* n_kv_heads, or 1: all heads alike */
+    const int32_t *first;       /* device [batch], or NULL: 0 */
+    const int32_t *count;       /* device [batch], or NULL: n_rows */
+    void *k_pool;               tq_type k_type;       float *k_scale;
+    void *v_pool;               tq_type v_type;       float *v_scale;
+    float *weights;             /* optional */
+    const int32_t *to_table;    /* device [batch][to_pages_per_seq], or NULL */
+    int64_t to_pages_per_seq;
+    int32_t *overflow;          /* device, optional */
+    int32_t *status;            /* as in tq_attention_q8_args: TQ_ERROR_TIMEOUT if a wait ran out (rows are then missing) */
+    void *workspace;            size_t workspace_bytes;
+} tq_kv_move_args;
+size_t tq_kv_move_workspace_size(const tq_kv_move_args *a, const tq_kv_pages *pages);
+tq_status tq_kv_move_paged_cuda(const tq_kv_move_args *a, const tq_kv_pages *pages, void *stream);
+
 /* log-sum-exp merge of n_parts partial results o[n_parts][n_rows][head_dim] with
  * natural-log lse[n_parts][n_rows] into out[n_rows][head_dim] (+ lse_out, optional):
  * the split-by-sequence combine of the multi-GPU path (new) */

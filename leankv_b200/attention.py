@@ -14,8 +14,8 @@ import struct
 import torch
 
 from . import _lib as L
-from .ops import (_DTYPES, _PAGES, _call, _check_lengths, _check_q8_pools, _check_rows, _check_table, _device_of,
-                  _need_cuda, _on, _own_rows, _row_strides, _stream)
+from .ops import (_DTYPES, _PAGES, _TYPE_OF_BYTES, DraftTree, _call, _check_lengths, _check_q8_pools, _check_rows, _check_status,
+                  _check_table, _check_weights, _device_of, _need_cuda, _on, _own_rows, _row_strides, _stream)
 
 
 class AttnArgs(C.Structure):
@@ -162,6 +162,8 @@ def decode_attention_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
 
 # tq_attention_q8_args (include/leankv_tq.h)
 _ATTN_Q8 = struct.Struct("iiiiqPiqqqPiqqqPPPPPPqfiiiPPPN")
+_MASK = struct.Struct("Pq")                                        # tq_draft_mask
+_WEIGHTS = struct.Struct("iiiiqPiqqqPiPPPPqqfiifPPPPN")            # tq_attention_weights_args
 
 
 def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
@@ -170,7 +172,7 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
                        sm_scale: float | None = None, causal: bool = True, rotate_q: bool = True,
                        v_rotated: bool = True, out_dtype: torch.dtype | None = None, return_lse: bool = False,
                        out: torch.Tensor | None = None, lse_out: torch.Tensor | None = None,
-                       status: torch.Tensor | None = None):
+                       status: torch.Tensor | None = None, tree=None):
     """Attention over 8-bit pages (tq_attention_q8_paged_cuda): one query token per sequence, a few, or prompts.
 
     q [B, Hq, n, D] of any batch, head and token strides, or [B, Hq, D] for one token; pools int8
@@ -187,6 +189,8 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     lse_out (float32 [B, Hq, n]): destinations.  status: int32 CUDA tensor [1], raised to 1 (TQ_ERROR_INVALID_VALUE)
     when a page id outside the pool is met or tokens behind max_kv_len are (they are left out), to 7 (TQ_ERROR_TIMEOUT)
     when a wait inside a kernel ran out (its rows are NaN); without one, last_status() tells.
+    tree: the query tokens are nodes of a tree of drafted tokens (ops.draft_tree, or masks of one's own, contiguous int32
+    [B or 1, n, ceil(n / 32)]): node i sees the tokens before the nodes and those nodes j < q_len[b] whose bit its mask has.
     """
     device = _device_of(q, k_pool, v_pool, k_scale, v_scale, page_table, kv_len, q_len, out, lse_out, status)
     single = q.dim() == 3
@@ -220,6 +224,17 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
         lse = torch.empty((B, Hq, n), dtype=torch.float32, device=q.device)
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise ValueError("status must be an int32 tensor")
+    masks = None
+    if tree is not None:
+        mask = tree.mask if isinstance(tree, DraftTree) else tree
+        _device_of(q, mask)
+        words = -(-n // 32)
+        if mask.dtype != torch.int32 or mask.dim() != 3 or mask.shape[0] not in (1, B) or mask.shape[1:] != (n, words) \
+                or not mask.is_contiguous():
+            raise ValueError(f"tree must be a contiguous int32 [{B} or 1, {n}, {words}] tensor of masks")
+        if not causal:
+            raise ValueError("the rows of a tree are causal")
+        masks = _MASK.pack(mask.data_ptr(), 0 if mask.shape[0] == 1 else n * words)
     fields = (B, Hq, Hkv, D, n, q.data_ptr(), _DTYPES[q.dtype], qs[0], qs[1], qs[2], out.data_ptr(), _DTYPES[out.dtype],
               os[0], os[1], os[2], k_pool.data_ptr(), k_scale.data_ptr(), v_pool.data_ptr(), v_scale.data_ptr(),
               kv_len.data_ptr(), 0 if q_len is None else q_len.data_ptr(), int(max_kv_len or 0), float(sm_scale or 0.0),
@@ -230,11 +245,72 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     need = _on(device, lib.tq_attention_q8_workspace_size, _ATTN_Q8.pack(*fields, 0, 0), pg)
     # from the allocator on every call: streams and captured graphs each get their own
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _call(device, lib.tq_attention_q8_paged_cuda, _ATTN_Q8.pack(*fields, ws.data_ptr() if need else 0, need), pg)
+    args = _ATTN_Q8.pack(*fields, ws.data_ptr() if need else 0, need)
+    if masks is None:
+        _call(device, lib.tq_attention_q8_paged_cuda, args, pg)
+    else:
+        _call(device, lib.tq_attention_q8_tree_paged_cuda, args, pg, masks)
     if single:
         out = out.squeeze(2)
         lse = lse.squeeze(2) if lse is not None and lse.dim() == 3 else lse
     return (out, lse) if return_lse else out
+
+
+def attention_weights_paged(q: torch.Tensor, k_pool: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
+                            lse: torch.Tensor, weights: torch.Tensor, k_scale: torch.Tensor | None = None,
+                            q_len: torch.Tensor | None = None, fresh: torch.Tensor | None = None, decay: float = 1.0,
+                            window: int | None = None, max_kv_len: int | None = None, sm_scale: float | None = None,
+                            causal: bool = True, rotate_q: bool = True, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Adds up the attention weights that cached tokens get from a step's queries (tq_attention_weights_paged_cuda).
+
+    weights float32 [num_pages, n_kv_heads, page_size], beside the pages: for each token t of sequence b and KV head
+    weights <- (t < fresh[b] ? decay * weights : 0) + sum of exp(score - lse) over the group's query heads and those of the last
+    `window` (default: all) query tokens that see t.  q, q_len, causal, max_kv_len, sm_scale, rotate_q and status as in
+    attention_q8_paged; lse float32 [B, Hq, n] (or [B, Hq] with q [B, Hq, D]), as the attention of these queries returned it.
+    k_pool: int8 pages with k_scale, or uint8 TQ blocks as decode_attention_paged takes them.  fresh: int32 [B], the first slot
+    whose earlier weight is not read (a step's new slots; default: none).  With decay 0 none is read.  Slots behind kv_len keep
+    theirs.  Returns weights."""
+    device = _device_of(q, k_pool, page_table, kv_len, lse, weights, k_scale, q_len, fresh, status)
+    if q.dim() == 3:
+        q = q.unsqueeze(2)
+    qs = _check_rows(q, "q")
+    B, Hq, n, D = q.shape
+    pages, H, page_size = _check_weights(weights)
+    if H == 0 or Hq == 0 or Hq % H:
+        raise ValueError("n_q_heads must be a multiple of n_kv_heads")
+    if k_pool.dtype == torch.int8:
+        if k_pool.shape != (pages, H, page_size, D) or not k_pool.is_contiguous():
+            raise ValueError("8-bit keys must be a contiguous int8 [num_pages, n_kv_heads, page_size, head_dim] tensor, pages as the weights'")
+        if k_scale is None or k_scale.dtype != torch.float32 or k_scale.shape != (pages, H, page_size // 16) or not k_scale.is_contiguous():
+            raise ValueError("8-bit keys need k_scale, a contiguous float32 [num_pages, n_kv_heads, page_size / 16] tensor")
+        kt = L.TYPE_Q8
+    else:
+        kt = _TYPE_OF_BYTES.get(k_pool.shape[-1])
+        if k_pool.dtype != torch.uint8 or kt is None or k_pool.shape != (pages, H, page_size, D // L.QK, L.BLOCK_BYTES[kt]) \
+                or not k_pool.is_contiguous():
+            raise ValueError("keys must be contiguous uint8 [num_pages, n_kv_heads, page_size, head_dim/32, bytes] blocks, pages as the weights'")
+        if k_scale is not None:
+            raise ValueError("TQ pools have no scales")
+    _check_table(page_table, B)
+    _check_lengths(kv_len, B, "kv_len")
+    for t, name in ((q_len, "q_len"), (fresh, "fresh")):
+        if t is not None:
+            _check_lengths(t, B, name)
+    if lse.dtype != torch.float32 or lse.numel() != B * Hq * n or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous float32 [B, Hq, n] tensor")
+    if window is not None and window < 1:
+        raise ValueError("window must be positive")
+    p = lambda t: 0 if t is None else t.data_ptr()   # noqa: E731
+    fields = (B, Hq, H, D, n, q.data_ptr(), _DTYPES[q.dtype], qs[0], qs[1], qs[2], k_pool.data_ptr(), kt, p(k_scale),
+              kv_len.data_ptr(), p(q_len), lse.data_ptr(), int(max_kv_len or 0), int(window or 0), float(sm_scale or 0.0),
+              int(causal), int(rotate_q), float(decay), p(fresh), weights.data_ptr(), _check_status(status))
+    pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
+    lib = L.load()
+    need = _on(device, lib.tq_attention_weights_workspace_size, _WEIGHTS.pack(*fields, 0, 0), pg)
+    # from the allocator on every call: streams and captured graphs each get their own
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _call(device, lib.tq_attention_weights_paged_cuda, _WEIGHTS.pack(*fields, ws.data_ptr() if need else 0, need), pg)
+    return weights
 
 
 def _btype(cache: torch.Tensor) -> int:

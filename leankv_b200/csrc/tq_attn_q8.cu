@@ -83,7 +83,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 }
 
 // One unit's share of tokens.  Partial results go to part / part_lse (splits > 1), else to out / lse.
-template <int D, int NT, bool LO>
+// TREE: rows see what their nodes' masks say (few rows: 64 bits a row).
+template <int D, int NT, bool LO, bool TREE>
 __global__ void __launch_bounds__(Q8_THREADS, Q8Cfg<D, NT, LO>::CTAS)
 attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ part, float* __restrict__ part_lse) {
     using C = Q8Cfg<D, NT, LO>;
@@ -96,6 +97,7 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
     float2* s_f = reinterpret_cast<float2*>(s_l + Q8_WARPS * ROWS);
     int* s_lim = reinterpret_cast<int*>(s_f + ROWS);          // last token seen
     float* s_lse = reinterpret_cast<float*>(s_lim + ROWS);
+    __shared__ uint64_t s_nodes[TREE ? ROWS : 1];             // nodes seen
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int split = blockIdx.x % splits, rt = (blockIdx.x / splits) % row_tiles;
@@ -108,7 +110,7 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
     int last_i = (row0 + ROWS - 1) / r.grp;
     if (last_i >= sl.q_len) last_i = sl.q_len - 1;
     const int first_i = row0 / r.grp;
-    const int kv_end = last_i < first_i ? 0 : last_seen(r, sl, last_i) + 1;
+    const int kv_end = last_i < first_i ? 0 : TREE ? sl.len : last_seen(r, sl, last_i) + 1;
     const int per = ((kv_end + splits - 1) / splits + 127) & ~127;
     const int64_t begin64 = (int64_t)split * per;
     const int begin = begin64 < kv_end ? (int)begin64 : kv_end;
@@ -213,7 +215,20 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
         if (lane % LPR == 0) {
             const float fr = top * r.sm_scale * LOG2E;
             s_f[row] = make_float2(fr * 0x1p24f, fr * 128.0f * sum);
-            s_lim[row] = live ? last_seen(r, sl, i) : -1;
+            if constexpr (TREE) {
+                const int lim = live ? last_before(sl, i) : -2;
+                uint64_t nodes = 0;
+                if (lim > -2) {
+                    const uint32_t* mask = node_mask(r, b, i);
+                    nodes = mask[0];
+                    if (r.tree_words > 1) nodes |= (uint64_t)mask[1] << 32;
+                    nodes &= (uint64_t(1) << sl.q_len) - 1;   // q_len <= n < 64 rows
+                }
+                s_lim[row] = lim;
+                s_nodes[row] = nodes;
+            } else {
+                s_lim[row] = live ? last_seen(r, sl, i) : -1;
+            }
         }
     }
     __syncthreads();
@@ -316,8 +331,16 @@ attn_q8_kernel(const Q8Run r, int row_tiles, int splits, float* __restrict__ par
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int left = s_lim[nt * 8 + 2 * t + e] - tok0 - g;   // last token seen, from this lane's first
-                    if (left < 0) s[nt][e] = -INFINITY;
-                    if (left < 8) s[nt][2 + e] = -INFINITY;
+                    if constexpr (TREE) {
+                        // tokens past the limit are nodes, or up to 15 slots behind the last one
+                        const uint64_t nodes = s_nodes[nt * 8 + 2 * t + e];
+                        const int node = tok0 + g - (sl.len - sl.q_len);
+                        if (left < 0 && !((nodes >> (node & 63)) & 1)) s[nt][e] = -INFINITY;
+                        if (left < 8 && !((nodes >> ((node + 8) & 63)) & 1)) s[nt][2 + e] = -INFINITY;
+                    } else {
+                        if (left < 0) s[nt][e] = -INFINITY;
+                        if (left < 8) s[nt][2 + e] = -INFINITY;
+                    }
                 }
         }
         bool over = false;
@@ -582,20 +605,21 @@ static size_t part_bytes(int D, const Q8Plan& p) {
 }
 size_t q8_workspace_bytes(int D, const Q8Plan& p) { return part_bytes(D, p) + p.tile_bytes; }
 
-template <int D, int NT, bool LO>
+template <int D, int NT, bool LO, bool TREE>
 static cudaError_t launch_one(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
     using C = Q8Cfg<D, NT, LO>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<D, NT, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<D, NT, LO, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)r.B * r.Hkv * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    attn_q8_kernel<D, NT, LO><<<(unsigned)grid, Q8_THREADS, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
+    attn_q8_kernel<D, NT, LO, TREE><<<(unsigned)grid, Q8_THREADS, C::SMEM, st>>>(r, p.row_tiles, p.splits, part, part_lse);
     return cudaGetLastError();
 }
 
 template <int D, int NT>
 static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
-    return p.lo ? launch_one<D, NT, true>(r, p, part, part_lse, st) : launch_one<D, NT, false>(r, p, part, part_lse, st);
+    if (r.tree) return p.lo ? launch_one<D, NT, true, true>(r, p, part, part_lse, st) : launch_one<D, NT, false, true>(r, p, part, part_lse, st);
+    return p.lo ? launch_one<D, NT, true, false>(r, p, part, part_lse, st) : launch_one<D, NT, false, false>(r, p, part, part_lse, st);
 }
 
 // raised by calls that bring no status word of their own; zero when the module is loaded

@@ -79,6 +79,27 @@ __device__ __forceinline__ int last_seen(const Q8Run& r, const SeqLens& s, int i
     return lim < 0 ? -1 : lim;
 }
 
+// Trees of drafted nodes.  Node i of a sequence is its cached token len - q_len + i; it sees all tokens before the
+// nodes and those nodes that its mask has.  last_before: the last token that it sees whatever the mask says, -1 if there
+// is none, -2 for a row that sees nothing (padding, nodes before the cache's first token).
+__device__ __forceinline__ int last_before(const SeqLens& s, int i) {
+    const int base = s.len - s.q_len;
+    if (i >= s.q_len || base + i < 0) return -2;
+    return base > 0 ? base - 1 : -1;
+}
+__device__ __forceinline__ const uint32_t* node_mask(const Q8Run& r, int b, int i) {
+    return r.tree + b * r.tree_stride + (int64_t)i * r.tree_words;
+}
+// bits of the nodes node0 .. node0 + 15 (node0 of any sign), those of 0 .. nodes - 1 only; a row without nodes has no mask
+__device__ __forceinline__ uint32_t mask16(const uint32_t* mask, int words, int node0, int nodes) {
+    if (nodes <= 0 || node0 <= -16 || node0 >= nodes) return 0;
+    const int w = node0 >> 5;
+    const uint32_t lo = w >= 0 ? mask[w] : 0u, hi = w + 1 < words ? mask[w + 1] : 0u;
+    uint32_t bits = __funnelshift_r(lo, hi, node0 & 31) & 0xFFFFu;
+    if (nodes - node0 < 16) bits &= (1u << (nodes - node0)) - 1u;
+    return bits;
+}
+
 // the 16-token block of a (sequence, KV head): its index in the pool (codes at 16 D times it, scale at it), or
 // -1 for a page outside the pool
 __device__ __forceinline__ int block_at(const Q8Run& r, int b, int h, int block) {

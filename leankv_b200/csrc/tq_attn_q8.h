@@ -28,6 +28,9 @@ struct Q8Run {
     int max_len = 0;                  // the caller's bound of kv_len
     float sm_scale = 0.0f;
     int causal = 1, rotate_q = 1, v_rotated = 1;
+    const uint32_t* tree = nullptr;   // masks of drafted nodes, [n][tree_words] a sequence (else: causal or all)
+    int64_t tree_stride = 0;          // words from one sequence's masks to the next one's (0: one tree for all)
+    int tree_words = 0;
     float norm = 1.0f;             // 1 / sqrt(D) of the Hadamard transform
     float* lse = nullptr;          // [B][Hq][n]
     int32_t* status = nullptr;

@@ -370,7 +370,8 @@ __device__ __forceinline__ void convert_tiles(const Q8Run& r, int b, int h, int 
 }
 
 // LO: q' as the sum of two f16 terms, the second one in TMEM (D / 2 columns, for which two row tiles leave no room)
-template <int D, bool DIRECT, int QTILES, bool LO>
+// TREE: rows see what their nodes' masks say
+template <int D, bool DIRECT, int QTILES, bool LO, bool TREE>
 __global__ void __launch_bounds__(PromptCfg<D, DIRECT, QTILES>::WARPS * 32, 1)
 attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, const uint8_t* __restrict__ kv_tiles,
                       const float4* __restrict__ factors, int row_tiles, int splits, float* __restrict__ part,
@@ -405,7 +406,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
     int last_i = (row0 + ROWS - 1) / r.grp;
     if (last_i >= sl.q_len) last_i = sl.q_len - 1;
     const int first_i = row0 / r.grp;
-    int kv_end = last_i < first_i ? 0 : last_seen(r, sl, last_i) + 1;
+    int kv_end = last_i < first_i ? 0 : TREE ? sl.len : last_seen(r, sl, last_i) + 1;
     if (!DIRECT && kv_end > r.max_len) {   // longer than the caller's bound: the work memory has no tiles for it
         kv_end = r.max_len;
         if (threadIdx.x == 0 && r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
@@ -482,7 +483,8 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
         }
         if (lane % LPR == 0) {
             s_f[row] = top * fabsf(r.sm_scale) * LOG2E;
-            s_lim[row] = live ? last_seen(r, sl, i) : -1;
+            if constexpr (TREE) s_lim[row] = live ? last_before(sl, i) : -2;
+            else s_lim[row] = live ? last_seen(r, sl, i) : -1;
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -527,7 +529,15 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
         constexpr float TINY = 1e-38f;   // least factor of a sum: -inf stays -inf where f or ks is zero
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
-        const bool idle = __all_sync(0xffffffffu, lim < 0);
+        const bool idle = __all_sync(0xffffffffu, lim < (TREE ? -1 : 0));
+        const uint32_t* mask = nullptr;   // TREE: the row's nodes
+        int nodes = 0;
+        if constexpr (TREE) {
+            if (lim > -2) {
+                mask = node_mask(r, b, (row0 + row) / r.grp);
+                nodes = sl.q_len;
+            }
+        }
         constexpr int BPH = C::BPT / TPR, CH = C::COLS / 32;
         for (int t = 0; t < tiles_n; ++t) {
             const int sb = QT == 2 ? qt : (t & 1);
@@ -564,10 +574,17 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
                     for (int bl = 0; bl < 2; ++bl) {
-                        const int left = lim - (tok0 + 32 * c + 16 * bl);   // last column seen
+                        const int first = tok0 + 32 * c + 16 * bl, left = lim - first;   // last column seen
+                        if constexpr (TREE) {
+                            const uint32_t seen = mask16(mask, r.tree_words, first - (sl.len - sl.q_len), nodes);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (j > left) raw[c][16 * bl + j] = 0xff800000u;   // -inf
+                            for (int j = 0; j < 16; ++j)
+                                if (j > left && !((seen >> j) & 1)) raw[c][16 * bl + j] = 0xff800000u;   // -inf
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (j > left) raw[c][16 * bl + j] = 0xff800000u;   // -inf
+                        }
                     }
             }
             // the largest exponent, from each scale block's largest sum (f and ks are not negative)
@@ -850,10 +867,10 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
 
 // Work memory: partial sums of split units, then tiles and factors, each of one pass's pairs.  A pass begins when the
 // one before has ended (its first kernel is launched in stream order), so they share it.
-template <int D, int QTILES, bool LO>
+template <int D, int QTILES, bool LO, bool TREE>
 static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, uint8_t* tiles, cudaStream_t st) {
     using C = PromptCfg<D, false, QTILES>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, false, QTILES, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, false, QTILES, LO, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * p.tiles_max * (2 * C::KV_TILE));
     const int64_t pairs = (int64_t)r.B * r.Hkv;
@@ -873,7 +890,7 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false, QTILES, LO>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
+        e = cudaLaunchKernelEx(&cfg, attn_q8_prompt_kernel<D, false, QTILES, LO, TREE>, r, pair0, now, p.tiles_max, (const uint8_t*)tiles,
                                (const float4*)factors, p.row_tiles, p.splits, part, part_lse);
         if (e == cudaSuccess && p.splits > 1) e = launch_q8_merge(r, p, pair0, now, part, part_lse, st);
         if (e != cudaSuccess) return e;
@@ -881,14 +898,14 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
     return cudaSuccess;
 }
 
-template <int D, bool LO>
+template <int D, bool LO, bool TREE>
 static cudaError_t launch_direct_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
     using C = PromptCfg<D, true, 1>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, true, 1, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(attn_q8_prompt_kernel<D, true, 1, LO, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t pairs = (int64_t)r.B * r.Hkv, grid = pairs * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    attn_q8_prompt_kernel<D, true, 1, LO><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, 0, (int)pairs, 0, nullptr, nullptr, p.row_tiles,
+    attn_q8_prompt_kernel<D, true, 1, LO, TREE><<<(unsigned)grid, C::WARPS * 32, C::SMEM, st>>>(r, 0, (int)pairs, 0, nullptr, nullptr, p.row_tiles,
                                                                                    p.splits, part, part_lse);
     e = cudaGetLastError();
     return e == cudaSuccess && p.splits > 1 ? launch_q8_merge(r, p, 0, (int)pairs, part, part_lse, st) : e;
@@ -896,13 +913,16 @@ static cudaError_t launch_direct_d(const Q8Run& r, const Q8Plan& p, float* part,
 
 cudaError_t launch_attention_q8_prompt(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, void* tiles, cudaStream_t st) {
     uint8_t* t = static_cast<uint8_t*>(tiles);
-    const auto run = [&](auto lo) {
-        constexpr bool LO = decltype(lo)::value;
-        if (p.direct) return r.D == 256 ? launch_direct_d<256, LO>(r, p, part, part_lse, st) : launch_direct_d<128, LO>(r, p, part, part_lse, st);
-        return r.D == 256 ? launch_prompt_d<256, 1, LO>(r, p, part, part_lse, t, st) : launch_prompt_d<128, 1, LO>(r, p, part, part_lse, t, st);
+    const auto run = [&](auto lo, auto tree) {
+        constexpr bool LO = decltype(lo)::value, TREE = decltype(tree)::value;
+        if (p.direct) return r.D == 256 ? launch_direct_d<256, LO, TREE>(r, p, part, part_lse, st) : launch_direct_d<128, LO, TREE>(r, p, part, part_lse, st);
+        if (!LO && p.rows == 256) return launch_prompt_d<128, 2, false, TREE>(r, p, part, part_lse, t, st);
+        return r.D == 256 ? launch_prompt_d<256, 1, LO, TREE>(r, p, part, part_lse, t, st) : launch_prompt_d<128, 1, LO, TREE>(r, p, part, part_lse, t, st);
     };
-    if (p.rows == 256) return launch_prompt_d<128, 2, false>(r, p, part, part_lse, t, st);
-    return p.lo ? run(std::true_type()) : run(std::false_type());
+    const std::true_type yes;
+    const std::false_type no;
+    if (r.tree) return p.lo ? run(yes, yes) : run(no, yes);
+    return p.lo ? run(yes, no) : run(no, no);
 }
 
 // Query rows of a CTA.  Two row tiles of D = 128 hide each other's softmax and products (8192-token prompt 597 us, with

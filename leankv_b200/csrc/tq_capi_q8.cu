@@ -212,13 +212,20 @@ extern "C" size_t tq_attention_q8_workspace_size(const tq_attention_q8_args* a, 
     return q8_workspace_bytes(r.D, p);
 }
 
-extern "C" tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args* a, const tq_kv_pages* pages, void* stream) {
-    clear_error();
+static tq_status q8_attention(const tq_attention_q8_args* a, const tq_kv_pages* pages, const tq_draft_mask* tree, void* stream) {
     Q8Run r;
     Q8Plan p;
     tq_status s = q8_check(a, pages, &r, &p);
     if (s) return s;
     if (r.B == 0 || r.n == 0) return TQ_SUCCESS;
+    if (tree) {
+        if (!r.causal) return set_error(TQ_ERROR_INVALID_VALUE, "a tree's rows are causal");
+        if (!tree->mask) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
+        if ((uintptr_t)tree->mask & 3) return set_error(TQ_ERROR_MISALIGNED, "masks not 4-byte aligned");
+        r.tree = tree->mask;
+        r.tree_stride = tree->batch_stride;
+        r.tree_words = (int)((r.n + 31) / 32);
+    }
     if (!r.q || !r.out || !r.k || !r.v || !r.ks || !r.vs || !r.kv_len) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
     uintptr_t m = (uintptr_t)r.q | (uintptr_t)r.out | (uintptr_t)r.k | (uintptr_t)r.v;
     for (int i = 0; i < 3; ++i)
@@ -232,6 +239,18 @@ extern "C" tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args* a, c
     if (need && ((uintptr_t)a->workspace & 15)) return set_error(TQ_ERROR_MISALIGNED, "workspace must be 16-byte aligned");
     if (!r.status && (s = cuda_status(q8_default_status(&r.status), "status word"))) return s;
     return cuda_status(launch_attention_q8(r, p, a->workspace, (cudaStream_t)stream), "attention launch");
+}
+
+extern "C" tq_status tq_attention_q8_paged_cuda(const tq_attention_q8_args* a, const tq_kv_pages* pages, void* stream) {
+    clear_error();
+    return q8_attention(a, pages, nullptr, stream);
+}
+
+extern "C" tq_status tq_attention_q8_tree_paged_cuda(const tq_attention_q8_args* a, const tq_kv_pages* pages, const tq_draft_mask* tree,
+                                                     void* stream) {
+    clear_error();
+    if (!tree) return set_error(TQ_ERROR_INVALID_VALUE, "null argument block");
+    return q8_attention(a, pages, tree, stream);
 }
 
 extern "C" tq_status tq_attention_q8_last_status(int32_t* status, void* stream) {

@@ -1,0 +1,267 @@
+// tq_move.cu — rows of a paged cache moved between token slots: the accepted path of a drafted tree, the tokens that an
+// eviction keeps.
+//
+// Row j of (sequence b, KV head h) goes from slot src[b][h][j] to slot first[b] + j: keys and values with their scales,
+// and the sums of attention weights.  TurboQuant rows are copied.  An 8-bit block of 16 slots has one scale for rows that
+// come from up to 16 blocks: where all of them have the same, codes and scale stay as they are; else
+//   scale = max over the rows of max |code| * scale / 127,  code = round(code * old scale / scale),
+// the rule by which the append makes them.  Rows of the first block in front of `first` take part in place.
+//
+// A CTA makes 64 slots (4 blocks of K and of V, a warp each), all in registers: rows are read once and written once.
+// What bounds it: the bytes of the rows, scattered reads of 56 bytes and up.
+//
+// In place, a slot may be written only after the row that it held has been read.  Slots only fall (src >= first + j,
+// checked), so that row is one of the same 64 or of an earlier 64.  CTAs take their 64 in the order in which they start (a
+// ticket), read, publish that they have read, and wait for the earlier ones of their (sequence, head) before they write:
+// what is waited for has started before and only reads, so every wait ends.  (Two kernels, out to work memory and back, would
+// move the bytes twice.)  A wait that runs out all the same ends with TQ_ERROR_TIMEOUT, its rows not written.
+#include "leankv_tq.h"
+#include "tq_common.cuh"
+#include "tq_evict.h"
+#include "tq_wait.h"
+
+namespace tq {
+
+constexpr int MOVE_WARPS = 8, MOVE_BLOCKS = 4, MOVE_SLOTS = 16 * MOVE_BLOCKS;
+
+__device__ __forceinline__ uint32_t flag_read(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ void flag_write(uint32_t* p, uint32_t v) {
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint64_t move_now() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+
+// One warp: until all chunks before `chunk` have been read.  A chunk's flag is 1 when it has been read, 2 when all before
+// it have been, too: the way back ends at a 2.
+__device__ __forceinline__ bool wait_earlier(const uint32_t* flags, int64_t chunk) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t base = chunk - 1; base >= 0; base -= 32) {
+        const uint64_t until = move_now() + WAIT_NS;
+        for (;;) {
+            const uint32_t f = base - lane >= 0 ? flag_read(flags + base - lane) : 2u;
+            const uint32_t read = __ballot_sync(0xffffffffu, f >= 1), all = __ballot_sync(0xffffffffu, f == 2);
+            const int stop = all ? __ffs(all) - 1 : 31;               // the nearest chunk that speaks for the rest
+            const uint32_t need = stop == 31 ? 0xffffffffu : (2u << stop) - 1;
+            if ((read & need) == need) {
+                if (all) return true;
+                break;
+            }
+            if (__any_sync(0xffffffffu, move_now() > until)) return false;
+        }
+    }
+    return true;
+}
+
+// where a slot's row lies, as a row of the pool (-1: outside the table or the pool)
+__device__ __forceinline__ int64_t row_at(const MoveRun& r, const int32_t* table, int64_t max_pages, int b, int h, int64_t slot) {
+    if (slot < 0 || slot >= (max_pages << r.page_shift)) return -1;
+    const int32_t pg = table[b * max_pages + (slot >> r.page_shift)];
+    if (pg < 0 || pg >= r.num_pages) return -1;
+    return (((int64_t)pg * r.Hkv + h) << r.page_shift) + (slot & ((int64_t(1) << r.page_shift) - 1));
+}
+
+// CTA-wide turn between reading and writing; `used` depends on all that the thread has read, so that the reads are over.
+// False: the rows must not be written.
+__device__ __forceinline__ bool move_turn(uint32_t* flags, int64_t chunk, uint32_t used, int* s_ok) {
+    __syncthreads_or(used == 0x9E3779B9u);
+    if (!flags) return true;   // one chunk, or other pages than those that are read
+    if (threadIdx.x < 32) {
+        if (threadIdx.x == 0) flag_write(flags + chunk, 1u);
+        const bool ok = wait_earlier(flags, chunk);
+        if (threadIdx.x == 0) {
+            if (ok) flag_write(flags + chunk, 2u);
+            *s_ok = ok;
+        }
+    }
+    __syncthreads();
+    return *s_ok != 0;
+}
+
+// What a lane knows of its row (lane & 15) of the warp's block
+struct MoveRow {
+    int64_t from = -1;   // pool row that is read, -1: none
+    bool moved = false;  // one of src (else an older row of the first block, or none)
+};
+
+__device__ __forceinline__ MoveRow move_row(const MoveRun& r, int b, int h, int64_t slot, int64_t to, int64_t first, int64_t count,
+                                            bool q8, bool counts) {
+    MoveRow m;
+    const int64_t j = slot - first;
+    if (j >= count) return m;
+    if (j < 0) {
+        if (q8) m.from = to;
+        return m;
+    }
+    const int64_t s = r.src[((int64_t)b * r.src_heads + (r.src_heads > 1 ? h : 0)) * r.n + j];
+    if (s < 0) return m;
+    if (to >= 0 && !(r.in_place && s < slot)) m.from = row_at(r, r.from, r.max_from, b, h, s);
+    m.moved = m.from >= 0;
+    if (!m.moved && counts && r.overflow) atomicAdd(r.overflow, 1);
+    return m;
+}
+
+__device__ __forceinline__ int64_t shfl64(int64_t v, int lane) { return __shfl_sync(0xffffffffu, (long long)v, lane); }
+
+// 8-bit rows of a block: D / 16 lanes a row, 16 codes each
+template <int D>
+__device__ __forceinline__ void move_block_q8(const MoveRun& r, const MoveSide& x, MoveRow m, int64_t to0, bool some, uint32_t used,
+                                              uint32_t* flags, int64_t chunk, int* s_ok) {
+    constexpr int LPR = D / 16, RPP = 32 / LPR, PASSES = 16 / RPP;
+    const int lane = threadIdx.x & 31, sub = lane / LPR, col = lane % LPR;
+    const bool valid = some && m.from >= 0;
+    const uint32_t rows = __ballot_sync(0xffffffffu, valid) & 0xFFFFu;
+    const int8_t* pool = reinterpret_cast<const int8_t*>(x.pool);
+    uint4 w[PASSES];
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int row = p * RPP + sub;
+        const int64_t from = shfl64(m.from, row);
+        w[p] = make_uint4(0, 0, 0, 0);
+        if ((rows >> row) & 1) w[p] = *reinterpret_cast<const uint4*>(pool + from * D + 16 * col);
+    }
+    const float scale = valid ? x.scale[m.from >> 4] : 0.0f;
+    used ^= __float_as_uint(scale);
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) used ^= w[p].x ^ w[p].y ^ w[p].z ^ w[p].w;
+
+    // rows' scales alike: nothing changes but the place
+    const float one = __shfl_sync(0xffffffffu, scale, rows ? __ffs(rows) - 1 : 0);
+    const bool alike = __all_sync(0xffffffffu, !valid || scale == one);
+    float now = one;
+    if (!alike) {
+        float top = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int row = p * RPP + sub;
+            uint32_t a = __vmaxu4(__vmaxu4(__vabs4(w[p].x), __vabs4(w[p].y)), __vmaxu4(__vabs4(w[p].z), __vabs4(w[p].w)));
+            a = __vmaxu4(a, a >> 16);
+            uint32_t most = max(a & 0xFFu, (a >> 8) & 0xFFu);
+#pragma unroll
+            for (int o = 1; o < LPR; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const float s = __shfl_sync(0xffffffffu, scale, row);
+            top = fmaxf(top, __fmul_rn(__fmul_rn((float)most, s), 1.0f / 127.0f));
+        }
+#pragma unroll
+        for (int o = LPR; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        now = top >= 0x1p-100f ? top : 0.0f;
+    }
+    const float ratio = now > 0.0f ? __fdiv_rn(scale, now) : 0.0f;   // of the lane's row
+    if (!move_turn(flags, chunk, used, s_ok) || !some) return;
+    int8_t* to = reinterpret_cast<int8_t*>(x.pool) + to0 * D + 16 * col;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int row = p * RPP + sub;
+        const float q = __shfl_sync(0xffffffffu, ratio, row);
+        if (!alike) {
+            uint32_t* words = reinterpret_cast<uint32_t*>(&w[p]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t acc = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    int c = __float2int_rn(__fmul_rn((float)(int8_t)(words[i] >> (8 * k)), q));
+                    c = c < -127 ? -127 : (c > 127 ? 127 : c);
+                    acc |= (uint32_t)(c & 0xFF) << (8 * k);
+                }
+                words[i] = acc;
+            }
+        }
+        if ((rows >> row) & 1) *reinterpret_cast<uint4*>(to + row * D) = w[p];
+    }
+    if (lane == 0) x.scale[to0 >> 4] = now;
+}
+
+// TurboQuant rows of a block: 8 U bytes a row, the block's 16 rows flat over the lanes
+template <int U>
+__device__ __forceinline__ void move_block_tq(const MoveSide& x, MoveRow m, int64_t to0, bool some, uint32_t used, uint32_t* flags,
+                                              int64_t chunk, int* s_ok) {
+    constexpr int N = 16 * U, PER = (N + 31) / 32;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rows = __ballot_sync(0xffffffffu, some && m.moved) & 0xFFFFu;
+    uint2 w[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int u = lane + 32 * i, row = u < N ? u / U : 0;
+        const int64_t from = shfl64(m.from, row);
+        w[i] = make_uint2(0, 0);
+        if (u < N && ((rows >> row) & 1)) w[i] = reinterpret_cast<const uint2*>(x.pool)[from * U + u % U];
+        used ^= w[i].x ^ w[i].y;
+    }
+    if (!move_turn(flags, chunk, used, s_ok) || !some) return;
+    uint2* to = reinterpret_cast<uint2*>(x.pool) + to0 * U;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int u = lane + 32 * i;
+        if (u < N && ((rows >> (u / U)) & 1)) to[u] = w[i];
+    }
+}
+
+// D: 8-bit rows of D elements (UK = UV = 0), or TurboQuant rows of 8 UK and 8 UV bytes
+template <int D, int UK, int UV>
+__global__ void __launch_bounds__(32 * MOVE_WARPS) move_kernel(const MoveRun r, int64_t chunks) {
+    __shared__ int64_t s_ticket;
+    __shared__ int s_ok;
+    int64_t ticket = blockIdx.x;
+    if (r.flags) {
+        if (threadIdx.x == 0) s_ticket = atomicAdd(r.flags, 1u);
+        __syncthreads();
+        ticket = s_ticket;
+    }
+    const int64_t pairs = (int64_t)r.B * r.Hkv, chunk = ticket / pairs, pair = ticket - chunk * pairs;
+    uint32_t* flags = r.flags ? r.flags + 1 + pair * chunks : nullptr;
+    const int b = (int)(pair / r.Hkv), h = (int)(pair % r.Hkv);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, side = warp & 1;
+    const int64_t cap = r.max_to << r.page_shift;
+    int64_t first = r.first ? r.first[b] : 0, count = r.count ? r.count[b] : r.n;
+    first = first < 0 ? 0 : (first > cap ? cap : first);
+    count = count < 0 ? 0 : (count > r.n ? r.n : count);
+
+    const int64_t slot0 = (first & ~int64_t(15)) + chunk * MOVE_SLOTS + (warp >> 1) * 16;
+    const int64_t to0 = row_at(r, r.to, r.max_to, b, h, slot0);
+    const int row = lane & 15;
+    MoveRow m = move_row(r, b, h, slot0 + row, to0 < 0 ? -1 : to0 + row, first, count, UK == 0, side == 0 && lane < 16);
+    // blocks of rows that all stay where they are, or of none, are left alone
+    const bool some = to0 >= 0 && __any_sync(0xffffffffu, m.moved && m.from != to0 + row);
+    float weight = 0.0f;
+    const bool weighs = r.weights && side == 0 && lane < 16 && some && m.moved;
+    if (weighs) weight = r.weights[m.from];
+    const uint32_t used = __float_as_uint(weight);
+    if constexpr (UK == 0) {
+        move_block_q8<D>(r, side ? r.v : r.k, m, to0, some, used, flags, chunk, &s_ok);
+    } else {
+        if (side) move_block_tq<UV>(r.v, m, to0, some, used, flags, chunk, &s_ok);
+        else move_block_tq<UK>(r.k, m, to0, some, used, flags, chunk, &s_ok);
+    }
+    if (flags && !s_ok) {
+        if (threadIdx.x == 0 && r.status) atomicMax(r.status, (int)TQ_ERROR_TIMEOUT);
+        return;
+    }
+    if (weighs) r.weights[to0 + row] = weight;
+}
+
+int64_t move_chunks(int64_t n, bool with_first) { return (n + (with_first ? 15 : 0) + MOVE_SLOTS - 1) / MOVE_SLOTS; }
+
+cudaError_t launch_move(const MoveRun& r, cudaStream_t st) {
+    const int64_t chunks = move_chunks(r.n, r.first != nullptr), grid = (int64_t)r.B * r.Hkv * chunks;
+    if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
+    if (r.flags) {
+        const cudaError_t e = cudaMemsetAsync(r.flags, 0, (size_t)(grid + 1) * sizeof(uint32_t), st);
+        if (e != cudaSuccess) return e;
+    }
+    const auto run = [&](auto kernel) {
+        kernel<<<(unsigned)grid, 32 * MOVE_WARPS, 0, st>>>(r, chunks);
+        return cudaGetLastError();
+    };
+    if (r.k.type == 8) return r.D == 256 ? run(move_kernel<256, 0, 0>) : run(move_kernel<128, 0, 0>);
+    if (r.D == 256) return r.k.type == 4 ? run(move_kernel<256, 18, 18>) : r.k.type == 3 ? run(move_kernel<256, 14, 18>) : run(move_kernel<256, 10, 18>);
+    return r.k.type == 4 ? run(move_kernel<128, 9, 9>) : r.k.type == 3 ? run(move_kernel<128, 7, 9>) : run(move_kernel<128, 5, 9>);
+}
+
+}  // namespace tq

@@ -1,0 +1,416 @@
+// tq_weights.cu — sums of the attention weights that cached tokens get from a step's queries, over 8-bit or TurboQuant keys.
+//
+// For token t of (sequence b, KV head h), over the group's query heads and the last `window` rows i of the sequence:
+//   w[t] <- (t < fresh[b] ? decay * w[t] : 0) + sum over rows that see t of exp(s_it - lse_i),  s_it = sm_scale q'_i . k_t
+// with the log-sum-exp that the attention of those rows has left.  V is not read, and no weight leaves the SM.
+//
+// Work.  A CTA takes a run of tokens of one (sequence, KV head); its 8 warps take every 8th block of 16 tokens, copied into
+// a ring of the warp's own in shared memory (cp.async).  Products are mma.sync m16n8k16 with the keys as the A operand (16
+// tokens x 16 elements) and 8 query rows as B: a thread's sums over the rows are then sums over its columns, which four
+// lanes add up at the end.  More than 32 rows are taken 32 at a time, the tokens' sums kept in shared memory between.
+//
+// What bounds it.  Single tokens: the keys' bytes.  Many rows: products and exponentials.
+//
+// Numbers.  Sums are fp32 results that later sums are added to, so weights are kept to fp32's size of error: q' is the sum of
+// two f16 terms (22 bits), 8-bit codes are exact in f16 (as subnormals (c + 128) 2^-24, the offset taken off in fp32, as in
+// the attention kernels), TurboQuant levels are the sum of two f16 terms, looked up by the pair.  Products are summed in fp32.
+#include <type_traits>
+
+#include "leankv_tq.h"
+#include "tq_attn_q8.cuh"
+#include "tq_evict.h"
+#include "tq_kernels.h"
+
+namespace tq {
+
+constexpr int WT_WARPS = 8, WT_THREADS = 32 * WT_WARPS, WT_TILES = 4, WT_ROWS = 8 * WT_TILES;
+constexpr int WT_TOKENS = 2048;   // tokens of a CTA whose sums wait in shared memory
+
+__device__ __forceinline__ void wt_cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 wt_lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 wt_lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint32_t wt_lds16(uint32_t a) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void wt_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D, int QT> struct WtCfg {
+    static constexpr int NK = D / 16;
+    static constexpr int ROWB = QT == 8 ? D : D / 32 * BlockBytes<QT == 8 ? 4 : QT>::value;
+    static constexpr int TILE = 16 * ROWB;                       // bytes of a block of 16 tokens
+    static constexpr int STAGES = QT == 8 && D == 256 ? 3 : 4;
+    static constexpr int RING = STAGES * TILE;                   // per warp
+    static constexpr int QPART = WT_TILES * NK * 256, QBYTES = 2 * QPART;
+    // pairs of levels as f16 terms: an entry for every lane of a half warp, so that lookups do not meet in a bank
+    static constexpr int PAIRS = QT == 4 ? 256 : QT == 3 ? 64 : QT == 2 ? 16 : 0, TABLE = PAIRS * 128;
+    static constexpr int SMEM = WT_WARPS * RING + QBYTES + TABLE;
+    static constexpr int CTAS = SMEM <= 74 * 1024 ? 3 : SMEM <= 112 * 1024 ? 2 : 1;
+};
+
+// two levels as the sum of two pairs of f16 terms
+template <int QT> __device__ __forceinline__ uint2 level_pair(int a, int b) {
+    float x = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int i = 0; i < (1 << QT); ++i) {
+        if (i == a) x = tq_level<QT>(i);
+        if (i == b) y = tq_level<QT>(i);
+    }
+    const __half2 hi = __floats2half2_rn(x, y);
+    const __half2 lo = __floats2half2_rn(x - __low2float(hi), y - __high2float(hi));
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&hi), *reinterpret_cast<const uint32_t*>(&lo));
+}
+
+template <int D, int QT>
+__global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel(const WeightsRun p, int splits, int row_chunks) {
+    using C = WtCfg<D, QT>;
+    constexpr int NK = C::NK, LPR = D / 16;
+    const Q8Run& r = p.q;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* s_q = smem + WT_WARPS * C::RING;
+    uint8_t* s_table = s_q + C::QBYTES;
+    __shared__ __align__(16) float2 s_f[WT_ROWS];   // a row's factor of the sums of codes, and that of 128 * sum of its q'
+    __shared__ float s_lse[WT_ROWS];                // its log-sum-exp in the log2 domain
+    __shared__ int s_lim[WT_ROWS];                  // last token that it sees
+    __shared__ float s_sum[WT_TOKENS];              // tokens' sums between chunks of rows
+
+    const int split = blockIdx.x % splits, pair = blockIdx.x / splits, h = pair % r.Hkv, b = pair / r.Hkv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const SeqLens sl = seq_lens(r, b);
+    const int per = ((sl.len + splits - 1) / splits + 127) & ~127;
+    const int64_t begin64 = (int64_t)split * per;
+    if (begin64 >= sl.len) return;
+    const int begin_all = (int)begin64, end_all = sl.len - begin_all < per ? sl.len : begin_all + per;
+    const int fresh = p.fresh ? p.fresh[b] : 0x7fffffff;
+    const int i0 = sl.q_len > p.window ? sl.q_len - (int)p.window : 0;
+    const int rows_all = (sl.q_len - i0) * r.grp;   // rows i0 .. of the sequence, row = token x head of group
+
+    if constexpr (QT != 8) {
+        for (int i = threadIdx.x; i < C::PAIRS * 16; i += WT_THREADS)
+            reinterpret_cast<uint2*>(s_table)[i] = level_pair<QT>((i >> 4) & ((1 << QT) - 1), (i >> 4) >> QT);
+    }
+
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * C::RING;
+    const uint32_t sq = (uint32_t)__cvta_generic_to_shared(s_q) + lane * 16;
+    const uint32_t table = (uint32_t)__cvta_generic_to_shared(s_table) + (lane & 15) * 8;
+
+    // with several chunks of rows, as many tokens at a time as have sums in shared memory
+    const int step = row_chunks > 1 ? WT_TOKENS : per;
+    for (int begin = begin_all; begin < end_all; begin += step) {
+    const int end = end_all - begin < step ? end_all : begin + step;
+    const int nblk_all = (end - begin + 15) >> 4, blk0 = begin >> 4;
+    const int mine = nblk_all > warp ? (nblk_all - warp + WT_WARPS - 1) / WT_WARPS : 0;
+    for (int chunk = 0; chunk < row_chunks; ++chunk) {
+        const int row0 = chunk * WT_ROWS, rows = rows_all - row0 < WT_ROWS ? rows_all - row0 : WT_ROWS;
+        if (chunk > 0 && rows <= 0) break;
+        const bool last = chunk + 1 == row_chunks || rows_all - row0 <= WT_ROWS;
+        const int tiles = rows > 0 ? (rows + 7) >> 3 : 0;
+
+        int nx_blk = -1, cu_blk = -1;                // windows of 32 blocks, one per lane
+        float nx_ks = 0.0f, cu_ks = 0.0f;
+        auto window = [&](int i) {
+            nx_blk = -1;
+            nx_ks = 0.0f;
+            if (i + lane < mine) {
+                nx_blk = block_at(r, b, h, blk0 + warp + (i + lane) * WT_WARPS);
+                if (nx_blk < 0) {
+                    if (r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
+                } else if (QT == 8) {
+                    nx_ks = r.ks[nx_blk];
+                }
+            }
+        };
+        uint32_t fill = ring;
+        auto issue = [&](int i) {
+            if (i < mine) {
+                if ((i & 31) == 0) window(i);
+                const int blk = __shfl_sync(0xffffffffu, nx_blk, i & 31);
+                if (blk >= 0) {
+                    const int8_t* kp = r.k + (int64_t)blk * C::TILE;
+#pragma unroll
+                    for (int e = 0; e < (C::TILE + 511) / 512; ++e) {
+                        const int c = lane + 32 * e;
+                        if (C::TILE % 512 == 0 || c < C::TILE / 16) {
+                            int to = c * 16;
+                            if constexpr (QT == 8) {   // chunk c of token x in a 128-byte half at c ^ (x & 7) of half * 2048 + x * 128
+                                const int x = c / LPR, cc = c % LPR;
+                                to = (cc >> 3) * 2048 + x * 128 + (((cc & 7) ^ (x & 7)) << 4);
+                            }
+                            wt_cp16(fill + to, kp + c * 16);
+                        }
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            fill += C::TILE;
+            if (fill == ring + C::RING) fill = ring;
+        };
+        if (chunk > 0 || begin > begin_all) __syncthreads();   // the rows before have been used
+#pragma unroll
+        for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
+
+        // ── q': Hadamard, row maximum, two f16 terms, in the order of the products' B fragments ──
+        for (int base = warp * (32 / LPR); base < tiles * 8; base += WT_WARPS * (32 / LPR)) {
+            const int row = base + lane / LPR, e0 = (lane % LPR) * 16;
+            const int gr = row0 + row, i = i0 + gr / r.grp, hq = h * r.grp + gr % r.grp;
+            float v[16];
+            const bool live = row < rows;
+            if (live) {
+                load_row16(r.q_dtype, r.q, b * r.qs[0] + hq * r.qs[1] + (int64_t)i * r.qs[2] + e0, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+            }
+            if (r.rotate_q) fwht16<D>(v, r.norm);
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+            for (int o = 1; o < LPR; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
+            float sum = 0.0f;
+            // Element e of the row goes where the keys' element meets it: half-word `odd` of word w (b0, b1 of one k-step, then of
+            // the next) of lane tt, pair of k-steps j2.  8 bits: a lane's elements are one run of 32 bytes in 128.  TurboQuant: a
+            // pair of k-steps is a block of 32 elements, lane tt has 8 of them: TQ4 the nibbles of bytes 4 tt .. 4 tt + 3 (e and
+            // e + 16 in a byte), TQ3 the group of 8 codes tt, TQ2 those of bytes 2 tt, 2 tt + 1.
+            __half* qh = reinterpret_cast<__half*>(s_q) + (row >> 3) * (NK / 2) * 256 + (row & 7) * 32;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int e = e0 + j;
+                const float x = v[j] * inv;
+                const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
+                sum += __half2float(hi) + __half2float(lo);
+                int j2, tt, w, odd;
+                if constexpr (QT == 8) {
+                    j2 = (e >> 7) * 4 + ((e & 31) >> 3); tt = (e & 127) >> 5; w = (e & 7) >> 1; odd = e & 1;
+                } else if constexpr (QT == 4) {
+                    j2 = e >> 5; tt = (e & 15) >> 2; w = e & 3; odd = (e >> 4) & 1;
+                } else {
+                    j2 = e >> 5; tt = (e & 31) >> 3; w = (e & 7) >> 1; odd = e & 1;
+                }
+                __half* to = qh + j2 * 256 + tt * 8 + w * 2 + odd;
+                to[0] = hi;
+                to[C::QPART / 2] = lo;
+            }
+#pragma unroll
+            for (int o = 1; o < LPR; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane % LPR == 0) {
+                const float fr = top * r.sm_scale * LOG2E;
+                s_f[row] = QT == 8 ? make_float2(fr * 0x1p24f, fr * 128.0f * sum) : make_float2(fr, 0.0f);
+                const float lse = live ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : INFINITY;
+                const bool sees = live && lse != -INFINITY;   // a row that saw nothing adds nothing
+                s_lse[row] = sees ? lse * LOG2E : INFINITY;
+                s_lim[row] = sees ? last_seen(r, sl, i) : 0x7fffffff;
+            }
+        }
+        __syncthreads();
+        int lim_min = 0x7fffffff;
+        if (lane < tiles * 8) lim_min = s_lim[lane];
+        lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+
+        // ── blocks of 16 tokens ──
+        uint32_t kt = ring - C::TILE;
+        for (int i = 0; i < mine; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
+            __syncwarp();
+            if ((i & 31) == 0) {
+                cu_blk = nx_blk;
+                cu_ks = nx_ks;
+            }
+            issue(i + C::STAGES - 1);
+            kt += C::TILE;
+            if (kt == ring + C::RING) kt = ring;
+            const int blk = __shfl_sync(0xffffffffu, cu_blk, i & 31);
+            if (blk < 0) continue;                   // a page outside the pool holds nothing
+            const float ks = __shfl_sync(0xffffffffu, cu_ks, i & 31);
+            const int tok0 = (blk0 + warp + i * WT_WARPS) << 4, tok = tok0 + g + 8 * (t & 1);   // the token that this lane writes
+            float* at = p.weights + ((int64_t)blk * 16 + (tok - tok0));
+            float held = 0.0f;
+            if (last && t < 2 && tok < end && tok < fresh && p.decay != 0.0f) held = *at;
+
+            float sum0 = 0.0f, sum1 = 0.0f;          // tokens g, g + 8, this lane's rows
+            auto add = [&](int nt, const float (&s)[4], float f, float off) {
+                // words 0, 1 of token g, words 2, 3 of token g + 8, for rows 2t and 2t + 1 of the tile
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = nt * 8 + 2 * t + e;
+                    const float2 fr = s_f[row];
+                    const float a = fr.x * f, c = fmaf(-fr.y, off, -s_lse[row]);
+                    float x = ex2(fmaf(s[e], a, c)), y = ex2(fmaf(s[2 + e], a, c));
+                    if (tok0 + 15 > lim_min) {
+                        const int left = s_lim[row] - tok0 - g;
+                        if (left < 0) x = 0.0f;
+                        if (left < 8) y = 0.0f;
+                    }
+                    sum0 += x;
+                    sum1 += y;
+                }
+            };
+            if constexpr (QT == 8) {
+                uint32_t kw[D / 128][2][8];
+#pragma unroll
+                for (int half = 0; half < D / 128; ++half)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t row = kt + half * 2048 + (x * 8 + g) * 128;
+                        const uint4 u = wt_lds128(row + (((2 * t) ^ g) << 4)), w = wt_lds128(row + (((2 * t + 1) ^ g) << 4));
+                        kw[half][x][0] = u.x; kw[half][x][1] = u.y; kw[half][x][2] = u.z; kw[half][x][3] = u.w;
+                        kw[half][x][4] = w.x; kw[half][x][5] = w.y; kw[half][x][6] = w.z; kw[half][x][7] = w.w;
+                    }
+                for (int nt = 0; nt < tiles; ++nt) {
+                    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sl4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int half = 0; half < D / 128; ++half)
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) {
+                            uint32_t a0[4], a1[4];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const uint32_t u = kw[half][x][j] ^ 0x80808080u, w = kw[half][x][j + 1] ^ 0x80808080u;
+                                a0[x] = __byte_perm(u, 0u, 0x4140); a0[2 + x] = __byte_perm(u, 0u, 0x4342);
+                                a1[x] = __byte_perm(w, 0u, 0x4140); a1[2 + x] = __byte_perm(w, 0u, 0x4342);
+                            }
+                            const uint32_t from = sq + (nt * (NK / 2) + half * 4 + j / 2) * 512;
+                            const uint4 q = wt_lds128(from), ql = wt_lds128(from + C::QPART);
+                            wt_mma(s, a0, q.x, q.y);
+                            wt_mma(sl4, a0, ql.x, ql.y);
+                            wt_mma(s, a1, q.z, q.w);
+                            wt_mma(sl4, a1, ql.z, ql.w);
+                        }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[e] += sl4[e];
+                    add(nt, s, ks, ks);
+                }
+            } else {
+                // a block of 32 elements is two k-steps; its scales are those of tokens g and g + 8
+                float acc[WT_TILES][4];
+#pragma unroll
+                for (int nt = 0; nt < WT_TILES; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
+                constexpr int BB = BlockBytes<QT>::value;
+#pragma unroll
+                for (int j2 = 0; j2 < D / 32; ++j2) {
+                    float d[2];
+                    uint2 lv[2][4];   // two f16 terms of the pairs of levels, tokens g and g + 8
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t row = kt + (x * 8 + g) * C::ROWB + j2 * BB;
+                        d[x] = half_decode(wt_lds16(row));
+                        uint32_t code[4];
+                        if constexpr (QT == 4) {
+                            const uint32_t w = wt_lds16(row + 2 + 4 * t) | wt_lds16(row + 4 + 4 * t) << 16;
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; ++i4) code[i4] = (w >> (8 * i4)) & 255u;
+                        } else if constexpr (QT == 3) {
+                            // bytes 3 t .. 3 t + 2 of the codes: two half-words, from byte 3 t or the one before
+                            const uint32_t from = row + 2 + ((3 * t) & ~1);
+                            uint32_t w = wt_lds16(from) | wt_lds16(from + 2) << 16;
+                            w >>= (t & 1) * 8;
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; ++i4) code[i4] = (w >> (6 * i4)) & 63u;
+                        } else {
+                            const uint32_t w = wt_lds16(row + 2 + 2 * t);
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; ++i4) code[i4] = (w >> (4 * i4)) & 15u;
+                        }
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; ++i4) lv[x][i4] = wt_lds64(table + code[i4] * 128);
+                    }
+                    const uint32_t h0[4] = {lv[0][0].x, lv[1][0].x, lv[0][1].x, lv[1][1].x}, h1[4] = {lv[0][2].x, lv[1][2].x, lv[0][3].x, lv[1][3].x};
+                    const uint32_t l0[4] = {lv[0][0].y, lv[1][0].y, lv[0][1].y, lv[1][1].y}, l1[4] = {lv[0][2].y, lv[1][2].y, lv[0][3].y, lv[1][3].y};
+#pragma unroll
+                    for (int nt = 0; nt < WT_TILES; ++nt) {
+                        if (nt >= tiles) break;
+                        const uint32_t from = sq + (nt * (NK / 2) + j2) * 512;
+                        const uint4 q = wt_lds128(from), ql = wt_lds128(from + C::QPART);
+                        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        wt_mma(s, h0, q.x, q.y);
+                        wt_mma(x, h0, ql.x, ql.y);
+                        wt_mma(s, h1, q.z, q.w);
+                        wt_mma(x, h1, ql.z, ql.w);
+                        wt_mma(x, l0, q.x, q.y);
+                        wt_mma(x, l1, q.z, q.w);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[nt][e] = fmaf(s[e] + x[e], d[e >> 1], acc[nt][e]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < WT_TILES; ++nt)
+                    if (nt < tiles) add(nt, acc[nt], 1.0f, 0.0f);
+            }
+            // the rows of the four lanes
+            sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
+            sum1 += __shfl_xor_sync(0xffffffffu, sum1, 1);
+            sum0 += __shfl_xor_sync(0xffffffffu, sum0, 2);
+            sum1 += __shfl_xor_sync(0xffffffffu, sum1, 2);
+            if (t < 2 && tok < end) {
+                float x = t ? sum1 : sum0;
+                if (chunk > 0) x += s_sum[tok - begin];
+                if (last) *at = tok < fresh && p.decay != 0.0f ? fmaf(p.decay, held, x) : x;
+                else s_sum[tok - begin] = x;
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (last) break;
+    }
+    }
+}
+
+WeightsPlan weights_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
+    WeightsPlan p;
+    const int64_t rows = n * grp, len = max_len > 0 ? max_len : 1, pairs = (int64_t)B * Hkv;
+    p.chunks = (int)((rows + WT_ROWS - 1) / WT_ROWS);
+    if (p.chunks < 1) p.chunks = 1;
+    const int64_t slots = 2 * (int64_t)sm_count();
+    // a CTA's time is its tokens plus a start worth some: the split with the least waves * (tokens + start)
+    int64_t best = INT64_MAX;
+    for (int s = 1; s <= 256; ++s) {
+        const int64_t per = ((len + s - 1) / s + 127) / 128 * 128;
+        if (s > 1 && (int64_t)(s - 1) * per >= len) continue;
+        const int64_t waves = (pairs * s + slots - 1) / slots, cost = waves * (per + 512);
+        if (cost < best) { best = cost; p.splits = s; }
+        if (waves > 8) break;
+    }
+    return p;
+}
+
+template <int D, int QT> static cudaError_t launch_weights_t(const WeightsRun& r, const WeightsPlan& p, cudaStream_t st) {
+    using C = WtCfg<D, QT>;
+    const cudaError_t e = cudaFuncSetAttribute(weights_kernel<D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t grid = (int64_t)r.q.B * r.q.Hkv * p.splits;
+    if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
+    weights_kernel<D, QT><<<(unsigned)grid, WT_THREADS, C::SMEM, st>>>(r, p.splits, p.chunks);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_weights(const WeightsRun& r, const WeightsPlan& p, void*, cudaStream_t st) {
+    const auto run = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        switch (r.k_type) {
+            case 8: return launch_weights_t<D, 8>(r, p, st);
+            case 4: return launch_weights_t<D, 4>(r, p, st);
+            case 3: return launch_weights_t<D, 3>(r, p, st);
+            default: return launch_weights_t<D, 2>(r, p, st);
+        }
+    };
+    return r.q.D == 256 ? run(std::integral_constant<int, 256>()) : run(std::integral_constant<int, 128>());
+}
+
+}  // namespace tq

@@ -467,6 +467,142 @@ def dequantize_q8(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype =
     return out
 
 
+# ── trees of drafted tokens, eviction ────────────────────────────────────────
+
+class DraftTree(NamedTuple):
+    """Trees of drafted tokens as the attention takes them: mask int32 [batch, n, ceil(n / 32)], bit j & 31 of word j >> 5
+    set where node i sees node j; depth int32 [batch, n], 0 for a root."""
+    mask: torch.Tensor
+    depth: torch.Tensor
+
+
+def draft_tree(parents: torch.Tensor) -> DraftTree:
+    """Ancestor masks and depths of trees of drafted tokens (tq_draft_tree_cuda).
+
+    parents: int32 CUDA [batch, n] (or [n], one tree for all sequences) of any batch stride, the parent of each node, which
+    comes before it, -1 for children of the cached tokens (other entries that do not come before their node are taken so, too).
+    A node sees itself and its ancestors; its position is that of the first token behind the cached ones plus its
+    depth.  At most 4096 nodes."""
+    device = _device_of(parents)
+    if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or (parents.shape[-1] > 1 and parents.stride(-1) != 1):
+        raise ValueError("parents must be an int32 [batch, n] or [n] tensor, n contiguous")
+    B, n = (1, parents.shape[0]) if parents.dim() == 1 else parents.shape
+    mask = torch.empty((B, n, -(-n // 32)), dtype=torch.int32, device=parents.device)
+    depth = torch.empty((B, n), dtype=torch.int32, device=parents.device)
+    stride = parents.stride(0) if parents.dim() == 2 else 0
+    _call(device, L.load().tq_draft_tree_cuda, parents.data_ptr(), stride, B, n, mask.data_ptr(), depth.data_ptr())
+    return DraftTree(mask, depth)
+
+
+_SELECT = struct.Struct("iiPPPqqqqPP")                # tq_select_args
+_MOVE = struct.Struct("iiiqPiPPPiPPiPPPqPPPN")        # tq_kv_move_args
+
+
+def _check_weights(t: torch.Tensor) -> tuple:
+    """(pages, heads, page_size) of a pool of summed attention weights."""
+    if t.dtype != torch.float32 or t.dim() != 3 or not t.is_contiguous():
+        raise ValueError("weights must be a contiguous float32 [num_pages, n_kv_heads, page_size] tensor")
+    return t.shape
+
+
+def _check_status(t: torch.Tensor | None, name: str = "status") -> int:
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or t.numel() < 1:
+        raise ValueError(f"{name} must be an int32 tensor")
+    return t.data_ptr()
+
+
+def select_tokens(weights: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, keep, sinks: int = 0,
+                  recent: int = 0, width: int | None = None, max_kv_len: int | None = None,
+                  out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """The cached tokens of each (sequence, KV head) that stay (tq_select_tokens_cuda).
+
+    weights float32 [num_pages, n_kv_heads, page_size], the sums that attention_weights_paged keeps; page_table int32
+    [B, max_pages_per_seq]; kv_len int32 [B].  keep: one number, or int32 CUDA [B] with width, their bound.  Of
+    k = min(keep, kv_len, width) tokens the last min(recent, k) stay, the first min(sinks, k - recent), and of the others
+    those with the largest weights, ties to the lowest slot, NaN as -inf.  Returns int32 [B, n_kv_heads, width] (in out):
+    slots, rising, -1 behind the last.  max_kv_len: an upper bound of kv_len that sizes the work (default: the capacity); tokens
+    behind it are left out, with status raised, as for pages outside the pool (attention.last_status() without status)."""
+    tensors = (weights, page_table, kv_len, out, status) + ((keep,) if isinstance(keep, torch.Tensor) else ())
+    device = _device_of(*tensors)
+    pages, H, page_size = _check_weights(weights)
+    B = page_table.shape[0]
+    _check_table(page_table, B)
+    _check_lengths(kv_len, B, "kv_len")
+    if isinstance(keep, torch.Tensor):
+        _check_lengths(keep, B, "keep")
+        if width is None:
+            raise ValueError("a tensor of numbers to keep needs width, their bound")
+        each = keep.data_ptr()
+    else:
+        if int(keep) < 0:
+            raise ValueError("keep must not be negative")
+        width, each = min(int(keep), int(keep) if width is None else int(width)), 0
+    if out is None:
+        out = torch.empty((B, H, width), dtype=torch.int32, device=weights.device)
+    elif out.dtype != torch.int32 or out.shape != (B, H, width) or not out.is_contiguous():
+        raise ValueError("out must be a contiguous int32 [B, n_kv_heads, width] tensor")
+    a = _SELECT.pack(B, H, weights.data_ptr(), kv_len.data_ptr(), each, width, int(sinks), int(recent), int(max_kv_len or 0),
+                     out.data_ptr(), _check_status(status))
+    _call(device, L.load().tq_select_tokens_cuda, a, _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size))
+    return out
+
+
+def kv_move_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor, src: torch.Tensor,
+                  first: torch.Tensor | None = None, count: torch.Tensor | None = None,
+                  k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                  weights: torch.Tensor | None = None, to_table: torch.Tensor | None = None,
+                  overflow: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Moves rows of a paged cache between token slots (tq_kv_move_paged_cuda): the accepted path of a drafted tree, the
+    tokens that stay after an eviction.
+
+    Row j of sequence b and KV head h goes from slot src[b, h, j] to slot first[b] + j (first: int32 [B], default 0).  src
+    int32 [B, n_kv_heads, n] or, for all heads alike, [B, n]; negative entries move nothing; rows j >= count[b] (int32
+    [B]) neither.  Pools as kv_append_rotary_paged writes them (TQ rows are copied; 8-bit blocks of rows of one scale keep
+    codes and scale, others get max |code| scale / 127).  weights: pool of summed attention weights, moved along.  In place
+    rows may only move down (src >= first + j); to_table (int32 [B, pages]) names other pages for the destination, none that
+    are read.  Rows without a place, or that would move up, are left and counted into overflow, one per head."""
+    device = _device_of(k_pool, v_pool, page_table, src, first, count, k_scale, v_scale, weights, to_table, overflow, status)
+    B = page_table.shape[0]
+    _check_table(page_table, B)
+    if k_pool.dtype == torch.int8:
+        H, D = (k_pool.shape[1], k_pool.shape[3]) if k_pool.dim() == 4 else (0, 0)
+        pages, page_size = _check_q8_pools(k_pool, v_pool, k_scale, v_scale, H, D)
+        kt = vt = Q8
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    else:
+        if k_pool.dim() != 5 or v_pool.dim() != 5 or k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 \
+                or k_pool.shape[:4] != v_pool.shape[:4] or v_pool.shape[4] != BLOCK_BYTES[TQ4_0] \
+                or k_pool.shape[4] not in _TYPE_OF_BYTES or not k_pool.is_contiguous() or not v_pool.is_contiguous():
+            raise ValueError("pools must be contiguous uint8 [num_pages, n_kv_heads, page_size, head_dim/32, bytes] "
+                             "blocks, TQ4_0 for the values")
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("TQ pools have no scales")
+        pages, H, page_size, D = k_pool.shape[0], k_pool.shape[1], k_pool.shape[2], k_pool.shape[3] * QK
+        kt, vt, ks, vs = _TYPE_OF_BYTES[k_pool.shape[4]], TQ4_0, 0, 0
+    if src.dtype != torch.int32 or src.dim() not in (2, 3) or src.shape[0] != B or not src.is_contiguous() \
+            or (src.dim() == 3 and src.shape[1] not in (1, H)):
+        raise ValueError("src must be a contiguous int32 [B, n_kv_heads, n] or [B, n] tensor")
+    for t, name in ((first, "first"), (count, "count")):
+        if t is not None:
+            _check_lengths(t, B, name)
+    if weights is not None and _check_weights(weights) != (pages, H, page_size):
+        raise ValueError(f"weights must be [{pages}, {H}, {page_size}], as the pools")
+    if to_table is not None:
+        _check_table(to_table, B)
+    p = lambda t: 0 if t is None else t.data_ptr()   # noqa: E731
+    fields = (B, H, D, src.shape[-1], src.data_ptr(), src.shape[1] if src.dim() == 3 else 1, p(first), p(count),
+              k_pool.data_ptr(), kt, ks, v_pool.data_ptr(), vt, vs, p(weights), p(to_table),
+              0 if to_table is None else to_table.shape[1], _check_status(overflow, "overflow"), _check_status(status))
+    pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
+    lib = L.load()
+    need = lib.tq_kv_move_workspace_size(_MOVE.pack(*fields, 0, 0), pg)
+    # from the allocator on every call: streams and captured graphs each get their own
+    ws = torch.empty(need, dtype=torch.uint8, device=k_pool.device) if need else None
+    _call(device, lib.tq_kv_move_paged_cuda, _MOVE.pack(*fields, ws.data_ptr() if need else 0, need), pg)
+
+
 TQ2_1_BYTES = 44   # block_tq2_1: a TQ3_0 block and three TQ2_0 blocks per 128 elements
 
 
