@@ -43,6 +43,20 @@ slots.  8-bit blocks that held a rejected row keep a scale that is large enough 
     ...                                          # append, attention, acceptance
     cache.commit(cache.batch([a, b], [2, 4]))
 
+A tree of drafted tokens (k_bits=8): its nodes are appended like a step's tokens, rotated by their depths, and see the
+cached tokens and their ancestors; the accepted path's rows then move up behind the cached ones.
+
+    step = cache.batch([a, b], n, tree=parents)  # parents of the n nodes, -1 for children of the cached tokens
+    q = cache.append(step, layer, k, v, rope=rope, q=q)
+    out = cache.attention(step, layer, q)
+    cache.accept(step, [[0, 2, 5], [1]])         # in place of the commit
+
+Eviction (track_weights=True): attention counts the weights that cached tokens get, evict drops those with the least of
+them, each KV head of each layer its own; positions go on counting from the tokens that a sequence has had.
+
+    out = cache.attention(step, layer, q, observe=1)   # the last query token of each sequence counts
+    cache.evict([a, b], keep=1024, sinks=4, recent=128)
+
 Page bookkeeping (PageTable) is host-side and needs no GPU.
 """
 from __future__ import annotations
@@ -67,6 +81,7 @@ class PageTable:
         self.max_seqs, self.max_pages_per_seq = max_seqs, max_pages_per_seq
         self.table = np.full((max_seqs, max_pages_per_seq), NO_PAGE, dtype=np.int32)
         self.lens = np.zeros(max_seqs, dtype=np.int64)
+        self.dropped = np.zeros(max_seqs, dtype=np.int64)   # tokens evicted: what positions are ahead of slots
         self.n_pages = np.zeros(max_seqs, dtype=np.int64)   # pages held per sequence
         self.active = np.zeros(max_seqs, dtype=bool)
         self._free = list(range(num_pages - 1, -1, -1))     # pop() hands out low pages first
@@ -88,6 +103,7 @@ class PageTable:
         s = int(idle[0])
         self.active[s] = True
         self.lens[s] = 0
+        self.dropped[s] = 0
         return s
 
     def free_sequence(self, s: int) -> None:
@@ -97,6 +113,7 @@ class PageTable:
         self.table[s, :] = NO_PAGE
         self.n_pages[s] = 0
         self.lens[s] = 0
+        self.dropped[s] = 0
         self.active[s] = False
         self.dirty.add(s)
 
@@ -138,6 +155,20 @@ class PageTable:
                 raise ValueError(f"sequence {s}: {n} tokens were not reserved")
             self.lens[s] += n
 
+    def truncate(self, s: int, length: int) -> None:
+        """The sequence keeps its first `length` tokens; pages behind them return to the pool."""
+        self._check(s)
+        if not 0 <= length <= self.lens[s]:
+            raise ValueError(f"sequence {s} has {int(self.lens[s])} tokens")
+        held = -(-length // self.page_size)
+        self._free.extend(int(p) for p in self.table[s, held: self.n_pages[s]][::-1])
+        if held < self.n_pages[s]:
+            self.table[s, held: self.n_pages[s]] = NO_PAGE
+            self.n_pages[s] = held
+            self.dirty.add(s)
+        self.dropped[s] += self.lens[s] - length
+        self.lens[s] = length
+
     def _check(self, s: int) -> None:
         if not (0 <= s < self.max_seqs) or not self.active[s]:
             raise ValueError(f"sequence {s} is not active")
@@ -155,6 +186,10 @@ class Batch:
     counts: "object" = None    # new tokens of each sequence where they differ (else n_new each)
     new_len: "object" = None   # int32 [B]: the same on the device
     seen_len: "object" = None  # int32 [B]: kv_len, 0 where a sequence has only padding (None: none has)
+    positions: "object" = None # int32 [B, n_new] where they are not the slots (trees, sequences with evicted tokens)
+    tree: "object" = None      # ops.DraftTree
+    parents: "object" = None   # the tree's, numpy [B or 1, n_new] (None: they came from the device)
+    starts: "object" = None    # pos on the host
 
 
 class PagedKVCache:
@@ -162,7 +197,7 @@ class PagedKVCache:
 
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, num_pages: int, page_size: int = 16,
                  max_seqs: int = 64, max_pages_per_seq: int | None = None, k_bits: int = 3, k_opt_passes: int = 0,
-                 device: str = "cuda"):
+                 device: str = "cuda", track_weights: bool = False):
         import torch
         if head_dim not in (128, 256):
             raise ValueError("head_dim must be 128 or 256 (fused decode attention)")
@@ -188,6 +223,10 @@ class PagedKVCache:
             self.k_scale = self.v_scale = [None] * n_layers
         self._table = torch.full((max_seqs, max_pages_per_seq), NO_PAGE, dtype=torch.int32, device=self.device)
         self._lens = torch.zeros(max_seqs, dtype=torch.int32, device=self.device)
+        # sums of attention weights beside the pages, every layer's
+        self._weights = torch.zeros((n_layers, num_pages, n_kv_heads, page_size), dtype=torch.float32, device=self.device) \
+            if track_weights else None
+        self.weights = [None] * n_layers if self._weights is None else list(self._weights)
 
     # sequence management (host bookkeeping; page-table rows reach the device in batch())
     def add_sequence(self) -> int:
@@ -201,36 +240,68 @@ class PagedKVCache:
     def seq_len(self, s: int) -> int:
         return int(self.pages.lens[s])
 
-    def batch(self, seqs: Sequence[int], n_new=1) -> Batch:
+    def batch(self, seqs: Sequence[int], n_new=1, tree=None) -> Batch:
         """Reserve pages for n_new tokens of every sequence and gather the step's device views.  With a count
-        for each sequence the step's tensors have max(n_new) rows, those behind a sequence's count are padding."""
+        for each sequence the step's tensors have max(n_new) rows, those behind a sequence's count are padding.
+
+        tree: the tokens are nodes of trees of drafted tokens: their parents, which come before them (-1: the cached
+        tokens), [max(n_new)] for all sequences or [B, max(n_new)], from the host or an int32 CUDA tensor."""
         import torch
         seqs = [int(s) for s in seqs]
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence may appear once per batch")
         counts = self.pages._counts(seqs, n_new)
+        rows = max(counts, default=0)
+        parents = None
+        if tree is not None:
+            if self.k_bits != 8:
+                raise ValueError("trees are attended in 8-bit pages (k_bits=8)")
+            if not isinstance(tree, torch.Tensor) or not tree.is_cuda:
+                parents = np.atleast_2d(np.asarray(tree, dtype=np.int32))
+                if parents.ndim != 2 or (parents >= np.arange(parents.shape[1])).any() or (parents < -1).any():
+                    raise ValueError("parents must come before their nodes, -1 for children of the cached tokens")
+                tree = torch.from_numpy(parents).to(self.device)
+            if tuple(tree.shape) not in ((rows,), (1, rows), (len(seqs), rows)):
+                raise ValueError(f"tree must have the step's {rows} nodes, one tree or {len(seqs)} of them")
+        fresh_pages = self.pages.n_pages[seqs].copy() if self._weights is not None else None
         self.pages.reserve(seqs, counts)
+        if fresh_pages is not None:
+            got = [int(p) for s, n in zip(seqs, fresh_pages) for p in self.pages.table[s, n: self.pages.n_pages[s]]]
+            if got:
+                self._weights.index_fill_(1, torch.tensor(got, dtype=torch.int64, device=self.device), 0.0)
         self._sync()
         idx = torch.tensor(seqs, dtype=torch.int64, device=self.device)
         pos = self._lens.index_select(0, idx)
         lens = self.pages.lens[seqs] + np.asarray(counts, dtype=np.int64)
-        rows = max(counts, default=0)
         alike = all(n == rows for n in counts)
         new_len = None if alike else torch.tensor(counts, dtype=torch.int32, device=self.device)
         kv_len = (pos + (rows if alike else new_len)).contiguous()
-        return Batch(seqs, rows, self._table.index_select(0, idx).contiguous(), pos.contiguous(), kv_len,
+        step = Batch(seqs, rows, self._table.index_select(0, idx).contiguous(), pos.contiguous(), kv_len,
                      int(lens.max()) if len(seqs) else 0, None if alike else counts, new_len,
-                     None if alike or min(counts) else kv_len * (new_len > 0))
+                     None if alike or min(counts) else kv_len * (new_len > 0), parents=parents,
+                     starts=[int(n) for n in self.pages.lens[seqs]])
+        dropped = self.pages.dropped[seqs]
+        if tree is not None or dropped.any():
+            from . import ops
+            first = pos + torch.from_numpy(dropped.astype(np.int32)).to(self.device)
+            ahead = torch.arange(rows, dtype=torch.int32, device=self.device)
+            if tree is not None:
+                step.tree = ops.draft_tree(tree)
+                ahead = step.tree.depth
+            step.positions = (first[:, None] + ahead).contiguous()
+        return step
 
     def append(self, step: Batch, layer: int, k, v, rope=None, positions=None, q=None):
         """Quantize-on-write of the step's new rows k, v [B, n_kv_heads, n_new, head_dim].
 
         rope (ops.Rotary): k (and q [B, n_q_heads, n_new, head_dim], whose rotated rows are returned) as they
-        leave the projection, any strides; turned by their positions (default: their slots; int32 [B, n_new]
-        or [axes, B, n_new] otherwise) in the same launch."""
+        leave the projection, any strides; turned by their positions (default: the tokens that came before, a tree's
+        nodes by their depths; int32 [B, n_new] or [axes, B, n_new] otherwise) in the same launch."""
         import torch
         from . import ops
         B = len(step.seqs)
+        if positions is None and rope is not None:
+            positions = step.positions
         for t, name in ((k, "k"), (v, "v")):
             if tuple(t.shape) != (B, self.n_kv_heads, step.n_new, self.head_dim):
                 raise ValueError(f"{name} must be [{B}, {self.n_kv_heads}, {step.n_new}, {self.head_dim}]")
@@ -254,26 +325,128 @@ class PagedKVCache:
         ops.kv_append_paged(v.contiguous(), self.v[layer], step.table, step.pos, qtype=4)
         return out
 
-    def attention(self, step: Batch, layer: int, q, sm_scale: float | None = None, out_dtype=None, out=None):
+    def attention(self, step: Batch, layer: int, q, sm_scale: float | None = None, out_dtype=None, out=None,
+                  return_lse: bool = False, observe: int = 0, decay: float = 1.0):
         """Attention over each sequence's tokens, this step's included: q [B, n_q_heads, head_dim], one token per
         sequence (its last), or, with k_bits=8, [B, n_q_heads, n_new, head_dim], each row seeing the tokens up to its
-        own; rows of padding, in the first form those of sequences without a token in a step of unequal counts, give
-        zeros.  attention.last_status() tells whether a kernel met a page id outside the pool or gave up a wait."""
+        own (a tree's node: its ancestors); rows of padding, in the first form those of sequences without a token in a step of
+        unequal counts, give zeros.  attention.last_status() tells whether a kernel met a page id outside the pool or gave up a wait.
+
+        observe: that many of each sequence's last query tokens count towards the weights by which evict() chooses, earlier
+        counts times decay (track_weights=True; after a tree's step the accepted rows count by observe())."""
         from . import attention as A
+        if observe and step.tree is not None:
+            raise ValueError("nodes of a tree may be rejected: observe() the accepted ones after accept()")
+        if observe:
+            self._need_weights()
+        want_lse = return_lse or bool(observe)
         if self.k_bits == 8:
             if q.dim() == 4 and q.shape[2] != step.n_new:
                 raise ValueError(f"q must have the step's {step.n_new} tokens")
+            if step.tree is not None and q.dim() == 3 and step.n_new != 1:
+                raise ValueError(f"q must have the step's {step.n_new} nodes")
             # one row per sequence out of several is the last one: a count above q's rows is taken as their number
-            return A.attention_q8_paged(q, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
-                                        step.table, step.kv_len, q_len=step.new_len,
-                                        max_kv_len=step.max_kv_len, sm_scale=sm_scale, out_dtype=out_dtype or q.dtype, out=out)
+            got = A.attention_q8_paged(q, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
+                                       step.table, step.kv_len, q_len=step.new_len, max_kv_len=step.max_kv_len,
+                                       sm_scale=sm_scale, out_dtype=out_dtype or q.dtype, out=out, return_lse=want_lse,
+                                       tree=step.tree)
+        else:
+            lens = step.kv_len if step.seen_len is None else step.seen_len
+            got = A.decode_attention_paged(q.contiguous(), self.k[layer], self.v[layer], step.table, lens,
+                                           max_kv_len=step.max_kv_len, sm_scale=sm_scale,
+                                           out_dtype=out_dtype or q.dtype, out=out, return_lse=want_lse)
+        if observe:
+            self.observe(step, layer, q, got[1], window=int(observe), decay=decay, sm_scale=sm_scale)
+        return got if return_lse or not want_lse else got[0]
+
+    def observe(self, step: Batch, layer: int, q, lse, window: int | None = None, decay: float = 1.0,
+                sm_scale: float | None = None) -> None:
+        """Counts the attention weights of the step's query rows (the last `window` of each sequence, default all), whose
+        attention left lse, towards the weights by which evict() chooses; earlier counts times decay.  Once a step and layer:
+        the step's own tokens begin at nothing.  After accept(), with the step it returns and the rows of q and lse of the
+        accepted nodes, as the rows of a chain."""
+        from . import attention as A
+        self._need_weights()
+        if step.tree is not None:
+            raise ValueError("nodes of a tree may be rejected: observe the accepted ones after accept()")
         lens = step.kv_len if step.seen_len is None else step.seen_len
-        return A.decode_attention_paged(q.contiguous(), self.k[layer], self.v[layer], step.table, lens,
-                                        max_kv_len=step.max_kv_len, sm_scale=sm_scale,
-                                        out_dtype=out_dtype or q.dtype, out=out)
+        A.attention_weights_paged(q, self.k[layer], step.table, lens, lse, self.weights[layer], k_scale=self.k_scale[layer],
+                                  q_len=step.new_len, fresh=step.pos, decay=decay, window=window,
+                                  max_kv_len=step.max_kv_len, sm_scale=sm_scale)
+
+    def accept(self, step: Batch, nodes: Sequence[Sequence[int]]) -> Batch:
+        """In place of the commit of a tree's step: of each sequence the nodes of a path (rising, none for a sequence that
+        accepts nothing) become its next tokens, the others are forgotten.  Returns the step of the accepted rows, committed."""
+        import torch
+        from . import ops
+        if step.tree is None:
+            raise ValueError("the step has no tree")
+        paths = [[int(x) for x in p] for p in nodes]
+        if len(paths) != len(step.seqs):
+            raise ValueError("nodes must have one path per sequence")
+        for i, path in enumerate(paths):
+            limit = step.n_new if step.counts is None else step.counts[i]
+            before = [-1] + path
+            if any(not a < x < limit for a, x in zip(before, path)):
+                raise ValueError(f"sequence {step.seqs[i]}: a path rises within its {limit} nodes")
+            if step.parents is not None:
+                row = step.parents[i if len(step.parents) > 1 else 0]
+                if any(int(row[x]) != a for a, x in zip(before, path)):
+                    raise ValueError(f"sequence {step.seqs[i]}: {path} is not a path of the tree")
+        for s, n in zip(step.seqs, step.starts):
+            if n != self.pages.lens[s]:
+                raise ValueError(f"sequence {s} has changed since the step")
+        rows = max((len(p) for p in paths), default=0)
+        if rows:
+            src = torch.tensor([p + [-1 << 30] * (rows - len(p)) for p in paths], dtype=torch.int32, device=self.device)
+            src = src + step.pos[:, None]
+            for layer in range(self.n_layers):
+                ops.kv_move_paged(self.k[layer], self.v[layer], step.table, src, first=step.pos, k_scale=self.k_scale[layer],
+                                  v_scale=self.v_scale[layer])
+        kept = self.batch(step.seqs, [len(p) for p in paths])
+        self.commit(kept)
+        return kept
+
+    def evict(self, seqs: Sequence[int], keep, sinks: int = 0, recent: int = 0) -> None:
+        """Drops tokens of the sequences until `keep` (one number, or one each) are left: in every layer each KV head keeps its
+        last `recent` and first `sinks` tokens and, of the others, those with the largest observed weights.  Pages that are
+        no longer needed return to the pool; later tokens' positions are not changed by it."""
+        import torch
+        from . import ops
+        self._need_weights()
+        seqs = [int(s) for s in seqs]
+        many = self.pages._counts(seqs, keep)
+        step = self.batch(seqs, 0)
+        left = [min(n, int(self.pages.lens[s])) for s, n in zip(seqs, many)]
+        width = max((n for s, n in zip(seqs, left) if n < self.pages.lens[s]), default=0)
+        if all(n == self.pages.lens[s] for s, n in zip(seqs, left)):
+            return
+        count = torch.tensor(left, dtype=torch.int32, device=self.device)
+        # sequences that keep all their tokens have nothing to move
+        moved = torch.tensor([n if n < self.pages.lens[s] else 0 for s, n in zip(seqs, left)], dtype=torch.int32, device=self.device)
+        for layer in range(self.n_layers if width else 0):
+            slots = ops.select_tokens(self.weights[layer], step.table, step.kv_len, moved, sinks=sinks, recent=recent,
+                                      width=width, max_kv_len=step.max_kv_len)
+            ops.kv_move_paged(self.k[layer], self.v[layer], step.table, slots, k_scale=self.k_scale[layer],
+                              v_scale=self.v_scale[layer], weights=self.weights[layer])
+        # slots behind the kept tokens begin at nothing
+        tail = [(int(self.pages.table[s, n // self.pages.page_size]), x) for s, n in zip(seqs, left) if n < self.pages.lens[s]
+                for x in range(n % self.pages.page_size, self.pages.page_size) if n % self.pages.page_size]
+        if tail:
+            page, slot = (torch.tensor(t, dtype=torch.int64, device=self.device) for t in zip(*tail))
+            self._weights[:, page, :, slot] = 0.0
+        for s, n in zip(seqs, left):
+            self.pages.truncate(s, n)
+        self._lens.index_copy_(0, torch.tensor(seqs, dtype=torch.int64, device=self.device), count)
+
+    def _need_weights(self) -> None:
+        if self._weights is None:
+            raise ValueError("weights are not tracked: PagedKVCache(track_weights=True)")
 
     def commit(self, step: Batch) -> None:
         """The step's rows are part of the sequences from now on."""
+        if step.tree is not None:
+            raise ValueError("a tree's step is committed by accept()")
         import torch
         self.pages.commit(step.seqs, step.n_new if step.counts is None else step.counts)
         idx = torch.tensor(step.seqs, dtype=torch.int64, device=self.device)
@@ -293,7 +466,7 @@ class PagedKVCache:
 
     def memory_summary(self) -> dict:
         pool = sum(t.numel() for t in self.k) + sum(t.numel() for t in self.v)
-        pool += sum(4 * t.numel() for t in self.k_scale + self.v_scale if t is not None)
+        pool += sum(4 * t.numel() for t in self.k_scale + self.v_scale + self.weights if t is not None)
         used = self.pages.num_pages - self.pages.free_pages
         return {"pool_bytes": pool, "pages": self.pages.num_pages, "pages_used": used,
                 "page_size": self.pages.page_size, "bytes_per_page_all_layers": pool // self.pages.num_pages,
