@@ -24,7 +24,7 @@ struct WeightsRun {
     float* weights = nullptr;         // [num_pages][Hkv][page]
 };
 struct WeightsPlan {
-    int chunks = 1;                   // of a KV head's query rows
+    int rows = 8, chunks = 1;         // query rows of a KV head at a time, and how often
     int splits = 1;                   // CTAs that share a (sequence, KV head)
     size_t bytes = 0;                 // work memory
 };

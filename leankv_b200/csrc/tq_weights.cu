@@ -5,15 +5,16 @@
 // with the log-sum-exp that the attention of those rows has left.  V is not read, and no weight leaves the SM.
 //
 // Work.  A CTA takes a run of tokens of one (sequence, KV head); its 8 warps take every 8th block of 16 tokens, copied into
-// a ring of the warp's own in shared memory (cp.async).  Products are mma.sync m16n8k16 with the keys as the A operand (16
-// tokens x 16 elements) and 8 query rows as B: a thread's sums over the rows are then sums over its columns, which four
+// a ring of the warp's own in shared memory (cp.async), their earlier weights with them.  Products are mma.sync with the keys as
+// the A operand (16 tokens) and 8 query rows as B: a thread's sums over the rows are then sums over its columns, which four
 // lanes add up at the end.  More than 32 rows are taken 32 at a time, the tokens' sums kept in shared memory between.
 //
-// What bounds it.  Single tokens: the keys' bytes.  Many rows: products and exponentials.
-//
-// Numbers.  Sums are fp32 results that later sums are added to, so weights are kept to fp32's size of error: q' is the sum of
-// two f16 terms (22 bits), 8-bit codes are exact in f16 (as subnormals (c + 128) 2^-24, the offset taken off in fp32, as in
-// the attention kernels), TurboQuant levels are the sum of two f16 terms, looked up by the pair.  Products are summed in fp32.
+// Numbers.  Sums are fp32 results that later sums are added to, so scores are kept to fp32's size of error.
+// 8 bits: codes enter s8 products (m16n8k32, exact in s32) as they lie in memory; a row of q' is scaled by its largest element
+// and is the sum of three terms of 8 bits, q1 + q2 / 254 + q3 / 254^2 (2^-24 of the largest element).  In f16 the codes have to be
+// converted and q' is two terms: as many operations on twice the instructions.  The sums start from the bits of 1.5 * 2^23, so that
+// they are floats as they are (their size is below 2^22).
+// TurboQuant: levels are the sum of two f16 terms, looked up by the pair, and so is q'; m16n8k16, fp32 sums.
 #include <type_traits>
 
 #include "leankv_tq.h"
@@ -23,7 +24,8 @@
 
 namespace tq {
 
-constexpr int WT_WARPS = 8, WT_THREADS = 32 * WT_WARPS, WT_TILES = 4, WT_ROWS = 8 * WT_TILES;
+constexpr int WT_WARPS = 8, WT_THREADS = 32 * WT_WARPS, WT_ROWS = 32;   // most rows at a time
+constexpr int WT_START = 256;     // what a CTA's start is worth, in tokens
 constexpr int WT_TOKENS = 2048;   // tokens of a CTA whose sums wait in shared memory
 
 __device__ __forceinline__ void wt_cp16(uint32_t dst, const void* src) {
@@ -39,10 +41,20 @@ __device__ __forceinline__ uint2 wt_lds64(uint32_t a) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
     return v;
 }
+__device__ __forceinline__ float wt_lds32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
 __device__ __forceinline__ uint32_t wt_lds16(uint32_t a) {
     uint16_t v;
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
     return v;
+}
+__device__ __forceinline__ void wt_imma(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void wt_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -50,16 +62,20 @@ __device__ __forceinline__ void wt_mma(float (&c)[4], const uint32_t (&a)[4], ui
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D, int QT> struct WtCfg {
-    static constexpr int NK = D / 16;
+// TILES: tiles of 8 rows at a time, 1 or 4
+template <int D, int QT, int TILES> struct WtCfg {
+    static constexpr int NK = D / 16, ROWS = 8 * TILES;
     static constexpr int ROWB = QT == 8 ? D : D / 32 * BlockBytes<QT == 8 ? 4 : QT>::value;
     static constexpr int TILE = 16 * ROWB;                       // bytes of a block of 16 tokens
+    static constexpr int STAGE = TILE + 64;                      // with their earlier weights
     static constexpr int STAGES = QT == 8 && D == 256 ? 3 : 4;
-    static constexpr int RING = STAGES * TILE;                   // per warp
-    static constexpr int QPART = WT_TILES * NK * 256, QBYTES = 2 * QPART;
+    static constexpr int RING = STAGES * STAGE;                  // per warp
+    // q': 8 bits three terms, [tile][pair of k-steps][3][lane] of 16 bytes; TurboQuant two parts of [tile][pair of k-steps][lane]
+    static constexpr int QPART = TILES * NK * 256, QBYTES = QT == 8 ? TILES * (D / 64) * 3 * 512 : 2 * QPART;
     // pairs of levels as f16 terms: an entry for every lane of a half warp, so that lookups do not meet in a bank
     static constexpr int PAIRS = QT == 4 ? 256 : QT == 3 ? 64 : QT == 2 ? 16 : 0, TABLE = PAIRS * 128;
-    static constexpr int SMEM = WT_WARPS * RING + QBYTES + TABLE;
+    static constexpr int SUMS = TILES > 1 ? WT_TOKENS * 4 : 0;   // tokens' sums between chunks of rows
+    static constexpr int SMEM = WT_WARPS * RING + QBYTES + TABLE + SUMS;
     static constexpr int CTAS = SMEM <= 74 * 1024 ? 3 : SMEM <= 112 * 1024 ? 2 : 1;
 };
 
@@ -76,18 +92,17 @@ template <int QT> __device__ __forceinline__ uint2 level_pair(int a, int b) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&hi), *reinterpret_cast<const uint32_t*>(&lo));
 }
 
-template <int D, int QT>
-__global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel(const WeightsRun p, int splits, int row_chunks) {
-    using C = WtCfg<D, QT>;
-    constexpr int NK = C::NK, LPR = D / 16;
+template <int D, int QT, int TILES>
+__global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights_kernel(const WeightsRun p, int splits, int row_chunks) {
+    using C = WtCfg<D, QT, TILES>;
+    constexpr int NK = C::NK, LPR = D / 16, ROWS = C::ROWS;
     const Q8Run& r = p.q;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* s_q = smem + WT_WARPS * C::RING;
     uint8_t* s_table = s_q + C::QBYTES;
-    __shared__ __align__(16) float2 s_f[WT_ROWS];   // a row's factor of the sums of codes, and that of 128 * sum of its q'
-    __shared__ float s_lse[WT_ROWS];                // its log-sum-exp in the log2 domain
-    __shared__ int s_lim[WT_ROWS];                  // last token that it sees
-    __shared__ float s_sum[WT_TOKENS];              // tokens' sums between chunks of rows
+    float* s_sum = reinterpret_cast<float*>(s_table + C::TABLE);
+    __shared__ __align__(16) float2 s_f[ROWS];      // a row's factor of the scores and its log-sum-exp, in the log2 domain
+    __shared__ int s_lim[ROWS];                     // last token that it sees
 
     const int split = blockIdx.x % splits, pair = blockIdx.x / splits, h = pair % r.Hkv, b = pair / r.Hkv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -116,10 +131,10 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
     const int nblk_all = (end - begin + 15) >> 4, blk0 = begin >> 4;
     const int mine = nblk_all > warp ? (nblk_all - warp + WT_WARPS - 1) / WT_WARPS : 0;
     for (int chunk = 0; chunk < row_chunks; ++chunk) {
-        const int row0 = chunk * WT_ROWS, rows = rows_all - row0 < WT_ROWS ? rows_all - row0 : WT_ROWS;
-        if (chunk > 0 && rows <= 0) break;
-        const bool last = chunk + 1 == row_chunks || rows_all - row0 <= WT_ROWS;
-        const int tiles = rows > 0 ? (rows + 7) >> 3 : 0;
+        const int row0 = chunk * ROWS, rows = rows_all - row0 < ROWS ? rows_all - row0 : ROWS;
+        const bool last = chunk + 1 == row_chunks || rows_all - row0 <= ROWS;
+        const int tiles = TILES == 1 ? 1 : rows > 0 ? (rows + 7) >> 3 : 0;
+        const bool reads = last && p.decay != 0.0f;   // the earlier weights, copied with the keys
 
         int nx_blk = -1, cu_blk = -1;                // windows of 32 blocks, one per lane
         float nx_ks = 0.0f, cu_ks = 0.0f;
@@ -135,29 +150,28 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
                 }
             }
         };
+        // 8 bits: 16-byte chunk c of token x in a 128-byte half goes to chunk c ^ (x & 7) of half * 2048 + x * 128; a lane takes
+        // every 32nd chunk of the block, and its places differ by constants and by the xor of constants
+        const uint32_t to0 = QT != 8 ? lane * 16 : D == 128 ? (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4)
+                                       : ((lane >> 3) & 1) * 2048 + (lane >> 4) * 128 + (((lane & 7) ^ (lane >> 4)) << 4);
         uint32_t fill = ring;
         auto issue = [&](int i) {
             if (i < mine) {
                 if ((i & 31) == 0) window(i);
                 const int blk = __shfl_sync(0xffffffffu, nx_blk, i & 31);
                 if (blk >= 0) {
-                    const int8_t* kp = r.k + (int64_t)blk * C::TILE;
+                    const int8_t* kp = r.k + (int64_t)blk * C::TILE + lane * 16;
 #pragma unroll
                     for (int e = 0; e < (C::TILE + 511) / 512; ++e) {
-                        const int c = lane + 32 * e;
-                        if (C::TILE % 512 == 0 || c < C::TILE / 16) {
-                            int to = c * 16;
-                            if constexpr (QT == 8) {   // chunk c of token x in a 128-byte half at c ^ (x & 7) of half * 2048 + x * 128
-                                const int x = c / LPR, cc = c % LPR;
-                                to = (cc >> 3) * 2048 + x * 128 + (((cc & 7) ^ (x & 7)) << 4);
-                            }
-                            wt_cp16(fill + to, kp + c * 16);
-                        }
+                        uint32_t to = to0 + e * 512;
+                        if constexpr (QT == 8) to = e * (D == 128 ? 512 : 256) + (to0 ^ (D == 128 ? (e & 1) << 6 : ((2 * e) & 7) << 4));
+                        if (C::TILE % 512 == 0 || lane + 32 * e < C::TILE / 16) wt_cp16(fill + to, kp + e * 512);
                     }
+                    if (reads && lane < 4) wt_cp16(fill + C::TILE + lane * 16, p.weights + (int64_t)blk * 16 + lane * 4);
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
-            fill += C::TILE;
+            fill += C::STAGE;
             if (fill == ring + C::RING) fill = ring;
         };
         if (chunk > 0 || begin > begin_all) __syncthreads();   // the rows before have been used
@@ -182,39 +196,52 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
             for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(v[j]));
 #pragma unroll
             for (int o = 1; o < LPR; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
-            float sum = 0.0f;
-            // Element e of the row goes where the keys' element meets it: half-word `odd` of word w (b0, b1 of one k-step, then of
-            // the next) of lane tt, pair of k-steps j2.  8 bits: a lane's elements are one run of 32 bytes in 128.  TurboQuant: a
-            // pair of k-steps is a block of 32 elements, lane tt has 8 of them: TQ4 the nibbles of bytes 4 tt .. 4 tt + 3 (e and
-            // e + 16 in a byte), TQ3 the group of 8 codes tt, TQ2 those of bytes 2 tt, 2 tt + 1.
-            __half* qh = reinterpret_cast<__half*>(s_q) + (row >> 3) * (NK / 2) * 256 + (row & 7) * 32;
+            if constexpr (QT == 8) {
+                // element e: byte e & 3 of word b (0, 1) of k-step s of lane tt, whose elements are one run of 32 in 128
+                const float inv = top >= 0x1p-100f ? __fdiv_rn(127.0f, top) : 0.0f;
+                uint32_t w[12];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int e = e0 + j;
-                const float x = v[j] * inv;
-                const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
-                sum += __half2float(hi) + __half2float(lo);
-                int j2, tt, w, odd;
-                if constexpr (QT == 8) {
-                    j2 = (e >> 7) * 4 + ((e & 31) >> 3); tt = (e & 127) >> 5; w = (e & 7) >> 1; odd = e & 1;
-                } else if constexpr (QT == 4) {
-                    j2 = e >> 5; tt = (e & 15) >> 2; w = e & 3; odd = (e >> 4) & 1;
-                } else {
-                    j2 = e >> 5; tt = (e & 31) >> 3; w = (e & 7) >> 1; odd = e & 1;
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t q1 = 0, q2 = 0, q3 = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float x = v[4 * j + k] * inv, a = rintf(x), y = (x - a) * 254.0f, c = rintf(y), d = rintf((y - c) * 254.0f);
+                        q1 |= ((uint32_t)(int)a & 0xFFu) << (8 * k);
+                        q2 |= ((uint32_t)(int)c & 0xFFu) << (8 * k);
+                        q3 |= ((uint32_t)(int)d & 0xFFu) << (8 * k);
+                    }
+                    w[(j >> 1) * 6 + (j & 1)] = q1;
+                    w[(j >> 1) * 6 + 2 + (j & 1)] = q2;
+                    w[(j >> 1) * 6 + 4 + (j & 1)] = q3;
                 }
-                __half* to = qh + j2 * 256 + tt * 8 + w * 2 + odd;
-                to[0] = hi;
-                to[C::QPART / 2] = lo;
-            }
+                const int half = e0 >> 7, tt = (e0 & 127) >> 5, pr = half * 2 + ((e0 & 31) >> 4);
+                uint4* to = reinterpret_cast<uint4*>(s_q) + ((row >> 3) * (D / 64) + pr) * 96 + (row & 7) * 4 + tt;
+                to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                to[32] = make_uint4(w[4], w[5], w[6], w[7]);
+                to[64] = make_uint4(w[8], w[9], w[10], w[11]);
+            } else {
+                const float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
+                // Element e of the row goes where the keys' element meets it: half-word `odd` of word w (b0, b1 of one k-step, then
+                // of the next) of lane tt, pair of k-steps j2.  A pair of k-steps is a block of 32 elements, lane tt has 8 of them:
+                // TQ4 the nibbles of bytes 4 tt .. 4 tt + 3 (e and e + 16 in a byte), TQ3 the group of 8 codes tt, TQ2 those of bytes
+                // 2 tt, 2 tt + 1.
+                __half* qh = reinterpret_cast<__half*>(s_q) + (row >> 3) * (NK / 2) * 256 + (row & 7) * 32;
 #pragma unroll
-            for (int o = 1; o < LPR; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                for (int j = 0; j < 16; ++j) {
+                    const int e = e0 + j;
+                    const float x = v[j] * inv;
+                    const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
+                    const int j2 = e >> 5, tt = QT == 4 ? (e & 15) >> 2 : (e & 31) >> 3, w = QT == 4 ? e & 3 : (e & 7) >> 1;
+                    const int odd = QT == 4 ? (e >> 4) & 1 : e & 1;
+                    __half* to = qh + j2 * 256 + tt * 8 + w * 2 + odd;
+                    to[0] = hi;
+                    to[C::QPART / 2] = lo;
+                }
+            }
             if (lane % LPR == 0) {
-                const float fr = top * r.sm_scale * LOG2E;
-                s_f[row] = QT == 8 ? make_float2(fr * 0x1p24f, fr * 128.0f * sum) : make_float2(fr, 0.0f);
                 const float lse = live ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : INFINITY;
                 const bool sees = live && lse != -INFINITY;   // a row that saw nothing adds nothing
-                s_lse[row] = sees ? lse * LOG2E : INFINITY;
+                s_f[row] = make_float2(top * (r.sm_scale * LOG2E * (QT == 8 ? 1.0f / 127.0f : 1.0f)), sees ? lse * LOG2E : INFINITY);
                 s_lim[row] = sees ? last_seen(r, sl, i) : 0x7fffffff;
             }
         }
@@ -224,7 +251,7 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
         lim_min = __reduce_min_sync(0xffffffffu, lim_min);
 
         // ── blocks of 16 tokens ──
-        uint32_t kt = ring - C::TILE;
+        uint32_t kt = ring - C::STAGE;
         for (int i = 0; i < mine; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
             __syncwarp();
@@ -233,74 +260,78 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
                 cu_ks = nx_ks;
             }
             issue(i + C::STAGES - 1);
-            kt += C::TILE;
+            kt += C::STAGE;
             if (kt == ring + C::RING) kt = ring;
             const int blk = __shfl_sync(0xffffffffu, cu_blk, i & 31);
             if (blk < 0) continue;                   // a page outside the pool holds nothing
             const float ks = __shfl_sync(0xffffffffu, cu_ks, i & 31);
             const int tok0 = (blk0 + warp + i * WT_WARPS) << 4, tok = tok0 + g + 8 * (t & 1);   // the token that this lane writes
             float* at = p.weights + ((int64_t)blk * 16 + (tok - tok0));
-            float held = 0.0f;
-            if (last && t < 2 && tok < end && tok < fresh && p.decay != 0.0f) held = *at;
 
             float sum0 = 0.0f, sum1 = 0.0f;          // tokens g, g + 8, this lane's rows
-            auto add = [&](int nt, const float (&s)[4], float f, float off) {
+            const bool edge = tok0 + 15 > lim_min;
+            auto add = [&](int nt, const float (&s)[4], float ks) {
                 // words 0, 1 of token g, words 2, 3 of token g + 8, for rows 2t and 2t + 1 of the tile
+                const float4 f = *reinterpret_cast<const float4*>(s_f + nt * 8 + 2 * t);
+                float x[4];
+                x[0] = ex2(fmaf(s[0], f.x * ks, -f.y));
+                x[1] = ex2(fmaf(s[1], f.z * ks, -f.w));
+                x[2] = ex2(fmaf(s[2], f.x * ks, -f.y));
+                x[3] = ex2(fmaf(s[3], f.z * ks, -f.w));
+                if (edge) {
+                    asm volatile("" ::: "memory");   // the last blocks only: kept a branch
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = nt * 8 + 2 * t + e;
-                    const float2 fr = s_f[row];
-                    const float a = fr.x * f, c = fmaf(-fr.y, off, -s_lse[row]);
-                    float x = ex2(fmaf(s[e], a, c)), y = ex2(fmaf(s[2 + e], a, c));
-                    if (tok0 + 15 > lim_min) {
-                        const int left = s_lim[row] - tok0 - g;
-                        if (left < 0) x = 0.0f;
-                        if (left < 8) y = 0.0f;
+                    for (int e = 0; e < 2; ++e) {
+                        const int left = s_lim[nt * 8 + 2 * t + e] - tok0 - g;
+                        if (left < 0) x[e] = 0.0f;
+                        if (left < 8) x[2 + e] = 0.0f;
                     }
-                    sum0 += x;
-                    sum1 += y;
                 }
+                sum0 += x[0] + x[1];
+                sum1 += x[2] + x[3];
             };
             if constexpr (QT == 8) {
-                uint32_t kw[D / 128][2][8];
+                uint32_t a[D / 32][4];
 #pragma unroll
                 for (int half = 0; half < D / 128; ++half)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const uint32_t row = kt + half * 2048 + (x * 8 + g) * 128;
                         const uint4 u = wt_lds128(row + (((2 * t) ^ g) << 4)), w = wt_lds128(row + (((2 * t + 1) ^ g) << 4));
-                        kw[half][x][0] = u.x; kw[half][x][1] = u.y; kw[half][x][2] = u.z; kw[half][x][3] = u.w;
-                        kw[half][x][4] = w.x; kw[half][x][5] = w.y; kw[half][x][6] = w.z; kw[half][x][7] = w.w;
+                        a[half * 4][x] = u.x; a[half * 4][2 + x] = u.y; a[half * 4 + 1][x] = u.z; a[half * 4 + 1][2 + x] = u.w;
+                        a[half * 4 + 2][x] = w.x; a[half * 4 + 2][2 + x] = w.y; a[half * 4 + 3][x] = w.z; a[half * 4 + 3][2 + x] = w.w;
                     }
                 for (int nt = 0; nt < tiles; ++nt) {
-                    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sl4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    int c[3][4];
 #pragma unroll
-                    for (int half = 0; half < D / 128; ++half)
+                    for (int k = 0; k < 3; ++k)
 #pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
-                            uint32_t a0[4], a1[4];
+                        for (int e = 0; e < 4; ++e) c[k][e] = 0x4B400000;   // 1.5 * 2^23
 #pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const uint32_t u = kw[half][x][j] ^ 0x80808080u, w = kw[half][x][j + 1] ^ 0x80808080u;
-                                a0[x] = __byte_perm(u, 0u, 0x4140); a0[2 + x] = __byte_perm(u, 0u, 0x4342);
-                                a1[x] = __byte_perm(w, 0u, 0x4140); a1[2 + x] = __byte_perm(w, 0u, 0x4342);
-                            }
-                            const uint32_t from = sq + (nt * (NK / 2) + half * 4 + j / 2) * 512;
-                            const uint4 q = wt_lds128(from), ql = wt_lds128(from + C::QPART);
-                            wt_mma(s, a0, q.x, q.y);
-                            wt_mma(sl4, a0, ql.x, ql.y);
-                            wt_mma(s, a1, q.z, q.w);
-                            wt_mma(sl4, a1, ql.z, ql.w);
-                        }
+                    for (int pr = 0; pr < D / 64; ++pr) {
+                        const uint32_t from = sq + (nt * (D / 64) + pr) * 1536;
+                        const uint4 u = wt_lds128(from), v = wt_lds128(from + 512), w = wt_lds128(from + 1024);
+                        wt_imma(c[0], a[2 * pr], u.x, u.y);
+                        wt_imma(c[1], a[2 * pr], u.z, u.w);
+                        wt_imma(c[2], a[2 * pr], v.x, v.y);
+                        wt_imma(c[0], a[2 * pr + 1], v.z, v.w);
+                        wt_imma(c[1], a[2 * pr + 1], w.x, w.y);
+                        wt_imma(c[2], a[2 * pr + 1], w.z, w.w);
+                    }
+                    float s[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[e] += sl4[e];
-                    add(nt, s, ks, ks);
+                    for (int e = 0; e < 4; ++e) {
+                        constexpr float ZERO = 12582912.0f;
+                        s[e] = fmaf(__int_as_float(c[2][e]) - ZERO, 1.0f / (254.0f * 254.0f), (__int_as_float(c[1][e]) - ZERO) * (1.0f / 254.0f));
+                        s[e] += __int_as_float(c[0][e]) - ZERO;
+                    }
+                    add(nt, s, ks);
                 }
             } else {
                 // a block of 32 elements is two k-steps; its scales are those of tokens g and g + 8
-                float acc[WT_TILES][4];
+                float acc[TILES][4];
 #pragma unroll
-                for (int nt = 0; nt < WT_TILES; ++nt)
+                for (int nt = 0; nt < TILES; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
                 constexpr int BB = BlockBytes<QT>::value;
@@ -335,7 +366,7 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
                     const uint32_t h0[4] = {lv[0][0].x, lv[1][0].x, lv[0][1].x, lv[1][1].x}, h1[4] = {lv[0][2].x, lv[1][2].x, lv[0][3].x, lv[1][3].x};
                     const uint32_t l0[4] = {lv[0][0].y, lv[1][0].y, lv[0][1].y, lv[1][1].y}, l1[4] = {lv[0][2].y, lv[1][2].y, lv[0][3].y, lv[1][3].y};
 #pragma unroll
-                    for (int nt = 0; nt < WT_TILES; ++nt) {
+                    for (int nt = 0; nt < TILES; ++nt) {
                         if (nt >= tiles) break;
                         const uint32_t from = sq + (nt * (NK / 2) + j2) * 512;
                         const uint4 q = wt_lds128(from), ql = wt_lds128(from + C::QPART);
@@ -351,8 +382,8 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
                     }
                 }
 #pragma unroll
-                for (int nt = 0; nt < WT_TILES; ++nt)
-                    if (nt < tiles) add(nt, acc[nt], 1.0f, 0.0f);
+                for (int nt = 0; nt < TILES; ++nt)
+                    if (nt < tiles) add(nt, acc[nt], 1.0f);
             }
             // the rows of the four lanes
             sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
@@ -362,7 +393,8 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
             if (t < 2 && tok < end) {
                 float x = t ? sum1 : sum0;
                 if (chunk > 0) x += s_sum[tok - begin];
-                if (last) *at = tok < fresh && p.decay != 0.0f ? fmaf(p.decay, held, x) : x;
+                if (reads && tok < fresh) x = fmaf(p.decay, wt_lds32(kt + C::TILE + (tok - tok0) * 4), x);
+                if (last) *at = x;
                 else s_sum[tok - begin] = x;
             }
         }
@@ -375,28 +407,30 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT>::CTAS) weights_kernel
 WeightsPlan weights_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
     WeightsPlan p;
     const int64_t rows = n * grp, len = max_len > 0 ? max_len : 1, pairs = (int64_t)B * Hkv;
-    p.chunks = (int)((rows + WT_ROWS - 1) / WT_ROWS);
+    p.rows = rows <= 8 ? 8 : WT_ROWS;
+    p.chunks = (int)((rows + p.rows - 1) / p.rows);
     if (p.chunks < 1) p.chunks = 1;
-    const int64_t slots = 2 * (int64_t)sm_count();
-    // a CTA's time is its tokens plus a start worth some: the split with the least waves * (tokens + start)
+    const int64_t slots = 3 * (int64_t)sm_count();
+    // A CTA's time is its tokens plus a start worth some.  Sequences differ in length, and the grid is made for the longest:
+    // rather several waves of short CTAs than one of long ones, as far as the start lets them.
     int64_t best = INT64_MAX;
     for (int s = 1; s <= 256; ++s) {
         const int64_t per = ((len + s - 1) / s + 127) / 128 * 128;
         if (s > 1 && (int64_t)(s - 1) * per >= len) continue;
-        const int64_t waves = (pairs * s + slots - 1) / slots, cost = waves * (per + 512);
+        const int64_t waves = (pairs * s + slots - 1) / slots, cost = waves * (per + WT_START) + per;
         if (cost < best) { best = cost; p.splits = s; }
-        if (waves > 8) break;
+        if (waves > 16) break;
     }
     return p;
 }
 
-template <int D, int QT> static cudaError_t launch_weights_t(const WeightsRun& r, const WeightsPlan& p, cudaStream_t st) {
-    using C = WtCfg<D, QT>;
-    const cudaError_t e = cudaFuncSetAttribute(weights_kernel<D, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+template <int D, int QT, int TILES> static cudaError_t launch_weights_t(const WeightsRun& r, const WeightsPlan& p, cudaStream_t st) {
+    using C = WtCfg<D, QT, TILES>;
+    const cudaError_t e = cudaFuncSetAttribute(weights_kernel<D, QT, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)r.q.B * r.q.Hkv * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-    weights_kernel<D, QT><<<(unsigned)grid, WT_THREADS, C::SMEM, st>>>(r, p.splits, p.chunks);
+    weights_kernel<D, QT, TILES><<<(unsigned)grid, WT_THREADS, C::SMEM, st>>>(r, p.splits, p.chunks);
     return cudaGetLastError();
 }
 
@@ -404,10 +438,10 @@ cudaError_t launch_weights(const WeightsRun& r, const WeightsPlan& p, void*, cud
     const auto run = [&](auto d) {
         constexpr int D = decltype(d)::value;
         switch (r.k_type) {
-            case 8: return launch_weights_t<D, 8>(r, p, st);
-            case 4: return launch_weights_t<D, 4>(r, p, st);
-            case 3: return launch_weights_t<D, 3>(r, p, st);
-            default: return launch_weights_t<D, 2>(r, p, st);
+            case 8: return p.rows == 8 ? launch_weights_t<D, 8, 1>(r, p, st) : launch_weights_t<D, 8, 4>(r, p, st);
+            case 4: return p.rows == 8 ? launch_weights_t<D, 4, 1>(r, p, st) : launch_weights_t<D, 4, 4>(r, p, st);
+            case 3: return p.rows == 8 ? launch_weights_t<D, 3, 1>(r, p, st) : launch_weights_t<D, 3, 4>(r, p, st);
+            default: return p.rows == 8 ? launch_weights_t<D, 2, 1>(r, p, st) : launch_weights_t<D, 2, 4>(r, p, st);
         }
     };
     return r.q.D == 256 ? run(std::integral_constant<int, 256>()) : run(std::integral_constant<int, 128>());
