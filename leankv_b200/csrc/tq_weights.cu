@@ -25,7 +25,7 @@
 namespace tq {
 
 constexpr int WT_WARPS = 8, WT_THREADS = 32 * WT_WARPS, WT_ROWS = 32;   // most rows at a time
-constexpr int WT_START = 256;     // what a CTA's start is worth, in tokens
+constexpr int WT_START = 1024;     // what a CTA's start is worth, in tokens
 constexpr int WT_TOKENS = 2048;   // tokens of a CTA whose sums wait in shared memory
 
 __device__ __forceinline__ void wt_cp16(uint32_t dst, const void* src) {
@@ -92,10 +92,53 @@ template <int QT> __device__ __forceinline__ uint2 level_pair(int a, int b) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&hi), *reinterpret_cast<const uint32_t*>(&lo));
 }
 
+// E consecutive elements (4 or 8) as float32
+template <int E> __device__ __forceinline__ void load_some(int dtype, const void* p, int64_t at, float (&v)[E]) {
+    if (dtype == DT_F32) {
+#pragma unroll
+        for (int j = 0; j < E / 4; ++j) {
+            const float4 x = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at)[j];
+            v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < E / 4; ++j) {
+            const uint2 x = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at)[j];
+            const uint32_t w[4] = {x.x & 0xFFFFu, x.x >> 16, x.y & 0xFFFFu, x.y >> 16};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[4 * j + k] = dtype == DT_F16 ? f16_bits_to_float(w[k]) : bf16_bits_to_float(w[k]);
+        }
+    }
+}
+// Hadamard transform of a row held E elements to a lane of the warp
+template <int E> __device__ __forceinline__ void fwht_warp(float (&v)[E], float norm) {
+#pragma unroll
+    for (int h = 1; h < E; h *= 2)
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            if (j & h) continue;
+            const float a = v[j], b = v[j + h];
+            v[j] = a + b;
+            v[j + h] = a - b;
+        }
+#pragma unroll
+    for (int bit = 1; bit < 32; bit *= 2) {
+        const float sg = (threadIdx.x & bit) ? -1.0f : 1.0f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = fmaf(v[j], sg, __shfl_xor_sync(0xffffffffu, v[j], bit));
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[j] *= norm;
+}
+// half_decode() in three operations: the bits moved to a float's place are the value times 2^-112, whatever the exponent
+__device__ __forceinline__ float scale_decode(uint32_t h) {
+    return __uint_as_float((h & 0x7FFFu) << 13 | (h & 0x8000u) << 16) * 0x1p112f;
+}
+
 template <int D, int QT, int TILES>
 __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights_kernel(const WeightsRun p, int splits, int row_chunks) {
     using C = WtCfg<D, QT, TILES>;
-    constexpr int NK = C::NK, LPR = D / 16, ROWS = C::ROWS;
+    constexpr int NK = C::NK, ROWS = C::ROWS;
     const Q8Run& r = p.q;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* s_q = smem + WT_WARPS * C::RING;
@@ -178,56 +221,54 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
 #pragma unroll
         for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
 
-        // ── q': Hadamard, row maximum, two f16 terms, in the order of the products' B fragments ──
-        for (int base = warp * (32 / LPR); base < tiles * 8; base += WT_WARPS * (32 / LPR)) {
-            const int row = base + lane / LPR, e0 = (lane % LPR) * 16;
-            const int gr = row0 + row, i = i0 + gr / r.grp, hq = h * r.grp + gr % r.grp;
-            float v[16];
+        // ── q': Hadamard, row maximum, terms in the order of the products' B fragments; a warp takes a row ──
+        for (int row = warp; row < tiles * 8; row += WT_WARPS) {
+            constexpr int E = D / 32;
+            const int e0 = lane * E, gr = row0 + row, i = i0 + gr / r.grp, hq = h * r.grp + gr % r.grp;
+            float v[E];
             const bool live = row < rows;
             if (live) {
-                load_row16(r.q_dtype, r.q, b * r.qs[0] + hq * r.qs[1] + (int64_t)i * r.qs[2] + e0, v);
+                load_some<E>(r.q_dtype, r.q, b * r.qs[0] + hq * r.qs[1] + (int64_t)i * r.qs[2] + e0, v);
             } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+                for (int j = 0; j < E; ++j) v[j] = 0.0f;
             }
-            if (r.rotate_q) fwht16<D>(v, r.norm);
+            const float lse = live ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : INFINITY;
+            if (r.rotate_q) fwht_warp<E>(v, r.norm);
             float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(v[j]));
+            for (int j = 0; j < E; ++j) top = fmaxf(top, fabsf(v[j]));
 #pragma unroll
-            for (int o = 1; o < LPR; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int o = 1; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float inv = top >= 0x1p-100f ? __fdiv_rn(QT == 8 ? 127.0f : 1.0f, top) : 0.0f;
             if constexpr (QT == 8) {
-                // element e: byte e & 3 of word b (0, 1) of k-step s of lane tt, whose elements are one run of 32 in 128
-                const float inv = top >= 0x1p-100f ? __fdiv_rn(127.0f, top) : 0.0f;
-                uint32_t w[12];
+                // element e: byte e & 3 of word b (0, 1) of a k-step of lane tt, whose elements are one run of 32 in 128
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t q1 = 0, q2 = 0, q3 = 0;
+                for (int j = 0; j < E / 4; ++j) {
+                    uint32_t q[3] = {0, 0, 0};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float x = v[4 * j + k] * inv, a = rintf(x), y = (x - a) * 254.0f, c = rintf(y), d = rintf((y - c) * 254.0f);
-                        q1 |= ((uint32_t)(int)a & 0xFFu) << (8 * k);
-                        q2 |= ((uint32_t)(int)c & 0xFFu) << (8 * k);
-                        q3 |= ((uint32_t)(int)d & 0xFFu) << (8 * k);
+                        q[0] |= ((uint32_t)(int)a & 0xFFu) << (8 * k);
+                        q[1] |= ((uint32_t)(int)c & 0xFFu) << (8 * k);
+                        q[2] |= ((uint32_t)(int)d & 0xFFu) << (8 * k);
                     }
-                    w[(j >> 1) * 6 + (j & 1)] = q1;
-                    w[(j >> 1) * 6 + 2 + (j & 1)] = q2;
-                    w[(j >> 1) * 6 + 4 + (j & 1)] = q3;
+                    const int e = e0 + 4 * j, word = (e & 31) >> 2, pr = (e >> 7) * 2 + (word >> 2), tt = (e & 127) >> 5;
+                    uint32_t* to = reinterpret_cast<uint32_t*>(s_q) + ((row >> 3) * (D / 64) + pr) * 384 + ((row & 7) * 4 + tt) * 4;
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        const int w = ((word >> 1) & 1) * 6 + k * 2 + (word & 1);   // of the pair of k-steps
+                        to[(w >> 2) * 128 + (w & 3)] = q[k];
+                    }
                 }
-                const int half = e0 >> 7, tt = (e0 & 127) >> 5, pr = half * 2 + ((e0 & 31) >> 4);
-                uint4* to = reinterpret_cast<uint4*>(s_q) + ((row >> 3) * (D / 64) + pr) * 96 + (row & 7) * 4 + tt;
-                to[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                to[32] = make_uint4(w[4], w[5], w[6], w[7]);
-                to[64] = make_uint4(w[8], w[9], w[10], w[11]);
             } else {
-                const float inv = top >= 0x1p-100f ? __fdiv_rn(1.0f, top) : 0.0f;
                 // Element e of the row goes where the keys' element meets it: half-word `odd` of word w (b0, b1 of one k-step, then
                 // of the next) of lane tt, pair of k-steps j2.  A pair of k-steps is a block of 32 elements, lane tt has 8 of them:
                 // TQ4 the nibbles of bytes 4 tt .. 4 tt + 3 (e and e + 16 in a byte), TQ3 the group of 8 codes tt, TQ2 those of bytes
                 // 2 tt, 2 tt + 1.
                 __half* qh = reinterpret_cast<__half*>(s_q) + (row >> 3) * (NK / 2) * 256 + (row & 7) * 32;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < E; ++j) {
                     const int e = e0 + j;
                     const float x = v[j] * inv;
                     const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
@@ -238,8 +279,7 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
                     to[C::QPART / 2] = lo;
                 }
             }
-            if (lane % LPR == 0) {
-                const float lse = live ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : INFINITY;
+            if (lane == 0) {
                 const bool sees = live && lse != -INFINITY;   // a row that saw nothing adds nothing
                 s_f[row] = make_float2(top * (r.sm_scale * LOG2E * (QT == 8 ? 1.0f / 127.0f : 1.0f)), sees ? lse * LOG2E : INFINITY);
                 s_lim[row] = sees ? last_seen(r, sl, i) : 0x7fffffff;
@@ -342,7 +382,7 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const uint32_t row = kt + (x * 8 + g) * C::ROWB + j2 * BB;
-                        d[x] = half_decode(wt_lds16(row));
+                        d[x] = scale_decode(wt_lds16(row));
                         uint32_t code[4];
                         if constexpr (QT == 4) {
                             const uint32_t w = wt_lds16(row + 2 + 4 * t) | wt_lds16(row + 4 + 4 * t) << 16;
