@@ -74,7 +74,7 @@ static tq_status weights_check(const tq_attention_weights_args* a, const tq_kv_p
     w->decay = a->decay;
     w->fresh = a->fresh;
     w->weights = a->weights;
-    *p = weights_plan(a->batch, a->n_kv_heads, (int)grp, a->head_dim, w->window, r.max_len);
+    *p = weights_plan(a->batch, a->n_kv_heads, (int)grp, a->head_dim, w->window, r.max_len, a->k_type == TQ_TYPE_Q8);
     return TQ_SUCCESS;
 }
 

@@ -26,10 +26,16 @@ struct WeightsRun {
 struct WeightsPlan {
     int rows = 8, chunks = 1;         // query rows of a KV head at a time, and how often
     int splits = 1;                   // CTAs that share a (sequence, KV head)
+    bool tensor = false;              // many rows, on tcgen05:
+    int tiles = 0;                    // row tiles of a (sequence, KV head) in the work memory
+    int pairs_pass = 0;               // (sequence, KV head) pairs that run at a time
     size_t bytes = 0;                 // work memory
 };
-WeightsPlan weights_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len);
+// n: query tokens that count
+WeightsPlan weights_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool q8);
 cudaError_t launch_weights(const WeightsRun& r, const WeightsPlan& p, void* workspace, cudaStream_t st);
+void weights_rows_plan(int64_t pairs, int D, int64_t rows, int64_t len, WeightsPlan* p);
+cudaError_t launch_weights_rows(const WeightsRun& r, const WeightsPlan& p, void* workspace, cudaStream_t st);
 
 struct SelectRun {
     int B = 0, Hkv = 0;

@@ -21,6 +21,7 @@
 #include "tq_attn_q8.cuh"
 #include "tq_evict.h"
 #include "tq_kernels.h"
+#include "tq_warp_rows.cuh"
 
 namespace tq {
 
@@ -92,44 +93,6 @@ template <int QT> __device__ __forceinline__ uint2 level_pair(int a, int b) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&hi), *reinterpret_cast<const uint32_t*>(&lo));
 }
 
-// E consecutive elements (4 or 8) as float32
-template <int E> __device__ __forceinline__ void load_some(int dtype, const void* p, int64_t at, float (&v)[E]) {
-    if (dtype == DT_F32) {
-#pragma unroll
-        for (int j = 0; j < E / 4; ++j) {
-            const float4 x = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at)[j];
-            v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < E / 4; ++j) {
-            const uint2 x = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at)[j];
-            const uint32_t w[4] = {x.x & 0xFFFFu, x.x >> 16, x.y & 0xFFFFu, x.y >> 16};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[4 * j + k] = dtype == DT_F16 ? f16_bits_to_float(w[k]) : bf16_bits_to_float(w[k]);
-        }
-    }
-}
-// Hadamard transform of a row held E elements to a lane of the warp
-template <int E> __device__ __forceinline__ void fwht_warp(float (&v)[E], float norm) {
-#pragma unroll
-    for (int h = 1; h < E; h *= 2)
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-            if (j & h) continue;
-            const float a = v[j], b = v[j + h];
-            v[j] = a + b;
-            v[j + h] = a - b;
-        }
-#pragma unroll
-    for (int bit = 1; bit < 32; bit *= 2) {
-        const float sg = (threadIdx.x & bit) ? -1.0f : 1.0f;
-#pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = fmaf(v[j], sg, __shfl_xor_sync(0xffffffffu, v[j], bit));
-    }
-#pragma unroll
-    for (int j = 0; j < E; ++j) v[j] *= norm;
-}
 // half_decode() in three operations: the bits moved to a float's place are the value times 2^-112, whatever the exponent
 __device__ __forceinline__ float scale_decode(uint32_t h) {
     return __uint_as_float((h & 0x7FFFu) << 13 | (h & 0x8000u) << 16) * 0x1p112f;
@@ -444,9 +407,15 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
     }
 }
 
-WeightsPlan weights_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len) {
+WeightsPlan weights_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool q8) {
     WeightsPlan p;
     const int64_t rows = n * grp, len = max_len > 0 ? max_len : 1, pairs = (int64_t)B * Hkv;
+    p.pairs_pass = (int)pairs;
+    p.tensor = q8 && rows > WT_ROWS;
+    if (p.tensor) {
+        weights_rows_plan(pairs, D, rows, len, &p);
+        return p;
+    }
     p.rows = rows <= 8 ? 8 : WT_ROWS;
     p.chunks = (int)((rows + p.rows - 1) / p.rows);
     if (p.chunks < 1) p.chunks = 1;
@@ -474,7 +443,8 @@ template <int D, int QT, int TILES> static cudaError_t launch_weights_t(const We
     return cudaGetLastError();
 }
 
-cudaError_t launch_weights(const WeightsRun& r, const WeightsPlan& p, void*, cudaStream_t st) {
+cudaError_t launch_weights(const WeightsRun& r, const WeightsPlan& p, void* workspace, cudaStream_t st) {
+    if (p.tensor) return launch_weights_rows(r, p, workspace, st);
     const auto run = [&](auto d) {
         constexpr int D = decltype(d)::value;
         switch (r.k_type) {
