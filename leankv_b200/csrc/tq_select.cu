@@ -6,11 +6,12 @@
 // the digit is the one in which the wanted rank falls.  Then the tokens above it, and as many of its equals as are
 // wanted, are written in the order of their slots, each at the count of those before it.
 //
-// A cluster of CTAs shares a (sequence, KV head): each takes a run of slots and keeps its keys in shared memory, so that
-// weights are read once; counts are added up over the cluster's shared memories.  What bounds it: the weights' bytes take
-// little time (16 x 8 heads of 32768 tokens: 17 MB); the rest is the chain of four passes with a barrier of the cluster after
-// each.  11 bits take the sign, the exponent and two bits of the fraction, so that weights of like size, which most are,
-// do not meet in one counter.
+// A CTA keeps the keys of up to 32768 slots in registers, 32 a thread, so that weights are read once; its counters are in
+// shared memory.  Where sequences are longer, or there are few (sequence, KV head)s, a cluster of CTAs shares one, and counts are
+// added up over their shared memories; a barrier of the cluster costs about as much as a pass over 8192 keys (128 of them of 32768
+// slots: 36 us in clusters of two, 48 and 110 us in clusters of four and eight).  What bounds it: the chain of four passes, counting
+// by atomics and barriers; the weights' bytes take little time (16 x 8 heads of 32768 tokens: 17 MB).  11 bits take the sign, the
+// exponent and two bits of the fraction, so that weights of like size, which most are, do not meet in one counter.
 #include <cooperative_groups.h>
 
 #include "leankv_tq.h"
@@ -21,10 +22,11 @@ namespace cg = cooperative_groups;
 
 namespace tq {
 
-constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2048;
+constexpr int SEL_THREADS = 1024, SEL_WARPS = 32, SEL_BINS = 2048;
 constexpr int SEL_MOST = 8;                          // CTAs of a cluster
-constexpr int SEL_KEYS = 40 * 1024;                  // keys that a CTA can keep
-constexpr int SEL_GROUP = SEL_THREADS;               // slots of a CTA come in multiples of this
+constexpr int SEL_KEYS = 32;                         // keys that a thread can keep
+constexpr int SEL_SHARE = 8192;                      // slots that make a CTA of a cluster worth its barriers
+constexpr int SEL_BATCH = 8;                         // weights of a thread that are under way together
 
 // larger weights have larger keys; NaN counts as -inf, -0 as 0; 0 is below all of them
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -35,18 +37,29 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 struct SelectShared {
-    uint32_t bins[3][SEL_BINS];
-    uint32_t warp_sums[SEL_WARPS];
+    uint32_t bins[3 * SEL_BINS];
+    uint32_t warp_sums[3][SEL_WARPS];
     uint32_t over[SEL_WARPS], same[SEL_WARPS];       // of a warp's slots: above the border, at it
     uint32_t totals[2];                              // of the CTA
-    uint32_t digit, left;
+    uint32_t digit[3], left[3];
 };
 
-// CACHED: keys are kept in shared memory; else (more slots than a cluster holds) weights are read in every pass
-template <bool CACHED>
-__global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelectRun r, int per_cta) {
-    extern __shared__ uint32_t s_keys[];
-    __shared__ SelectShared sh;
+// the sum of the values of the lanes before this one, and of all
+__device__ __forceinline__ uint32_t before_lane(uint32_t x, uint32_t* all) {
+    uint32_t y = x;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const uint32_t z = __shfl_up_sync(0xffffffffu, y, o);
+        if ((threadIdx.x & 31) >= o) y += z;
+    }
+    *all = __shfl_sync(0xffffffffu, y, 31);
+    return y - x;
+}
+
+// KPT: keys of a thread; 0: more slots than a cluster keeps, weights are read in every pass
+template <int KPT>
+__global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectRun r, int per_warp) {
+    __shared__ __align__(16) SelectShared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int64_t pair = blockIdx.x / size;
@@ -75,80 +88,123 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelectRun r, 
     }
     if (want == 0) return;                             // for all CTAs of the cluster
 
-    const int begin = rank * per_cta;                  // this CTA's slots, a warp's run of them
-    const int per_warp = per_cta / SEL_WARPS, w0 = begin + warp * per_warp;
+    // this warp's run of slots, 32 at a time
+    const int64_t w64 = ((int64_t)rank * SEL_WARPS + warp) * per_warp;
+    const int w0 = (int)(w64 < hi ? w64 : hi);
+    const int turns = KPT ? KPT : ((hi - w0 < per_warp ? hi - w0 : per_warp) + 31) >> 5;
     const float* pool = r.weights;
     const int32_t* pages = r.pages + (int64_t)b * r.max_pages;
     const int in_page = (1 << r.page_shift) - 1;
-    auto load = [&](int slot) -> uint32_t {
-        const int32_t pg = pages[slot >> r.page_shift];
-        if (pg < 0 || pg >= r.num_pages) {             // holds nothing: goes before all others
-            if (r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
-            return 0u;
+    auto inside = [&](int i) { return w0 + 32 * i + lane >= lo && w0 + 32 * i + lane < hi; };
+    uint32_t keys[KPT ? KPT : 1];
+    // f(i, key) for the warp's turns i0 .. (those of this lane that are candidates), weights as they come from memory
+    auto read = [&](auto f) {
+#pragma unroll
+        for (int i0 = 0; i0 < (KPT ? KPT : turns); i0 += SEL_BATCH) {
+            int32_t pg[SEL_BATCH];
+            float w[SEL_BATCH];
+#pragma unroll
+            for (int u = 0; u < SEL_BATCH; ++u) {
+                pg[u] = -1;
+                if ((!KPT || i0 + u < KPT) && i0 + u < turns && inside(i0 + u)) pg[u] = pages[(w0 + 32 * (i0 + u) + lane) >> r.page_shift];
+            }
+#pragma unroll
+            for (int u = 0; u < SEL_BATCH; ++u) {
+                w[u] = 0.0f;
+                if (pg[u] >= 0 && pg[u] < r.num_pages)
+                    w[u] = pool[((((int64_t)pg[u] * r.Hkv + h) << r.page_shift)) + ((w0 + 32 * (i0 + u) + lane) & in_page)];
+            }
+#pragma unroll
+            for (int u = 0; u < SEL_BATCH; ++u) {
+                if ((KPT && i0 + u >= KPT) || i0 + u >= turns) continue;
+                uint32_t key = 0;                      // of a page outside the pool: goes before all others
+                if (inside(i0 + u)) {
+                    if (pg[u] >= 0 && pg[u] < r.num_pages) key = weight_key(w[u]);
+                    else if (r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
+                }
+                f(i0 + u, key);
+            }
         }
-        return weight_key(pool[((((int64_t)pg * r.Hkv + h) << r.page_shift)) + (slot & in_page)]);
     };
-    for (int i = threadIdx.x; i < 3 * SEL_BINS; i += SEL_THREADS) sh.bins[0][i] = 0;
+    for (int i = threadIdx.x; i < 3 * SEL_BINS; i += SEL_THREADS) sh.bins[i] = 0;
+    if constexpr (KPT > 0) {
+#pragma unroll
+        for (int i0 = 0; i0 < KPT; i0 += SEL_BATCH) {
+            int32_t pg[SEL_BATCH];
+#pragma unroll
+            for (int u = 0; u < SEL_BATCH; ++u) {
+                pg[u] = -1;
+                if (i0 + u < KPT && inside(i0 + u)) pg[u] = pages[(w0 + 32 * (i0 + u) + lane) >> r.page_shift];
+            }
+#pragma unroll
+            for (int u = 0; u < SEL_BATCH; ++u) {
+                if (i0 + u >= KPT) continue;
+                float w = 0.0f;
+                const bool there = pg[u] >= 0 && pg[u] < r.num_pages;
+                if (there) w = pool[((((int64_t)pg[u] * r.Hkv + h) << r.page_shift)) + ((w0 + 32 * (i0 + u) + lane) & in_page)];
+                else if (inside(i0 + u) && r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
+                keys[i0 + u] = there ? weight_key(w) : 0u;
+            }
+        }
+    }
     __syncthreads();
     uint32_t border = 0, left = want;                  // digits found so far; rank among those that agree with them
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-        uint32_t* bins = sh.bins[pass];
-        for (int i = lane; i < per_warp; i += 32) {
-            const int slot = w0 + i;
-            if (slot >= hi) break;
-            uint32_t key;
-            if (pass == 0 || !CACHED) {
-                if (slot < lo) continue;
-                key = load(slot);
-                if (CACHED) s_keys[slot - begin] = key;
-            } else {
-                if (slot < lo) continue;
-                key = s_keys[slot - begin];
-            }
+        uint32_t* bins = sh.bins + pass * SEL_BINS;
+        auto count = [&](int i, uint32_t key) {
+            if (!inside(i)) return;
             if (pass == 0 || (key >> (shift + bits)) == (border >> (shift + bits))) atomicAdd(bins + ((key >> shift) & ((1u << bits) - 1)), 1u);
-        }
-        cluster.sync();
-        // bins from the top: a thread has four of them
-        const int at = SEL_BINS - 4 - 4 * threadIdx.x;
-        uint4 sum = make_uint4(0, 0, 0, 0);
-        for (int c = 0; c < size; ++c) {
-            const uint4 x = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(bins, c) + at);
-            sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-        }
-        uint32_t before = sum.x + sum.y + sum.z + sum.w;
-        const uint32_t mine = before;
+        };
+        if constexpr (KPT > 0) {
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += x;
+            for (int i = 0; i < KPT; ++i) count(i, keys[i]);
+        } else {
+            read(count);
         }
-        if (lane == 31) sh.warp_sums[warp] = before;
+        // bins from the top: a thread has two of them
+        const int at = SEL_BINS - 2 - 2 * threadIdx.x;
+        uint2 sum;
+        if (size > 1) {
+            cluster.sync();
+            sum = make_uint2(0, 0);
+            for (int c = 0; c < size; ++c) {
+                const uint2 x = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(bins, c) + at);
+                sum.x += x.x; sum.y += x.y;
+            }
+        } else {
+            __syncthreads();
+            sum = *reinterpret_cast<const uint2*>(bins + at);
+        }
+        const uint32_t mine = sum.x + sum.y;
+        uint32_t all, before = before_lane(mine, &all);
+        if (lane == 31) sh.warp_sums[pass][warp] = all;
         __syncthreads();
-        before -= mine;
-        for (int w = 0; w < warp; ++w) before += sh.warp_sums[w];
+        uint32_t rest;
+        const uint32_t others = before_lane(sh.warp_sums[pass][lane], &rest);
+        before += __shfl_sync(0xffffffffu, others, warp);
         if (before < left && before + mine >= left) {
-            uint32_t x[4] = {sum.w, sum.z, sum.y, sum.x};
-            int d = 0;
-            while (d < 3 && before + x[d] < left) before += x[d++];
-            sh.digit = (uint32_t)(at + 3 - d);
-            sh.left = left - before;
+            const bool second = before + sum.y < left;   // the upper bin does not reach
+            sh.digit[pass] = (uint32_t)(at + (second ? 0 : 1));
+            sh.left[pass] = left - before - (second ? sum.y : 0);
         }
         __syncthreads();
-        border |= sh.digit << shift;
-        left = sh.left;
+        border |= sh.digit[pass] << shift;
+        left = sh.left[pass];
     }
 
     // those above the border all stay, and the first `left` of those at it
     uint32_t over = 0, same = 0;
-    for (int i = lane; i < per_warp; i += 32) {
-        const int slot = w0 + i;
-        if (slot >= hi) break;
-        if (slot < lo) continue;
-        const uint32_t key = CACHED ? s_keys[slot - begin] : load(slot);
-        over += key > border;
-        same += key == border;
+    auto tally = [&](int i, uint32_t key) {
+        over += inside(i) && key > border;
+        same += inside(i) && key == border;
+    };
+    if constexpr (KPT > 0) {
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) tally(i, keys[i]);
+    } else {
+        read(tally);
     }
     over = __reduce_add_sync(0xffffffffu, over);
     same = __reduce_add_sync(0xffffffffu, same);
@@ -157,52 +213,46 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelectRun r, 
         sh.same[warp] = same;
     }
     __syncthreads();
-    if (threadIdx.x < 2) {
-        uint32_t t = 0;
-        for (int w = 0; w < SEL_WARPS; ++w) t += threadIdx.x ? sh.same[w] : sh.over[w];
-        sh.totals[threadIdx.x] = t;
+    // before this warp's slots
+    uint32_t all_over, all_same;
+    const uint32_t o32 = before_lane(sh.over[lane], &all_over), s32 = before_lane(sh.same[lane], &all_same);
+    over = __shfl_sync(0xffffffffu, o32, warp);
+    same = __shfl_sync(0xffffffffu, s32, warp);
+    if (size > 1) {
+        if (threadIdx.x == 0) {
+            sh.totals[0] = all_over;
+            sh.totals[1] = all_same;
+        }
+        cluster.sync();
+        for (int c = 0; c < rank; ++c) {
+            const uint32_t* t = cluster.map_shared_rank(sh.totals, c);
+            over += t[0];
+            same += t[1];
+        }
     }
-    cluster.sync();
-    over = same = 0;                                   // before this warp's slots
-    for (int c = 0; c < rank; ++c) {
-        const uint32_t* t = cluster.map_shared_rank(sh.totals, c);
-        over += t[0];
-        same += t[1];
-    }
-    for (int w = 0; w < warp; ++w) {
-        over += sh.over[w];
-        same += sh.same[w];
-    }
-    for (int i = 0; i < per_warp && w0 + i < hi; i += 32) {
-        const int slot = w0 + i + lane;
-        const bool in = slot >= lo && slot < hi;
-        const uint32_t key = in ? (CACHED ? s_keys[slot - begin] : load(slot)) : 0u;
+    const uint32_t below = (1u << lane) - 1;
+    auto place = [&](int i, uint32_t key) {
+        const bool in = inside(i);
         const uint32_t up = __ballot_sync(0xffffffffu, in && key > border), eq = __ballot_sync(0xffffffffu, in && key == border);
-        const uint32_t below = (1u << lane) - 1;
         const uint32_t o = over + __popc(up & below), e = same + __popc(eq & below);
         const bool stays = ((up >> lane) & 1) || (((eq >> lane) & 1) && e < left);
-        if (stays) out[sinks + o + (e < left ? e : left)] = slot;
+        if (stays) out[sinks + o + (e < left ? e : left)] = w0 + 32 * i + lane;
         over += __popc(up);
         same += __popc(eq);
+    };
+    if constexpr (KPT > 0) {
+#pragma unroll
+        for (int i = 0; i < KPT; ++i) place(i, keys[i]);
+    } else {
+        read(place);
     }
-    cluster.sync();                                    // no CTA ends while another one may still read its shared memory
+    if (size > 1) cluster.sync();                      // no CTA ends while another one may still read its shared memory
 }
 
-cudaError_t launch_select(const SelectRun& r, cudaStream_t st) {
-    const int64_t pairs = (int64_t)r.B * r.Hkv;
-    // CTAs of a (sequence, KV head): as many as are resident together (three a SM by their threads and bins), none with
-    // fewer than 2048 slots to look at, since each adds to the counting over the cluster
-    int size = 1;
-    while (size < SEL_MOST && pairs * size * 2 <= 3 * (int64_t)sm_count() && r.max_len > size * 2048) size *= 2;
-    while (size < SEL_MOST && r.max_len > (int64_t)size * SEL_KEYS) size *= 2;
-    const int64_t per64 = ((r.max_len + size - 1) / size + SEL_GROUP - 1) / SEL_GROUP * SEL_GROUP;
-    const int per = (int)per64;
-    const bool cached = per <= SEL_KEYS;
-    if (pairs * size >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
+template <int KPT> static cudaError_t launch_select_k(const SelectRun& r, int size, int per_warp, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(pairs * size));
+    cfg.gridDim = dim3((unsigned)((int64_t)r.B * r.Hkv * size));
     cfg.blockDim = dim3(SEL_THREADS);
-    cfg.dynamicSmemBytes = cached ? (size_t)per * sizeof(uint32_t) : 0;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -210,10 +260,22 @@ cudaError_t launch_select(const SelectRun& r, cudaStream_t st) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (!cached) return cudaLaunchKernelEx(&cfg, select_kernel<false>, r, per);
-    const cudaError_t e = cudaFuncSetAttribute(select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_KEYS * (int)sizeof(uint32_t));
-    if (e != cudaSuccess) return e;
-    return cudaLaunchKernelEx(&cfg, select_kernel<true>, r, per);
+    return cudaLaunchKernelEx(&cfg, select_kernel<KPT>, r, per_warp);
+}
+
+cudaError_t launch_select(const SelectRun& r, cudaStream_t st) {
+    const int64_t pairs = (int64_t)r.B * r.Hkv;
+    // CTAs of a (sequence, KV head): one, but where SMs would be idle as many as look at SEL_SHARE slots each, and as many as it
+    // takes to keep the keys
+    int size = 1;
+    while (size < SEL_MOST && pairs * size * 2 <= sm_count() && r.max_len > (int64_t)size * SEL_SHARE) size *= 2;
+    while (size < SEL_MOST && r.max_len > (int64_t)size * SEL_THREADS * SEL_KEYS) size *= 2;
+    if (pairs * size >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
+    const int64_t per = (r.max_len + size - 1) / size;       // slots of a CTA
+    if (per <= 2 * SEL_THREADS) return launch_select_k<2>(r, size, 2 * 32, st);
+    if (per <= 8 * SEL_THREADS) return launch_select_k<8>(r, size, 8 * 32, st);
+    if (per <= SEL_KEYS * SEL_THREADS) return launch_select_k<SEL_KEYS>(r, size, SEL_KEYS * 32, st);
+    return launch_select_k<0>(r, size, (int)((per + SEL_THREADS - 1) / SEL_THREADS * 32), st);
 }
 
 }  // namespace tq
