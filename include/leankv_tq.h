@@ -507,7 +507,7 @@ tq_status tq_attention_q8_tree_paged_cuda(const tq_attention_q8_args *a, const t
 /* ── eviction from paged caches ──────────────────────────────────────────────
  *
  * Three steps: sums of the attention weights that cached tokens get, kept beside the pages as
- *   weights  float [num_pages][n_kv_heads][page_size]
+ *   weights  float [num_pages][n_kv_heads][page_size], on a 16-byte boundary
  * the selection of the tokens of each (sequence, KV head) that stay, and moving their rows together.  No counterpart in the
  * reference.  Page ids outside the pool are treated as holding nothing (TQ_ERROR_INVALID_VALUE in *status).
  *

@@ -95,11 +95,11 @@ extern "C" tq_status tq_attention_weights_paged_cuda(const tq_attention_weights_
     if (r.B == 0 || r.max_pages == 0) return TQ_SUCCESS;
     if ((r.n > 0 && (!r.q || !w.lse)) || !r.k || !r.kv_len || !w.weights || (w.k_type == TQ_TYPE_Q8 && !r.ks))
         return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
-    uintptr_t m = (uintptr_t)r.q | (uintptr_t)r.k;
+    uintptr_t m = (uintptr_t)r.q | (uintptr_t)r.k | (uintptr_t)w.weights;
     for (int i = 0; i < 3; ++i) m |= (uintptr_t)(r.qs[i] * (int64_t)dtype_bytes(r.q_dtype));
-    if (m & 15) return set_error(TQ_ERROR_MISALIGNED, "keys and the rows of q must start on 16-byte boundaries");
-    if (((uintptr_t)r.ks | (uintptr_t)r.kv_len | (uintptr_t)r.q_len | (uintptr_t)w.lse | (uintptr_t)w.fresh | (uintptr_t)w.weights | (uintptr_t)r.status) & 3)
-        return set_error(TQ_ERROR_MISALIGNED, "scales, lengths, lse, weights or status not 4-byte aligned");
+    if (m & 15) return set_error(TQ_ERROR_MISALIGNED, "keys, weights and the rows of q must start on 16-byte boundaries");
+    if (((uintptr_t)r.ks | (uintptr_t)r.kv_len | (uintptr_t)r.q_len | (uintptr_t)w.lse | (uintptr_t)w.fresh | (uintptr_t)r.status) & 3)
+        return set_error(TQ_ERROR_MISALIGNED, "scales, lengths, lse or status not 4-byte aligned");
     if (p.bytes && (!a->workspace || a->workspace_bytes < p.bytes)) return set_error(TQ_ERROR_INVALID_VALUE, "workspace of %zu bytes needed", p.bytes);
     if (p.bytes && ((uintptr_t)a->workspace & 15)) return set_error(TQ_ERROR_MISALIGNED, "workspace must be 16-byte aligned");
     if (!r.status && (s = cuda_status(q8_default_status(&r.status), "status word"))) return s;
@@ -120,8 +120,9 @@ extern "C" tq_status tq_select_tokens_cuda(const tq_select_args* a, const tq_kv_
     if (a->max_kv_len < 0 || a->max_kv_len > cap) return set_error(TQ_ERROR_INVALID_VALUE, "max_kv_len outside [0, capacity]");
     if (a->batch == 0 || a->width == 0) return TQ_SUCCESS;
     if (!a->weights || !a->kv_len || !a->slots) return set_error(TQ_ERROR_INVALID_VALUE, "null pointer");
-    if (((uintptr_t)a->weights | (uintptr_t)a->kv_len | (uintptr_t)a->keep | (uintptr_t)a->slots | (uintptr_t)a->status) & 3)
-        return set_error(TQ_ERROR_MISALIGNED, "weights, lengths, slots or status not 4-byte aligned");
+    if ((uintptr_t)a->weights & 15) return set_error(TQ_ERROR_MISALIGNED, "weights must be 16-byte aligned");
+    if (((uintptr_t)a->kv_len | (uintptr_t)a->keep | (uintptr_t)a->slots | (uintptr_t)a->status) & 3)
+        return set_error(TQ_ERROR_MISALIGNED, "lengths, slots or status not 4-byte aligned");
     r.B = a->batch; r.Hkv = a->n_kv_heads;
     r.weights = a->weights;
     r.pages = pg->page_table; r.max_pages = pg->max_pages_per_seq; r.num_pages = pg->num_pages;

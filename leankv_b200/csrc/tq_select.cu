@@ -26,9 +26,11 @@ constexpr int SEL_THREADS = 1024, SEL_WARPS = 32, SEL_BINS = 2048;
 constexpr int SEL_MOST = 8;                          // CTAs of a cluster
 constexpr int SEL_KEYS = 32;                         // keys that a thread can keep
 constexpr int SEL_SHARE = 8192;                      // slots that make a CTA of a cluster worth its barriers
-constexpr int SEL_BATCH = 8;                         // weights of a thread that are under way together
+constexpr int SEL_BATCH = 4;                         // fours of weights of a thread that are under way together
 
-// larger weights have larger keys; NaN counts as -inf, -0 as 0; 0 is below all of them
+// larger weights have larger keys; NaN counts as -inf, -0 as 0.  Below all of them are KEY_LOST (of a page outside the pool) and
+// 0 (no candidate: counted with the lowest bin or not at all, and never reached from the top)
+constexpr uint32_t KEY_LOST = 1;
 __device__ __forceinline__ uint32_t weight_key(float w) {
     uint32_t u = __float_as_uint(w);
     if (u == 0x80000000u) u = 0u;
@@ -56,7 +58,7 @@ __device__ __forceinline__ uint32_t before_lane(uint32_t x, uint32_t* all) {
     return y - x;
 }
 
-// KPT: keys of a thread; 0: more slots than a cluster keeps, weights are read in every pass
+// KPT: keys of a thread, a multiple of 4; 0: more slots than a cluster keeps, weights are read in every pass
 template <int KPT>
 __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectRun r, int per_warp) {
     __shared__ __align__(16) SelectShared sh;
@@ -88,64 +90,66 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectRun 
     }
     if (want == 0) return;                             // for all CTAs of the cluster
 
-    // this warp's run of slots, 32 at a time
+    // this warp's run of slots, 128 at a time, four consecutive ones (of one page) a lane
     const int64_t w64 = ((int64_t)rank * SEL_WARPS + warp) * per_warp;
     const int w0 = (int)(w64 < hi ? w64 : hi);
-    const int turns = KPT ? KPT : ((hi - w0 < per_warp ? hi - w0 : per_warp) + 31) >> 5;
-    const float* pool = r.weights;
+    const int turns = KPT ? KPT / 4 : ((hi - w0 < per_warp ? hi - w0 : per_warp) + 127) >> 7;
+    const float* pool = r.weights + ((int64_t)h << r.page_shift);
     const int32_t* pages = r.pages + (int64_t)b * r.max_pages;
     const int in_page = (1 << r.page_shift) - 1;
-    auto inside = [&](int i) { return w0 + 32 * i + lane >= lo && w0 + 32 * i + lane < hi; };
+    const int64_t page_step = (int64_t)r.Hkv << r.page_shift;
     uint32_t keys[KPT ? KPT : 1];
-    // f(i, key) for the warp's turns i0 .. (those of this lane that are candidates), weights as they come from memory
-    auto read = [&](auto f) {
+    // f(turn, four keys) for `n` turns of the warp from i0 on, weights as they come from memory: SEL_BATCH a lane under way together,
+    // pages first
+    auto read = [&](int i0, int n, auto f) {
+        int32_t pg[SEL_BATCH];
+        float4 w[SEL_BATCH];
 #pragma unroll
-        for (int i0 = 0; i0 < (KPT ? KPT : turns); i0 += SEL_BATCH) {
-            int32_t pg[SEL_BATCH];
-            float w[SEL_BATCH];
+        for (int u = 0; u < SEL_BATCH; ++u) {
+            const int slot = w0 + 128 * (i0 + u) + 4 * lane;
+            pg[u] = -2;
+            if (u < n && slot + 3 >= lo && slot < hi) pg[u] = pages[slot >> r.page_shift];
+        }
 #pragma unroll
-            for (int u = 0; u < SEL_BATCH; ++u) {
-                pg[u] = -1;
-                if ((!KPT || i0 + u < KPT) && i0 + u < turns && inside(i0 + u)) pg[u] = pages[(w0 + 32 * (i0 + u) + lane) >> r.page_shift];
+        for (int u = 0; u < SEL_BATCH; ++u)
+            if (pg[u] >= 0 && pg[u] < r.num_pages)
+                w[u] = *reinterpret_cast<const float4*>(pool + pg[u] * page_step + ((w0 + 128 * (i0 + u) + 4 * lane) & in_page));
+#pragma unroll
+        for (int u = 0; u < SEL_BATCH; ++u) {
+            if (u >= n) continue;
+            uint32_t key[4] = {0, 0, 0, 0};
+            if (pg[u] >= 0 && pg[u] < r.num_pages) {
+                key[0] = weight_key(w[u].x); key[1] = weight_key(w[u].y);
+                key[2] = weight_key(w[u].z); key[3] = weight_key(w[u].w);
+            } else if (pg[u] != -2) {
+                key[0] = key[1] = key[2] = key[3] = KEY_LOST;
+                if (r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
             }
+            const int slot = w0 + 128 * (i0 + u) + 4 * lane;
+            if (slot < lo || slot + 3 >= hi) {   // the ends of the candidates
 #pragma unroll
-            for (int u = 0; u < SEL_BATCH; ++u) {
-                w[u] = 0.0f;
-                if (pg[u] >= 0 && pg[u] < r.num_pages)
-                    w[u] = pool[((((int64_t)pg[u] * r.Hkv + h) << r.page_shift)) + ((w0 + 32 * (i0 + u) + lane) & in_page)];
+                for (int v = 0; v < 4; ++v)
+                    if (slot + v < lo || slot + v >= hi) key[v] = 0;
             }
+            f(i0 + u, key);
+        }
+    };
+    auto every = [&](auto f) {
+        if constexpr (KPT > 0) {
 #pragma unroll
-            for (int u = 0; u < SEL_BATCH; ++u) {
-                if ((KPT && i0 + u >= KPT) || i0 + u >= turns) continue;
-                uint32_t key = 0;                      // of a page outside the pool: goes before all others
-                if (inside(i0 + u)) {
-                    if (pg[u] >= 0 && pg[u] < r.num_pages) key = weight_key(w[u]);
-                    else if (r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
-                }
-                f(i0 + u, key);
-            }
+            for (int i = 0; i < KPT / 4; ++i) f(i, keys + 4 * i);
+        } else {
+            for (int i = 0; i < turns; i += SEL_BATCH) read(i, turns - i, f);
         }
     };
     for (int i = threadIdx.x; i < 3 * SEL_BINS; i += SEL_THREADS) sh.bins[i] = 0;
     if constexpr (KPT > 0) {
 #pragma unroll
-        for (int i0 = 0; i0 < KPT; i0 += SEL_BATCH) {
-            int32_t pg[SEL_BATCH];
+        for (int i0 = 0; i0 < KPT / 4; i0 += SEL_BATCH)
+            read(i0, KPT / 4 - i0, [&](int i, const uint32_t* key) {
 #pragma unroll
-            for (int u = 0; u < SEL_BATCH; ++u) {
-                pg[u] = -1;
-                if (i0 + u < KPT && inside(i0 + u)) pg[u] = pages[(w0 + 32 * (i0 + u) + lane) >> r.page_shift];
-            }
-#pragma unroll
-            for (int u = 0; u < SEL_BATCH; ++u) {
-                if (i0 + u >= KPT) continue;
-                float w = 0.0f;
-                const bool there = pg[u] >= 0 && pg[u] < r.num_pages;
-                if (there) w = pool[((((int64_t)pg[u] * r.Hkv + h) << r.page_shift)) + ((w0 + 32 * (i0 + u) + lane) & in_page)];
-                else if (inside(i0 + u) && r.status) atomicMax(r.status, (int)TQ_ERROR_INVALID_VALUE);
-                keys[i0 + u] = there ? weight_key(w) : 0u;
-            }
-        }
+                for (int v = 0; v < 4; ++v) keys[4 * i + v] = key[v];
+            });
     }
     __syncthreads();
     uint32_t border = 0, left = want;                  // digits found so far; rank among those that agree with them
@@ -153,16 +157,12 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectRun 
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
         uint32_t* bins = sh.bins + pass * SEL_BINS;
-        auto count = [&](int i, uint32_t key) {
-            if (!inside(i)) return;
-            if (pass == 0 || (key >> (shift + bits)) == (border >> (shift + bits))) atomicAdd(bins + ((key >> shift) & ((1u << bits) - 1)), 1u);
-        };
-        if constexpr (KPT > 0) {
+        every([&](int, const uint32_t* key) {
 #pragma unroll
-            for (int i = 0; i < KPT; ++i) count(i, keys[i]);
-        } else {
-            read(count);
-        }
+            for (int v = 0; v < 4; ++v)
+                if (pass == 0 ? key[v] != 0 : (key[v] >> (shift + bits)) == (border >> (shift + bits)))
+                    atomicAdd(bins + (pass == 0 ? key[v] >> shift : (key[v] >> shift) & ((1u << bits) - 1)), 1u);
+        });
         // bins from the top: a thread has two of them
         const int at = SEL_BINS - 2 - 2 * threadIdx.x;
         uint2 sum;
@@ -196,16 +196,13 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectRun 
 
     // those above the border all stay, and the first `left` of those at it
     uint32_t over = 0, same = 0;
-    auto tally = [&](int i, uint32_t key) {
-        over += inside(i) && key > border;
-        same += inside(i) && key == border;
-    };
-    if constexpr (KPT > 0) {
+    every([&](int, const uint32_t* key) {
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) tally(i, keys[i]);
-    } else {
-        read(tally);
-    }
+        for (int v = 0; v < 4; ++v) {
+            over += key[v] > border;
+            same += key[v] == border;
+        }
+    });
     over = __reduce_add_sync(0xffffffffu, over);
     same = __reduce_add_sync(0xffffffffu, same);
     if (lane == 0) {
@@ -230,22 +227,25 @@ __global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectRun 
             same += t[1];
         }
     }
-    const uint32_t below = (1u << lane) - 1;
-    auto place = [&](int i, uint32_t key) {
-        const bool in = inside(i);
-        const uint32_t up = __ballot_sync(0xffffffffu, in && key > border), eq = __ballot_sync(0xffffffffu, in && key == border);
-        const uint32_t o = over + __popc(up & below), e = same + __popc(eq & below);
-        const bool stays = ((up >> lane) & 1) || (((eq >> lane) & 1) && e < left);
-        if (stays) out[sinks + o + (e < left ? e : left)] = w0 + 32 * i + lane;
-        over += __popc(up);
-        same += __popc(eq);
-    };
-    if constexpr (KPT > 0) {
+    int32_t* at = out + sinks;
+    every([&](int i, const uint32_t* key) {
+        // tokens above the border and at it, in the lanes before and in this one (16 bits each: at most 128)
+        uint32_t mine = 0;
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) place(i, keys[i]);
-    } else {
-        read(place);
-    }
+        for (int v = 0; v < 4; ++v) mine += (key[v] > border ? 1u : 0u) + (key[v] == border ? 0x10000u : 0u);
+        uint32_t all, o = before_lane(mine, &all), e = same + (o >> 16);
+        o = over + (o & 0xFFFFu);
+        const int slot = w0 + 128 * i + 4 * lane;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const bool up = key[v] > border, eq = key[v] == border;
+            if (up || (eq && e < left)) at[o + (e < left ? e : left)] = slot + v;
+            o += up;
+            e += eq;
+        }
+        over += all & 0xFFFFu;
+        same += all >> 16;
+    });
     if (size > 1) cluster.sync();                      // no CTA ends while another one may still read its shared memory
 }
 
@@ -272,10 +272,10 @@ cudaError_t launch_select(const SelectRun& r, cudaStream_t st) {
     while (size < SEL_MOST && r.max_len > (int64_t)size * SEL_THREADS * SEL_KEYS) size *= 2;
     if (pairs * size >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
     const int64_t per = (r.max_len + size - 1) / size;       // slots of a CTA
-    if (per <= 2 * SEL_THREADS) return launch_select_k<2>(r, size, 2 * 32, st);
+    if (per <= 4 * SEL_THREADS) return launch_select_k<4>(r, size, 4 * 32, st);
     if (per <= 8 * SEL_THREADS) return launch_select_k<8>(r, size, 8 * 32, st);
     if (per <= SEL_KEYS * SEL_THREADS) return launch_select_k<SEL_KEYS>(r, size, SEL_KEYS * 32, st);
-    return launch_select_k<0>(r, size, (int)((per + SEL_THREADS - 1) / SEL_THREADS * 32), st);
+    return launch_select_k<0>(r, size, (int)((per + 4 * SEL_THREADS - 1) / (4 * SEL_THREADS) * 128), st);
 }
 
 }  // namespace tq

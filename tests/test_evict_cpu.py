@@ -39,7 +39,7 @@ def _move(pages=PAGES, **change):
     (INVALID, dict(B=-1)), (INVALID, dict(Hq=3)), (INVALID, dict(H=0)), (INVALID, dict(n=-1)), (INVALID, dict(most=129)), (INVALID, dict(window=-1)),
     (INVALID, dict(sm=float("nan"))), (INVALID, dict(decay=float("inf"))), (INVALID, dict(qt=7)), (UNSUPPORTED, dict(D=64)),
     (UNSUPPORTED, dict(kt=5)), (UNSUPPORTED, dict(n=1 << 31)), (UNSUPPORTED, dict(n=1 << 62)), (UNSUPPORTED, dict(B=1 << 30)),
-    (MISALIGNED, dict(q=68)), (MISALIGNED, dict(q1=127)), (MISALIGNED, dict(k=72)), (MISALIGNED, dict(w=66)), (MISALIGNED, dict(lse=65)),
+    (MISALIGNED, dict(q=68)), (MISALIGNED, dict(q1=127)), (MISALIGNED, dict(k=72)), (MISALIGNED, dict(w=66)), (MISALIGNED, dict(w=72)), (MISALIGNED, dict(lse=65)),
     (INVALID, dict(pages=(0, 8, 8, 16))), (INVALID, dict(pages=(64, 8, 8, 24))), (UNSUPPORTED, dict(pages=(64, 1 << 30, 8, 16)))])
 def test_weights_refusals(want, change):
     assert _weights(**change) == want
@@ -48,7 +48,7 @@ def test_weights_refusals(want, change):
 @pytest.mark.parametrize("want,change", [
     (INVALID, dict(w=0)), (INVALID, dict(kv_len=0)), (INVALID, dict(out=0)), (INVALID, dict(width=-1)), (INVALID, dict(sinks=-1)),
     (INVALID, dict(recent=-1)), (INVALID, dict(most=129)), (INVALID, dict(H=0)), (INVALID, dict(B=-1)), (UNSUPPORTED, dict(width=1 << 31)),
-    (UNSUPPORTED, dict(B=1 << 30)), (MISALIGNED, dict(w=66)), (MISALIGNED, dict(keep=65)), (INVALID, dict(pages=(64, 0, 8, 16)))])
+    (UNSUPPORTED, dict(B=1 << 30)), (MISALIGNED, dict(w=66)), (MISALIGNED, dict(w=72)), (MISALIGNED, dict(keep=65)), (INVALID, dict(pages=(64, 0, 8, 16)))])
 def test_select_refusals(want, change):
     assert _select(**change) == want
 
