@@ -165,6 +165,8 @@ static tq_status move_check(const tq_kv_move_args* a, const tq_kv_pages* pg, Mov
     r->max_to = a->to_table ? a->to_pages_per_seq : pg->max_pages_per_seq;
     r->overflow = a->overflow;
     r->status = a->status;
+    if (pg->num_pages >= (int64_t(1) << 32) / (((int64_t)a->n_kv_heads) << r->page_shift))
+        return set_error(TQ_ERROR_UNSUPPORTED, "pools must have fewer than 2^32 rows");
     const int64_t chunks = move_chunks(r->n, r->first != nullptr), pairs = (int64_t)r->B * r->Hkv;
     if (pairs > 0 && chunks > INT32_MAX / pairs) return set_error(TQ_ERROR_UNSUPPORTED, "more than 2^37 rows");
     *bytes = r->in_place && chunks > 1 ? (size_t)(pairs * chunks + 1) * sizeof(uint32_t) : 0;

@@ -59,12 +59,14 @@ __device__ __forceinline__ bool wait_earlier(const uint32_t* flags, int64_t chun
     return true;
 }
 
-// where a slot's row lies, as a row of the pool (-1: outside the table or the pool)
-__device__ __forceinline__ int64_t row_at(const MoveRun& r, const int32_t* table, int64_t max_pages, int b, int h, int64_t slot) {
-    if (slot < 0 || slot >= (max_pages << r.page_shift)) return -1;
-    const int32_t pg = table[b * max_pages + (slot >> r.page_shift)];
-    if (pg < 0 || pg >= r.num_pages) return -1;
-    return (((int64_t)pg * r.Hkv + h) << r.page_shift) + (slot & ((int64_t(1) << r.page_shift) - 1));
+// where a slot's row lies, as a row of the pool (a row of K and V takes 112 bytes and more, so that 32 bits number all that a GPU
+// holds), or NO_ROW: outside the table or the pool
+constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t row_at(const MoveRun& r, const int32_t* table, uint32_t cap, int h, uint32_t slot) {
+    if (slot >= cap) return NO_ROW;
+    const int32_t pg = table[slot >> r.page_shift];
+    if (pg < 0 || pg >= r.num_pages) return NO_ROW;
+    return (((uint32_t)pg * r.Hkv + h) << r.page_shift) + (slot & ((1u << r.page_shift) - 1));
 }
 
 // CTA-wide turn between reading and writing; `used` depends on all that the thread has read, so that the reads are over.
@@ -86,28 +88,39 @@ __device__ __forceinline__ bool move_turn(uint32_t* flags, int64_t chunk, uint32
 
 // What a lane knows of its row (lane & 15) of the warp's block
 struct MoveRow {
-    int64_t from = -1;   // pool row that is read, -1: none
-    bool moved = false;  // one of src (else an older row of the first block, or none)
+    uint32_t from = NO_ROW;   // pool row that is read
+    bool moved = false;       // one of src (else an older row of the first block, or none)
 };
 
-__device__ __forceinline__ MoveRow move_row(const MoveRun& r, int b, int h, int64_t slot, int64_t to, int64_t first, int64_t count,
-                                            bool q8, bool counts) {
+// src, from: of the (sequence, head), the sequence; slots below 2^31, so that differences of them are signed words
+__device__ __forceinline__ MoveRow move_row(const MoveRun& r, const int32_t* src, const int32_t* from, uint32_t cap, int h, uint32_t slot, uint32_t to,
+                                            uint32_t first, int count, bool q8, bool counts) {
     MoveRow m;
-    const int64_t j = slot - first;
+    const int j = (int)(slot - first);
     if (j >= count) return m;
     if (j < 0) {
         if (q8) m.from = to;
         return m;
     }
-    const int64_t s = r.src[((int64_t)b * r.src_heads + (r.src_heads > 1 ? h : 0)) * r.n + j];
+    const int s = src[j];
     if (s < 0) return m;
-    if (to >= 0 && !(r.in_place && s < slot)) m.from = row_at(r, r.from, r.max_from, b, h, s);
-    m.moved = m.from >= 0;
+    if (to != NO_ROW && !(r.in_place && (uint32_t)s < slot)) m.from = row_at(r, from, cap, h, (uint32_t)s);
+    m.moved = m.from != NO_ROW;
     if (!m.moved && counts && r.overflow) atomicAdd(r.overflow, 1);
     return m;
 }
 
-__device__ __forceinline__ int64_t shfl64(int64_t v, int lane) { return __shfl_sync(0xffffffffu, (long long)v, lane); }
+// the larger and the smaller of two pairs of 16-bit whole numbers
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.s16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.s16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 
 // round(code * q) of four codes, |code * q| < 127.5: codes as floats from the bits of 2^23 + 128 + code, the product rounded as
 // any, then to a whole number by adding 1.5 * 2^23, whose low byte it is (conversions by instruction would go through a unit that
@@ -128,20 +141,20 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t codes, float q) {
 
 // 8-bit rows of a block: D / 16 lanes a row, 16 codes each
 template <int D>
-__device__ __forceinline__ void move_block_q8(const MoveRun& r, const MoveSide& x, MoveRow m, int64_t to0, bool some, uint32_t used,
+__device__ __forceinline__ void move_block_q8(const MoveRun& r, const MoveSide& x, MoveRow m, uint32_t to0, bool some, uint32_t used,
                                               uint32_t* flags, int64_t chunk, int* s_ok) {
     constexpr int LPR = D / 16, RPP = 32 / LPR, PASSES = 16 / RPP;
     const int lane = threadIdx.x & 31, sub = lane / LPR, col = lane % LPR;
-    const bool valid = some && m.from >= 0;
+    const bool valid = some && m.from != NO_ROW;
     const uint32_t rows = __ballot_sync(0xffffffffu, valid) & 0xFFFFu;
     const int8_t* pool = reinterpret_cast<const int8_t*>(x.pool);
     uint4 w[PASSES];
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
         const int row = p * RPP + sub;
-        const int64_t from = shfl64(m.from, row);
+        const uint32_t from = __shfl_sync(0xffffffffu, m.from, row);
         w[p] = make_uint4(0, 0, 0, 0);
-        if ((rows >> row) & 1) w[p] = *reinterpret_cast<const uint4*>(pool + from * D + 16 * col);
+        if ((rows >> row) & 1) w[p] = *reinterpret_cast<const uint4*>(pool + (size_t)from * D + 16 * col);
     }
     const float scale = valid ? x.scale[m.from >> 4] : 0.0f;
     used ^= __float_as_uint(scale);
@@ -161,8 +174,8 @@ __device__ __forceinline__ void move_block_q8(const MoveRun& r, const MoveSide& 
             const uint32_t in[4] = {w[p].x, w[p].y, w[p].z, w[p].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                most = __vimax3_s16x2(most, in[i], in[i] << 8);
-                least = __vimin3_s16x2(least, in[i], in[i] << 8);
+                most = max2(most, max2(in[i], in[i] << 8));
+                least = min2(least, min2(in[i], in[i] << 8));
             }
             const int hi = max((int)(int16_t)most, (int)most >> 16) >> 8, lo = min((int)(int16_t)least, (int)least >> 16) >> 8;
             const float s = __shfl_sync(0xffffffffu, scale, p * RPP + sub);
@@ -174,7 +187,7 @@ __device__ __forceinline__ void move_block_q8(const MoveRun& r, const MoveSide& 
     }
     const float ratio = now > 0.0f ? __fdiv_rn(scale, now) : 0.0f;   // of the lane's row
     if (!move_turn(flags, chunk, used, s_ok) || !some) return;
-    int8_t* to = reinterpret_cast<int8_t*>(x.pool) + to0 * D + 16 * col;
+    int8_t* to = reinterpret_cast<int8_t*>(x.pool) + (size_t)to0 * D + 16 * col;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
         const int row = p * RPP + sub;
@@ -189,7 +202,7 @@ __device__ __forceinline__ void move_block_q8(const MoveRun& r, const MoveSide& 
 
 // TurboQuant rows of a block: 8 U bytes a row, the block's 16 rows flat over the lanes
 template <int U>
-__device__ __forceinline__ void move_block_tq(const MoveSide& x, MoveRow m, int64_t to0, bool some, uint32_t used, uint32_t* flags,
+__device__ __forceinline__ void move_block_tq(const MoveSide& x, MoveRow m, uint32_t to0, bool some, uint32_t used, uint32_t* flags,
                                               int64_t chunk, int* s_ok) {
     constexpr int N = 16 * U, PER = (N + 31) / 32;
     const int lane = threadIdx.x & 31;
@@ -198,13 +211,13 @@ __device__ __forceinline__ void move_block_tq(const MoveSide& x, MoveRow m, int6
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int u = lane + 32 * i, row = u < N ? u / U : 0;
-        const int64_t from = shfl64(m.from, row);
+        const uint32_t from = __shfl_sync(0xffffffffu, m.from, row);
         w[i] = make_uint2(0, 0);
-        if (u < N && ((rows >> row) & 1)) w[i] = reinterpret_cast<const uint2*>(x.pool)[from * U + u % U];
+        if (u < N && ((rows >> row) & 1)) w[i] = reinterpret_cast<const uint2*>(x.pool)[(size_t)from * U + u % U];
         used ^= w[i].x ^ w[i].y;
     }
     if (!move_turn(flags, chunk, used, s_ok) || !some) return;
-    uint2* to = reinterpret_cast<uint2*>(x.pool) + to0 * U;
+    uint2* to = reinterpret_cast<uint2*>(x.pool) + (size_t)to0 * U;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int u = lane + 32 * i;
@@ -214,30 +227,32 @@ __device__ __forceinline__ void move_block_tq(const MoveSide& x, MoveRow m, int6
 
 // D: 8-bit rows of D elements (UK = UV = 0), or TurboQuant rows of 8 UK and 8 UV bytes
 template <int D, int UK, int UV>
-__global__ void __launch_bounds__(32 * MOVE_WARPS) move_kernel(const MoveRun r, int64_t chunks) {
-    __shared__ int64_t s_ticket;
+__global__ void __launch_bounds__(32 * MOVE_WARPS, D == 128 && UK == 0 ? 7 : 4) move_kernel(const MoveRun r, uint32_t chunks) {
+    __shared__ uint32_t s_ticket;
     __shared__ int s_ok;
-    int64_t ticket = blockIdx.x;
+    uint32_t ticket = blockIdx.x;
     if (r.flags) {
         if (threadIdx.x == 0) s_ticket = atomicAdd(r.flags, 1u);
         __syncthreads();
         ticket = s_ticket;
     }
-    const int64_t pairs = (int64_t)r.B * r.Hkv, chunk = ticket / pairs, pair = ticket - chunk * pairs;
-    uint32_t* flags = r.flags ? r.flags + 1 + pair * chunks : nullptr;
-    const int b = (int)(pair / r.Hkv), h = (int)(pair % r.Hkv);
+    const uint32_t pairs = (uint32_t)r.B * r.Hkv, chunk = ticket / pairs, pair = ticket - chunk * pairs;
+    uint32_t* flags = r.flags ? r.flags + 1 + (size_t)pair * chunks : nullptr;
+    const int b = (int)(pair / r.Hkv), h = (int)(pair - (uint32_t)b * r.Hkv);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, side = warp & 1;
-    const int64_t cap = r.max_to << r.page_shift;
-    int64_t first = r.first ? r.first[b] : 0, count = r.count ? r.count[b] : r.n;
-    first = first < 0 ? 0 : (first > cap ? cap : first);
-    count = count < 0 ? 0 : (count > r.n ? r.n : count);
+    const uint32_t cap = (uint32_t)(r.max_to << r.page_shift), from_cap = (uint32_t)(r.max_from << r.page_shift);   // at most 2^30
+    int first32 = r.first ? r.first[b] : 0, count = (int)r.n;
+    if (r.count) count = r.count[b] < 0 ? 0 : (r.count[b] > count ? count : r.count[b]);
+    const uint32_t first = first32 < 0 ? 0 : ((uint32_t)first32 > cap ? cap : (uint32_t)first32);
 
-    const int64_t slot0 = (first & ~int64_t(15)) + chunk * MOVE_SLOTS + (warp >> 1) * 16;
-    const int64_t to0 = row_at(r, r.to, r.max_to, b, h, slot0);
+    const uint32_t slot0 = (first & ~15u) + chunk * MOVE_SLOTS + (warp >> 1) * 16;
+    const int32_t* to_table = r.to + (int64_t)b * r.max_to;
+    const uint32_t to0 = row_at(r, to_table, cap, h, slot0);
     const int row = lane & 15;
-    MoveRow m = move_row(r, b, h, slot0 + row, to0 < 0 ? -1 : to0 + row, first, count, UK == 0, side == 0 && lane < 16);
+    MoveRow m = move_row(r, r.src + ((int64_t)b * r.src_heads + (r.src_heads > 1 ? h : 0)) * r.n, r.from + (int64_t)b * r.max_from, from_cap, h,
+                         slot0 + row, to0 == NO_ROW ? NO_ROW : to0 + row, first, count, UK == 0, side == 0 && lane < 16);
     // blocks of rows that all stay where they are, or of none, are left alone
-    const bool some = to0 >= 0 && __any_sync(0xffffffffu, m.moved && m.from != to0 + row);
+    const bool some = to0 != NO_ROW && __any_sync(0xffffffffu, m.moved && m.from != to0 + row);
     float weight = 0.0f;
     const bool weighs = r.weights && side == 0 && lane < 16 && some && m.moved;
     if (weighs) weight = r.weights[m.from];
@@ -265,7 +280,7 @@ cudaError_t launch_move(const MoveRun& r, cudaStream_t st) {
         if (e != cudaSuccess) return e;
     }
     const auto run = [&](auto kernel) {
-        kernel<<<(unsigned)grid, 32 * MOVE_WARPS, 0, st>>>(r, chunks);
+        kernel<<<(unsigned)grid, 32 * MOVE_WARPS, 0, st>>>(r, (uint32_t)chunks);
         return cudaGetLastError();
     };
     if (r.k.type == 8) return r.D == 256 ? run(move_kernel<256, 0, 0>) : run(move_kernel<128, 0, 0>);
