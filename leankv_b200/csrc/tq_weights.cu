@@ -57,6 +57,12 @@ __device__ __forceinline__ void wt_imma(int (&c)[4], const uint32_t (&a)[4], uin
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the sums begin with this product
+__device__ __forceinline__ void wt_mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void wt_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -73,25 +79,13 @@ template <int D, int QT, int TILES> struct WtCfg {
     static constexpr int RING = STAGES * STAGE;                  // per warp
     // q': 8 bits three terms, [tile][pair of k-steps][3][lane] of 16 bytes; TurboQuant two parts of [tile][pair of k-steps][lane]
     static constexpr int QPART = TILES * NK * 256, QBYTES = QT == 8 ? TILES * (D / 64) * 3 * 512 : 2 * QPART;
-    // pairs of levels as f16 terms: an entry for every lane of a half warp, so that lookups do not meet in a bank
-    static constexpr int PAIRS = QT == 4 ? 256 : QT == 3 ? 64 : QT == 2 ? 16 : 0, TABLE = PAIRS * 128;
+    // pairs of levels as f16 terms: an entry of 256 bytes, 8 for every lane, so that lookups do not meet in a bank and a lookup's
+    // address is the pair's number in one byte and the lane's in the next
+    static constexpr int PAIRS = QT == 4 ? 256 : QT == 3 ? 64 : QT == 2 ? 16 : 0, TABLE = PAIRS * 256;
     static constexpr int SUMS = TILES > 1 ? WT_TOKENS * 4 : 0;   // tokens' sums between chunks of rows
-    static constexpr int SMEM = WT_WARPS * RING + QBYTES + TABLE + SUMS;
+    static constexpr int SMEM = TABLE + WT_WARPS * RING + QBYTES + SUMS;
     static constexpr int CTAS = SMEM <= 74 * 1024 ? 3 : SMEM <= 112 * 1024 ? 2 : 1;
 };
-
-// two levels as the sum of two pairs of f16 terms
-template <int QT> __device__ __forceinline__ uint2 level_pair(int a, int b) {
-    float x = 0.0f, y = 0.0f;
-#pragma unroll
-    for (int i = 0; i < (1 << QT); ++i) {
-        if (i == a) x = tq_level<QT>(i);
-        if (i == b) y = tq_level<QT>(i);
-    }
-    const __half2 hi = __floats2half2_rn(x, y);
-    const __half2 lo = __floats2half2_rn(x - __low2float(hi), y - __high2float(hi));
-    return make_uint2(*reinterpret_cast<const uint32_t*>(&hi), *reinterpret_cast<const uint32_t*>(&lo));
-}
 
 // half_decode() in three operations: the bits moved to a float's place are the value times 2^-112, whatever the exponent
 __device__ __forceinline__ float scale_decode(uint32_t h) {
@@ -104,9 +98,8 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
     constexpr int NK = C::NK, ROWS = C::ROWS;
     const Q8Run& r = p.q;
     extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t* s_q = smem + WT_WARPS * C::RING;
-    uint8_t* s_table = s_q + C::QBYTES;
-    float* s_sum = reinterpret_cast<float*>(s_table + C::TABLE);
+    uint8_t* s_q = smem + C::TABLE + WT_WARPS * C::RING;   // the table comes first
+    float* s_sum = reinterpret_cast<float*>(s_q + C::QBYTES);
     __shared__ __align__(16) float2 s_f[ROWS];      // a row's factor of the scores and its log-sum-exp, in the log2 domain
     __shared__ int s_lim[ROWS];                     // last token that it sees
 
@@ -122,13 +115,26 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
     const int rows_all = (sl.q_len - i0) * r.grp;   // rows i0 .. of the sequence, row = token x head of group
 
     if constexpr (QT != 8) {
-        for (int i = threadIdx.x; i < C::PAIRS * 16; i += WT_THREADS)
-            reinterpret_cast<uint2*>(s_table)[i] = level_pair<QT>((i >> 4) & ((1 << QT) - 1), (i >> 4) >> QT);
+        __shared__ float s_level[1 << (QT & 7)];
+        if (threadIdx.x < (1 << QT)) {
+            float x = 0.0f;
+#pragma unroll
+            for (int i = 0; i < (1 << QT); ++i)
+                if (i == threadIdx.x) x = tq_level<QT>(i);
+            s_level[threadIdx.x] = x;
+        }
+        __syncthreads();
+        for (int i = warp; i < C::PAIRS; i += WT_WARPS) {   // two levels as the sum of two pairs of f16 terms
+            const float x = s_level[i & ((1 << QT) - 1)], y = s_level[i >> QT];
+            const __half2 hi = __floats2half2_rn(x, y);
+            reinterpret_cast<uint2*>(smem)[i * 32 + lane] =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&hi), pack_h2(x - __low2float(hi), y - __high2float(hi)));
+        }
     }
 
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * C::RING;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + C::TABLE + warp * C::RING;
     const uint32_t sq = (uint32_t)__cvta_generic_to_shared(s_q) + lane * 16;
-    const uint32_t table = (uint32_t)__cvta_generic_to_shared(s_table) + (lane & 15) * 8;
+    const uint32_t lane8 = lane * 8;
 
     // with several chunks of rows, as many tokens at a time as have sums in shared memory
     const int step = row_chunks > 1 ? WT_TOKENS : per;
@@ -346,42 +352,46 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
                     for (int x = 0; x < 2; ++x) {
                         const uint32_t row = kt + (x * 8 + g) * C::ROWB + j2 * BB;
                         d[x] = scale_decode(wt_lds16(row));
-                        uint32_t code[4];
+                        uint32_t at[4];   // of the pairs in the table
                         if constexpr (QT == 4) {
                             const uint32_t w = wt_lds16(row + 2 + 4 * t) | wt_lds16(row + 4 + 4 * t) << 16;
 #pragma unroll
-                            for (int i4 = 0; i4 < 4; ++i4) code[i4] = (w >> (8 * i4)) & 255u;
+                            for (int i4 = 0; i4 < 4; ++i4) at[i4] = __byte_perm(w, lane8, 0x5504 | i4 << 4);   // lane8 is below 256
                         } else if constexpr (QT == 3) {
                             // bytes 3 t .. 3 t + 2 of the codes: two half-words, from byte 3 t or the one before
                             const uint32_t from = row + 2 + ((3 * t) & ~1);
                             uint32_t w = wt_lds16(from) | wt_lds16(from + 2) << 16;
-                            w >>= (t & 1) * 8;
+                            w = (t & 1) ? w : w << 8;   // the 24 bits in the upper three bytes
 #pragma unroll
-                            for (int i4 = 0; i4 < 4; ++i4) code[i4] = (w >> (6 * i4)) & 63u;
+                            for (int i4 = 0; i4 < 4; ++i4) at[i4] = ((w >> (6 * i4)) & 0x3F00u) | lane8;
                         } else {
-                            const uint32_t w = wt_lds16(row + 2 + 2 * t);
+                            const uint32_t w = wt_lds16(row + 2 + 2 * t) << 8;
 #pragma unroll
-                            for (int i4 = 0; i4 < 4; ++i4) code[i4] = (w >> (4 * i4)) & 15u;
+                            for (int i4 = 0; i4 < 4; ++i4) at[i4] = ((w >> (4 * i4)) & 0xF00u) | lane8;
                         }
 #pragma unroll
-                        for (int i4 = 0; i4 < 4; ++i4) lv[x][i4] = wt_lds64(table + code[i4] * 128);
+                        for (int i4 = 0; i4 < 4; ++i4) lv[x][i4] = *reinterpret_cast<const uint2*>(smem + at[i4]);
                     }
-                    const uint32_t h0[4] = {lv[0][0].x, lv[1][0].x, lv[0][1].x, lv[1][1].x}, h1[4] = {lv[0][2].x, lv[1][2].x, lv[0][3].x, lv[1][3].x};
-                    const uint32_t l0[4] = {lv[0][0].y, lv[1][0].y, lv[0][1].y, lv[1][1].y}, l1[4] = {lv[0][2].y, lv[1][2].y, lv[0][3].y, lv[1][3].y};
+                    // A product takes 8 tokens: the first terms of their levels in its rows 0 .. 7, the second ones in rows 8 .. 15, as
+                    // the lookups give them (16 tokens a product and a product for each term would be 6 of them instead of 8,
+                    // and 16 moves of registers)
 #pragma unroll
                     for (int nt = 0; nt < TILES; ++nt) {
                         if (nt >= tiles) break;
                         const uint32_t from = sq + (nt * (NK / 2) + j2) * 512;
                         const uint4 q = wt_lds128(from), ql = wt_lds128(from + C::QPART);
-                        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        wt_mma(s, h0, q.x, q.y);
-                        wt_mma(x, h0, ql.x, ql.y);
-                        wt_mma(s, h1, q.z, q.w);
-                        wt_mma(x, h1, ql.z, ql.w);
-                        wt_mma(x, l0, q.x, q.y);
-                        wt_mma(x, l1, q.z, q.w);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[nt][e] = fmaf(s[e] + x[e], d[e >> 1], acc[nt][e]);
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t a0[4] = {lv[x][0].x, lv[x][0].y, lv[x][1].x, lv[x][1].y};
+                            const uint32_t a1[4] = {lv[x][2].x, lv[x][2].y, lv[x][3].x, lv[x][3].y};
+                            float s[4];
+                            wt_mma_first(s, a0, q.x, q.y);
+                            wt_mma(s, a1, q.z, q.w);
+                            wt_mma(s, a0, ql.x, ql.y);
+                            wt_mma(s, a1, ql.z, ql.w);
+                            acc[nt][2 * x] = fmaf(s[0] + s[2], d[x], acc[nt][2 * x]);
+                            acc[nt][2 * x + 1] = fmaf(s[1] + s[3], d[x], acc[nt][2 * x + 1]);
+                        }
                     }
                 }
 #pragma unroll
