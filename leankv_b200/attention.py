@@ -15,7 +15,7 @@ import torch
 
 from . import _lib as L
 from .ops import (_DTYPES, _PAGES, _TYPE_OF_BYTES, DraftTree, _call, _check_lengths, _check_q8_pools, _check_rows, _check_status,
-                  _check_table, _check_weights, _device_of, _need_cuda, _on, _own_rows, _row_strides, _stream)
+                  _check_table, _check_weights, _device_of, _need_cuda, _own_rows, _row_strides, _stream, _work_bytes)
 
 
 class AttnArgs(C.Structure):
@@ -221,7 +221,7 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
         if lse.dtype != torch.float32 or lse.numel() != B * Hq * n or not lse.is_contiguous():
             raise ValueError("lse_out must be a contiguous float32 [B, Hq, n] tensor")
     elif return_lse:
-        lse = torch.empty((B, Hq, n), dtype=torch.float32, device=q.device)
+        lse = torch.empty(B, Hq, n, dtype=torch.float32, device=q.device)
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise ValueError("status must be an int32 tensor")
     masks = None
@@ -242,7 +242,8 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
               0 if status is None else status.data_ptr())
     pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
     lib = L.load()
-    need = _on(device, lib.tq_attention_q8_workspace_size, _ATTN_Q8.pack(*fields, 0, 0), pg)
+    key = ("attention", device, B, Hq, Hkv, D, n, out.dtype, fields[21], page_table.shape[1], pages, page_size)
+    need = _work_bytes(key, device, lib.tq_attention_q8_workspace_size, _ATTN_Q8, fields, pg)
     # from the allocator on every call: streams and captured graphs each get their own
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     args = _ATTN_Q8.pack(*fields, ws.data_ptr() if need else 0, need)
@@ -306,7 +307,8 @@ def attention_weights_paged(q: torch.Tensor, k_pool: torch.Tensor, page_table: t
               int(causal), int(rotate_q), float(decay), p(fresh), weights.data_ptr(), _check_status(status))
     pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
     lib = L.load()
-    need = _on(device, lib.tq_attention_weights_workspace_size, _WEIGHTS.pack(*fields, 0, 0), pg)
+    key = ("weights", device, B, Hq, H, D, n, kt, fields[16], fields[17], page_table.shape[1], pages, page_size)
+    need = _work_bytes(key, device, lib.tq_attention_weights_workspace_size, _WEIGHTS, fields, pg)
     # from the allocator on every call: streams and captured graphs each get their own
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _call(device, lib.tq_attention_weights_paged_cuda, _WEIGHTS.pack(*fields, ws.data_ptr() if need else 0, need), pg)

@@ -608,7 +608,8 @@ size_t q8_workspace_bytes(int D, const Q8Plan& p) { return part_bytes(D, p) + p.
 template <int D, int NT, bool LO, bool TREE>
 static cudaError_t launch_one(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
     using C = Q8Cfg<D, NT, LO>;
-    cudaError_t e = cudaFuncSetAttribute(attn_q8_kernel<D, NT, LO, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = allow_smem(attn_q8_kernel<D, NT, LO, TREE>, C::SMEM, allowed);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)r.B * r.Hkv * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;

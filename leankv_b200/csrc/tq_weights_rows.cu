@@ -407,7 +407,8 @@ void weights_rows_plan(int64_t pairs, int D, int64_t rows, int64_t len, WeightsP
 template <int D>
 static cudaError_t launch_weights_rows_d(const WeightsRun& r, const WeightsPlan& p, uint8_t* ws, cudaStream_t st) {
     using C = WrCfg<D>;
-    cudaError_t e = cudaFuncSetAttribute(weights_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = allow_smem(weights_rows_kernel<D>, C::SMEM, allowed);
     if (e != cudaSuccess) return e;
     RowMeta* meta = reinterpret_cast<RowMeta*>(ws + (size_t)p.pairs_pass * p.tiles * C::QTILE);
     const int64_t pairs = (int64_t)r.q.B * r.q.Hkv;

@@ -263,6 +263,22 @@ def _on(device: int, fn, *args):
         return fn(*args)
 
 
+_work_sizes: dict = {}
+
+
+def _work_bytes(key: tuple, device: int, fn, fmt: struct.Struct, fields: tuple, pg: bytes) -> int:
+    """Bytes of work memory of a call, which depend on its sizes and its device (key) alone."""
+    n = _work_sizes.get(key)
+    if n is None:
+        n = _on(device, fn, fmt.pack(*fields, 0, 0), pg)
+        if n == 0 and L.load().tq_last_error_string():
+            return 0   # arguments that are refused: the call itself says why
+        if len(_work_sizes) >= 4096:
+            _work_sizes.clear()
+        _work_sizes[key] = n
+    return n
+
+
 def _call(device: int, fn, *args) -> None:
     """A library call on the device's current stream."""
     status = _on(device, fn, *args, _raw_stream(device))
@@ -524,13 +540,13 @@ def select_tokens(weights: torch.Tensor, page_table: torch.Tensor, kv_len: torch
     those with the largest weights, ties to the lowest slot, NaN as -inf.  Returns int32 [B, n_kv_heads, width] (in out):
     slots, rising, -1 behind the last.  max_kv_len: an upper bound of kv_len that sizes the work (default: the capacity); tokens
     behind it are left out, with status raised, as for pages outside the pool (attention.last_status() without status)."""
-    tensors = (weights, page_table, kv_len, out, status) + ((keep,) if isinstance(keep, torch.Tensor) else ())
-    device = _device_of(*tensors)
+    by_sequence = isinstance(keep, torch.Tensor)
+    device = _device_of(weights, page_table, kv_len, out, status, keep if by_sequence else None)
     pages, H, page_size = _check_weights(weights)
-    B = page_table.shape[0]
+    B, per = page_table.shape if page_table.dim() == 2 else (0, 0)
     _check_table(page_table, B)
     _check_lengths(kv_len, B, "kv_len")
-    if isinstance(keep, torch.Tensor):
+    if by_sequence:
         _check_lengths(keep, B, "keep")
         if width is None:
             raise ValueError("a tensor of numbers to keep needs width, their bound")
@@ -540,12 +556,12 @@ def select_tokens(weights: torch.Tensor, page_table: torch.Tensor, kv_len: torch
             raise ValueError("keep must not be negative")
         width, each = min(int(keep), int(keep) if width is None else int(width)), 0
     if out is None:
-        out = torch.empty((B, H, width), dtype=torch.int32, device=weights.device)
+        out = torch.empty(B, H, width, dtype=torch.int32, device=weights.device)
     elif out.dtype != torch.int32 or out.shape != (B, H, width) or not out.is_contiguous():
         raise ValueError("out must be a contiguous int32 [B, n_kv_heads, width] tensor")
     a = _SELECT.pack(B, H, weights.data_ptr(), kv_len.data_ptr(), each, width, int(sinks), int(recent), int(max_kv_len or 0),
                      out.data_ptr(), _check_status(status))
-    _call(device, L.load().tq_select_tokens_cuda, a, _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size))
+    _call(device, L.load().tq_select_tokens_cuda, a, _PAGES.pack(page_table.data_ptr(), per, pages, page_size))
     return out
 
 
@@ -597,7 +613,8 @@ def kv_move_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.
               0 if to_table is None else to_table.shape[1], _check_status(overflow, "overflow"), _check_status(status))
     pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
     lib = L.load()
-    need = lib.tq_kv_move_workspace_size(_MOVE.pack(*fields, 0, 0), pg)
+    key = ("move", device, B, H, D, src.shape, kt, first is None, to_table is None, page_table.shape[1], pages, page_size)
+    need = _work_bytes(key, device, lib.tq_kv_move_workspace_size, _MOVE, fields, pg)
     # from the allocator on every call: streams and captured graphs each get their own
     ws = torch.empty(need, dtype=torch.uint8, device=k_pool.device) if need else None
     _call(device, lib.tq_kv_move_paged_cuda, _MOVE.pack(*fields, ws.data_ptr() if need else 0, need), pg)
