@@ -500,7 +500,8 @@ typedef struct {
 } tq_draft_mask;
 /* tq_attention_q8_paged_cuda with the rows of q as nodes of a tree.  a->causal must be set (the tokens before the nodes are seen
  * whole); bits of nodes i >= q_len[b] are ignored.  Rows that see nothing, padding and nodes before the cache's first token among
- * them, give zeros and -inf.  Work memory as for tq_attention_q8_paged_cuda. */
+ * them, give zeros and -inf.  Work memory: tq_attention_q8_tree_workspace_size() bytes, as for tq_attention_q8_paged_cuda. */
+size_t tq_attention_q8_tree_workspace_size(const tq_attention_q8_args *a, const tq_kv_pages *pages);
 tq_status tq_attention_q8_tree_paged_cuda(const tq_attention_q8_args *a, const tq_kv_pages *pages, const tq_draft_mask *tree,
                                           void *stream);
 

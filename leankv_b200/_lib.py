@@ -113,6 +113,7 @@ SIGNATURES = {
     "tq_attention_q8_last_status": (_i32, [_v, _v]),
     # trees of drafted tokens, eviction from paged caches (argument blocks: leankv_b200.ops, leankv_b200.attention)
     "tq_draft_tree_cuda": (_i32, [_v, _i64, _i32, _i32, _v, _v, _v]),
+    "tq_attention_q8_tree_workspace_size": (C.c_size_t, [_v, _v]),
     "tq_attention_q8_tree_paged_cuda": (_i32, [_v, _v, _v, _v]),
     "tq_attention_weights_workspace_size": (C.c_size_t, [_v, _v]),
     "tq_attention_weights_paged_cuda": (_i32, [_v, _v, _v]),

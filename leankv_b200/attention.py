@@ -242,8 +242,9 @@ def attention_q8_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
               0 if status is None else status.data_ptr())
     pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
     lib = L.load()
-    key = ("attention", device, B, Hq, Hkv, D, n, out.dtype, fields[21], page_table.shape[1], pages, page_size)
-    need = _work_bytes(key, device, lib.tq_attention_q8_workspace_size, _ATTN_Q8, fields, pg)
+    key = ("attention" if masks is None else "tree", device, B, Hq, Hkv, D, n, out.dtype, fields[21], page_table.shape[1], pages, page_size)
+    size = lib.tq_attention_q8_workspace_size if masks is None else lib.tq_attention_q8_tree_workspace_size
+    need = _work_bytes(key, device, size, _ATTN_Q8, fields, pg)
     # from the allocator on every call: streams and captured graphs each get their own
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     args = _ATTN_Q8.pack(*fields, ws.data_ptr() if need else 0, need)

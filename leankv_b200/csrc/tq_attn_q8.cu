@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8Run r, int64
 constexpr int DIRECT_ROWS_128 = 49, DIRECT_ROWS_256 = 33, PROMPT_ROWS = 449;
 
 // lo: q' as the sum of two f16 terms
-Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo) {
+Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo, bool tree) {
     Q8Plan p;
     p.lo = lo;
     const int64_t rows = n * grp, len = max_len > 0 ? max_len : 1;
@@ -590,7 +590,15 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool 
     for (int s = 1; s <= 256; ++s) {
         const int64_t per = ((len + s - 1) / s + 127) / 128 * 128;
         if (s > 1 && (int64_t)(s - 1) * per >= len) continue;   // the last split would be empty
-        const int64_t waves = (units * s + slots - 1) / slots, cost = waves * (per + start + (s > 1 ? join : 0));
+        const int64_t each = per + start + (s > 1 ? join : 0), waves = (units * s + slots - 1) / slots;
+        int64_t cost = waves * each;
+        if (tree) {
+            // A verification step's sequences have grown to lengths of all kinds: half of the weight to lengths even between
+            // none and the bound, whose time is the longest CTA's or the mean one's (16 sequences of up to 9000 tokens, 104 rows:
+            // one split 123 us, two 99, four 97, six 111).
+            const double mean = (double)units * (double)(len / 2 + s * (each - per)) / (double)slots;
+            cost += mean > (double)each ? (int64_t)(mean < 0x1p60 ? mean : 0x1p60) : each;
+        }
         if (cost < best) { best = cost; p.splits = s; }
         if (waves > 8) break;   // finer splits only add starts
     }

@@ -49,7 +49,7 @@ struct Q8Plan {
     size_t tile_bytes = 0;
 };
 
-Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo);
+Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool lo, bool tree);
 size_t q8_workspace_bytes(int D, const Q8Plan& p);
 int q8_prompt_rows(int64_t pairs, int64_t rows, int D, bool direct, bool lo);
 void q8_prompt_tiles(int64_t pairs, int D, int64_t max_len, Q8Plan* p);

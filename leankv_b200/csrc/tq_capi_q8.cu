@@ -162,7 +162,7 @@ extern "C" tq_status tq_dequantize_q8_cuda(const int8_t* codes, const float* sca
 
 // ── attention ────────────────────────────────────────────────────────────────
 
-static tq_status q8_check(const tq_attention_q8_args* a, const tq_kv_pages* pg, Q8Run* r, Q8Plan* p) {
+static tq_status q8_check(const tq_attention_q8_args* a, const tq_kv_pages* pg, bool tree, Q8Run* r, Q8Plan* p) {
     if (!a) return set_error(TQ_ERROR_INVALID_VALUE, "null argument block");
     if (a->batch < 0 || a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->n_new < 0)
         return set_error(TQ_ERROR_INVALID_VALUE, "bad batch / head / token counts");
@@ -200,7 +200,7 @@ static tq_status q8_check(const tq_attention_q8_args* a, const tq_kv_pages* pg, 
     r->lse = a->lse; r->status = a->status;
     r->max_len = (int)(a->max_kv_len > 0 ? a->max_kv_len : cap);
     *p = q8_plan(a->batch, a->n_kv_heads, (int)grp, a->head_dim, a->n_new, a->max_kv_len > 0 ? a->max_kv_len : cap,
-                 a->out_dtype != TQ_DTYPE_BF16);   // a bf16 output has 8 bits: one term of 11 does
+                 a->out_dtype != TQ_DTYPE_BF16, tree);   // a bf16 output has 8 bits: one term of 11 does
     return TQ_SUCCESS;
 }
 
@@ -208,14 +208,22 @@ extern "C" size_t tq_attention_q8_workspace_size(const tq_attention_q8_args* a, 
     clear_error();
     Q8Run r;
     Q8Plan p;
-    if (q8_check(a, pages, &r, &p) != TQ_SUCCESS) return 0;
+    if (q8_check(a, pages, false, &r, &p) != TQ_SUCCESS) return 0;
+    return q8_workspace_bytes(r.D, p);
+}
+
+extern "C" size_t tq_attention_q8_tree_workspace_size(const tq_attention_q8_args* a, const tq_kv_pages* pages) {
+    clear_error();
+    Q8Run r;
+    Q8Plan p;
+    if (q8_check(a, pages, true, &r, &p) != TQ_SUCCESS) return 0;
     return q8_workspace_bytes(r.D, p);
 }
 
 static tq_status q8_attention(const tq_attention_q8_args* a, const tq_kv_pages* pages, const tq_draft_mask* tree, void* stream) {
     Q8Run r;
     Q8Plan p;
-    tq_status s = q8_check(a, pages, &r, &p);
+    tq_status s = q8_check(a, pages, tree != nullptr, &r, &p);
     if (s) return s;
     if (r.B == 0 || r.n == 0) return TQ_SUCCESS;
     if (tree) {

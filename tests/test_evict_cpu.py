@@ -86,6 +86,16 @@ def test_tree_refusals():
     assert call(args(causal=0), _MASK.pack(64, 0)) == INVALID and call(args(), _MASK.pack(66, 0)) == MISALIGNED
 
 
+def test_tree_work_memory_at_the_largest_sizes():
+    """Rows and tokens whose products pass 64 bits are planned for all the same."""
+    lib = L.load()
+    args = lambda B, n: _ATTN_Q8.pack(B, 4, 2, 128, n, 64, 1, 1536, 128, 512, 64, 1, 1536, 128, 512, 64, 64, 64, 64, 64, 0, 0, 0.0,   # noqa: E731
+                                      1, 1, 1, 0, 64, 0, 0)
+    pages = ops._PAGES.pack(64, 1 << 26, 8, 16)
+    for B, n in ((1, 1 << 29), (1 << 29, 1), (1 << 20, 1 << 18)):
+        assert lib.tq_attention_q8_tree_workspace_size(args(B, n), pages) > 0
+
+
 def test_truncated_sequences_give_pages_back_and_keep_count():
     pt = PageTable(num_pages=10, page_size=16, max_seqs=2, max_pages_per_seq=8)
     a, b = pt.add_sequence(), pt.add_sequence()
