@@ -190,6 +190,7 @@ class Batch:
     tree: "object" = None      # ops.DraftTree
     parents: "object" = None   # the tree's, numpy [B or 1, n_new] (None: they came from the device)
     starts: "object" = None    # pos on the host
+    dropped: "object" = None   # tokens evicted from each sequence when the step was made
 
 
 class PagedKVCache:
@@ -279,7 +280,7 @@ class PagedKVCache:
         step = Batch(seqs, rows, self._table.index_select(0, idx).contiguous(), pos.contiguous(), kv_len,
                      int(lens.max()) if len(seqs) else 0, None if alike else counts, new_len,
                      None if alike or min(counts) else kv_len * (new_len > 0), parents=parents,
-                     starts=[int(n) for n in self.pages.lens[seqs]])
+                     starts=[int(n) for n in self.pages.lens[seqs]], dropped=[int(n) for n in self.pages.dropped[seqs]])
         dropped = self.pages.dropped[seqs]
         if tree is not None or dropped.any():
             from . import ops
@@ -393,7 +394,9 @@ class PagedKVCache:
                 row = step.parents[i if len(step.parents) > 1 else 0]
                 if any(int(row[x]) != a for a, x in zip(before, path)):
                     raise ValueError(f"sequence {step.seqs[i]}: {path} is not a path of the tree")
+        self._check_evicted(step)
         for s, n in zip(step.seqs, step.starts):
+            self.pages._check(s)
             if n != self.pages.lens[s]:
                 raise ValueError(f"sequence {s} has changed since the step")
         rows = max((len(p) for p in paths), default=0)
@@ -439,6 +442,10 @@ class PagedKVCache:
             self.pages.truncate(s, n)
         self._lens.index_copy_(0, torch.tensor(seqs, dtype=torch.int64, device=self.device), count)
 
+    def _check_evicted(self, step: Batch) -> None:
+        if step.dropped is not None and any(n != self.pages.dropped[s] for s, n in zip(step.seqs, step.dropped)):
+            raise ValueError("tokens have been evicted since the step was made: its slots and pages are no longer those of its sequences")
+
     def _need_weights(self) -> None:
         if self._weights is None:
             raise ValueError("weights are not tracked: PagedKVCache(track_weights=True)")
@@ -447,6 +454,7 @@ class PagedKVCache:
         """The step's rows are part of the sequences from now on."""
         if step.tree is not None:
             raise ValueError("a tree's step is committed by accept()")
+        self._check_evicted(step)
         import torch
         self.pages.commit(step.seqs, step.n_new if step.counts is None else step.counts)
         idx = torch.tensor(step.seqs, dtype=torch.int64, device=self.device)

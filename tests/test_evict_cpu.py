@@ -136,3 +136,67 @@ def test_argument_blocks_have_the_header_s_sizes():
         _fields_ = [("i", C.c_int * 2), ("p", C.c_void_p * 3), ("n", C.c_int64 * 4), ("o", C.c_void_p * 2)]
 
     assert (_WEIGHTS.size, ops._MOVE.size, ops._SELECT.size, _MASK.size) == (C.sizeof(W), C.sizeof(M), C.sizeof(S), 16)
+
+
+class _Library:
+    """Plans by the current device; a launch refuses work memory of another device's plan, as the library does."""
+
+    def __init__(self, current):
+        self.current, self.seen = current, []
+
+    def _size(self, *_):
+        self.seen.append(("size", self.current[0]))
+        return {0: 1 << 10, 1: 1 << 12}[self.current[0]]
+
+    def _launch(self, fmt):
+        def call(args, *rest):
+            self.seen.append(("launch", self.current[0], rest[-1]))
+            return 0 if fmt is None or fmt.unpack(args)[-1] >= {0: 1 << 10, 1: 1 << 12}[self.current[0]] else 1
+        return call
+
+    tq_attention_weights_workspace_size = tq_kv_move_workspace_size = tq_attention_q8_tree_workspace_size = _size
+    tq_attention_weights_paged_cuda = property(lambda self: self._launch(_WEIGHTS))
+    tq_kv_move_paged_cuda = property(lambda self: self._launch(ops._MOVE))
+    tq_attention_q8_tree_paged_cuda = property(lambda self: self._launch(_ATTN_Q8))
+    tq_select_tokens_cuda = property(lambda self: self._launch(None))
+
+    @staticmethod
+    def tq_last_error_string():
+        return b"workspace too small"
+
+
+def test_calls_of_tensors_on_another_device(monkeypatch):
+    """Work memory is sized, and work launched, on the tensors' device and its stream."""
+    import contextlib
+
+    import torch
+
+    from leankv_b200 import attention
+    current = [0]
+    lib = _Library(current)
+
+    @contextlib.contextmanager
+    def guard(device):
+        before, current[0] = current[0], device
+        yield
+        current[0] = before
+
+    for module in (attention, ops):
+        monkeypatch.setattr(module, "_device_of", lambda *ts: 1)
+    monkeypatch.setattr(L, "load", lambda: lib)
+    monkeypatch.setattr(ops, "_current_device", lambda: current[0])
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 100 + device)
+    monkeypatch.setattr(ops, "_work_sizes", {})
+    monkeypatch.setattr(torch.cuda, "device", guard)
+    pool, scale, w = torch.zeros(4, 1, 16, 128, dtype=torch.int8), torch.zeros(4, 1, 1), torch.zeros(4, 1, 16)
+    table, lens = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    q, src = torch.zeros(1, 2, 3, 128), torch.zeros(1, 1, 40, dtype=torch.int32)
+    both = [("size", 1), ("launch", 1, 101)]
+    attention.attention_weights_paged(q, pool, table, lens, torch.zeros(1, 2, 3), w, k_scale=scale)
+    assert lib.seen == both
+    lib.seen.clear()
+    ops.kv_move_paged(pool, pool, table, src, k_scale=scale, v_scale=scale)
+    assert lib.seen == both
+    lib.seen.clear()
+    ops.select_tokens(w, table, lens, 4)
+    assert lib.seen == both[1:] and current == [0]

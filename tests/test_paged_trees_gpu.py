@@ -259,6 +259,19 @@ def test_refusals():
                  lambda: plain.batch([s], 2, tree=[[-1, 0], [-1, 0]])):
         with pytest.raises(ValueError):
             call()
+    # a step made before an eviction, and one of a sequence that has gone
+    kept = PagedKVCache(1, H, D, num_pages=8, page_size=16, max_seqs=2, k_bits=8, track_weights=True)
+    s = kept.add_sequence()
+    kept.commit(kept.batch([s], 20))
+    old, tree = kept.batch([s], 1), kept.batch([s], 2, tree=[-1, 0])
+    kept.evict([s], 10)
+    for call in (lambda: kept.commit(old), lambda: kept.accept(tree, [[0]])):
+        with pytest.raises(ValueError):
+            call()
+    tree = kept.batch([s], 2, tree=[-1, 0])
+    kept.free_sequence(s)
+    with pytest.raises(ValueError):
+        kept.accept(tree, [[0]])
     tq = PagedKVCache(1, H, D, num_pages=8, page_size=16, max_seqs=2, k_bits=3)
     with pytest.raises(ValueError):
         tq.batch([tq.add_sequence()], 2, tree=[-1, 0])
