@@ -88,16 +88,16 @@ def dequantize(blocks: torch.Tensor, qtype=4, dtype: torch.dtype = torch.float32
     q = _qtype(qtype)
     if blocks.dtype != torch.uint8 or not blocks.is_contiguous():
         raise ValueError("blocks must be a contiguous uint8 tensor")
-    bb = BLOCK_BYTES[q]
-    if blocks.numel() % bb:
+    bb, held = BLOCK_BYTES[q], blocks.shape
+    nb, rest = divmod(blocks.numel(), bb)
+    if rest:
         raise ValueError("block buffer size is not a multiple of the block size")
-    nb = blocks.numel() // bb
-    if blocks.dim() >= 2 and blocks.shape[-1] == bb:
-        shape = (*blocks.shape[:-2], blocks.shape[-2] * QK)
+    if len(held) >= 2 and held[-1] == bb:
+        shape = (*held[:-2], held[-2] * QK)
     else:
         shape = (nb * QK,)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=blocks.device)
+        out = torch.empty(*shape, dtype=dtype, device=blocks.device)
     else:
         _need_cuda(out)
         if out.numel() != nb * QK or not out.is_contiguous() or out.dtype not in _DTYPES:
@@ -467,19 +467,23 @@ def dequantize_q8(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype =
     """Values of 8-bit pages: int8 [..., tokens, head_dim] (tokens a multiple of 16, head_dim 128 or 256)
     times float32 [..., tokens / 16], rounded to dtype."""
     device = _device_of(codes, scale, out)
-    if codes.dtype != torch.int8 or not codes.is_contiguous() or codes.dim() < 2 or codes.shape[-2] % Q8_BLOCK:
+    shape = codes.shape
+    if codes.dtype != torch.int8 or not codes.is_contiguous() or len(shape) < 2 or shape[-2] % Q8_BLOCK:
         raise ValueError("codes must be a contiguous int8 [..., tokens, head_dim] tensor, tokens a multiple of 16")
-    if scale.dtype != torch.float32 or not scale.is_contiguous() \
-            or scale.shape != (*codes.shape[:-2], codes.shape[-2] // Q8_BLOCK):
+    blocks = scale.shape
+    if scale.dtype != torch.float32 or not scale.is_contiguous() or len(blocks) != len(shape) - 1 \
+            or blocks[:-1] != shape[:-2] or blocks[-1] * Q8_BLOCK != shape[-2]:
         raise ValueError("scale must be a contiguous float32 [..., tokens / 16] tensor")
     if out is None:
-        out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-    elif out.shape != codes.shape or not out.is_contiguous():
+        if dtype not in _DTYPES:
+            raise TypeError(f"unsupported dtype {dtype}")
+        out = torch.empty_like(codes, dtype=dtype)   # contiguous as the codes are
+    elif out.shape != shape or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of the codes' shape")
-    if out.dtype not in _DTYPES:
+    kind = _DTYPES.get(out.dtype)
+    if kind is None:
         raise TypeError(f"unsupported dtype {out.dtype}")
-    _call(device, L.load().tq_dequantize_q8_cuda, codes.data_ptr(), scale.data_ptr(), out.data_ptr(), _DTYPES[out.dtype],
-          scale.numel(), codes.shape[-1])
+    _call(device, L.load().tq_dequantize_q8_cuda, codes.data_ptr(), scale.data_ptr(), out.data_ptr(), kind, scale.numel(), shape[-1])
     return out
 
 
@@ -607,13 +611,14 @@ def kv_move_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.
         raise ValueError(f"weights must be [{pages}, {H}, {page_size}], as the pools")
     if to_table is not None:
         _check_table(to_table, B)
-    p = lambda t: 0 if t is None else t.data_ptr()   # noqa: E731
-    fields = (B, H, D, src.shape[-1], src.data_ptr(), src.shape[1] if src.dim() == 3 else 1, p(first), p(count),
-              k_pool.data_ptr(), kt, ks, v_pool.data_ptr(), vt, vs, p(weights), p(to_table),
+    rows, per = src.shape[-1], page_table.shape[1]
+    fields = (B, H, D, rows, src.data_ptr(), src.shape[1] if src.dim() == 3 else 1, 0 if first is None else first.data_ptr(),
+              0 if count is None else count.data_ptr(), k_pool.data_ptr(), kt, ks, v_pool.data_ptr(), vt, vs,
+              0 if weights is None else weights.data_ptr(), 0 if to_table is None else to_table.data_ptr(),
               0 if to_table is None else to_table.shape[1], _check_status(overflow, "overflow"), _check_status(status))
-    pg = _PAGES.pack(page_table.data_ptr(), page_table.shape[1], pages, page_size)
+    pg = _PAGES.pack(page_table.data_ptr(), per, pages, page_size)
     lib = L.load()
-    key = ("move", device, B, H, D, src.shape, kt, first is None, to_table is None, page_table.shape[1], pages, page_size)
+    key = ("move", device, B, H, D, rows, kt, first is None, to_table is None, per, pages, page_size)
     need = _work_bytes(key, device, lib.tq_kv_move_workspace_size, _MOVE, fields, pg)
     # from the allocator on every call: streams and captured graphs each get their own
     ws = torch.empty(need, dtype=torch.uint8, device=k_pool.device) if need else None
