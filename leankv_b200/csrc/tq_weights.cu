@@ -195,14 +195,15 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
             constexpr int E = D / 32;
             const int e0 = lane * E, gr = row0 + row, i = i0 + gr / r.grp, hq = h * r.grp + gr % r.grp;
             float v[E];
-            const bool live = row < rows;
-            if (live) {
+            // a row that saw nothing adds nothing, whatever q holds there
+            const float lse = row < rows ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : -INFINITY;
+            const bool sees = lse != -INFINITY;
+            if (sees) {
                 load_some<E>(r.q_dtype, r.q, b * r.qs[0] + hq * r.qs[1] + (int64_t)i * r.qs[2] + e0, v);
             } else {
 #pragma unroll
                 for (int j = 0; j < E; ++j) v[j] = 0.0f;
             }
-            const float lse = live ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : INFINITY;
             if (r.rotate_q) fwht_warp<E>(v, r.norm);
             float top = 0.0f;
 #pragma unroll
@@ -249,7 +250,6 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
                 }
             }
             if (lane == 0) {
-                const bool sees = live && lse != -INFINITY;   // a row that saw nothing adds nothing
                 s_f[row] = make_float2(top * (r.sm_scale * LOG2E * (QT == 8 ? 1.0f / 127.0f : 1.0f)), sees ? lse * LOG2E : INFINITY);
                 s_lim[row] = sees ? last_seen(r, sl, i) : 0x7fffffff;
             }

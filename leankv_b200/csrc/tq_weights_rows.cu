@@ -6,13 +6,13 @@
 // leave the kernel as one float.
 //
 // Products are of 8-bit whole numbers with 32-bit sums (kind::i8): codes enter as they lie in the pages.  A row of q' is the sum
-// of three terms of 8 bits, q1 + q2 / 128 + q3 / 128^2, in units of 1/127 of the largest element of its 64 rows; the terms are
-// rows of the same product, N = 3 x 64.  Two f16 terms take as many operations, but the codes have to be converted on their way
+// of three terms of 8 bits, q1 + q2 / 128 + q3 / 128^2, in units of 1/127 of its largest element; the terms are rows of the same
+// product, N = 3 x 64.  Two f16 terms take as many operations, but the codes have to be converted on their way
 // (38 us for a window of 64 tokens of 32 heads over 2 x 16100 tokens, bound by shared memory's bandwidth: conversion, products and
 // the rows' factors) and their fp32 sums were off by 4e-6 of the result; sums of whole numbers are exact.
 //
-// weights_rows_prepare_kernel: q' (Hadamard, common scale, terms) into images of the shared-memory tiles, once per call (a row is
-// read by every CTA of its KV head); with each row's log-sum-exp and last token.
+// weights_rows_prepare_kernel: q' (Hadamard, the row's scale, terms) into images of the shared-memory tiles, once per call (a row is
+// read by every CTA of its KV head); with each row's scale, log-sum-exp and last token.
 //
 // weights_rows_kernel: a CTA takes a run of tokens of one (sequence, KV head) and QN rows at a time, whose images stay in shared
 // memory while the run's keys come by, 128 tokens at a time.  Warps:
@@ -53,6 +53,7 @@ constexpr uint32_t WR_ZERO = 0x4B400000u;
 
 struct RowMeta {
     float nl;      // negative log-sum-exp, in the log2 domain
+    float f;       // of its scores, into that domain
     int lim;       // last token that the row sees, -1: none
 };
 
@@ -80,41 +81,40 @@ __device__ __forceinline__ void wr_wait(uint32_t (&x)[3][8]) {
         asm volatile("" : "+r"(x[k][0]), "+r"(x[k][1]), "+r"(x[k][2]), "+r"(x[k][3]), "+r"(x[k][4]), "+r"(x[k][5]), "+r"(x[k][6]), "+r"(x[k][7]));
 }
 
-// One CTA: 64 rows of a (sequence, KV head), 8 a warp, all in registers until their largest element is known.
+// One CTA: 64 rows of a (sequence, KV head), 8 a warp.
 template <int D>
 __global__ void __launch_bounds__(256) weights_rows_prepare_kernel(const WeightsRun p, int64_t pair0, int subs, uint8_t* __restrict__ images,
-                                                                   RowMeta* __restrict__ meta, float* __restrict__ factors) {
+                                                                   RowMeta* __restrict__ meta) {
     using C = WrCfg<D>;
     constexpr int E = D / 32, ROWS = WR_SUB / 8;
     const Q8Run& r = p.q;
-    __shared__ float s_top[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t slot = blockIdx.x / subs, pair = pair0 + slot;
     const int sub = blockIdx.x % subs, h = (int)(pair % r.Hkv), b = (int)(pair / r.Hkv);
     const SeqLens sl = seq_lens(r, b);
     const int i0 = sl.q_len > p.window ? sl.q_len - (int)p.window : 0;
-    float v[ROWS][E], top = 0.0f;
+    // Row k's log-sum-exp.  A row that saw nothing adds nothing, whatever q holds there.
+    const auto lse_of = [&](int i, int hq) { return i < sl.q_len ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : -INFINITY; };
+    float v[ROWS][E], inv[ROWS];
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
         const int at = sub * WR_SUB + warp * ROWS + k, i = i0 + at / r.grp, hq = h * r.grp + at % r.grp;
 #pragma unroll
         for (int j = 0; j < E; ++j) v[k][j] = 0.0f;
-        if (i < sl.q_len) load_some<E>(r.q_dtype, r.q, b * r.qs[0] + hq * r.qs[1] + (int64_t)i * r.qs[2] + lane * E, v[k]);
+        if (lse_of(i, hq) != -INFINITY) load_some<E>(r.q_dtype, r.q, b * r.qs[0] + hq * r.qs[1] + (int64_t)i * r.qs[2] + lane * E, v[k]);
     }
+    float mine = 0.0f;   // lane k < ROWS: the largest element of row k
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
         if (r.rotate_q) fwht_warp<E>(v[k], r.norm);
+        float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < E; ++j) top = fmaxf(top, fabsf(v[k][j]));
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));   // floats from 0 on are in the order of their bits
+        if (lane == k) mine = top;
+        inv[k] = top >= 0x1p-100f ? __fdiv_rn(127.0f, top) : 0.0f;
     }
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) s_top[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_top[w]);
-    const float inv = top >= 0x1p-100f ? __fdiv_rn(127.0f, top) : 0.0f;
     uint8_t* image = images + (slot * subs + sub) * C::QSUB;
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256) weights_rows_prepare_kernel(const Weights
             q[0][j] = q[1][j] = q[2][j] = 0;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const float y = v[k][4 * j + x] * inv, a = rintf(y), z = (y - a) * 128.0f, d = rintf(z), f = rintf((z - d) * 128.0f);
+                const float y = v[k][4 * j + x] * inv[k], a = rintf(y), z = (y - a) * 128.0f, d = rintf(z), f = rintf((z - d) * 128.0f);
                 q[0][j] |= ((uint32_t)(int)a & 0xFFu) << (8 * x);
                 q[1][j] |= ((uint32_t)(int)d & 0xFFu) << (8 * x);
                 q[2][j] |= ((uint32_t)(int)f & 0xFFu) << (8 * x);
@@ -139,28 +139,27 @@ __global__ void __launch_bounds__(256) weights_rows_prepare_kernel(const Weights
             for (int j = 0; j < E / 4; ++j) reinterpret_cast<uint32_t*>(to)[j] = q[term][j];
         }
     }
-    if (threadIdx.x < WR_SUB) {
-        const int at = sub * WR_SUB + threadIdx.x, i = i0 + at / r.grp, hq = h * r.grp + at % r.grp;
-        const float lse = i < sl.q_len ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : -INFINITY;
-        const bool sees = lse != -INFINITY;   // a row that saw nothing adds nothing
+    if (lane < ROWS) {
+        const int at = sub * WR_SUB + warp * ROWS + lane, i = i0 + at / r.grp, hq = h * r.grp + at % r.grp;
+        const float lse = lse_of(i, hq);
+        const bool sees = lse != -INFINITY;
         RowMeta m;
         m.nl = sees ? -lse * LOG2E : -INFINITY;
+        m.f = mine * (r.sm_scale * LOG2E * (1.0f / 127.0f));
         m.lim = sees ? last_seen(r, sl, i) : -1;
-        meta[(slot * subs + sub) * WR_SUB + threadIdx.x] = m;
+        meta[(slot * subs + sub) * WR_SUB + warp * ROWS + lane] = m;
     }
-    if (threadIdx.x == 0) factors[slot * subs + sub] = top * (r.sm_scale * LOG2E * (1.0f / 127.0f));
 }
 
 template <int D>
 __global__ void __launch_bounds__(WrCfg<D>::THREADS, 1)
-weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, const uint8_t* __restrict__ images, const RowMeta* __restrict__ meta,
-                    const float* __restrict__ factors) {
+weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, const uint8_t* __restrict__ images, const RowMeta* __restrict__ meta) {
     using C = WrCfg<D>;
     constexpr int QN = C::QN, NS = C::NS, STAGES = C::STAGES;
     const Q8Run& r = p.q;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[16];
-    __shared__ __align__(16) float s_nl[QN];
+    __shared__ __align__(16) float s_row[2 * QN];   // of two rows: their nl, their f
     __shared__ int s_lim[QN], s_most, s_least;   // last tokens of the rows; the largest and the least of them
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
@@ -237,7 +236,8 @@ weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, con
         __syncthreads();
         if (threadIdx.x < ns * WR_SUB) {
             const RowMeta m = meta[sub0 * WR_SUB + threadIdx.x];
-            s_nl[threadIdx.x] = m.nl;
+            s_row[(threadIdx.x >> 1) * 4 + (threadIdx.x & 1)] = m.nl;
+            s_row[(threadIdx.x >> 1) * 4 + 2 + (threadIdx.x & 1)] = m.f;
             s_lim[threadIdx.x] = m.lim;
             const int most = __reduce_max_sync(0xffffffffu, m.lim), least = __reduce_min_sync(0xffffffffu, m.lim < 0 ? 0x7fffffff : m.lim);
             if (lane == 0) {
@@ -253,12 +253,6 @@ weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, con
             // ── weights and sums: thread = token and 32 of the rows of every other product ──
             const int odd = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane, part = odd * 2 + half;
             const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + odd * 256 + half * 32;
-            float factor[(NS + 1) / 2];
-#pragma unroll
-            for (int i = 0; i < (NS + 1) / 2; ++i) {   // this warp's products of a tile: the j with (prod + j) odd or even
-                const int j = 2 * i + ((prod + odd) & 1);
-                factor[i] = j < ns ? factors[sub0 + j] : 0.0f;
-            }
             // the token's scale a tile ahead, and its page two (what is loaded is not looked at before its turn: the warp would wait)
             int next_page = -1;
             float next_ks = 0.0f;
@@ -278,7 +272,7 @@ weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, con
             bool ok = true;
             for (int t = 0; t < all; ++t) {
                 const int tok0 = begin + t * 128, tok = tok0 + row;
-                const float ks = next_ks;
+                const float2 ks = make_float2(next_ks, next_ks);
                 fetch(t + 1);
                 locate(t + 2);
                 float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
@@ -292,8 +286,6 @@ weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, con
                         ok = ok && __all_sync(0xffffffffu, mbar_wait(s_full + 8 * odd, (n >> 1) & 1, &s_failed));
                         if (!ok) continue;
                         tc_fence_after();
-                        const float f = (ns & 1) ? factors[sub0 + j] : factor[i];   // an odd number of products: the turns change
-                        const float2 a = make_float2(f * ks, f * ks);
                         uint32_t raw[2][3][8];   // 8 rows' terms are loaded while those before are used
                         wr_load(from, raw[0]);
 #pragma unroll
@@ -305,7 +297,7 @@ weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, con
                             float e[8];
 #pragma unroll
                             for (int k = 0; k < 8; k += 4) {
-                                const float4 l = *reinterpret_cast<const float4*>(s_nl + r0 + k);
+                                const float4 l = *reinterpret_cast<const float4*>(s_row + 2 * (r0 + k)), m = *reinterpret_cast<const float4*>(s_row + 2 * (r0 + k) + 4);
                                 // c1 + (c2 + c3 / 128) / 128 to half of 1/128 of c1's unit, floats from the bits of 1.5 * 2^23 + c
                                 const float2 off = make_float2(-12681216.0f, -12681216.0f), m1 = make_float2(0x1p-7f, 0x1p-7f);
                                 const auto sum = [&](int u) {
@@ -314,8 +306,8 @@ weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, con
                                                                   __uint_as_float(x[1][k + u + 1] + (uint32_t)((int)x[2][k + u + 1] >> 7) + WR_ZERO));
                                     return __ffma2_rn(lo, m1, __fadd2_rn(hi, off));
                                 };
-                                const float2 y = __ffma2_rn(sum(0), a, make_float2(l.x, l.y));
-                                const float2 z = __ffma2_rn(sum(2), a, make_float2(l.z, l.w));
+                                const float2 y = __ffma2_rn(sum(0), __fmul2_rn(make_float2(l.z, l.w), ks), make_float2(l.x, l.y));
+                                const float2 z = __ffma2_rn(sum(2), __fmul2_rn(make_float2(m.z, m.w), ks), make_float2(m.x, m.y));
                                 e[k] = ex2(y.x);
                                 e[k + 1] = ex2(y.y);
                                 e[k + 2] = ex2(z.x);
@@ -453,8 +445,8 @@ weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, con
     }
 }
 
-// bytes of the work memory for a product's rows: image, meta, factor
-template <int D> constexpr size_t wr_sub_bytes() { return WrCfg<D>::QSUB + WR_SUB * sizeof(RowMeta) + sizeof(float); }
+// bytes of the work memory for a product's rows: image, meta
+template <int D> constexpr size_t wr_sub_bytes() { return WrCfg<D>::QSUB + WR_SUB * sizeof(RowMeta); }
 
 // A CTA's time is its tokens for each chunk of rows plus a start for each; one CTA an SM.  Its tokens at most fill the sums'
 // place once where there are several chunks (beyond, it would read the rows again).
@@ -487,13 +479,12 @@ static cudaError_t launch_weights_rows_d(const WeightsRun& r, const WeightsPlan&
     if (e != cudaSuccess) return e;
     const size_t all = (size_t)p.pairs_pass * p.tiles;
     RowMeta* meta = reinterpret_cast<RowMeta*>(ws + all * C::QSUB);
-    float* factors = reinterpret_cast<float*>(meta + all * WR_SUB);
     const int64_t pairs = (int64_t)r.q.B * r.q.Hkv;
     for (int64_t pair0 = 0; pair0 < pairs; pair0 += p.pairs_pass) {
         const int now = (int)(pairs - pair0 < p.pairs_pass ? pairs - pair0 : p.pairs_pass);
         const int64_t prepare = (int64_t)now * p.tiles, grid = (int64_t)now * p.splits;
         if (prepare >= (int64_t(1) << 31) || grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;
-        weights_rows_prepare_kernel<D><<<(unsigned)prepare, 256, 0, st>>>(r, pair0, p.tiles, ws, meta, factors);
+        weights_rows_prepare_kernel<D><<<(unsigned)prepare, 256, 0, st>>>(r, pair0, p.tiles, ws, meta);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)grid);
@@ -505,7 +496,7 @@ static cudaError_t launch_weights_rows_d(const WeightsRun& r, const WeightsPlan&
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, weights_rows_kernel<D>, r, pair0, p.splits, p.tiles, (const uint8_t*)ws, (const RowMeta*)meta, (const float*)factors);
+        e = cudaLaunchKernelEx(&cfg, weights_rows_kernel<D>, r, pair0, p.splits, p.tiles, (const uint8_t*)ws, (const RowMeta*)meta);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;

@@ -40,7 +40,7 @@ def _keys(kind, pages, H, P, D, seed):
 
 
 def _check(kind, B, H, grp, n, D, P, dtype, lens, q_len=None, fresh=None, decay=1.0, window=None, causal=True, rotate_q=True, sm=None,
-           seed=0, lse_of=None, table=None, three=False):
+           seed=0, lse_of=None, table=None, three=False, q_of=None):
     per = -(-max(16, max(lens)) // P)
     pool, scale, val, size = _keys(kind, B * per + 2, H, P, D, seed)
     g = torch.Generator().manual_seed(seed)
@@ -48,6 +48,8 @@ def _check(kind, B, H, grp, n, D, P, dtype, lens, q_len=None, fresh=None, decay=
         table = torch.randperm(B * per + 2, generator=g)[: B * per].view(B, per).to(torch.int32).to(DEV)
     gq = torch.Generator(device=DEV).manual_seed(seed + 2)
     q = torch.randn(B, n, H * grp, D, device=DEV, generator=gq).to(dtype).transpose(1, 2)
+    if q_of is not None:
+        q = q_of(q)
     w0 = torch.rand(B * per + 2, H, P, device=DEV, generator=gq)
     had, s_scale = _hadamard(D), D ** -0.5 if sm is None else sm
     want, tol = w0.double(), torch.zeros(w0.shape, device=DEV).double()
@@ -138,6 +140,34 @@ def test_rows_that_saw_nothing_add_nothing():
         lse[1] = -math.inf
         return lse
     _check(8, 2, 2, 4, 3, 128, 16, torch.bfloat16, [400, 33], lse_of=some, seed=7)
+
+
+@pytest.mark.parametrize("kind,n", [(8, 1), (8, 5), (8, 70), (8, 300), (3, 1), (4, 9)])
+def test_rows_that_saw_nothing_may_hold_anything(kind, n):
+    B, H, P, D = 2, 2, 16, 128
+    pool, scale, _, _ = _keys(kind, 20, H, P, D, 1)
+    table = torch.arange(20, dtype=torch.int32, device=DEV).view(2, 10)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    q = torch.randn(B, 4, n, D, device=DEV, generator=g)
+    lens = torch.tensor([150, 140], dtype=torch.int32, device=DEV)
+    lse = torch.rand(B, 4, n, device=DEV, generator=g) + 5.0
+    lse[:, 1::2, : (n + 1) // 2] = -math.inf
+    bad = q.clone()
+    for i, x in enumerate((math.inf, -math.inf, math.nan)):
+        bad[:, 1::2, i: (n + 1) // 2: 3, 7 * i] = x
+    one, two = torch.rand(20, H, P, device=DEV, generator=g).repeat(2, 1, 1, 1)
+    attention.attention_weights_paged(q, pool, table, lens, lse, one, k_scale=scale, causal=False)
+    attention.attention_weights_paged(bad, pool, table, lens, lse, two, k_scale=scale, causal=False)
+    assert bool(one.isfinite().all()) and torch.equal(one, two)
+
+
+@pytest.mark.parametrize("kind,n", [(8, 5), (8, 16), (8, 100), (3, 5)])
+def test_rows_of_unlike_sizes(kind, n):
+    # each row keeps the accuracy of its own size
+    def some(q):
+        small = torch.arange(q.shape[1] * n, device=DEV).view(1, -1, n, 1) % 5 > 0
+        return torch.where(small, q * 2.0 ** -10, q * 4)
+    _check(kind, 2, 2, 4, n, 128, 32, torch.float32, [400, n], q_of=some, seed=n)
 
 
 def test_earlier_weights_are_not_read_where_they_do_not_count():
