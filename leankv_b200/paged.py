@@ -228,11 +228,13 @@ class PagedKVCache:
         self._weights = torch.zeros((n_layers, num_pages, n_kv_heads, page_size), dtype=torch.float32, device=self.device) \
             if track_weights else None
         self.weights = [None] * n_layers if self._weights is None else list(self._weights)
+        self._observed = np.zeros(max_seqs, dtype=np.int64)   # slots that have been given weights: drafted ones may be rejected
 
     # sequence management (host bookkeeping; page-table rows reach the device in batch())
     def add_sequence(self) -> int:
         s = self.pages.add_sequence()
         self._lens[s] = 0
+        self._observed[s] = 0
         return s
 
     def free_sequence(self, s: int) -> None:
@@ -374,6 +376,8 @@ class PagedKVCache:
         A.attention_weights_paged(q, self.k[layer], step.table, lens, lse, self.weights[layer], k_scale=self.k_scale[layer],
                                   q_len=step.new_len, fresh=step.pos, decay=decay, window=window,
                                   max_kv_len=step.max_kv_len, sm_scale=sm_scale)
+        ends = np.asarray(step.starts) + np.asarray(step.n_new if step.counts is None else step.counts)
+        self._observed[step.seqs] = np.maximum(self._observed[step.seqs], ends)
 
     def accept(self, step: Batch, nodes: Sequence[Sequence[int]]) -> Batch:
         """In place of the commit of a tree's step: of each sequence the nodes of a path (rising, none for a sequence that
@@ -432,15 +436,23 @@ class PagedKVCache:
                                       width=width, max_kv_len=step.max_kv_len)
             ops.kv_move_paged(self.k[layer], self.v[layer], step.table, slots, k_scale=self.k_scale[layer],
                               v_scale=self.v_scale[layer], weights=self.weights[layer])
-        # slots behind the kept tokens begin at nothing
-        tail = [(int(self.pages.table[s, n // self.pages.page_size]), x) for s, n in zip(seqs, left) if n < self.pages.lens[s]
-                for x in range(n % self.pages.page_size, self.pages.page_size) if n % self.pages.page_size]
-        if tail:
-            page, slot = (torch.tensor(t, dtype=torch.int64, device=self.device) for t in zip(*tail))
-            self._weights[:, page, :, slot] = 0.0
         for s, n in zip(seqs, left):
+            if n < self.pages.lens[s]:
+                self._observed[s] = self.pages.capacity
             self.pages.truncate(s, n)
+        self._forget(seqs)
         self._lens.index_copy_(0, torch.tensor(seqs, dtype=torch.int64, device=self.device), count)
+
+    def _forget(self, seqs: Sequence[int]) -> None:
+        """Slots behind the sequences' tokens begin at nothing (pages that join a sequence do anyway)."""
+        import torch
+        size, t = self.pages.page_size, self.pages
+        tail = [(int(t.table[s, x // size]), x % size) for s in seqs
+                for x in range(int(t.lens[s]), min(int(self._observed[s]), int(t.n_pages[s]) * size))]
+        self._observed[seqs] = np.minimum(self._observed[seqs], t.lens[seqs])
+        if tail:
+            page, slot = (torch.tensor(i, dtype=torch.int64, device=self.device) for i in zip(*tail))
+            self._weights[:, page, :, slot] = 0.0
 
     def _check_evicted(self, step: Batch) -> None:
         if step.dropped is not None and any(n != self.pages.dropped[s] for s, n in zip(step.seqs, step.dropped)):
@@ -459,6 +471,8 @@ class PagedKVCache:
         self.pages.commit(step.seqs, step.n_new if step.counts is None else step.counts)
         idx = torch.tensor(step.seqs, dtype=torch.int64, device=self.device)
         self._lens.index_copy_(0, idx, step.kv_len)
+        if self._weights is not None:
+            self._forget(step.seqs)
 
     def _sync(self) -> None:
         import torch

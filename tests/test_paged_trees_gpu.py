@@ -249,6 +249,34 @@ def test_observed_after_acceptance():
     _near(now, 0.5 * had_before + p, 1e-5)
 
 
+@pytest.mark.parametrize("k_bits", [8, 3])
+def test_rejected_drafts_leave_no_weights(k_bits):
+    cache, rope, g = _make(k_bits, track_weights=True)
+    s = cache.add_sequence()
+
+    def held():
+        pages = torch.tensor(cache.pages.table[s, : cache.pages.n_pages[s]], device=DEV).long()
+        return torch.stack([w[pages].transpose(0, 1).flatten(1) for w in cache.weights])
+
+    step = cache.batch([s], 30)
+    _step(cache, rope, g, step) if k_bits == 8 else None
+    if k_bits != 8:   # TurboQuant keys: one query a sequence
+        for layer in range(2):
+            k, v = (torch.randn(1, H, 30, D, device=DEV, generator=g).bfloat16() for _ in range(2))
+            cache.append(step, layer, k, v)
+    cache.commit(step)
+    drafted = cache.batch([s], 6)
+    for layer in range(2):
+        k, v, q = (torch.randn(1, h, 6, D, device=DEV, generator=g).bfloat16() for h in (H, H, H * GRP))
+        cache.append(drafted, layer, k, v)
+        cache.attention(drafted, layer, q if k_bits == 8 else q[:, :, -1], observe=6)
+    assert bool((held()[..., :36] > 0).all())
+    cache.commit(cache.batch([s], 3))   # slots 33 .. 35 held rejected tokens
+    assert bool((held()[..., :33] > 0).all()) and bool((held()[..., 33:] == 0).all())
+    cache.commit(cache.batch([s], 20))   # not observed
+    assert bool((held()[..., :33] > 0).all()) and bool((held()[..., 33:] == 0).all())
+
+
 def test_refusals():
     plain = PagedKVCache(1, H, D, num_pages=8, page_size=16, max_seqs=2, k_bits=8)
     s = plain.add_sequence()
