@@ -20,6 +20,12 @@
 // tokens with 5 drafted tokens of 8 heads take 119 us, against 34 us for the bytes (issue 40 %, one CTA of 8 warps
 // per SM by its 220 registers).  Short caches: the launches (9.7 us for one sequence of 1001 tokens).
 //
+// Trees of drafted nodes (TREE) differ in what a row sees of the nodes alone, so only blocks behind the first node look at masks, 64 bits a
+// row in shared memory.  10 nodes of 4 heads behind 1000 tokens: 12.8 us.  Trees of more rows go to the tcgen05 kernels as drafted
+// tokens do: 16 sequences of up to 9000 tokens with 26 nodes of 4 heads 100 us, 24 for the bytes (issue 37 %, tensor 22 %: the
+// converting warps' chain); 3 sequences of 12000 tokens with 63 nodes of 8 heads of 256, float16, 300 us, 138 for the products of
+// two terms (202 us of them attention, tensor 54 %, then the tiles' expansion and the merge).
+//
 // Numbers.  A row of q' is scaled by its largest element and rounded to f16; where the output has more than bf16's 8
 // bits (LO) it is the sum of two f16 terms (float16 answers of 8 to 20 rows off by 2.4e-4 to 2.6e-4 of their norm
 // instead of 4.1e-4, 2.1e-4 of it the output's rounding, in the same time).  Codes are integers of 8 bits and exact in

@@ -7,7 +7,17 @@
 // Work.  A CTA takes a run of tokens of one (sequence, KV head); its 8 warps take every 8th block of 16 tokens, copied into
 // a ring of the warp's own in shared memory (cp.async), their earlier weights with them.  Products are mma.sync with the keys as
 // the A operand (16 tokens) and 8 query rows as B: a thread's sums over the rows are then sums over its columns, which four
-// lanes add up at the end.  More than 32 rows are taken 32 at a time, the tokens' sums kept in shared memory between.
+// lanes add up at the end.  More than 32 rows of TurboQuant keys are taken 32 at a time, the tokens' sums kept in shared memory
+// between; of 8-bit keys they go to tq_weights_rows.cu.  us with this file's kernel and with that one, 2 x 16000 tokens of 8 KV heads:
+//   rows          36         64         128         256
+//   D = 128    39 | 27    55 | 27    107 | 33    210 | 50
+//   D = 256    68 | 33    95 | 34    186 | 42    367 | 70
+//
+// What bounds it.  8 bits: the keys' bytes, 16 sequences of 32768 tokens of 8 KV heads (0.57 GB with the earlier weights) in 102 us,
+// 5.6 TB/s (86 % of the measured copy rate; a fourth of them in 36 us: issue 60 %, integer pipe 34 %, DRAM 48 %).  With f16 products
+// of converted codes the same took 129 us.  TurboQuant: instructions and the lookups' shared memory, 32 sequences of up to 9000
+// tokens of TQ3 keys in 60 us, floor 11 (8 of 9000 in 35 us: issue 60 %, shared-memory wavefronts 61 %, integer pipe 43 %,
+// DRAM 12 %); 136 us with levels made by arithmetic and a product for each term.  One sequence of 1001 tokens: the launch, 4.2 us.
 //
 // Numbers.  Sums are fp32 results that later sums are added to, so scores are kept to fp32's size of error.
 // 8 bits: codes enter s8 products (m16n8k32, exact in s32) as they lie in memory; a row of q' is scaled by its largest element
@@ -26,7 +36,7 @@
 namespace tq {
 
 constexpr int WT_WARPS = 8, WT_THREADS = 32 * WT_WARPS, WT_ROWS = 32;   // most rows at a time
-constexpr int WT_START = 1024;     // what a CTA's start is worth, in tokens
+constexpr int WT_START = 1024;     // what a CTA's start is worth, in tokens (256, 512 and 4096 are all slower)
 constexpr int WT_TOKENS = 2048;   // tokens of a CTA whose sums wait in shared memory
 
 __device__ __forceinline__ void wt_cp16(uint32_t dst, const void* src) {
@@ -421,7 +431,7 @@ WeightsPlan weights_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_
     WeightsPlan p;
     const int64_t rows = n * grp, len = max_len > 0 ? max_len : 1, pairs = (int64_t)B * Hkv;
     p.pairs_pass = (int)pairs;
-    p.tensor = q8 && rows > WT_ROWS;
+    p.tensor = q8 && rows > WT_ROWS;   // both sides measured: the table above
     if (p.tensor) {
         weights_rows_plan(pairs, D, rows, len, &p);
         return p;

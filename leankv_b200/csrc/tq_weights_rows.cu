@@ -7,9 +7,14 @@
 //
 // Products are of 8-bit whole numbers with 32-bit sums (kind::i8): codes enter as they lie in the pages.  A row of q' is the sum
 // of three terms of 8 bits, q1 + q2 / 128 + q3 / 128^2, in units of 1/127 of its largest element; the terms are rows of the same
-// product, N = 3 x 64.  Two f16 terms take as many operations, but the codes have to be converted on their way
-// (38 us for a window of 64 tokens of 32 heads over 2 x 16100 tokens, bound by shared memory's bandwidth: conversion, products and
-// the rows' factors) and their fp32 sums were off by 4e-6 of the result; sums of whole numbers are exact.
+// product, N = 3 x 64.  Two f16 terms take as many operations, but the codes have to be converted on their way and the
+// fp32 sums were off by 4e-6 of the result, where this is off by 1e-6: sums of whole numbers are exact.
+//
+// What bounds it: the way from TMEM to the weights, about 11 instructions for each of them, in two groups of warps that take turns.  The
+// last 64 tokens of 32 heads over 2 x 16100 tokens (256 rows a KV head): 54 us with the preparing kernel, 48 of them this
+// one's, floor 10 (issue 55 %, special function unit 35 %, tensor pipe 26 %); with f16 products 38 us, with mma.sync 210.
+// One scale for 64 rows: 50 us, but rows much smaller than their neighbours lost bits.  Four converting warps more, deeper rings, sums
+// begun from the bits of 1.5 * 2^23 in TMEM (61 to 88 us): slower.
 //
 // weights_rows_prepare_kernel: q' (Hadamard, the row's scale, terms) into images of the shared-memory tiles, once per call (a row is
 // read by every CTA of its KV head); with each row's scale, log-sum-exp and last token.
