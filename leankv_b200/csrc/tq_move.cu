@@ -8,7 +8,7 @@
 // the rule by which the append makes them.  Rows of the first block in front of `first` take part in place.
 //
 // A CTA makes 64 slots (4 blocks of K and of V, a warp each), all in registers: rows are read once and written once.
-// What bounds it: instructions of the rescaling, about 3 a code, then the scattered reads.  16 x 8 heads of 8192 kept tokens of 128
+// What bounds it: instructions of the rescaling, about 6 a code, then the scattered reads.  16 x 8 heads of 8192 kept tokens of 128
 // elements in 8 bits with their weights (0.55 GB read and written): 143 us, floor 84 (6 of the 16 sequences: 63 us, issue 67 %, integer
 // pipe 60 %, DRAM 32 %); 206 us with conversions by instruction, 166 and 158 us with five and six CTAs an SM (eight spill: 145).
 // TQ3 rows, 20 heads of up to 3001 tokens of 256 elements: 18.6 us with the reading back of the pages.

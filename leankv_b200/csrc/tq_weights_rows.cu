@@ -10,7 +10,7 @@
 // product, N = 3 x 64.  Two f16 terms take as many operations, but the codes have to be converted on their way and the
 // fp32 sums were off by 4e-6 of the result, where this is off by 1e-6: sums of whole numbers are exact.
 //
-// What bounds it: the way from TMEM to the weights, about 11 instructions for each of them, in two groups of warps that take turns.  The
+// What bounds it: the way from TMEM to the weights, 14 instructions issued for each of them, half of them its arithmetic.  The
 // last 64 tokens of 32 heads over 2 x 16100 tokens (256 rows a KV head): 54 us with the preparing kernel, 48 of them this
 // one's, floor 10 (issue 55 %, special function unit 35 %, tensor pipe 26 %); with f16 products 38 us, with mma.sync 210.
 // One scale for 64 rows: 50 us, but rows much smaller than their neighbours lost bits.  Four converting warps more, deeper rings, sums
