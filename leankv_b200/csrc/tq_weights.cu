@@ -15,16 +15,18 @@
 //
 // What bounds it.  8 bits: the keys' bytes, 16 sequences of 32768 tokens of 8 KV heads (0.57 GB with the earlier weights) in 102 us,
 // 5.6 TB/s (86 % of the measured copy rate; a fourth of them in 36 us: issue 60 %, integer pipe 34 %, DRAM 48 %).  With f16 products
-// of converted codes the same took 129 us.  TurboQuant: instructions and the lookups' shared memory, 32 sequences of up to 9000
-// tokens of TQ3 keys in 60 us, floor 11 (8 of 9000 in 35 us: issue 60 %, shared-memory wavefronts 61 %, integer pipe 43 %,
-// DRAM 12 %); 136 us with levels made by arithmetic and a product for each term.  One sequence of 1001 tokens: the launch, 4.2 us.
+// of converted codes the same took 129 us.  TurboQuant: instructions and their latency, 32 sequences of up to 9000 tokens
+// of TQ3 keys in 54 us, floor 11 (8 of 9000 in 34 us: issue 59 %, integer pipe 47 %, DRAM 12 %); 60 us with pairs of levels as
+// f16 terms from a table in shared memory (its wavefronts 61 %), 136 us with levels made by arithmetic.  One sequence of 1001 tokens: the launch, 4.2 us.
 //
 // Numbers.  Sums are fp32 results that later sums are added to, so scores are kept to fp32's size of error.
 // 8 bits: codes enter s8 products (m16n8k32, exact in s32) as they lie in memory; a row of q' is scaled by its largest element
 // and is the sum of three terms of 8 bits, q1 + q2 / 254 + q3 / 254^2 (2^-24 of the largest element).  In f16 the codes have to be
 // converted and q' is two terms: as many operations on twice the instructions.  The sums start from the bits of 1.5 * 2^23, so that
 // they are floats as they are (their size is below 2^22).
-// TurboQuant: levels are the sum of two f16 terms, looked up by the pair, and so is q'; m16n8k16, fp32 sums.
+// TQ2, TQ3: levels are sums of three such terms, too, whose bytes a byte permute looks up four at a time; of the nine products of
+// terms those below 2^-23 of the largest elements are left out, six remain.  TQ4 has more levels than a permute takes: its levels
+// are the sum of two f16 terms, looked up by the pair in shared memory, and so is q'; m16n8k16, fp32 sums.
 #include <type_traits>
 
 #include "leankv_tq.h"
@@ -36,7 +38,7 @@
 namespace tq {
 
 constexpr int WT_WARPS = 8, WT_THREADS = 32 * WT_WARPS, WT_ROWS = 32;   // most rows at a time
-constexpr int WT_START = 1024;     // what a CTA's start is worth, in tokens (256, 512 and 4096 are all slower)
+constexpr int WT_START = 1024;     // what a CTA's start is worth, in tokens (512 is slower for 8-bit keys, 2048 for TQ3 ones, 256 for both)
 constexpr int WT_TOKENS = 2048;   // tokens of a CTA whose sums wait in shared memory
 
 __device__ __forceinline__ void wt_cp16(uint32_t dst, const void* src) {
@@ -62,12 +64,22 @@ __device__ __forceinline__ uint32_t wt_lds16(uint32_t a) {
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
     return v;
 }
+__device__ __forceinline__ int wt_lds16s(uint32_t a) {
+    int16_t v;
+    asm volatile("ld.shared.s16 %0, [%1];" : "=h"(v) : "r"(a));
+    return v;
+}
 __device__ __forceinline__ void wt_imma(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// the sums begin with this product
+// the sums begin with this product, at `zero`
+__device__ __forceinline__ void wt_imma_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int zero) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(zero));
+}
 __device__ __forceinline__ void wt_mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -79,6 +91,29 @@ __device__ __forceinline__ void wt_mma(float (&c)[4], const uint32_t (&a)[4], ui
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The eight (TQ3) or four (TQ2) levels in units of 1/127 of the largest one, as the sum of three terms of 8 bits, l1 + l2 / 254 +
+// l3 / 254^2: term k of levels 4 w .. 4 w + 3 in the bytes of a word.
+template <int QT> constexpr uint32_t wt_levels(int k, int w) {
+    uint32_t bytes = 0;
+    for (int i = 0; i < 4; ++i) {
+        double x = (double)tq_level<QT>((4 * w + i) & ((1 << QT) - 1)) / (double)tq_level<QT>((1 << QT) - 1) * 127.0;
+        int term = 0;
+        for (int j = 0; j <= k; ++j) {
+            term = (int)(x < 0.0 ? x - 0.5 : x + 0.5);
+            x = (x - term) * 254.0;
+        }
+        bytes |= (uint32_t)(term & 0xFF) << (8 * i);
+    }
+    return bytes;
+}
+__device__ __forceinline__ uint32_t wt_either(uint32_t mask, uint32_t a, uint32_t b) { return (a & mask) | (b & ~mask); }
+// byte i of the result: byte (nibble i of s, 0 .. 7) of lo and hi
+__device__ __forceinline__ uint32_t wt_prmt(uint32_t lo, uint32_t hi, uint32_t s) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(lo), "r"(hi), "r"(s));
+    return d;
+}
+
 // TILES: tiles of 8 rows at a time, 1 or 4
 template <int D, int QT, int TILES> struct WtCfg {
     static constexpr int NK = D / 16, ROWS = 8 * TILES;
@@ -87,19 +122,22 @@ template <int D, int QT, int TILES> struct WtCfg {
     static constexpr int STAGE = TILE + 64;                      // with their earlier weights
     static constexpr int STAGES = QT == 8 && D == 256 ? 3 : 4;
     static constexpr int RING = STAGES * STAGE;                  // per warp
-    // q': 8 bits three terms, [tile][pair of k-steps][3][lane] of 16 bytes; TurboQuant two parts of [tile][pair of k-steps][lane]
-    static constexpr int QPART = TILES * NK * 256, QBYTES = QT == 8 ? TILES * (D / 64) * 3 * 512 : 2 * QPART;
-    // pairs of levels as f16 terms: an entry of 256 bytes, 8 for every lane, so that lookups do not meet in a bank and a lookup's
+    // q': 8 bits three terms, [tile][pair of k-steps][3][lane] of 16 bytes; TQ2 and TQ3 three terms, [tile][block of 32 elements], the first
+    // two [lane] of 16 bytes and the third [lane] of 8; TQ4 two parts of [tile][pair of k-steps][lane]
+    static constexpr int QPART = TILES * NK * 256, QBLOCK = 768, QBYTES = QT == 4 ? 2 * QPART : TILES * (D / 32) * QBLOCK;
+    // TQ4: pairs of levels as f16 terms, an entry of 256 bytes, 8 for every lane, so that lookups do not meet in a bank and a lookup's
     // address is the pair's number in one byte and the lane's in the next
-    static constexpr int PAIRS = QT == 4 ? 256 : QT == 3 ? 64 : QT == 2 ? 16 : 0, TABLE = PAIRS * 256;
+    static constexpr int PAIRS = QT == 4 ? 256 : 0, TABLE = PAIRS * 256;
+    // what a sum of products counts: TQ2 and TQ3 levels are in units of 1/127 of the largest one, too
+    static constexpr float UNIT = QT == 4 ? 1.0f : QT == 8 ? 1.0f / 127.0f : tq_level<QT == 8 ? 4 : QT>((1 << (QT & 3)) - 1) / (127.0f * 127.0f);
     static constexpr int SUMS = TILES > 1 ? WT_TOKENS * 4 : 0;   // tokens' sums between chunks of rows
     static constexpr int SMEM = TABLE + WT_WARPS * RING + QBYTES + SUMS;
     static constexpr int CTAS = SMEM <= 74 * 1024 ? 3 : SMEM <= 112 * 1024 ? 2 : 1;
 };
 
 // half_decode() in three operations: the bits moved to a float's place are the value times 2^-112, whatever the exponent
-__device__ __forceinline__ float scale_decode(uint32_t h) {
-    return __uint_as_float((h & 0x7FFFu) << 13 | (h & 0x8000u) << 16) * 0x1p112f;
+__device__ __forceinline__ float scale_decode(int h) {   // sign-extended, so that the sign is in its place, and in those of the exponent's top
+    return __uint_as_float(((uint32_t)h << 13) & 0x8FFFFFFFu) * 0x1p112f;
 }
 
 template <int D, int QT, int TILES>
@@ -124,7 +162,7 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
     const int i0 = sl.q_len > p.window ? sl.q_len - (int)p.window : 0;
     const int rows_all = (sl.q_len - i0) * r.grp;   // rows i0 .. of the sequence, row = token x head of group
 
-    if constexpr (QT != 8) {
+    if constexpr (QT == 4) {
         __shared__ float s_level[1 << (QT & 7)];
         if (threadIdx.x < (1 << QT)) {
             float x = 0.0f;
@@ -145,6 +183,16 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + C::TABLE + warp * C::RING;
     const uint32_t sq = (uint32_t)__cvta_generic_to_shared(s_q) + lane * 16;
     const uint32_t lane8 = lane * 8;
+    uint32_t levels[3][2];   // TQ2, TQ3
+    if constexpr (QT == 2 || QT == 3) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            constexpr uint32_t w[3][2] = {{wt_levels<QT>(0, 0), wt_levels<QT>(0, 1)}, {wt_levels<QT>(1, 0), wt_levels<QT>(1, 1)},
+                                          {wt_levels<QT>(2, 0), wt_levels<QT>(2, 1)}};
+            levels[k][0] = w[k][0];
+            levels[k][1] = w[k][1];
+        }
+    }
 
     // with several chunks of rows, as many tokens at a time as have sums in shared memory
     const int step = row_chunks > 1 ? WT_TOKENS : per;
@@ -220,9 +268,9 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
             for (int j = 0; j < E; ++j) top = fmaxf(top, fabsf(v[j]));
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float inv = top >= 0x1p-100f ? __fdiv_rn(QT == 8 ? 127.0f : 1.0f, top) : 0.0f;
-            if constexpr (QT == 8) {
-                // element e: byte e & 3 of word b (0, 1) of a k-step of lane tt, whose elements are one run of 32 in 128
+            const float inv = top >= 0x1p-100f ? __fdiv_rn(QT == 4 ? 1.0f : 127.0f, top) : 0.0f;
+            if constexpr (QT != 4) {
+                // 8 bits: element e is byte e & 3 of word b (0, 1) of a k-step of lane tt, whose elements are one run of 32 in 128
 #pragma unroll
                 for (int j = 0; j < E / 4; ++j) {
                     uint32_t q[3] = {0, 0, 0};
@@ -232,6 +280,15 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
                         q[0] |= ((uint32_t)(int)a & 0xFFu) << (8 * k);
                         q[1] |= ((uint32_t)(int)c & 0xFFu) << (8 * k);
                         q[2] |= ((uint32_t)(int)d & 0xFFu) << (8 * k);
+                    }
+                    if constexpr (QT != 8) {
+                        // elements 8 tt .. 8 tt + 7 of a block, as the codes lie: b0 and b1 of lane tt
+                        const int e = e0 + 4 * j, half = (e >> 2) & 1, at = (row & 7) * 4 + ((e & 31) >> 3);
+                        uint8_t* to = s_q + ((row >> 3) * (D / 32) + (e >> 5)) * C::QBLOCK;
+                        reinterpret_cast<uint32_t*>(to)[at * 4 + half] = q[0];
+                        reinterpret_cast<uint32_t*>(to)[at * 4 + 2 + half] = q[1];
+                        reinterpret_cast<uint32_t*>(to + 512)[at * 2 + half] = q[2];
+                        continue;
                     }
                     const int e = e0 + 4 * j, word = (e & 31) >> 2, pr = (e >> 7) * 2 + (word >> 2), tt = (e & 127) >> 5;
                     uint32_t* to = reinterpret_cast<uint32_t*>(s_q) + ((row >> 3) * (D / 64) + pr) * 384 + ((row & 7) * 4 + tt) * 4;
@@ -243,24 +300,23 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
                 }
             } else {
                 // Element e of the row goes where the keys' element meets it: half-word `odd` of word w (b0, b1 of one k-step, then
-                // of the next) of lane tt, pair of k-steps j2.  A pair of k-steps is a block of 32 elements, lane tt has 8 of them:
-                // TQ4 the nibbles of bytes 4 tt .. 4 tt + 3 (e and e + 16 in a byte), TQ3 the group of 8 codes tt, TQ2 those of bytes
-                // 2 tt, 2 tt + 1.
+                // of the next) of lane tt, pair of k-steps j2.  A pair of k-steps is a block of 32 elements, lane tt has the nibbles of
+                // bytes 4 tt .. 4 tt + 3, e and e + 16 in a byte.
                 __half* qh = reinterpret_cast<__half*>(s_q) + (row >> 3) * (NK / 2) * 256 + (row & 7) * 32;
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
                     const int e = e0 + j;
                     const float x = v[j] * inv;
                     const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
-                    const int j2 = e >> 5, tt = QT == 4 ? (e & 15) >> 2 : (e & 31) >> 3, w = QT == 4 ? e & 3 : (e & 7) >> 1;
-                    const int odd = QT == 4 ? (e >> 4) & 1 : e & 1;
+                    const int j2 = e >> 5, tt = (e & 15) >> 2, w = e & 3;
+                    const int odd = (e >> 4) & 1;
                     __half* to = qh + j2 * 256 + tt * 8 + w * 2 + odd;
                     to[0] = hi;
                     to[C::QPART / 2] = lo;
                 }
             }
             if (lane == 0) {
-                s_f[row] = make_float2(top * (r.sm_scale * LOG2E * (QT == 8 ? 1.0f / 127.0f : 1.0f)), sees ? lse * LOG2E : INFINITY);
+                s_f[row] = make_float2(top * (r.sm_scale * LOG2E * C::UNIT), sees ? lse * LOG2E : INFINITY);
                 s_lim[row] = sees ? last_seen(r, sl, i) : 0x7fffffff;
             }
         }
@@ -346,6 +402,72 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
                     }
                     add(nt, s, ks);
                 }
+            } else if constexpr (QT != 4) {
+                // A block of 32 elements is a k-step; a lane takes the 8 codes of elements 8 t .. 8 t + 7 of tokens g and g + 8.  Codes
+                // become the nibbles of a byte permute's selector, which looks up four levels' terms at a time.
+                constexpr int BB = BlockBytes<QT>::value;
+                constexpr float Z = 12582912.0f, R2 = 1.0f / (254.0f * 254.0f);
+                float2 acc[TILES][2];
+#pragma unroll
+                for (int nt = 0; nt < TILES; ++nt) acc[nt][0] = acc[nt][1] = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int j2 = 0; j2 < D / 32; ++j2) {
+                    float d[2];
+                    uint32_t a[3][4];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t row = kt + (x * 8 + g) * C::ROWB + j2 * BB;
+                        d[x] = scale_decode(wt_lds16s(row));
+                        uint32_t v;
+                        if constexpr (QT == 3) {
+                            // bytes 3 t .. 3 t + 2 of the codes: two half-words, from byte 3 t or the one before
+                            const uint32_t from = row + 2 + ((3 * t) & ~1);
+                            v = wt_prmt(wt_lds16(from), wt_lds16(from + 2), (t & 1) ? 0x5541u : 0x5410u);
+                            v = wt_either(0x0000FFFFu, v, v << 4);   // 12 bits in 16
+                            v = wt_either(0x00FF00FFu, v, v << 2);   // 6 in 8
+                            v = (v & 0x07070707u) | ((v << 1) & 0x70707070u);
+                        } else {
+                            const uint32_t w = wt_lds16(row + 2 + 2 * t);
+                            v = wt_either(0x0000FFFFu, w, w << 8);
+                            v = wt_either(0x00FF00FFu, v, v << 4);
+                            v = (v & 0x03030303u) | ((v << 2) & 0x30303030u);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) {
+                            a[k][x] = wt_prmt(levels[k][0], levels[k][1], v);
+                            a[k][2 + x] = wt_prmt(levels[k][0], levels[k][1], v >> 16);
+                        }
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < TILES; ++nt) {
+                        if (nt >= tiles) break;
+                        const uint32_t from = (uint32_t)__cvta_generic_to_shared(s_q) + (nt * (D / 32) + j2) * C::QBLOCK;
+                        const uint4 q = wt_lds128(from + lane * 16);
+                        const uint2 q3 = wt_lds64(from + 512 + lane8);
+                        // products by the size of their terms; those below 2^-23 of the largest elements are left out
+                        int c[3][4];
+                        wt_imma_first(c[0], a[0], q.x, q.y, 0x4B400000);
+                        wt_imma_first(c[1], a[0], q.z, q.w, 0x4B400000);
+                        wt_imma_first(c[2], a[0], q3.x, q3.y, 0x4B400000);
+                        wt_imma(c[1], a[1], q.x, q.y);
+                        wt_imma(c[2], a[1], q.z, q.w);
+                        wt_imma(c[2], a[2], q.x, q.y);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const auto pair = [&](int k) { return make_float2(__int_as_float(c[k][2 * x]), __int_as_float(c[k][2 * x + 1])); };
+                            // -Z R2 is rounded by 2^-17 of the first term's unit
+                            float2 y = __ffma2_rn(pair(2), make_float2(R2, R2), make_float2(-Z * R2, -Z * R2));
+                            y = __ffma2_rn(__fadd2_rn(pair(1), make_float2(-Z, -Z)), make_float2(1.0f / 254.0f, 1.0f / 254.0f), y);
+                            y = __fadd2_rn(y, __fadd2_rn(pair(0), make_float2(-Z, -Z)));
+                            acc[nt][x] = __ffma2_rn(y, make_float2(d[x], d[x]), acc[nt][x]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < TILES; ++nt) {
+                    const float y[4] = {acc[nt][0].x, acc[nt][0].y, acc[nt][1].x, acc[nt][1].y};
+                    if (nt < tiles) add(nt, y, 1.0f);
+                }
             } else {
                 // a block of 32 elements is two k-steps; its scales are those of tokens g and g + 8
                 float acc[TILES][4];
@@ -361,24 +483,11 @@ __global__ void __launch_bounds__(WT_THREADS, WtCfg<D, QT, TILES>::CTAS) weights
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const uint32_t row = kt + (x * 8 + g) * C::ROWB + j2 * BB;
-                        d[x] = scale_decode(wt_lds16(row));
+                        d[x] = scale_decode(wt_lds16s(row));
                         uint32_t at[4];   // of the pairs in the table
-                        if constexpr (QT == 4) {
-                            const uint32_t w = wt_lds16(row + 2 + 4 * t) | wt_lds16(row + 4 + 4 * t) << 16;
+                        const uint32_t w = wt_lds16(row + 2 + 4 * t) | wt_lds16(row + 4 + 4 * t) << 16;
 #pragma unroll
-                            for (int i4 = 0; i4 < 4; ++i4) at[i4] = __byte_perm(w, lane8, 0x5504 | i4 << 4);   // lane8 is below 256
-                        } else if constexpr (QT == 3) {
-                            // bytes 3 t .. 3 t + 2 of the codes: two half-words, from byte 3 t or the one before
-                            const uint32_t from = row + 2 + ((3 * t) & ~1);
-                            uint32_t w = wt_lds16(from) | wt_lds16(from + 2) << 16;
-                            w = (t & 1) ? w : w << 8;   // the 24 bits in the upper three bytes
-#pragma unroll
-                            for (int i4 = 0; i4 < 4; ++i4) at[i4] = ((w >> (6 * i4)) & 0x3F00u) | lane8;
-                        } else {
-                            const uint32_t w = wt_lds16(row + 2 + 2 * t) << 8;
-#pragma unroll
-                            for (int i4 = 0; i4 < 4; ++i4) at[i4] = ((w >> (4 * i4)) & 0xF00u) | lane8;
-                        }
+                        for (int i4 = 0; i4 < 4; ++i4) at[i4] = __byte_perm(w, lane8, 0x5504 | i4 << 4);   // lane8 is below 256
 #pragma unroll
                         for (int i4 = 0; i4 < 4; ++i4) lv[x][i4] = *reinterpret_cast<const uint2*>(smem + at[i4]);
                     }

@@ -2,8 +2,10 @@
 
 Tolerance.  A score's roundings: the Hadamard transform in fp32 (log2 D + 1 roundings of values of at most sum |q| / sqrt(D)), q'
 divided by its largest element (two roundings of 2^-24) and taken as two f16 terms (what they leave is at most 2^-23 of the largest
-element): (log2 D + 3) 2^-24 sum|q| / sqrt(D) + 2^-22 max|q'| on each element of q', times sum |k_d|.  TurboQuant levels as two f16
-terms are off by 2^-22 of each.  The products of a score are summed by at most 3 D / 16 matrix instructions, each off by at most
+element): (log2 D + 3) 2^-24 sum|q| / sqrt(D) + 2^-22 max|q'| on each element of q', times sum |k_d|.  TQ4 levels as two f16
+terms are off by 2^-22 of each.  TQ2 and TQ3 levels are three terms of 8 bits, off by 2^-24 of the largest level, and products of
+terms below 2^-23 of the largest level and element are left out; their sums are of whole numbers and exact, so that on these
+inputs the part for the matrix instructions (D = 128: 25 times 2^-22 of the products' sizes) is far above both.  The products of a score are summed by at most 3 D / 16 matrix instructions, each off by at most
 2^-22 of the sum of the products' sizes (8 bits: of codes + 128).  In the exponent four more roundings of 2^-24 of the sizes of
 score and lse; the power 2^-22; the sum over the rows 2^-23 for each of them; the earlier weight's part 2^-23."""
 import math
