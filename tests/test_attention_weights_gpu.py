@@ -117,6 +117,13 @@ def test_many_rows(kind, D, grp, n, causal):
     _check(kind, 5, 2, grp, n, D, 32, torch.float16, lens, q_len=[n, n, n, n, 2 * n // 3], fresh=[900 - n, 0, 7, 0, 100], causal=causal, seed=n)
 
 
+@pytest.mark.parametrize("kind", [2, 3, 4])
+@pytest.mark.parametrize("D,grp,n,P", [(128, 3, 3, 16), (256, 8, 4, 64), (256, 5, 13, 16), (128, 16, 5, 128)])
+def test_turboquant_rows(kind, D, grp, n, P):
+    # one to three times the rows that are taken at a time; tokens of a CTA beyond the sums that it holds
+    _check(kind, 3, 2, grp, n, D, P, torch.bfloat16, [4500, n, 17], q_len=[n, n, n - 1], fresh=[4500 - n, 0, 16], decay=0.5, seed=n)
+
+
 @pytest.mark.parametrize("window", [1, 3, 40, 64, 99, 1000])
 def test_window(window):
     n = 99
