@@ -203,28 +203,30 @@ __device__ __forceinline__ void move_block_q8(const MoveRun& r, const MoveSide& 
     if (lane == 0) x.scale[to0 >> 4] = now;
 }
 
-// TurboQuant rows of a block: 8 U bytes a row, the block's 16 rows flat over the lanes
-template <int U>
-__device__ __forceinline__ void move_block_tq(const MoveSide& x, MoveRow m, uint32_t to0, bool some, uint32_t used, uint32_t* flags,
-                                              int64_t chunk, int* s_ok) {
-    constexpr int N = 16 * U, PER = (N + 31) / 32;
+// TurboQuant rows of a block: 8 U bytes a row, the block's 16 rows flat over the lanes.  Reading and writing are apart, so that
+// the warps of K and of V, whose rows differ in size, meet at one and the same turn between them.
+template <int U> constexpr int tq_words() { return (16 * U + 31) / 32; }   // of a lane
+template <int U, int M>
+__device__ __forceinline__ uint32_t read_block_tq(const MoveSide& x, uint32_t from_row, uint32_t rows, uint2 (&w)[M]) {
     const int lane = threadIdx.x & 31;
-    const uint32_t rows = __ballot_sync(0xffffffffu, some && m.moved) & 0xFFFFu;
-    uint2 w[PER];
+    uint32_t used = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int u = lane + 32 * i, row = u < N ? u / U : 0;
-        const uint32_t from = __shfl_sync(0xffffffffu, m.from, row);
+    for (int i = 0; i < tq_words<U>(); ++i) {
+        const int u = lane + 32 * i, row = u < 16 * U ? u / U : 0;
+        const uint32_t from = __shfl_sync(0xffffffffu, from_row, row);
         w[i] = make_uint2(0, 0);
-        if (u < N && ((rows >> row) & 1)) w[i] = reinterpret_cast<const uint2*>(x.pool)[(size_t)from * U + u % U];
+        if (u < 16 * U && ((rows >> row) & 1)) w[i] = reinterpret_cast<const uint2*>(x.pool)[(size_t)from * U + u % U];
         used ^= w[i].x ^ w[i].y;
     }
-    if (!move_turn(flags, chunk, used, s_ok) || !some) return;
+    return used;
+}
+template <int U, int M>
+__device__ __forceinline__ void write_block_tq(const MoveSide& x, uint32_t to0, uint32_t rows, const uint2 (&w)[M]) {
     uint2* to = reinterpret_cast<uint2*>(x.pool) + (size_t)to0 * U;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int u = lane + 32 * i;
-        if (u < N && ((rows >> (u / U)) & 1)) to[u] = w[i];
+    for (int i = 0; i < tq_words<U>(); ++i) {
+        const int u = (threadIdx.x & 31) + 32 * i;
+        if (u < 16 * U && ((rows >> (u / U)) & 1)) to[u] = w[i];
     }
 }
 
@@ -263,8 +265,14 @@ __global__ void __launch_bounds__(32 * MOVE_WARPS, D == 128 && UK == 0 ? 7 : 4) 
     if constexpr (UK == 0) {
         move_block_q8<D>(r, side ? r.v : r.k, m, to0, some, used, flags, chunk, &s_ok);
     } else {
-        if (side) move_block_tq<UV>(r.v, m, to0, some, used, flags, chunk, &s_ok);
-        else move_block_tq<UK>(r.k, m, to0, some, used, flags, chunk, &s_ok);
+        uint2 w[tq_words<(UK > UV ? UK : UV)>()];
+        const uint32_t rows = __ballot_sync(0xffffffffu, some && m.moved) & 0xFFFFu;
+        const uint32_t read = side ? read_block_tq<UV>(r.v, m.from, rows, w) : read_block_tq<UK>(r.k, m.from, rows, w);
+        const bool go = move_turn(flags, chunk, used ^ read, &s_ok);
+        if (go && some) {
+            if (side) write_block_tq<UV>(r.v, to0, rows, w);
+            else write_block_tq<UK>(r.k, to0, rows, w);
+        }
     }
     if (flags && !s_ok) {
         if (threadIdx.x == 0 && r.status) atomicMax(r.status, (int)TQ_ERROR_TIMEOUT);
