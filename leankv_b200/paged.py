@@ -84,6 +84,8 @@ class PageTable:
         self.dropped = np.zeros(max_seqs, dtype=np.int64)   # tokens evicted: what positions are ahead of slots
         self.n_pages = np.zeros(max_seqs, dtype=np.int64)   # pages held per sequence
         self.active = np.zeros(max_seqs, dtype=bool)
+        self.given_back = np.zeros(max_seqs, dtype=np.int64)   # how often a sequence slot has given tokens or pages back
+        self.times_given_back = 0                              # all slots together
         self._free = list(range(num_pages - 1, -1, -1))     # pop() hands out low pages first
         self.dirty: set = set()                             # sequence rows changed since the last sync
 
@@ -115,6 +117,7 @@ class PageTable:
         self.lens[s] = 0
         self.dropped[s] = 0
         self.active[s] = False
+        self._gives_back(s)
         self.dirty.add(s)
 
     @staticmethod
@@ -162,12 +165,18 @@ class PageTable:
             raise ValueError(f"sequence {s} has {int(self.lens[s])} tokens")
         held = -(-length // self.page_size)
         self._free.extend(int(p) for p in self.table[s, held: self.n_pages[s]][::-1])
+        if held < self.n_pages[s] or length < self.lens[s]:
+            self._gives_back(s)
         if held < self.n_pages[s]:
             self.table[s, held: self.n_pages[s]] = NO_PAGE
             self.n_pages[s] = held
             self.dirty.add(s)
         self.dropped[s] += self.lens[s] - length
         self.lens[s] = length
+
+    def _gives_back(self, s: int) -> None:
+        self.given_back[s] += 1
+        self.times_given_back += 1
 
     def _check(self, s: int) -> None:
         if not (0 <= s < self.max_seqs) or not self.active[s]:
@@ -190,7 +199,8 @@ class Batch:
     tree: "object" = None      # ops.DraftTree
     parents: "object" = None   # the tree's, numpy [B or 1, n_new] (None: they came from the device)
     starts: "object" = None    # pos on the host
-    dropped: "object" = None   # tokens evicted from each sequence when the step was made
+    given_back: "object" = None      # the sequences' PageTable.given_back when the step was made
+    times_given_back: "object" = None
 
 
 class PagedKVCache:
@@ -282,7 +292,8 @@ class PagedKVCache:
         step = Batch(seqs, rows, self._table.index_select(0, idx).contiguous(), pos.contiguous(), kv_len,
                      int(lens.max()) if len(seqs) else 0, None if alike else counts, new_len,
                      None if alike or min(counts) else kv_len * (new_len > 0), parents=parents,
-                     starts=[int(n) for n in self.pages.lens[seqs]], dropped=[int(n) for n in self.pages.dropped[seqs]])
+                     starts=[int(n) for n in self.pages.lens[seqs]], given_back=self.pages.given_back[seqs],
+                     times_given_back=self.pages.times_given_back)
         dropped = self.pages.dropped[seqs]
         if tree is not None or dropped.any():
             from . import ops
@@ -302,6 +313,7 @@ class PagedKVCache:
         nodes by their depths; int32 [B, n_new] or [axes, B, n_new] otherwise) in the same launch."""
         import torch
         from . import ops
+        self._check_step(step)
         B = len(step.seqs)
         if positions is None and rope is not None:
             positions = step.positions
@@ -338,6 +350,7 @@ class PagedKVCache:
         observe: that many of each sequence's last query tokens count towards the weights by which evict() chooses, earlier
         counts times decay (track_weights=True; after a tree's step the accepted rows count by observe())."""
         from . import attention as A
+        self._check_step(step)
         if observe and step.tree is not None:
             raise ValueError("nodes of a tree may be rejected: observe() the accepted ones after accept()")
         if observe:
@@ -369,6 +382,7 @@ class PagedKVCache:
         the step's own tokens begin at nothing.  After accept(), with the step it returns and the rows of q and lse of the
         accepted nodes, as the rows of a chain."""
         from . import attention as A
+        self._check_step(step)
         self._need_weights()
         if step.tree is not None:
             raise ValueError("nodes of a tree may be rejected: observe the accepted ones after accept()")
@@ -398,9 +412,8 @@ class PagedKVCache:
                 row = step.parents[i if len(step.parents) > 1 else 0]
                 if any(int(row[x]) != a for a, x in zip(before, path)):
                     raise ValueError(f"sequence {step.seqs[i]}: {path} is not a path of the tree")
-        self._check_evicted(step)
+        self._check_step(step)
         for s, n in zip(step.seqs, step.starts):
-            self.pages._check(s)
             if n != self.pages.lens[s]:
                 raise ValueError(f"sequence {s} has changed since the step")
         rows = max((len(p) for p in paths), default=0)
@@ -417,7 +430,8 @@ class PagedKVCache:
     def evict(self, seqs: Sequence[int], keep, sinks: int = 0, recent: int = 0) -> None:
         """Drops tokens of the sequences until `keep` (one number, or one each) are left: in every layer each KV head keeps its
         last `recent` and first `sinks` tokens and, of the others, those with the largest observed weights.  Pages that are
-        no longer needed return to the pool; later tokens' positions are not changed by it."""
+        no longer needed return to the pool; later tokens' positions are not changed by it.  Steps made before an eviction are
+        refused from then on where it took tokens from one of their sequences."""
         import torch
         from . import ops
         self._need_weights()
@@ -454,9 +468,14 @@ class PagedKVCache:
             page, slot = (torch.tensor(i, dtype=torch.int64, device=self.device) for i in zip(*tail))
             self._weights[:, page, :, slot] = 0.0
 
-    def _check_evicted(self, step: Batch) -> None:
-        if step.dropped is not None and any(n != self.pages.dropped[s] for s, n in zip(step.seqs, step.dropped)):
-            raise ValueError("tokens have been evicted since the step was made: its slots and pages are no longer those of its sequences")
+    def _check_step(self, step: Batch) -> None:
+        """A step has its own copy of page-table rows: of a sequence that has been freed or evicted from they name pages that
+        others may hold by now."""
+        if step.times_given_back == self.pages.times_given_back or step.given_back is None:
+            return
+        if (self.pages.given_back[step.seqs] != step.given_back).any():
+            raise ValueError("a sequence has been freed or evicted from since the step was made: its slots and pages are no longer those of "
+                             "the step")
 
     def _need_weights(self) -> None:
         if self._weights is None:
@@ -466,7 +485,7 @@ class PagedKVCache:
         """The step's rows are part of the sequences from now on."""
         if step.tree is not None:
             raise ValueError("a tree's step is committed by accept()")
-        self._check_evicted(step)
+        self._check_step(step)
         import torch
         self.pages.commit(step.seqs, step.n_new if step.counts is None else step.counts)
         idx = torch.tensor(step.seqs, dtype=torch.int64, device=self.device)
