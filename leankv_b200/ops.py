@@ -581,8 +581,9 @@ def kv_move_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.
     int32 [B, n_kv_heads, n] or, for all heads alike, [B, n]; negative entries move nothing; rows j >= count[b] (int32
     [B]) neither.  Pools as kv_append_rotary_paged writes them (TQ rows are copied; 8-bit blocks of rows of one scale keep
     codes and scale, others get max |code| scale / 127).  weights: pool of summed attention weights, moved along.  In place
-    rows may only move down (src >= first + j); to_table (int32 [B, pages]) names other pages for the destination, none that
-    are read.  Rows without a place, or that would move up, are left and counted into overflow, one per head."""
+    (no to_table, or page_table itself) rows may only move down (src >= first + j); another to_table (int32 [B, pages]) names
+    other pages for the destination, none that are read.  Rows without a place, or that would move up, are left and counted into
+    overflow, one per head."""
     device = _device_of(k_pool, v_pool, page_table, src, first, count, k_scale, v_scale, weights, to_table, overflow, status)
     B = page_table.shape[0]
     _check_table(page_table, B)
@@ -618,7 +619,9 @@ def kv_move_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.
               0 if to_table is None else to_table.shape[1], _check_status(overflow, "overflow"), _check_status(status))
     pg = _PAGES.pack(page_table.data_ptr(), per, pages, page_size)
     lib = L.load()
-    key = ("move", device, B, H, D, rows, kt, first is None, to_table is None, per, pages, page_size)
+    # a table of the destinations that is the pages' own is in place, too
+    in_place = to_table is None or to_table.data_ptr() == page_table.data_ptr()
+    key = ("move", device, B, H, D, rows, kt, first is None, in_place, per, pages, page_size)
     need = _work_bytes(key, device, lib.tq_kv_move_workspace_size, _MOVE, fields, pg)
     # from the allocator on every call: streams and captured graphs each get their own
     ws = torch.empty(need, dtype=torch.uint8, device=k_pool.device) if need else None
