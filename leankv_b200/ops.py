@@ -612,6 +612,8 @@ def kv_move_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.
         raise ValueError(f"weights must be [{pages}, {H}, {page_size}], as the pools")
     if to_table is not None:
         _check_table(to_table, B)
+        if to_table.shape[1] == 0:
+            raise ValueError("to_table must have a page for each sequence at least")   # (without one its address is that of no table)
     rows, per = src.shape[-1], page_table.shape[1]
     fields = (B, H, D, rows, src.data_ptr(), src.shape[1] if src.dim() == 3 else 1, 0 if first is None else first.data_ptr(),
               0 if count is None else count.data_ptr(), k_pool.data_ptr(), kt, ks, v_pool.data_ptr(), vt, vs,

@@ -44,3 +44,11 @@ def test_work_memory_does_not_depend_on_the_order_of_calls(library, order):
         _move(to)
     assert all(given == needed for given, needed in library.given)
     assert [needed > 0 for _, needed in library.given] == [to != "other" for to in order]
+
+
+def test_a_destination_without_pages_is_refused(library):
+    pool, scale = torch.zeros(4, H, P, D, dtype=torch.int8), torch.zeros(4, H, P // 16)
+    with pytest.raises(ValueError):
+        ops.kv_move_paged(pool, pool, torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, H, 3, dtype=torch.int32), k_scale=scale,
+                          v_scale=scale, to_table=torch.zeros(1, 0, dtype=torch.int32))
+    assert not library.given
