@@ -201,6 +201,7 @@ class Batch:
     starts: "object" = None    # pos on the host
     given_back: "object" = None      # the sequences' PageTable.given_back when the step was made
     times_given_back: "object" = None
+    written: "object" = None         # layers whose rows have been appended (caches that track weights)
 
 
 class PagedKVCache:
@@ -238,13 +239,17 @@ class PagedKVCache:
         self._weights = torch.zeros((n_layers, num_pages, n_kv_heads, page_size), dtype=torch.float32, device=self.device) \
             if track_weights else None
         self.weights = [None] * n_layers if self._weights is None else list(self._weights)
-        self._observed = np.zeros(max_seqs, dtype=np.int64)   # slots that have been given weights: drafted ones may be rejected
+        # Drafted tokens may be observed and rejected.  Of each sequence: the slots behind its tokens that may hold weights end at
+        # _observed; in a layer, the weights from _valid on are of rows that others have been written over.
+        self._observed = np.zeros(max_seqs, dtype=np.int64)
+        self._valid = np.zeros((n_layers, max_seqs), dtype=np.int64)
 
     # sequence management (host bookkeeping; page-table rows reach the device in batch())
     def add_sequence(self) -> int:
         s = self.pages.add_sequence()
         self._lens[s] = 0
         self._observed[s] = 0
+        self._valid[:, s] = 0
         return s
 
     def free_sequence(self, s: int) -> None:
@@ -314,6 +319,11 @@ class PagedKVCache:
         import torch
         from . import ops
         self._check_step(step)
+        if self._weights is not None and step.starts is not None:
+            if not step.written or layer in step.written:   # once for all layers, and again when the step's rows are written anew
+                self._valid[:, step.seqs] = np.minimum(self._valid[:, step.seqs], step.starts)
+                step.written = set()
+            step.written.add(layer)
         B = len(step.seqs)
         if positions is None and rope is not None:
             positions = step.positions
@@ -392,6 +402,7 @@ class PagedKVCache:
                                   max_kv_len=step.max_kv_len, sm_scale=sm_scale)
         ends = np.asarray(step.starts) + np.asarray(step.n_new if step.counts is None else step.counts)
         self._observed[step.seqs] = np.maximum(self._observed[step.seqs], ends)
+        self._valid[layer, step.seqs] = ends
 
     def accept(self, step: Batch, nodes: Sequence[Sequence[int]]) -> Batch:
         """In place of the commit of a tree's step: of each sequence the nodes of a path (rising, none for a sequence that
@@ -454,19 +465,29 @@ class PagedKVCache:
             if n < self.pages.lens[s]:
                 self._observed[s] = self.pages.capacity
             self.pages.truncate(s, n)
-        self._forget(seqs)
+        self._forget(seqs, left)
         self._lens.index_copy_(0, torch.tensor(seqs, dtype=torch.int64, device=self.device), count)
 
-    def _forget(self, seqs: Sequence[int]) -> None:
-        """Slots behind the sequences' tokens begin at nothing (pages that join a sequence do anyway)."""
+    def _forget(self, seqs: Sequence[int], starts: Sequence[int]) -> None:
+        """Slots behind the sequences' tokens begin at nothing (pages that join a sequence do anyway), and so do those from
+        starts on whose weights are of other rows than they hold."""
         import torch
         size, t = self.pages.page_size, self.pages
-        tail = [(int(t.table[s, x // size]), x % size) for s in seqs
-                for x in range(int(t.lens[s]), min(int(self._observed[s]), int(t.n_pages[s]) * size))]
+        tails: dict = {}   # layers (None: all) -> (page, slot) of each
+        for s, start in zip(seqs, starts):
+            top, length = min(int(self._observed[s]), int(t.n_pages[s]) * size), int(t.lens[s])
+            if top > start:
+                firsts = np.clip(self._valid[:, s], start, length)
+                for first in np.unique(firsts):
+                    layers = None if (firsts == first).all() else tuple(np.flatnonzero(firsts == first))
+                    tails.setdefault(layers, []).extend((int(t.table[s, x // size]), x % size) for x in range(int(first), top))
         self._observed[seqs] = np.minimum(self._observed[seqs], t.lens[seqs])
-        if tail:
-            page, slot = (torch.tensor(i, dtype=torch.int64, device=self.device) for i in zip(*tail))
-            self._weights[:, page, :, slot] = 0.0
+        self._valid[:, seqs] = np.minimum(self._valid[:, seqs], t.lens[seqs])
+        for layers, tail in tails.items():
+            if tail:
+                page, slot = (torch.tensor(i, dtype=torch.int64, device=self.device) for i in zip(*tail))
+                for weights in [self._weights] if layers is None else [self._weights[n: n + 1] for n in layers]:
+                    weights[:, page, :, slot] = 0.0
 
     def _check_step(self, step: Batch) -> None:
         """A step has its own copy of page-table rows: of a sequence that has been freed or evicted from they name pages that
@@ -487,11 +508,12 @@ class PagedKVCache:
             raise ValueError("a tree's step is committed by accept()")
         self._check_step(step)
         import torch
+        starts = [int(n) for n in self.pages.lens[step.seqs]]
         self.pages.commit(step.seqs, step.n_new if step.counts is None else step.counts)
         idx = torch.tensor(step.seqs, dtype=torch.int64, device=self.device)
         self._lens.index_copy_(0, idx, step.kv_len)
         if self._weights is not None:
-            self._forget(step.seqs)
+            self._forget(step.seqs, starts)
 
     def _sync(self) -> None:
         import torch
