@@ -461,11 +461,12 @@ class PagedKVCache:
                                       width=width, max_kv_len=step.max_kv_len)
             ops.kv_move_paged(self.k[layer], self.v[layer], step.table, slots, k_scale=self.k_scale[layer],
                               v_scale=self.v_scale[layer], weights=self.weights[layer])
-        for s, n in zip(seqs, left):
-            if n < self.pages.lens[s]:
-                self._observed[s] = self.pages.capacity
+        # (the others keep what a step under way has reserved and observed)
+        cut = [(s, n) for s, n in zip(seqs, left) if n < self.pages.lens[s]]
+        for s, n in cut:
+            self._observed[s] = self.pages.capacity
             self.pages.truncate(s, n)
-        self._forget(seqs, left)
+        self._forget([s for s, _ in cut], [n for _, n in cut])
         self._lens.index_copy_(0, torch.tensor(seqs, dtype=torch.int64, device=self.device), count)
 
     def _forget(self, seqs: Sequence[int], starts: Sequence[int]) -> None:

@@ -86,3 +86,20 @@ def test_a_step_written_twice():
     _run(cache, g, step)      # other rows, not observed
     cache.commit(step)
     assert bool((_held(cache, s) == 0).all())
+
+
+@pytest.mark.parametrize("bits", [8, 3])
+def test_a_step_under_way_beside_an_eviction(bits):
+    """A sequence that keeps all its tokens keeps the pages and the weights of a step that is still to be committed."""
+    cache, g = _cache(bits)
+    a, b = cache.add_sequence(), cache.add_sequence()
+    step = cache.batch([a, b], 30)
+    _run(cache, g, step, range(LAYERS))
+    cache.commit(step)
+    step = cache.batch([b], 5)            # its last three slots are on a page that no token has yet
+    _run(cache, g, step, range(LAYERS))
+    before, held = _held(cache, b), list(cache.pages.table[b])
+    cache.evict([a, b], [12, 100], sinks=1, recent=2)
+    assert (cache.seq_len(a), cache.seq_len(b)) == (12, 30) and list(cache.pages.table[b]) == held
+    cache.commit(step)
+    assert cache.seq_len(b) == 35 and torch.equal(_held(cache, b), before) and bool((before[..., :35] > 0).all())
