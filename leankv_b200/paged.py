@@ -268,6 +268,8 @@ class PagedKVCache:
         seqs = [int(s) for s in seqs]
         if len(set(seqs)) != len(seqs):
             raise ValueError("a sequence may appear once per batch")
+        for s in seqs:
+            self.pages._check(s)
         counts = self.pages._counts(seqs, n_new)
         rows = max(counts, default=0)
         parents = None
