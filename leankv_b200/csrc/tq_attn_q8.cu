@@ -640,23 +640,17 @@ static cudaError_t launch_rows(const Q8Run& r, const Q8Plan& p, float* part, flo
 // raised by calls that bring no status word of their own; zero when the module is loaded
 __device__ int32_t q8_status_word;
 
-// its address on the current device (asked for once a device; the first call may be a captured one)
+// Its address on the current device.  Asked for on every call (about 0.1 us): it is another one after cudaDeviceReset.  The first
+// call, which loads the module, may be a captured one.
 cudaError_t q8_default_status(int32_t** word) {
-    static std::atomic<int32_t*> known[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const bool keep = dev >= 0 && dev < 64;
-    if (keep && (*word = known[dev].load(std::memory_order_relaxed)) != nullptr) return cudaSuccess;
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    if ((e = cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) return e;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return e;
     void* at = nullptr;
     e = cudaGetSymbolAddress(&at, q8_status_word);
     const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
-    if (e != cudaSuccess || back != cudaSuccess) return e != cudaSuccess ? e : back;
     *word = static_cast<int32_t*>(at);
-    if (keep) known[dev].store(*word, std::memory_order_relaxed);
-    return cudaSuccess;
+    return e != cudaSuccess ? e : back;
 }
 
 cudaError_t launch_q8_merge(const Q8Run& r, const Q8Plan& p, int64_t pair0, int pairs, const float* part, const float* part_lse,
