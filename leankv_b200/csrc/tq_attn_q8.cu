@@ -36,7 +36,6 @@
 // of f16 numbers near their row's largest, whatever the scales of other blocks; the sum of weights l takes
 // p_j / vs in fp32.  m is the largest s + log2 vs seen up to a slack of 8: rows are rescaled only when a score
 // exceeds m by more than that (p stays below 2^14, and is exact to f16's 11 bits down to 2^-20 of the largest).
-#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -622,8 +621,7 @@ size_t q8_workspace_bytes(int D, const Q8Plan& p) { return part_bytes(D, p) + p.
 template <int D, int NT, bool LO, bool TREE>
 static cudaError_t launch_one(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
     using C = Q8Cfg<D, NT, LO>;
-    static std::atomic<uint64_t> allowed{0};
-    cudaError_t e = allow_smem(attn_q8_kernel<D, NT, LO, TREE>, C::SMEM, allowed);
+    cudaError_t e = allow_smem(attn_q8_kernel<D, NT, LO, TREE>, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)r.B * r.Hkv * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;

@@ -717,8 +717,7 @@ attn_q8_prompt_kernel(const Q8Run r, int64_t pair0, int pairs, int tiles_max, co
 template <int D, int QTILES, bool LO, bool TREE>
 static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, uint8_t* tiles, cudaStream_t st) {
     using C = PromptCfg<D, false, QTILES>;
-    static std::atomic<uint64_t> allowed{0};
-    cudaError_t e = allow_smem(attn_q8_prompt_kernel<D, false, QTILES, LO, TREE>, C::SMEM, allowed);
+    cudaError_t e = allow_smem(attn_q8_prompt_kernel<D, false, QTILES, LO, TREE>, C::SMEM);
     if (e != cudaSuccess) return e;
     float4* factors = reinterpret_cast<float4*>(tiles + (size_t)p.pairs_pass * p.tiles_max * (2 * C::KV_TILE));
     const int64_t pairs = (int64_t)r.B * r.Hkv;
@@ -749,8 +748,7 @@ static cudaError_t launch_prompt_d(const Q8Run& r, const Q8Plan& p, float* part,
 template <int D, bool LO, bool TREE>
 static cudaError_t launch_direct_d(const Q8Run& r, const Q8Plan& p, float* part, float* part_lse, cudaStream_t st) {
     using C = PromptCfg<D, true, 1>;
-    static std::atomic<uint64_t> allowed{0};
-    cudaError_t e = allow_smem(attn_q8_prompt_kernel<D, true, 1, LO, TREE>, C::SMEM, allowed);
+    cudaError_t e = allow_smem(attn_q8_prompt_kernel<D, true, 1, LO, TREE>, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t pairs = (int64_t)r.B * r.Hkv, grid = pairs * p.row_tiles * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;

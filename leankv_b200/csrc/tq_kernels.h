@@ -1,7 +1,6 @@
 // tq_kernels.h — internal launchers (C++ linkage, not part of the public ABI).
 #pragma once
 
-#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -9,17 +8,11 @@ namespace tq {
 
 int sm_count();
 
-// Lets a kernel use `bytes` of dynamic shared memory, once a device (about 1 us a call): `done` is the kernel's own, a bit per device.
+// Lets a kernel use `bytes` of dynamic shared memory.  On every call (0.06 us where it does already): the limit goes with the context,
+// and cudaDeviceReset makes another one.
 template <typename Kernel>
-inline cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
-    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
-    return e;
+inline cudaError_t allow_smem(Kernel kernel, int bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 // Placement of quantized head rows in a KV cache (cap == 0: contiguous output).

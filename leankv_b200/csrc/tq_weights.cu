@@ -564,8 +564,7 @@ WeightsPlan weights_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_
 
 template <int D, int QT, int TILES> static cudaError_t launch_weights_t(const WeightsRun& r, const WeightsPlan& p, cudaStream_t st) {
     using C = WtCfg<D, QT, TILES>;
-    static std::atomic<uint64_t> allowed{0};
-    const cudaError_t e = allow_smem(weights_kernel<D, QT, TILES>, C::SMEM, allowed);
+    const cudaError_t e = allow_smem(weights_kernel<D, QT, TILES>, C::SMEM);
     if (e != cudaSuccess) return e;
     const int64_t grid = (int64_t)r.q.B * r.q.Hkv * p.splits;
     if (grid >= (int64_t(1) << 31)) return cudaErrorInvalidConfiguration;

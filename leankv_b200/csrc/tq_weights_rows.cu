@@ -479,8 +479,7 @@ void weights_rows_plan(int64_t pairs, int D, int64_t rows, int64_t len, WeightsP
 template <int D>
 static cudaError_t launch_weights_rows_d(const WeightsRun& r, const WeightsPlan& p, uint8_t* ws, cudaStream_t st) {
     using C = WrCfg<D>;
-    static std::atomic<uint64_t> allowed{0};
-    cudaError_t e = allow_smem(weights_rows_kernel<D>, C::SMEM, allowed);
+    cudaError_t e = allow_smem(weights_rows_kernel<D>, C::SMEM);
     if (e != cudaSuccess) return e;
     const size_t all = (size_t)p.pairs_pass * p.tiles;
     RowMeta* meta = reinterpret_cast<RowMeta*>(ws + all * C::QSUB);

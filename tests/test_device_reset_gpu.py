@@ -107,3 +107,7 @@ def _run(what):
 
 def test_the_word_of_calls_without_a_status():
     _run("select")
+
+
+def test_kernels_with_more_shared_memory_than_the_default():
+    _run("attend")
