@@ -99,8 +99,9 @@ __global__ void __launch_bounds__(256) weights_rows_prepare_kernel(const Weights
     const int sub = blockIdx.x % subs, h = (int)(pair % r.Hkv), b = (int)(pair / r.Hkv);
     const SeqLens sl = seq_lens(r, b);
     const int i0 = sl.q_len > p.window ? sl.q_len - (int)p.window : 0;
-    // Row k's log-sum-exp.  A row that saw nothing adds nothing, whatever q holds there.
-    const auto lse_of = [&](int i, int hq) { return i < sl.q_len ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : -INFINITY; };
+    // Row k's log-sum-exp, -inf for a row that sees no token, whatever was left for it.  Such a row, and one of -inf, adds nothing,
+    // whatever q holds there.
+    const auto lse_of = [&](int i, int hq) { return last_seen(r, sl, i) >= 0 ? p.lse[((int64_t)b * r.Hq + hq) * r.n + i] : -INFINITY; };
     float v[ROWS][E], inv[ROWS];
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
