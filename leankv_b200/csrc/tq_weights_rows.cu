@@ -304,13 +304,14 @@ weights_rows_kernel(const WeightsRun p, int64_t pair0, int splits, int subs, con
 #pragma unroll
                             for (int k = 0; k < 8; k += 4) {
                                 const float4 l = *reinterpret_cast<const float4*>(s_row + 2 * (r0 + k)), m = *reinterpret_cast<const float4*>(s_row + 2 * (r0 + k) + 4);
-                                // c1 + (c2 + c3 / 128) / 128 to half of 1/128 of c1's unit, floats from the bits of 1.5 * 2^23 + c
-                                const float2 off = make_float2(-12681216.0f, -12681216.0f), m1 = make_float2(0x1p-7f, 0x1p-7f);
+                                // c1 + (c2 + c3 / 128) / 128, floats from the bits of 1.5 * 2^23 + c.  c2 + c3 / 128 is rounded to a
+                                // whole number there, the nearest, so that scores are off by up to half of 1/128 of c1's unit, either way.
+                                const float2 off = make_float2(-12681984.0f, -12681984.0f), m1 = make_float2(0x1p-7f, 0x1p-7f);
+                                const auto term = [&](int t, int u) {
+                                    return make_float2(__uint_as_float(x[t][k + u] + WR_ZERO), __uint_as_float(x[t][k + u + 1] + WR_ZERO));
+                                };
                                 const auto sum = [&](int u) {
-                                    const float2 hi = make_float2(__uint_as_float(x[0][k + u] + WR_ZERO), __uint_as_float(x[0][k + u + 1] + WR_ZERO));
-                                    const float2 lo = make_float2(__uint_as_float(x[1][k + u] + (uint32_t)((int)x[2][k + u] >> 7) + WR_ZERO),
-                                                                  __uint_as_float(x[1][k + u + 1] + (uint32_t)((int)x[2][k + u + 1] >> 7) + WR_ZERO));
-                                    return __ffma2_rn(lo, m1, __fadd2_rn(hi, off));
+                                    return __ffma2_rn(__ffma2_rn(term(2, u), m1, term(1, u)), m1, __fadd2_rn(term(0, u), off));
                                 };
                                 const float2 y = __ffma2_rn(sum(0), __fmul2_rn(make_float2(l.z, l.w), ks), make_float2(l.x, l.y));
                                 const float2 z = __ffma2_rn(sum(2), __fmul2_rn(make_float2(m.z, m.w), ks), make_float2(m.x, m.y));
