@@ -564,6 +564,8 @@ tq_status tq_select_tokens_cuda(const tq_select_args *a, const tq_kv_pages *page
  * copied.  A destination block of 8-bit rows (TQ_Q8_BLOCK slots) whose rows had one scale all keeps codes and scale; else its scale becomes
  * max |code| * scale / 127 over the rows that are moved into it and those in it before slot first[b], and codes are rounded to it;
  * codes of the block's other slots stay as they are, under its new scale.
+ * (A step of a drafted tree may so round the rows of its first block twice: where the append raises the block's scale for a
+ * node, and where the accepted path's move sets it back; each by up to half of the scale.)
  * to_table NULL or the pages' own table (the same address): in place; a row may only move down (src >= first + j), and the rows
  * of a call may come in any order.  Otherwise destination slots are looked up in to_table, whose pages must be none that the
  * call reads.  Rows that would move up, from or to slots without a page, are left and counted in *overflow, one per head.  Two

@@ -44,7 +44,10 @@ slots.  8-bit blocks that held a rejected row keep a scale that is large enough 
     cache.commit(cache.batch([a, b], [2, 4]))
 
 A tree of drafted tokens (k_bits=8): its nodes are appended like a step's tokens, rotated by their depths, and see the
-cached tokens and their ancestors; the accepted path's rows then move up behind the cached ones.
+cached tokens and their ancestors; the accepted path's rows then move up behind the cached ones.  A step
+rounds the rows of the block of 16 slots that it begins in up to twice more, when a node raises the block's scale and when the
+path's move sets it back: the rows that stay are off by about 1.4 times what a chain of the same tokens leaves (200 steps of
+26 nodes and 4 accepted, rows of unlike size: 2.4e-2 of the norm, the chain 1.6e-2).
 
     step = cache.batch([a, b], n, tree=parents)  # parents of the n nodes, -1 for children of the cached tokens
     q = cache.append(step, layer, k, v, rope=rope, q=q)
