@@ -510,7 +510,8 @@ tq_status tq_attention_q8_tree_paged_cuda(const tq_attention_q8_args *a, const t
  * Three steps: sums of the attention weights that cached tokens get, kept beside the pages as
  *   weights  float [num_pages][n_kv_heads][page_size], on a 16-byte boundary
  * the selection of the tokens of each (sequence, KV head) that stay, and moving their rows together.  No counterpart in the
- * reference.  Page ids outside the pool are treated as holding nothing (TQ_ERROR_INVALID_VALUE in *status).
+ * reference.  Page ids outside the pool are treated as holding nothing (TQ_ERROR_INVALID_VALUE in *status; the move leaves their
+ * rows and counts them in *overflow instead).
  *
  * tq_attention_weights_paged_cuda: for the tokens t < kv_len[b] of sequence b and KV head h
  *   w[t] <- (t < fresh[b] ? decay * w[t] : 0) + sum exp(s_it - lse_i),   s_it = sm_scale * q'_i . k_t,
@@ -518,7 +519,10 @@ tq_status tq_attention_q8_tree_paged_cuda(const tq_attention_q8_args *a, const t
  * rotate_q.  q, lengths, causal, pages and status are those of tq_attention_q8_paged_cuda, lse the log-sum-exps that the
  * attention of these rows has left (after an accepted path of a tree has moved, its rows see what they saw).  Rows of -inf
  * add nothing.  With decay 0, and from fresh[b] on, w is not read.  Slots from kv_len[b] on stay as they are.  Keys: TQ_TYPE_Q8 with
- * k_scale, or TQ2_0 / TQ3_0 / TQ4_0 blocks.  Sums are fp32; a weight is off by about 2^-20 of itself for each unit of its score.
+ * k_scale, or TQ2_0 / TQ3_0 / TQ4_0 blocks.  Sums are fp32.  A score is off by the sizes of its products, however much of them
+ * cancels: by up to sm_scale * sum |k_d| * (2^-22 max |q'| + (log2 head_dim + 3) 2^-24 sum |q_d| / sqrt(head_dim)) and 2^-22 of
+ * |s| + |lse| (TQ4_0 keys: besides (3 head_dim / 16 + 1) 2^-22 sm_scale * sum |q'_d k_d|), and a weight by as much of itself.
+ * max_kv_len sizes the work split; tokens behind it are counted all the same.
  * Sequences of a call must not share pages.  Work memory: tq_attention_weights_workspace_size() bytes.
  */
 typedef struct {

@@ -267,8 +267,9 @@ def attention_weights_paged(q: torch.Tensor, k_pool: torch.Tensor, page_table: t
 
     weights float32 [num_pages, n_kv_heads, page_size], beside the pages: for each token t of sequence b and KV head
     weights <- (t < fresh[b] ? decay * weights : 0) + sum of exp(score - lse) over the group's query heads and those of the last
-    `window` (default: all) query tokens that see t.  q, q_len, causal, max_kv_len, sm_scale, rotate_q and status as in
-    attention_q8_paged; lse float32 [B, Hq, n] (or [B, Hq] with q [B, Hq, D]), as the attention of these queries returned it.
+    `window` (default: all) query tokens that see t.  q, q_len, causal, sm_scale, rotate_q and status as in attention_q8_paged;
+    max_kv_len, an upper bound of kv_len, sizes the work split; lse float32 [B, Hq, n] (or [B, Hq] with q [B, Hq, D]), as the
+    attention of these queries returned it.
     k_pool: int8 pages with k_scale, or uint8 TQ blocks as decode_attention_paged takes them.  fresh: int32 [B], the first slot
     whose earlier weight is not read (a step's new slots; default: none).  With decay 0 none is read.  Slots behind kv_len keep
     theirs.  Returns weights."""

@@ -21,7 +21,8 @@
 // per SM by its 220 registers).  Short caches: the launches (9.7 us for one sequence of 1001 tokens).
 //
 // Trees of drafted nodes (TREE) differ in what a row sees of the nodes alone, so only blocks behind the first node look at masks, 64 bits a
-// row in shared memory.  10 nodes of 4 heads behind 1000 tokens: 12.8 us.  Trees of more rows go to the tcgen05 kernels as drafted
+// row in shared memory.  10 nodes of 4 heads behind 1000 tokens: 12.8 us, as a chain of as many tokens (12.4): two units of 24 rows, a
+// few blocks of tokens a CTA, then the merge; alone the two kernels take 9 us each, chains of dependent steps both.  Trees of more rows go to the tcgen05 kernels as drafted
 // tokens do: 16 sequences of up to 9000 tokens with 26 nodes of 4 heads 100 us, 24 for the bytes (issue 37 %, tensor 22 %: the
 // converting warps' chain); 3 sequences of 12000 tokens with 63 nodes of 8 heads of 256, float16, 300 us, 138 for the products of
 // two terms (202 us of them attention, tensor 54 %, then the tiles' expansion and the merge).
@@ -600,7 +601,9 @@ Q8Plan q8_plan(int B, int Hkv, int grp, int D, int64_t n, int64_t max_len, bool 
         if (tree) {
             // A verification step's sequences have grown to lengths of all kinds: half of the weight to lengths even between
             // none and the bound, whose time is the longest CTA's or the mean one's (16 sequences of up to 9000 tokens, 104 rows:
-            // one split 123 us, two 99, four 97, six 111).
+            // one split 123 us, two 99, four 97, six 111; other lengths to 9000: 128 us, planned as drafted tokens 133).  Lengths all
+            // alike pay for it where splits do not fill the SMs evenly: 16 x 9000 tokens 165 us (145), 4 x 16000 102 (86); 8 x 3000,
+            // 32 x 2000, 2 x 8000 and 1 x 30000 tokens take the same either way.
             const double mean = (double)units * (double)(len / 2 + s * (each - per)) / (double)slots;
             cost += mean > (double)each ? (int64_t)(mean < 0x1p60 ? mean : 0x1p60) : each;
         }

@@ -10,8 +10,9 @@
 // A CTA makes 64 slots (4 blocks of K and of V, a warp each), all in registers: rows are read once and written once.
 // What bounds it: instructions of the rescaling, about 6 a code, then the scattered reads.  16 x 8 heads of 8192 kept tokens of 128
 // elements in 8 bits with their weights (0.55 GB read and written): 143 us, floor 84 (6 of the 16 sequences: 63 us, issue 67 %, integer
-// pipe 60 %, DRAM 32 %); 206 us with conversions by instruction, 166 and 158 us with five and six CTAs an SM (eight spill: 145).
-// TQ3 rows, 20 heads of up to 3001 tokens of 256 elements: 18.6 us with the reading back of the pages.
+// pipe 60 %, DRAM 32 %); 206 us with conversions by instruction, 166 and 158 us with five and six CTAs an SM, 145 with eight (seven
+// spill 8 bytes a thread, eight more).  To other pages, without waits: 118 us of 140 (no weights).  TQ3 rows of 128 elements, the same
+// tokens: 123 us; 20 heads of up to 3001 tokens of 256 elements: 16 us with the reading back of the pages.
 //
 // In place, a slot may be written only after the row that it held has been read.  Slots only fall (src >= first + j,
 // checked), so that row is one of the same 64 or of an earlier 64.  CTAs take their 64 in the order in which they start (a

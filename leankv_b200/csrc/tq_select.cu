@@ -6,13 +6,15 @@
 // the digit is the one in which the wanted rank falls.  Then the tokens above it, and as many of its equals as are
 // wanted, are written in the order of their slots, each at the count of those before it.
 //
-// A CTA keeps the keys of up to 32768 slots in registers, 32 a thread, so that weights are read once; its counters are in
-// shared memory.  Where sequences are longer, or there are few (sequence, KV head)s, a cluster of CTAs shares one, and counts are
-// added up over their shared memories; a barrier of the cluster costs about as much as a pass over 8192 keys (128 of them of 32768
-// slots: 36 us in clusters of two, 48 and 110 us in clusters of four and eight).  What bounds it: the chain of four passes, counting
-// by atomics and barriers; the weights' bytes take little time (16 x 8 heads of 32768 tokens, 17 MB: 20 us, floor 3; issue 61 %,
-// integer pipe 55 %; 42 us when every pass read them again).  One sequence of 1025 tokens: 6.5 us.  11 bits take the sign, the
-// exponent and two bits of the fraction, so that weights of like size, which most are, do not meet in one counter.
+// A CTA keeps the keys of up to 32768 slots, 32 a thread, so that weights are read once: in registers, but 28 words of a thread's
+// (112 bytes stored, 128 loaded), which 64 registers for each of 1024 threads do not hold.  Its counters are in shared memory.
+// Where sequences are longer, or there are few (sequence, KV head)s, a cluster of CTAs shares one, and counts are added up over
+// their shared memories; a barrier of the cluster costs about as much as a pass over 8192 keys (128 of them of 32768 slots: 36 us
+// in clusters of two, 48 and 110 us in clusters of four and eight).  What bounds it: the chain of four passes, counting by atomics
+// and barriers; the weights' bytes take little time (16 x 8 heads of 32768 tokens, 17 MB: 20 us, floor 3; issue 61 %, integer pipe
+// 55 %; 42 us when every pass read them again).  Weights that are all alike, whose counting meets in one word: 19 us.  One sequence
+// of 1025 tokens: 6.5 us.  11 bits take the sign, the exponent and two bits of the fraction, so that weights of like size, which
+// most are, do not meet in one counter.
 #include <cooperative_groups.h>
 
 #include "leankv_tq.h"

@@ -9,15 +9,19 @@
 // the A operand (16 tokens) and 8 query rows as B: a thread's sums over the rows are then sums over its columns, which four
 // lanes add up at the end.  More than 32 rows of TurboQuant keys are taken 32 at a time, the tokens' sums kept in shared memory
 // between; of 8-bit keys they go to tq_weights_rows.cu.  us with this file's kernel and with that one, 2 x 16000 tokens of 8 KV heads:
-//   rows          36         64         128         256
-//   D = 128    39 | 27    55 | 27    107 | 33    210 | 50
-//   D = 256    68 | 33    95 | 34    186 | 42    367 | 70
+//   rows       32        36         64         128         256
+//   D = 128    28     39 | 29    55 | 29    107 | 36    210 | 55
+//   D = 256    50     68 | 35    95 | 36    186 | 45    367 | 76
+// The bound of 32 rows is that of D = 128; heads of 256 with 32 rows would be faster there (about 35 us), with 8 they are not.
 //
 // What bounds it.  8 bits: the keys' bytes, 16 sequences of 32768 tokens of 8 KV heads (0.57 GB with the earlier weights) in 102 us,
 // 5.6 TB/s (86 % of the measured copy rate; a fourth of them in 36 us: issue 60 %, integer pipe 34 %, DRAM 48 %).  With f16 products
 // of converted codes the same took 129 us.  TurboQuant: instructions and their latency, 32 sequences of up to 9000 tokens
 // of TQ3 keys in 54 us, floor 11 (8 of 9000 in 34 us: issue 59 %, integer pipe 47 %, DRAM 12 %); 60 us with pairs of levels as
-// f16 terms from a table in shared memory (its wavefronts 61 %), 136 us with levels made by arithmetic.  One sequence of 1001 tokens: the launch, 4.2 us.
+// f16 terms from a table in shared memory (its wavefronts 61 %), 136 us with levels made by arithmetic.  32 other ragged sequences to
+// 9000 tokens of 8 KV heads, one token of 64 heads, us for 8 bits, TQ4, TQ3, TQ2: heads of 128 42, 67, 59, 56; heads of 256 60, 134, 98, 90.
+// More rows of 8-bit keys (16, 24, 32 rows over 16 x 9000 tokens of 8 KV heads): 59, 77, 92 us, of heads of 256 116, 148, 182: the
+// products and powers of a tile of 8 rows.  One sequence of 1001 tokens: the launch, 4.7 us.
 //
 // Numbers.  Sums are fp32 results that later sums are added to, so scores are kept to fp32's size of error.
 // 8 bits: codes enter s8 products (m16n8k32, exact in s32) as they lie in memory; a row of q' is scaled by its largest element

@@ -10,10 +10,11 @@
 // product, N = 3 x 64.  Two f16 terms take as many operations, but the codes have to be converted on their way and the
 // fp32 sums were off by 4e-6 of the result, where this is off by 1e-6: sums of whole numbers are exact.
 //
-// What bounds it: the way from TMEM to the weights, 14 instructions issued for each of them, half of them its arithmetic.  The
-// last 64 tokens of 32 heads over 2 x 16100 tokens (256 rows a KV head): 54 us with the preparing kernel, 48 of them this
-// one's, floor 10 (issue 55 %, special function unit 35 %, tensor pipe 26 %); with f16 products 38 us, with mma.sync 210.
-// One scale for 64 rows: 50 us, but rows much smaller than their neighbours lost bits.  Four converting warps more, deeper rings, sums
+// What bounds it: the way from TMEM to the weights, 13 instructions issued for each of them, half of them its arithmetic, and their
+// latency: no pipe is full.  The last 64 tokens of 32 heads over 2 x 16100 tokens (256 rows a KV head): 56 us with the preparing
+// kernel, floor 10 (this kernel alone: issue 55 %, FMA pipe 41 %, special function unit 33 %, tensor pipe 25 %, 20 warps an SM); with
+// f16 products 38 us, with mma.sync 210.  Terms joined by a shift, which rounds down, took 53 us and made all scores too small.
+// One scale for 64 rows: 4 us less, but rows much smaller than their neighbours lost bits.  Four converting warps more, deeper rings, sums
 // begun from the bits of 1.5 * 2^23 in TMEM (61 to 88 us): slower.
 //
 // weights_rows_prepare_kernel: q' (Hadamard, the row's scale, terms) into images of the shared-memory tiles, once per call (a row is
