@@ -201,7 +201,9 @@ class Batch:
     positions: "object" = None # int32 [B, n_new] where they are not the slots (trees, sequences with evicted tokens)
     tree: "object" = None      # ops.DraftTree
     parents: "object" = None   # the tree's, numpy [B or 1, n_new] (None: they came from the device)
-    starts: "object" = None    # pos on the host
+    starts: "object" = None    # pos and kv_len on the host
+    ends: "object" = None
+    index: "object" = None     # seqs as an array
     given_back: "object" = None      # the sequences' PageTable.given_back when the step was made
     times_given_back: "object" = None
     written: "object" = None         # layers whose rows have been appended (caches that track weights)
@@ -295,14 +297,15 @@ class PagedKVCache:
         self._sync()
         idx = torch.tensor(seqs, dtype=torch.int64, device=self.device)
         pos = self._lens.index_select(0, idx)
-        lens = self.pages.lens[seqs] + np.asarray(counts, dtype=np.int64)
+        index = np.asarray(seqs, dtype=np.int64)
+        lens = self.pages.lens[index] + np.asarray(counts, dtype=np.int64)
         alike = all(n == rows for n in counts)
         new_len = None if alike else torch.tensor(counts, dtype=torch.int32, device=self.device)
         kv_len = (pos + (rows if alike else new_len)).contiguous()
         step = Batch(seqs, rows, self._table.index_select(0, idx).contiguous(), pos.contiguous(), kv_len,
                      int(lens.max()) if len(seqs) else 0, None if alike else counts, new_len,
                      None if alike or min(counts) else kv_len * (new_len > 0), parents=parents,
-                     starts=[int(n) for n in self.pages.lens[seqs]], given_back=self.pages.given_back[seqs],
+                     starts=self.pages.lens[index], ends=lens, index=index, given_back=self.pages.given_back[index],
                      times_given_back=self.pages.times_given_back)
         dropped = self.pages.dropped[seqs]
         if tree is not None or dropped.any():
@@ -326,7 +329,7 @@ class PagedKVCache:
         self._check_step(step)
         if self._weights is not None and step.starts is not None:
             if not step.written or layer in step.written:   # once for all layers, and again when the step's rows are written anew
-                self._valid[:, step.seqs] = np.minimum(self._valid[:, step.seqs], step.starts)
+                self._valid[:, step.index] = np.minimum(self._valid[:, step.index], step.starts)
                 step.written = set()
             step.written.add(layer)
         B = len(step.seqs)
@@ -405,9 +408,8 @@ class PagedKVCache:
         A.attention_weights_paged(q, self.k[layer], step.table, lens, lse, self.weights[layer], k_scale=self.k_scale[layer],
                                   q_len=step.new_len, fresh=step.pos, decay=decay, window=window,
                                   max_kv_len=step.max_kv_len, sm_scale=sm_scale)
-        ends = np.asarray(step.starts) + np.asarray(step.n_new if step.counts is None else step.counts)
-        self._observed[step.seqs] = np.maximum(self._observed[step.seqs], ends)
-        self._valid[layer, step.seqs] = ends
+        self._observed[step.index] = np.maximum(self._observed[step.index], step.ends)
+        self._valid[layer, step.index] = step.ends
 
     def accept(self, step: Batch, nodes: Sequence[Sequence[int]]) -> Batch:
         """In place of the commit of a tree's step: of each sequence the nodes of a path (rising, none for a sequence that
@@ -479,16 +481,16 @@ class PagedKVCache:
         starts on whose weights are of other rows than they hold."""
         import torch
         size, t = self.pages.page_size, self.pages
+        lengths, tops = t.lens[seqs], np.minimum(self._observed[seqs], t.n_pages[seqs] * size)
+        firsts = np.clip(self._valid[:, seqs], starts, lengths)
         tails: dict = {}   # layers (None: all) -> (page, slot) of each
-        for s, start in zip(seqs, starts):
-            top, length = min(int(self._observed[s]), int(t.n_pages[s]) * size), int(t.lens[s])
-            if top > start:
-                firsts = np.clip(self._valid[:, s], start, length)
-                for first in np.unique(firsts):
-                    layers = None if (firsts == first).all() else tuple(np.flatnonzero(firsts == first))
-                    tails.setdefault(layers, []).extend((int(t.table[s, x // size]), x % size) for x in range(int(first), top))
-        self._observed[seqs] = np.minimum(self._observed[seqs], t.lens[seqs])
-        self._valid[:, seqs] = np.minimum(self._valid[:, seqs], t.lens[seqs])
+        for i in np.flatnonzero((firsts < tops).any(0)):
+            for first in np.unique(firsts[:, i]):
+                here = firsts[:, i] == first
+                layers = None if here.all() else tuple(np.flatnonzero(here))
+                tails.setdefault(layers, []).extend((int(t.table[seqs[i], x // size]), x % size) for x in range(int(first), int(tops[i])))
+        self._observed[seqs] = np.minimum(self._observed[seqs], lengths)
+        self._valid[:, seqs] = np.minimum(self._valid[:, seqs], lengths)
         for layers, tail in tails.items():
             if tail:
                 page, slot = (torch.tensor(i, dtype=torch.int64, device=self.device) for i in zip(*tail))
@@ -500,7 +502,7 @@ class PagedKVCache:
         others may hold by now."""
         if step.times_given_back == self.pages.times_given_back or step.given_back is None:
             return
-        if (self.pages.given_back[step.seqs] != step.given_back).any():
+        if (self.pages.given_back[step.index] != step.given_back).any():
             raise ValueError("a sequence has been freed or evicted from since the step was made: its slots and pages are no longer those of "
                              "the step")
 
