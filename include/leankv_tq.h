@@ -521,7 +521,8 @@ tq_status tq_attention_q8_tree_paged_cuda(const tq_attention_q8_args *a, const t
  * add nothing.  With decay 0, and from fresh[b] on, w is not read.  Slots from kv_len[b] on stay as they are.  Keys: TQ_TYPE_Q8 with
  * k_scale, or TQ2_0 / TQ3_0 / TQ4_0 blocks.  Sums are fp32.  A score is off by the sizes of its products, however much of them
  * cancels: by up to sm_scale * sum |k_d| * (2^-22 max |q'| + (log2 head_dim + 3) 2^-24 sum |q_d| / sqrt(head_dim)) and 2^-22 of
- * |s| + |lse| (TQ4_0 keys: besides (3 head_dim / 16 + 1) 2^-22 sm_scale * sum |q'_d k_d|), and a weight by as much of itself.
+ * |s| + |lse|; TQ4_0 keys: besides (3 head_dim / 16 + 1) 2^-22 sm_scale * sum |q'_d k_d|; more than 32 rows of 8-bit keys: besides
+ * 2^-15 sm_scale * max |q'| * the key's scale.  A weight is off by as much of itself.
  * max_kv_len sizes the work split; tokens behind it are counted all the same.
  * Sequences of a call must not share pages.  Work memory: tq_attention_weights_workspace_size() bytes.
  */

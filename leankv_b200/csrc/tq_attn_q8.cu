@@ -22,7 +22,8 @@
 //
 // Trees of drafted nodes (TREE) differ in what a row sees of the nodes alone, so only blocks behind the first node look at masks, 64 bits a
 // row in shared memory.  10 nodes of 4 heads behind 1000 tokens: 12.8 us, as a chain of as many tokens (12.4): two units of 24 rows, a
-// few blocks of tokens a CTA, then the merge; alone the two kernels take 9 us each, chains of dependent steps both.  Trees of more rows go to the tcgen05 kernels as drafted
+// few blocks of tokens a CTA, then the merge; alone the two kernels take 9 us each, chains of dependent steps both.
+// Trees of more rows go to the tcgen05 kernels as drafted
 // tokens do: 16 sequences of up to 9000 tokens with 26 nodes of 4 heads 100 us, 24 for the bytes (issue 37 %, tensor 22 %: the
 // converting warps' chain); 3 sequences of 12000 tokens with 63 nodes of 8 heads of 256, float16, 300 us, 138 for the products of
 // two terms (202 us of them attention, tensor 54 %, then the tiles' expansion and the merge).

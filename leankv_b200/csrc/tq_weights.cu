@@ -12,7 +12,7 @@
 //   rows       32        36         64         128         256
 //   D = 128    28     39 | 29    55 | 29    107 | 36    210 | 55
 //   D = 256    50     68 | 35    95 | 36    186 | 45    367 | 76
-// The bound of 32 rows is that of D = 128; heads of 256 with 32 rows would be faster there (about 35 us), with 8 they are not.
+// The bound of 32 rows is that of D = 128; heads of 256 with 32 rows would be faster there (about 35 us).
 //
 // What bounds it.  8 bits: the keys' bytes, 16 sequences of 32768 tokens of 8 KV heads (0.57 GB with the earlier weights) in 102 us,
 // 5.6 TB/s (86 % of the measured copy rate; a fourth of them in 36 us: issue 60 %, integer pipe 34 %, DRAM 48 %).  With f16 products

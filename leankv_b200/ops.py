@@ -542,8 +542,9 @@ def select_tokens(weights: torch.Tensor, page_table: torch.Tensor, kv_len: torch
     [B, max_pages_per_seq]; kv_len int32 [B].  keep: one number, or int32 CUDA [B] with width, their bound.  Of
     k = min(keep, kv_len, width) tokens the last min(recent, k) stay, the first min(sinks, k - recent), and of the others
     those with the largest weights, ties to the lowest slot, NaN as -inf.  Returns int32 [B, n_kv_heads, width] (in out; with one
-    number, keep or the smaller width): slots, rising, -1 behind the last.  max_kv_len: an upper bound of kv_len that sizes the work (default: the capacity); tokens
-    behind it are left out, with status raised, as for pages outside the pool (attention.last_status() without status)."""
+    number, keep or the smaller width): slots, rising, -1 behind the last.  max_kv_len: an upper bound of kv_len that sizes the
+    work (default: the capacity); tokens behind it are left out, with status raised, as for pages outside the pool
+    (attention.last_status() without status)."""
     by_sequence = isinstance(keep, torch.Tensor)
     device = _device_of(weights, page_table, kv_len, out, status, keep if by_sequence else None)
     pages, H, page_size = _check_weights(weights)
